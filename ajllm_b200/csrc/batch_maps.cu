@@ -1,0 +1,179 @@
+// Block tables, cache slots, positions and row offsets of a ragged batch from its request lengths.
+//
+// With counts[i] cache blocks and q[i] new tokens per sequence, F[i] = sum counts[:i], S[i] = sum q[:i]:
+//   table[i, j]  = ids[F[i] + j]               (j < counts[i], else pad)
+//   position[t]  = cached[i] + t - S[i]        (S[i] <= t < S[i + 1])
+//   slot[t]      = ids[F[i] + position / B] * B + position % B
+// Nothing is computed to speak of: a call lasts as long as one dependent chain (lengths -> sums -> block id -> store),
+// plus the time to write the tables when they are large. So there is one launch and no second pass over partial sums:
+// every CTA sums all lengths itself (a few KB out of L2, n / 256 per thread) and then takes its share of the output in
+// pieces of four elements, 16 bytes a store. Lengths are read as at least 0, and sums saturate at 2^30 - 1, so no input
+// reaches an index out of range: a token whose sequence has no block for it, and a row behind the last sequence, gets
+// the pad block.
+#include "common.cuh"
+
+namespace ajb {
+namespace maps {
+
+constexpr int kThreads = 256;
+constexpr int kMaxSeqs = 16384;              // two sums of 4 bytes per sequence in shared memory
+constexpr int kCap = (1 << 30) - 1;
+
+__device__ __forceinline__ int sat_add(int a, int b) { return min(a + b, kCap); }     // both in [0, kCap]
+
+struct Params {
+  const int *ids, *counts, *cached, *q_lens;
+  int n_ids, seqs, total, width, block_size, pad;
+  int *tables, *positions;
+  long long* slots;
+  int *q_start, *context;
+};
+
+// sums[i] = saturated sum of max(0, x[:i]) for i in [0, n]; all threads of the CTA, `n` uniform
+__device__ void prefix_sums(const int* __restrict__ x, int n, int* sums, int* warp_sums) {
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  int carry = 0;
+  for (int base = 0; base < n; base += kThreads) {
+    const int i = base + t;
+    int v = i < n ? min(max(x[i], 0), kCap) : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v = sat_add(v, up);
+    }
+    if (lane == 31) warp_sums[warp] = v;
+    __syncthreads();
+    int before = carry, all = carry;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w == warp) before = all;
+      all = sat_add(all, warp_sums[w]);
+    }
+    // saturated sums cannot be taken back apart: the exclusive sum comes from the neighbour's inclusive one
+    const int left = __shfl_up_sync(0xffffffffu, v, 1);
+    if (i < n) sums[i] = lane > 0 ? sat_add(before, left) : before;
+    carry = all;
+    __syncthreads();
+  }
+  if (t == 0) sums[n] = carry;
+}
+
+// last i in [0, n) with sums[i] <= t (n >= 1, sums[0] = 0 <= t)
+__device__ __forceinline__ int find(const int* sums, int n, int t) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (sums[mid] <= t) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(kThreads) batch_maps_kernel(const Params p) {
+  extern __shared__ int sums[];
+  __shared__ int warp_sums[kThreads / 32];
+  int* first_block = sums;
+  int* first_token = sums + p.seqs + 1;
+  prefix_sums(p.counts, p.seqs, first_block, warp_sums);
+  prefix_sums(p.q_lens, p.seqs, first_token, warp_sums);
+  __syncthreads();
+  const int tokens = min(first_token[p.seqs], p.total);        // rows that belong to a sequence
+  const long long thread = blockIdx.x * (long long)kThreads + threadIdx.x, threads = (long long)gridDim.x * kThreads;
+
+  for (long long i = thread; i <= p.seqs; i += threads) {
+    p.q_start[i] = min(first_token[i], p.total);
+    if (i < p.seqs) p.context[i] = (int)min((long long)max(p.cached[i], 0) + max(p.q_lens[i], 0), 0x7fffffffll);
+  }
+
+  // four tokens per thread: one search, then a step to the next sequence where one ends
+  const int token_pieces = (p.total + 3) >> 2;
+  for (long long piece = thread; piece < token_pieces; piece += threads) {
+    const int t0 = (int)piece * 4;
+    int pos[4];
+    long long slot[4];
+    int i = t0 < tokens ? find(first_token, p.seqs, t0) : p.seqs;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int t = t0 + k;
+      pos[k] = 0;
+      slot[k] = (long long)p.pad * p.block_size;
+      if (t < tokens) {
+        while (first_token[i + 1] <= t) ++i;                   // empty sequences are stepped over
+        const long long at = (long long)max(p.cached[i], 0) + (t - first_token[i]);
+        const long long b = at / p.block_size;
+        const int offset = (int)(at - b * p.block_size);
+        const bool has = b < first_block[i + 1] - first_block[i] && first_block[i] + b < p.n_ids;
+        const int id = has ? p.ids[first_block[i] + b] : p.pad;
+        pos[k] = (int)min(at, 0x7fffffffll);
+        slot[k] = (long long)id * p.block_size + offset;
+      }
+    }
+    if (t0 + 4 <= p.total) {
+      *reinterpret_cast<int4*>(p.positions + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+      *reinterpret_cast<longlong2*>(p.slots + t0) = make_longlong2(slot[0], slot[1]);
+      *reinterpret_cast<longlong2*>(p.slots + t0 + 2) = make_longlong2(slot[2], slot[3]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (t0 + k < p.total) {
+          p.positions[t0 + k] = pos[k];
+          p.slots[t0 + k] = slot[k];
+        }
+    }
+  }
+
+  // four table entries per thread; rows of any width, so a piece may end in the next row
+  const long long cells = (long long)p.seqs * p.width;
+  for (long long piece = thread; piece < (cells + 3) >> 2; piece += threads) {
+    const long long c0 = piece * 4;
+    int row = (int)(c0 / p.width), col = (int)(c0 - (long long)row * p.width);
+    int v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[k] = p.pad;
+      if (row < p.seqs) {
+        const long long at = (long long)first_block[row] + col;
+        if (at < first_block[row + 1] && at < p.n_ids) v[k] = p.ids[at];
+      }
+      if (++col == p.width) { col = 0; ++row; }
+    }
+    if (c0 + 4 <= cells) {
+      *reinterpret_cast<int4*>(p.tables + c0) = make_int4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (c0 + k < cells) p.tables[c0 + k] = v[k];
+    }
+  }
+}
+
+}  // namespace maps
+}  // namespace ajb
+
+// ids [n_ids] block ids of all sequences, one after another; counts / cached / q_lens [seqs]; all int32 on the device.
+// tables [seqs, width], positions [total], slots [total] (int64), q_start [seqs + 1], context [seqs]; tables, positions
+// and slots 16-byte aligned.
+extern "C" int ajb_batch_maps(const void* ids, const void* counts, const void* cached, const void* q_lens, int n_ids, int seqs,
+                              int total, int width, int block_size, int pad, void* tables, void* positions, void* slots,
+                              void* q_start, void* context, void* stream) {
+  using namespace ajb;
+  AJB_REQUIRE(seqs >= 0 && seqs <= maps::kMaxSeqs, "batch maps: %d sequences (at most %d)", seqs, maps::kMaxSeqs);
+  AJB_REQUIRE(total >= 0 && total <= maps::kCap && n_ids >= 0 && n_ids <= maps::kCap && width >= 1 && block_size >= 1,
+              "batch maps: %d tokens, %d block ids, %d blocks per table row, %d tokens per block are out of range", total, n_ids,
+              width, block_size);
+  AJB_REQUIRE(((reinterpret_cast<uintptr_t>(tables) | reinterpret_cast<uintptr_t>(positions) | reinterpret_cast<uintptr_t>(slots)) & 15) == 0,
+              "batch maps: tables, positions and slots must be 16-byte aligned");
+  maps::Params p;
+  p.ids = (const int*)ids; p.counts = (const int*)counts; p.cached = (const int*)cached; p.q_lens = (const int*)q_lens;
+  p.n_ids = n_ids; p.seqs = seqs; p.total = total; p.width = width; p.block_size = block_size; p.pad = pad;
+  p.tables = (int*)tables; p.positions = (int*)positions; p.slots = (long long*)slots; p.q_start = (int*)q_start;
+  p.context = (int*)context;
+  const int smem = 2 * (seqs + 1) * (int)sizeof(int);
+  if (smem > 48 * 1024)      // per device and cheap next to a batch of thousands of sequences: set on every such call
+    AJB_CUDA_OK(cudaFuncSetAttribute(maps::batch_maps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  const long long pieces = ((long long)total + 3) / 4 + ((long long)seqs * width + 3) / 4 + 1;
+  const long long blocks = (pieces + maps::kThreads - 1) / maps::kThreads;
+  maps::batch_maps_kernel<<<(int)(blocks < 4ll * sm_count() ? blocks : 4ll * sm_count()), maps::kThreads, smem,
+                            reinterpret_cast<cudaStream_t>(stream)>>>(p);
+  AJB_CUDA_OK(cudaGetLastError());
+  return 0;
+}

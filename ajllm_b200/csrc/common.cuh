@@ -37,6 +37,8 @@ const char* last_error();
     }                                       \
   } while (0)
 
+constexpr int kMaxDevices = 16;   // devices of one process that per-device state is kept for
+
 // Device status words written by kernels whose bounded waits expired. Index = kernel id.
 enum KernelId : int { kGemm = 0, kFlashFwd = 1, kFlashBwdKV = 2, kFlashBwdQ = 3, kCommGemm = 4, kFlashBwdFused = 8, kNumKernelIds = 16 };
 struct DeviceStatus {

@@ -37,7 +37,12 @@
 // Layouts: q [tokens, Hq, hd] bf16 (rows of a sequence are contiguous, `q_start[seq]` is its first
 // row); caches [num_blocks, block_size = 16, Hkv, hd] bf16; block_tables [num_seqs, max_blocks] int32;
 // out like q.
+//
+// Behind a shared prefix (csrc/prefix_attention.cu) the kernel covers the rest of every sequence: it starts at key
+// `first_key`, always leaves un-normalised parts, and sequences with more query rows than one CTA holds are cut into
+// `chunks` of q_len tokens each.
 #include "common.cuh"
+#include "paged_attention.h"
 
 namespace ajb {
 namespace paged {
@@ -46,7 +51,7 @@ constexpr int TILE = 64;           // keys per step
 constexpr int QROWS = 128;         // rows of the query / probability operand tiles (the MMA's M)
 constexpr int BLOCK_TOKENS = 16;   // tokens per cache block
 constexpr int kThreads = 192;
-constexpr int kMaxRows = 64;       // group * q_len
+constexpr int kMaxRows = 64;       // group * q_len of a plain launch
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kPagedKernelId = 5;
 constexpr int kReplTileBytes = 32 * 128;   // REPL variant: the 32 meaningful rows of a probability tile (64 keys x 2 bytes per row)
@@ -69,15 +74,31 @@ struct Params {
   __nv_bfloat16* out;
   const int* block_tables;
   const int* context_lens;
-  const int* q_start;
+  const int* q_start;         // null: sequence i's rows start at i * q_total
+  long long q_pitch;          // elements between the rows of two tokens in q
   int max_blocks;
   int heads, kv_heads, q_len;
+  int q_total;                // new tokens per sequence; q_len of them are a CTA's, chunk after chunk
+  int first_key;              // first cached token this launch looks at (a multiple of the block size)
   float scale;
-  int splits;                 // CTAs per (sequence, KV head); > 1: partial results go to the workspace
-  float* part_o;              // [tokens, Hq, splits, hd] fp32, un-normalised
-  float2* part_ml;            // [tokens, Hq, splits] (reference maximum in log2 units, row sum); sum 0 = no keys seen
+  int splits;                 // CTAs per (sequence, KV head, chunk)
+  int part_stride, part_base; // parts per row in the workspace and the first one of this launch; part_stride 0: no parts
+  float* part_o;              // [tokens, Hq, part_stride, hd] fp32, un-normalised
+  float2* part_ml;            // [tokens, Hq, part_stride] (reference maximum in log2 units, row sum); sum 0 = no keys seen
   DeviceStatus* status;
 };
+
+// Rows [first, TILE) of a V tile become zero: they belong to no key (the unused end of the last block, or a block fetched
+// again to fill the tile), their probabilities are zero, and zero times whatever an old sequence left there (an
+// infinity, a NaN) must not reach the sums. `t` is the caller's index among the 128 threads that share the work.
+template <int HD>
+__device__ __forceinline__ void zero_value_rows(uint8_t* tile, int first, int t) {
+  constexpr int kBoxes = HD / 64;
+  for (int i = first * 8 + t; i < TILE * 8; i += 128) {
+#pragma unroll
+    for (int b = 0; b < kBoxes; ++b) reinterpret_cast<uint4*>(tile + b * (TILE * 128))[i] = make_uint4(0, 0, 0, 0);
+  }
+}
 
 // 16-byte chunk `ch` of row `row` of a K-major operand tile of QROWS rows (128-byte swizzle, 64-element boxes).
 __device__ __forceinline__ void store_chunk(uint8_t* tile, int row, int ch, uint4 val) {
@@ -115,17 +136,24 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int seq = blockIdx.x, kv_head = blockIdx.y;
+  const int seq = blockIdx.x, kv_head = (int)blockIdx.y % p.kv_heads;
   const int group = p.heads / p.kv_heads;
-  const int rows = group * p.q_len;                 // real rows, packed head-major: row = h_in_group * q_len + i
-  const int ctx = p.context_lens[seq];
-  const int all_tiles = (ctx + TILE - 1) / TILE;
+  const int q0 = ((int)blockIdx.y / p.kv_heads) * p.q_len;          // first of this CTA's new tokens
+  const int q_len = min(p.q_len, p.q_total - q0);
+  const int rows = group * q_len;                   // real rows, packed head-major: row = h_in_group * q_len + i
+  const int token0 = (p.q_start != nullptr ? p.q_start[seq] : seq * p.q_total) + q0;
+  // keys are counted from first_key; the block table bounds them whatever the context length says
+  const int ctx = p.context_lens[seq] - (p.q_total - q0 - q_len) - p.first_key;
+  const int keys = min(max(ctx, 0), p.max_blocks * BLOCK_TOKENS - p.first_key);
+  const int all_tiles = (keys + TILE - 1) / TILE;
   // this CTA's share of the sequence's tiles: [t0, t0 + n_tiles)
   const int per_split = (all_tiles + p.splits - 1) / p.splits;
   const int t0 = min(all_tiles, (int)blockIdx.z * per_split);
   const int n_tiles = min(all_tiles - t0, per_split);
   const int active_quarters = (rows + 31) / 32;
-  const int* table = p.block_tables + (size_t)seq * p.max_blocks;
+  // the tile that the last key does not fill, if it is this CTA's (always its last one)
+  const int ragged_tile = (keys % TILE != 0 && n_tiles > 0 && t0 + n_tiles == all_tiles) ? n_tiles - 1 : -1;
+  const int* table = p.block_tables + (size_t)seq * p.max_blocks + p.first_key / BLOCK_TOKENS;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -153,8 +181,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     const int t = threadIdx.x - 64;                 // 0..127 == tile row
     const int qr = REPL ? (t & 31) : t;             // REPL: every quarter holds a copy of the query rows
     const bool real = qr < rows;
-    const int h = real ? qr / p.q_len : 0, i = real ? qr % p.q_len : 0;
-    const __nv_bfloat16* src = p.q + ((size_t)(p.q_start[seq] + i) * p.heads + kv_head * group + h) * HD;
+    const int h = real ? qr / q_len : 0, i = real ? qr % q_len : 0;
+    const __nv_bfloat16* src = p.q + (size_t)(token0 + i) * p.q_pitch + (size_t)(kv_head * group + h) * HD;
 #pragma unroll
     for (int ch = 0; ch < HD / 8; ++ch) {
       const uint4 v = real ? reinterpret_cast<const uint4*>(src)[ch] : make_uint4(0, 0, 0, 0);
@@ -173,7 +201,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     // its copies would cost more than the copies themselves.
     constexpr int kBlocksPerTile = TILE / BLOCK_TOKENS;
     constexpr int kTilesPerGroup = 32 / kBlocksPerTile;
-    const int last_block = (ctx + BLOCK_TOKENS - 1) / BLOCK_TOKENS - 1;
+    const int last_block = (keys + BLOCK_TOKENS - 1) / BLOCK_TOKENS - 1;
     // blocks past the end of the sequence re-read the last valid block (masked later); keeps the byte count fixed
     auto fetch_ids = [&](int group) { return table[max(0, min(last_block, (t0 + group * kTilesPerGroup) * kBlocksPerTile + lane))]; };
     int ids_next = n_tiles > 0 ? fetch_ids(0) : 0;
@@ -287,8 +315,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     // ---- at most 32 query rows, copied into every quarter: warp q handles key columns [16 q, 16 q + 16)
     const int quarter = warp & 3;
     const bool real = lane < rows;
-    const int h = real ? lane / p.q_len : 0, qi = real ? lane % p.q_len : 0;
-    const int k_max = real ? ctx - p.q_len + qi : -1;   // last visible key
+    const int h = real ? lane / q_len : 0, qi = real ? lane % q_len : 0;
+    const int k_max = real ? min(ctx - q_len + qi, keys - 1) : -1;   // last visible key
     const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
     const float sl = p.scale * kLog2e;
     float m_run = -INFINITY, l_run = 0.0f;              // l_run: this warp's 16 columns of every tile only
@@ -364,6 +392,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 #pragma unroll
       for (int ch = 0; ch < 2; ++ch)
         store_chunk(tile_p, lane, quarter * 2 + ch, make_uint4(pk[ch * 4], pk[ch * 4 + 1], pk[ch * 4 + 2], pk[ch * 4 + 3]));
+      if (ragged_tile == j) {
+        if (!mbar_wait(&v_full[s], ((uint32_t)j >> 1) & 1, abort_flag, p.status, kPagedKernelId, 11)) { ok = false; break; }
+        zero_value_rows<HD>(sKV + s * 2 * C::kTile + C::kTile, keys - (t0 + j) * TILE, quarter * 32 + lane);
+      }
       if (j > 0 && __any_sync(0xffffffffu, moved)) {
         // O changes scale: every product up to tile j - 1 must have landed first (all warps wait, so that none
         // announces its part of P before the rescaled O is in place ... the first warp rescales)
@@ -397,18 +429,19 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         ok = collect((uint32_t)n_tiles, sums);
       }
     }
-    const size_t out_row = (size_t)(p.q_start[seq] + qi) * p.heads + kv_head * group + h;
-    if (p.splits > 1 && quarter == 0 && real && (n_tiles == 0 || !ok))
-      p.part_ml[out_row * p.splits + blockIdx.z] = make_float2(0.0f, 0.0f);        // nothing to merge from this part
+    const size_t out_row = (size_t)(token0 + qi) * p.heads + kv_head * group + h;
+    const size_t part_row = out_row * p.part_stride + p.part_base + blockIdx.z;
+    if (p.part_stride > 0 && quarter == 0 && real && (n_tiles == 0 || !ok))
+      p.part_ml[part_row] = make_float2(0.0f, 0.0f);        // nothing to merge from this part
     if (ok && quarter == 0 && n_tiles > 0 &&
         mbar_wait(&pv_done[(n_tiles - 1) & 1], (((uint32_t)(n_tiles - 1)) >> 1) & 1, abort_flag, p.status, kPagedKernelId, 8)) {
       tc_fence_after_sync();
       const float l_all = (sums[0] + sums[1]) + (sums[2] + sums[3]);
       const float inv_l = l_all > 0.0f ? 1.0f / l_all : 0.0f;
       __nv_bfloat16* dst = p.out + out_row * HD;
-      if (p.splits > 1) {
-        if (real) p.part_ml[out_row * p.splits + blockIdx.z] = make_float2(m_run == -INFINITY ? 0.0f : m_run * sl, l_all);
-        float* part = p.part_o + (out_row * p.splits + blockIdx.z) * HD;
+      if (p.part_stride > 0) {
+        if (real) p.part_ml[part_row] = make_float2(m_run == -INFINITY ? 0.0f : m_run * sl, l_all);
+        float* part = p.part_o + part_row * HD;
 #pragma unroll 1
         for (int c = 0; c < HD / 32; ++c) {
           uint32_t ov[32];
@@ -444,8 +477,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     const int row = quarter * 32 + lane;
     const bool active = quarter < active_quarters;     // warp-uniform
     const bool real = row < rows;
-    const int h = real ? row / p.q_len : 0, qi = real ? row % p.q_len : 0;
-    const int k_max = real ? ctx - p.q_len + qi : -1;   // last visible key
+    const int h = real ? row / q_len : 0, qi = real ? row % q_len : 0;
+    const int k_max = real ? min(ctx - q_len + qi, keys - 1) : -1;   // last visible key
     const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
     const float sl = p.scale * kLog2e;
     float m_run = -INFINITY, l_run = 0.0f;
@@ -507,6 +540,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 #pragma unroll
         for (int ch = 0; ch < TILE / 8; ++ch) store_chunk(sP, row, ch, make_uint4(pk[ch * 4], pk[ch * 4 + 1], pk[ch * 4 + 2], pk[ch * 4 + 3]));
       }
+      if (ragged_tile == j) {
+        if (!mbar_wait(&v_full[s], ((uint32_t)j >> 1) & 1, abort_flag, p.status, kPagedKernelId, 11)) { ok = false; break; }
+        zero_value_rows<HD>(sKV + s * 2 * C::kTile + C::kTile, keys - (t0 + j) * TILE, quarter * 32 + lane);
+      }
       if (active && j > 0 && __any_sync(0xffffffffu, moved)) {
 #pragma unroll 1
         for (int c = 0; c < HD / 32; ++c) {
@@ -524,14 +561,15 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_ready[0]);
     }
-    const size_t out_row = (size_t)(p.q_start[seq] + qi) * p.heads + kv_head * group + h;
-    if (p.splits > 1 && real && (n_tiles == 0 || !ok))
-      p.part_ml[out_row * p.splits + blockIdx.z] = make_float2(0.0f, 0.0f);        // nothing to merge from this part
+    const size_t out_row = (size_t)(token0 + qi) * p.heads + kv_head * group + h;
+    const size_t part_row = out_row * p.part_stride + p.part_base + blockIdx.z;
+    if (p.part_stride > 0 && real && (n_tiles == 0 || !ok))
+      p.part_ml[part_row] = make_float2(0.0f, 0.0f);        // nothing to merge from this part
     if (ok && n_tiles > 0 && mbar_wait(&pv_done[0], (uint32_t)(n_tiles - 1) & 1, abort_flag, p.status, kPagedKernelId, 8)) {
       tc_fence_after_sync();
-      if (active && p.splits > 1) {
-        if (real) p.part_ml[out_row * p.splits + blockIdx.z] = make_float2(m_run == -INFINITY ? 0.0f : m_run * sl, l_run);
-        float* part = p.part_o + (out_row * p.splits + blockIdx.z) * HD;
+      if (active && p.part_stride > 0) {
+        if (real) p.part_ml[part_row] = make_float2(m_run == -INFINITY ? 0.0f : m_run * sl, l_run);
+        float* part = p.part_o + part_row * HD;
 #pragma unroll 1
         for (int c = 0; c < HD / 32; ++c) {
           uint32_t ov[32];
@@ -586,7 +624,7 @@ __global__ void merge_splits_kernel(const float* __restrict__ part_o, const floa
   const long long local_row = w / heads;
   const int head = (int)(w - local_row * heads);
   const int seq = (int)(local_row / q_len), i = (int)(local_row - (long long)seq * q_len);
-  const size_t out_row = (size_t)(q_start[seq] + i) * heads + head;
+  const size_t out_row = (q_start != nullptr ? (size_t)(q_start[seq] + i) : (size_t)local_row) * heads + head;
   float m_max = -INFINITY;
   for (int z = 0; z < splits; ++z) {
     const float2 ml = part_ml[out_row * splits + z];
@@ -612,21 +650,21 @@ __global__ void merge_splits_kernel(const float* __restrict__ part_o, const floa
 }
 
 template <int HD>
-static int launch(const void* q, const void* k_cache, const void* v_cache, const void* block_tables,
-                  const void* context_lens, const void* q_start, void* out, int num_seqs, int num_blocks, int max_blocks,
-                  int heads, int kv_heads, int q_len, float scale, int splits, void* part_o, void* part_ml,
-                  cudaStream_t stream) {
+static int launch_kernel(const Launch& a, cudaStream_t stream) {
   using C = Cfg<HD>;
   CUtensorMap map_k, map_v;
-  const uint64_t row_pitch = (uint64_t)kv_heads * HD * 2;
-  int rc = make_tensor_map_3d(&map_k, k_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, num_blocks, BLOCK_TOKENS,
-                              (uint64_t)kv_heads * HD, row_pitch * BLOCK_TOKENS, row_pitch, BLOCK_TOKENS, 64);
+  const uint64_t row_pitch = (uint64_t)a.kv_heads * HD * 2;
+  int rc = make_tensor_map_3d(&map_k, a.k_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.num_blocks, BLOCK_TOKENS,
+                              (uint64_t)a.kv_heads * HD, row_pitch * BLOCK_TOKENS, row_pitch, BLOCK_TOKENS, 64);
   if (rc) return rc;
-  rc = make_tensor_map_3d(&map_v, v_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, num_blocks, BLOCK_TOKENS,
-                          (uint64_t)kv_heads * HD, row_pitch * BLOCK_TOKENS, row_pitch, BLOCK_TOKENS, 64);
+  rc = make_tensor_map_3d(&map_v, a.v_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.num_blocks, BLOCK_TOKENS,
+                          (uint64_t)a.kv_heads * HD, row_pitch * BLOCK_TOKENS, row_pitch, BLOCK_TOKENS, 64);
   if (rc) return rc;
-  static bool configured = false;
-  if (!configured) {
+  // function attributes belong to a device: set once on each
+  static bool configured[kMaxDevices] = {};
+  int dev = 0;
+  AJB_CUDA_OK(cudaGetDevice(&dev));
+  if (dev >= kMaxDevices || !configured[dev]) {
     AJB_CUDA_OK(cudaFuncSetAttribute(paged_attention_kernel<HD, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
     AJB_CUDA_OK(cudaFuncSetAttribute(paged_attention_kernel<HD, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
     // two CTAs per SM need the whole shared-memory carve-out
@@ -634,28 +672,54 @@ static int launch(const void* q, const void* k_cache, const void* v_cache, const
                                      cudaSharedmemCarveoutMaxShared));
     AJB_CUDA_OK(cudaFuncSetAttribute(paged_attention_kernel<HD, true>, cudaFuncAttributePreferredSharedMemoryCarveout,
                                      cudaSharedmemCarveoutMaxShared));
-    configured = true;
+    if (dev < kMaxDevices) configured[dev] = true;
   }
   Params p;
-  p.q = (const __nv_bfloat16*)q; p.out = (__nv_bfloat16*)out; p.block_tables = (const int*)block_tables;
-  p.context_lens = (const int*)context_lens; p.q_start = (const int*)q_start; p.max_blocks = max_blocks;
-  p.heads = heads; p.kv_heads = kv_heads; p.q_len = q_len; p.scale = scale; p.status = device_status_buffer();
-  p.splits = splits; p.part_o = (float*)part_o; p.part_ml = (float2*)part_ml;
-  if ((heads / kv_heads) * q_len <= 32)
-    paged_attention_kernel<HD, true><<<dim3(num_seqs, kv_heads, splits), kThreads, C::kSmem, stream>>>(map_k, map_v, p);
+  p.q = (const __nv_bfloat16*)a.q; p.out = (__nv_bfloat16*)a.out; p.block_tables = (const int*)a.block_tables;
+  p.context_lens = (const int*)a.context_lens; p.q_start = (const int*)a.q_start; p.q_pitch = a.q_pitch;
+  p.max_blocks = a.max_blocks; p.heads = a.heads; p.kv_heads = a.kv_heads; p.q_len = a.q_len; p.q_total = a.q_total;
+  p.first_key = a.first_key; p.scale = a.scale; p.status = device_status_buffer();
+  p.splits = a.splits; p.part_stride = a.part_stride; p.part_base = a.part_base;
+  p.part_o = (float*)a.part_o; p.part_ml = (float2*)a.part_ml;
+  const int chunks = (a.q_total + a.q_len - 1) / a.q_len;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.num_seqs, a.kv_heads * chunks, a.splits);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = a.beside_previous ? 1 : 0;
+  if ((a.heads / a.kv_heads) * a.q_len <= 32)
+    AJB_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_attention_kernel<HD, true>, map_k, map_v, p));
   else
-    paged_attention_kernel<HD, false><<<dim3(num_seqs, kv_heads, splits), kThreads, C::kSmem, stream>>>(map_k, map_v, p);
-  AJB_CUDA_OK(cudaGetLastError());
-  if (splits > 1) {
-    const long long pairs = (long long)num_seqs * q_len * heads;
-    const int threads = 128;
-    const long long blocks = (pairs * 32 + threads - 1) / threads;
-    merge_splits_kernel<HD><<<(unsigned)blocks, threads, 0, stream>>>((const float*)part_o, (const float2*)part_ml,
-                                                                      (__nv_bfloat16*)out, (const int*)q_start, q_len, heads,
-                                                                      splits, pairs);
-    AJB_CUDA_OK(cudaGetLastError());
-  }
+    AJB_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_attention_kernel<HD, false>, map_k, map_v, p));
   return 0;
+}
+
+int launch(const Launch& a, int head_dim, cudaStream_t stream) {
+  if (head_dim == 128) return launch_kernel<128>(a, stream);
+  if (head_dim == 64) return launch_kernel<64>(a, stream);
+  set_error("paged attention: head_dim %d is not supported (64 and 128 are)", head_dim);
+  return 2;
+}
+
+template <int HD>
+static int launch_merge(const Launch& a, cudaStream_t stream) {
+  const long long pairs = (long long)a.num_seqs * a.q_total * a.heads;
+  const int threads = 128;
+  const long long blocks = (pairs * 32 + threads - 1) / threads;
+  merge_splits_kernel<HD><<<(unsigned)blocks, threads, 0, stream>>>((const float*)a.part_o, (const float2*)a.part_ml,
+                                                                    (__nv_bfloat16*)a.out, (const int*)a.q_start, a.q_total,
+                                                                    a.heads, a.part_stride, pairs);
+  AJB_CUDA_OK(cudaGetLastError());
+  return 0;
+}
+
+int merge_parts(const Launch& a, int head_dim, cudaStream_t stream) {
+  return head_dim == 128 ? launch_merge<128>(a, stream) : launch_merge<64>(a, stream);
 }
 
 }  // namespace paged
@@ -677,12 +741,14 @@ extern "C" int ajb_paged_attention(const void* q, const void* k_cache, const voi
               "paged attention: (heads / kv_heads) * q_len = %d exceeds %d", (heads / kv_heads) * q_len, paged::kMaxRows);
   if (num_seqs <= 0) return 0;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (head_dim == 128)
-    return paged::launch<128>(q, k_cache, v_cache, block_tables, context_lens, q_start, out, num_seqs, num_blocks,
-                              max_blocks, heads, kv_heads, q_len, scale, splits, part_o, part_ml, s);
-  if (head_dim == 64)
-    return paged::launch<64>(q, k_cache, v_cache, block_tables, context_lens, q_start, out, num_seqs, num_blocks,
-                             max_blocks, heads, kv_heads, q_len, scale, splits, part_o, part_ml, s);
-  set_error("paged attention: head_dim %d is not supported (64 and 128 are)", head_dim);
-  return 2;
+  paged::Launch a;
+  a.q = q; a.k_cache = k_cache; a.v_cache = v_cache; a.block_tables = block_tables; a.context_lens = context_lens;
+  a.q_start = q_start; a.out = out; a.q_pitch = (long long)heads * head_dim;
+  a.num_seqs = num_seqs; a.num_blocks = num_blocks; a.max_blocks = max_blocks; a.heads = heads; a.kv_heads = kv_heads;
+  a.q_len = q_len; a.q_total = q_len; a.first_key = 0; a.scale = scale; a.splits = splits;
+  a.part_stride = splits > 1 ? splits : 0; a.part_base = 0; a.part_o = part_o; a.part_ml = part_ml;
+  a.beside_previous = false;
+  int rc = paged::launch(a, head_dim, s);
+  if (rc == 0 && splits > 1) rc = paged::merge_parts(a, head_dim, s);
+  return rc;
 }

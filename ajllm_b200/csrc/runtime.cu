@@ -21,7 +21,6 @@ void set_error(const char* fmt, ...) {
 
 const char* last_error() { return g_error; }
 
-static constexpr int kMaxDevices = 16;
 static DeviceStatus* g_status[kMaxDevices] = {nullptr};
 static int g_sm_count[kMaxDevices] = {0};
 static std::mutex g_mutex;

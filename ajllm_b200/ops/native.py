@@ -71,6 +71,9 @@ _SIGNATURES: dict[str, list] = {
     "ajb_sample_rows": [c_void, c_long, c_int, c_int, c_void, c_void, c_void, c_void, c_void, c_int, c_void, c_void],
     "ajb_spec_verify": [c_void, c_void, c_void, c_int, c_int, c_int, c_void, c_void, c_void, c_void, c_void],
     "ajb_paged_attention": [c_void] * 7 + [c_int] * 8 + [c_float, c_int, c_void, c_void, c_void],
+    "ajb_shared_prefix_attention": [c_void] * 6 + [c_long] + [c_int] * 9 + [c_float, c_int, c_int, c_void, c_void, c_void],
+    "ajb_batch_maps": [c_void] * 4 + [c_int] * 6 + [c_void] * 6,
+    "ajb_process_logits": [c_void, c_int, c_long, c_void, c_int, c_int, c_void, c_long, c_int] + [c_void] * 7 + [c_int, c_void, c_long, c_void],
     "ajb_flash_bwd": [c_void, c_void, c_void, c_void, c_void, c_void, c_void, c_int, c_int, c_int, c_int, c_int,
                       c_long, c_int, c_float, c_void],
 }
@@ -132,7 +135,7 @@ class PeerTimeout(RuntimeError):
     def __init__(self, code: int) -> None:
         self.code, self.kernel_id, self.stage = code, (code & 0xFF) - 1, code >> 8
         names = {0: "gemm", 1: "flash forward", 2: "flash backward (dK/dV)", 3: "flash backward (dQ)", 4: "tensor-parallel gemm",
-                 5: "paged attention", 6: "fp8 gemm", 7: "expert exchange", 8: "flash backward (fused)", 9: "gradient reduce-scatter", 10: "gemm (CTA pairs)", 11: "decoding gemm (cluster)"}
+                 5: "paged attention", 6: "fp8 gemm", 7: "expert exchange", 8: "flash backward (fused)", 9: "gradient reduce-scatter", 10: "gemm (CTA pairs)", 11: "decoding gemm (cluster)", 12: "shared-prefix attention"}
         super().__init__(f"kernel '{names.get(self.kernel_id, self.kernel_id)}' stopped waiting at stage {self.stage} "
                          f"(status word {code:#x}); its outputs are incomplete")
 
@@ -169,7 +172,8 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 
 # kernels launched per entry point (everything else launches one)
-_LAUNCHES_PER_CALL = {"ajb_flash_bwd": 3, "ajb_sumsq_f32": 2, "ajb_gemm_bf16_decode": 2, "ajb_gemm_bf16_skinny_pair": 2}
+_LAUNCHES_PER_CALL = {"ajb_flash_bwd": 3, "ajb_sumsq_f32": 2, "ajb_gemm_bf16_decode": 2, "ajb_gemm_bf16_skinny_pair": 2,
+                      "ajb_shared_prefix_attention": 3}
 launch_count = 0
 
 

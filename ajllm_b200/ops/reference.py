@@ -156,6 +156,96 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     return out
 
 
+def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                            context_lens: torch.Tensor, prefix_len: int, q_len: int = 1,
+                            scale: float | None = None) -> torch.Tensor:
+    """Decode / verify attention of sequences that share their first ``prefix_len`` tokens (whole blocks of them are
+    looked up in the first row of ``block_tables``). ``q`` is ``[num_seqs * q_len, Hq, hd]``; query row ``j`` of a
+    sequence sees the shared blocks and its own tokens up to position ``context_len - q_len + j``; a row that sees
+    nothing comes out as zeros."""
+    block, kv_heads, hd = k_cache.shape[1:]
+    heads = q.shape[1]
+    scale = scale if scale is not None else 1.0 / math.sqrt(hd)
+    columns = prefix_len // block
+    shared = columns * block
+    out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+    for i in range(block_tables.shape[0]):
+        context = int(context_lens[i])
+        length = max(shared, min(context, block_tables.shape[1] * block))
+        ids = torch.cat((block_tables[0, :columns], block_tables[i, columns:(length + block - 1) // block])).long()
+        keys, values = (c[ids].reshape(-1, kv_heads, hd)[:length].float().repeat_interleave(heads // kv_heads, dim=1)
+                        for c in (k_cache, v_cache))
+        rows = q[i * q_len:(i + 1) * q_len].float()
+        scores = torch.einsum("ihd,shd->ihs", rows, keys) * scale
+        last = (context - q_len + torch.arange(q_len, device=q.device)).clamp(min=shared - 1)
+        scores = scores.masked_fill(torch.arange(length, device=q.device)[None, None, :] > last[:, None, None], float("-inf"))
+        probs = torch.nan_to_num(torch.softmax(scores, dim=-1)) if shared == 0 else torch.softmax(scores, dim=-1)
+        out[i * q_len:(i + 1) * q_len] = torch.einsum("ihs,shd->ihd", probs, values).to(q.dtype)
+    return out
+
+
+def batch_maps(block_ids: torch.Tensor, block_counts: torch.Tensor, cached_lens: torch.Tensor, q_lens: torch.Tensor,
+               total_tokens: int, max_blocks: int, block_size: int, pad_block: int) -> tuple[torch.Tensor, ...]:
+    """Block tables ``[n, max_blocks]``, positions and cache slots ``[total_tokens]``, row offsets ``[n + 1]`` and
+    context lengths ``[n]`` of a ragged batch; what no sequence owns is filled from ``pad_block``."""
+    n = block_counts.shape[0]
+    int32 = dict(dtype=torch.int32, device=block_ids.device)
+    tables = torch.full((n, max_blocks), pad_block, **int32)
+    positions = torch.zeros(total_tokens, **int32)
+    slots = torch.full((total_tokens,), pad_block * block_size, dtype=torch.int64, device=block_ids.device)
+    starts, contexts = [0], []
+    ids = block_ids.tolist()
+    first = 0
+    for i, (count, cached, new) in enumerate(zip(block_counts.tolist(), cached_lens.tolist(), q_lens.tolist())):
+        count, cached, new = max(0, count), max(0, cached), max(0, new)
+        own = ids[first:first + count]
+        first += count
+        tables[i, :min(len(own), max_blocks)] = torch.tensor(own[:max_blocks], **int32)
+        lo, hi = starts[-1], min(starts[-1] + new, total_tokens)
+        for t in range(lo, hi):
+            at = cached + t - lo
+            positions[t] = at
+            block = own[at // block_size] if at // block_size < len(own) else pad_block
+            slots[t] = block * block_size + at % block_size
+        starts.append(hi)
+        contexts.append(cached + new)
+    return tables, positions, slots, torch.tensor(starts, **int32), torch.tensor(contexts, **int32)
+
+
+def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None, prompt_lens: torch.Tensor | None = None,
+                   history_lens: torch.Tensor | None = None, repetition: torch.Tensor | None = None,
+                   presence: torch.Tensor | None = None, frequency: torch.Tensor | None = None,
+                   bias_ids: torch.Tensor | None = None, bias_values: torch.Tensor | None = None,
+                   token_mask: torch.Tensor | None = None) -> torch.Tensor:
+    """Penalties for repeated tokens, then biases, then the grammar mask, in fp32 (see ``ops.serving.process_logits``)."""
+    x = logits.float().clone()
+    rows, vocab = x.shape
+    if history is not None:
+        place = torch.arange(history.shape[1], device=x.device)[None, :]
+        known = (place < history_lens[:, None]) & (history >= 0) & (history < vocab)
+        made = known & (place >= prompt_lens[:, None])
+        ids = history.long().clamp(0, vocab - 1)
+        seen, count = (torch.zeros(rows, vocab, dtype=torch.int32, device=x.device).scatter_add_(1, ids, hit.int())
+                       for hit in (known, made))
+        if repetition is not None:
+            factor = repetition[:, None]
+            x = torch.where(seen > 0, torch.where(x > 0, x / factor, x * factor), x)
+        if frequency is not None:
+            x = torch.where(count > 0, x - frequency[:, None] * count, x)
+        if presence is not None:
+            x = torch.where(count > 0, x - presence[:, None], x)
+    if bias_ids is not None:
+        index = torch.arange(rows, device=x.device)
+        for j in range(bias_ids.shape[1]):
+            token = bias_ids[:, j].long()
+            hit = (token >= 0) & (token < vocab)
+            x[index[hit], token[hit]] += bias_values[hit, j]
+    if token_mask is not None:
+        bit = torch.arange(vocab, device=x.device)
+        x = x.masked_fill((token_mask[:, bit // 32] >> (bit % 32)) & 1 == 0, float("-inf"))
+    return x
+
+
 def quantize_weight_fp8_blocks(weight: torch.Tensor, block: int = 128) -> tuple[torch.Tensor, torch.Tensor]:
     """e4m3 weights with one fp32 scale per ``block x block`` tile: ``w ≈ q * scale``."""
     out_f, in_f = weight.shape

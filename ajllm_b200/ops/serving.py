@@ -1,14 +1,17 @@
 """GPU entry points of the serving path: in-place RoPE on packed rows with explicit positions, paged
 attention for decode / verify rows, the training flash kernel for prompts that start from an empty
-cache, and the batched sampler."""
+cache, and the batched sampler; block tables and slot maps built on the device, paged attention of a batch
+behind a shared prefix, and logits processing (these three take CPU tensors too and then run the plain
+statements of :mod:`ajllm_b200.ops.reference`)."""
 
 from __future__ import annotations
 
 import math
+from typing import NamedTuple
 
 import torch
 
-from ajllm_b200.ops import native
+from ajllm_b200.ops import native, reference
 
 _MAX_ROWS = 64
 
@@ -140,3 +143,250 @@ def spec_verify(target_logits: torch.Tensor, draft_logits: torch.Tensor, draft_t
                 draft_tokens.contiguous().data_ptr(), seqs, k1 - 1, vocab, temperature.data_ptr(), seeds.data_ptr(),
                 counters.data_ptr(), result.data_ptr(), native.stream_ptr())
     return result
+
+
+# ----------------------------------------------------------------------------- shared by the operators below
+
+
+def _require(condition: bool, message: str) -> None:
+    if not condition:
+        raise ValueError(message)
+
+
+def _int32(op: str, device: torch.device, **tensors: torch.Tensor) -> None:
+    for name, t in tensors.items():
+        if t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
+            raise ValueError(f"{op}: {name} must be a contiguous int32 tensor on {device} (got {t.dtype} on {t.device})")
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the memory ranges that two non-empty tensors span have a byte in common."""
+    def span(t):
+        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+# ----------------------------------------------------------------------------- block tables and slot maps
+
+
+class BatchMaps(NamedTuple):
+    """What the kernels of one serving step need to know about a ragged batch of ``n`` sequences."""
+
+    tables: torch.Tensor          # int32 [n, max_blocks]: block ids of every sequence, padded
+    positions: torch.Tensor       # int32 [total_tokens]: position of every new token in its sequence
+    slots: torch.Tensor           # int64 [total_tokens]: cache slot of every new token
+    q_start: torch.Tensor         # int32 [n + 1]: first row of every sequence, and the end of the last
+    context_lens: torch.Tensor    # int32 [n]: cached plus new tokens
+
+
+def batch_maps(block_ids: torch.Tensor, block_counts: torch.Tensor, cached_lens: torch.Tensor, q_lens: torch.Tensor,
+               total_tokens: int, max_blocks: int, *, block_size: int = 16, pad_block: int = 0,
+               out: "BatchMaps | tuple[torch.Tensor, ...] | None" = None) -> BatchMaps:
+    """Block tables, positions, cache slots, row offsets and context lengths of a ragged batch, built on the device.
+
+    ``block_ids`` holds the cache blocks of all sequences one after another, ``block_counts[i]`` of them for sequence
+    ``i``, which has ``cached_lens[i]`` tokens in the cache and brings ``q_lens[i]`` new ones (any of them may be 0);
+    all four are int32. ``total_tokens`` is the number of rows of the step: rows behind the last sequence, and tokens
+    for which a sequence has no block, are sent to ``pad_block`` (the former to position 0 and the block's first slot),
+    which must be a block that no sequence owns. Table rows keep a sequence's first ``max_blocks`` blocks and are filled
+    up with ``pad_block``. At most 16384 sequences per call.
+
+    ``out`` may hold the five result tensors (buffers a captured graph reads); they are overwritten and returned.
+    """
+    n, device = block_counts.shape[0], block_ids.device
+    _int32("batch_maps", device, block_ids=block_ids, block_counts=block_counts, cached_lens=cached_lens, q_lens=q_lens)
+    _require(block_ids.dim() == 1 and block_counts.dim() == 1 and cached_lens.shape == block_counts.shape == q_lens.shape,
+             "batch_maps: block_ids is one flat list, block_counts / cached_lens / q_lens have one entry per sequence")
+    _require(total_tokens >= 0 and max_blocks >= 1 and block_size >= 1 and pad_block >= 0,
+             "batch_maps: total_tokens and pad_block must not be negative, max_blocks and block_size must be positive")
+    _require(n <= 16384, f"batch_maps: {n} sequences are too many (at most 16384)")
+    if out is not None:
+        out = BatchMaps(*out)
+        _int32("batch_maps", device, tables=out.tables, positions=out.positions, q_start=out.q_start, context_lens=out.context_lens)
+        slots = out.slots
+        _require(slots.dtype == torch.int64 and slots.device == device and slots.is_contiguous() and slots.shape == (total_tokens,)
+                 and out.tables.shape == (n, max_blocks) and out.positions.shape == (total_tokens,)
+                 and out.q_start.shape == (n + 1,) and out.context_lens.shape == (n,),
+                 "batch_maps: the tensors in out do not have the shapes and types of the results")
+    if device.type != "cuda":
+        found = reference.batch_maps(block_ids, block_counts, cached_lens, q_lens, total_tokens, max_blocks, block_size, pad_block)
+        if out is None:
+            return BatchMaps(*found)
+        for mine, theirs in zip(out, found):
+            mine.copy_(theirs)
+        return out
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return batch_maps(block_ids, block_counts, cached_lens, q_lens, total_tokens, max_blocks, block_size=block_size,
+                              pad_block=pad_block, out=out)
+    if out is None:
+        out = BatchMaps(torch.empty(n, max_blocks, dtype=torch.int32, device=device),
+                        torch.empty(total_tokens, dtype=torch.int32, device=device),
+                        torch.empty(total_tokens, dtype=torch.int64, device=device),
+                        torch.empty(n + 1, dtype=torch.int32, device=device),
+                        torch.empty(n, dtype=torch.int32, device=device))
+    tables, positions, slots, q_start, context_lens = out
+    native.call("ajb_batch_maps", block_ids.data_ptr(), block_counts.data_ptr(), cached_lens.data_ptr(), q_lens.data_ptr(),
+                block_ids.shape[0], n, total_tokens, max_blocks, block_size, pad_block, tables.data_ptr(), positions.data_ptr(),
+                slots.data_ptr(), q_start.data_ptr(), context_lens.data_ptr(), native.stream_ptr())
+    return out
+
+
+# ----------------------------------------------------------------------------- attention behind a shared prefix
+
+_PREFIX_TILE = 128         # query rows and keys per step of the prefix kernel
+
+
+def prefix_parts(query_rows: int, kv_heads: int, shared: int) -> int:
+    """Parts that the shared prefix is cut into: one CTA per SM, and no part without a tile of keys."""
+    if not _SM_COUNT:
+        _SM_COUNT.append(int(native.lib().ajb_sm_count()))
+    units = -(-query_rows // _PREFIX_TILE) * kv_heads
+    return max(1, min(_SM_COUNT[0] // units, -(-shared // _PREFIX_TILE), 16))
+
+
+def shared_prefix_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, block_tables: torch.Tensor,
+                            context_lens: torch.Tensor, prefix_len: int, *, q_len: int = 1, scale: float | None = None,
+                            max_context: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Paged attention of a batch of sequences that all begin with the same ``prefix_len`` cached tokens.
+
+    Same result as :func:`paged_attention`, but the keys and values of the prefix are read once for the whole batch and
+    multiplied with all its query rows at once. ``q`` is ``[n * q_len, Hq, hd]``, ``q_len`` newest tokens of every
+    sequence one after another (1 for decoding, ``k + 1`` for verification, more for the chunk of a prompt); token
+    ``j`` of sequence ``i`` attends to its first ``context_lens[i] - q_len + j + 1`` tokens. ``block_tables`` (int32
+    ``[n, max_blocks]``) and ``context_lens`` (int32 ``[n]``, new tokens included) cover the whole context; the blocks
+    of the prefix are taken from the first row. New tokens lie behind the prefix
+    (``context_lens[i] - q_len >= prefix_len``): the whole prefix is visible to every row. A prefix that ends inside a
+    block is shared up to that block. Heads are 64 or 128 wide, ``Hq / Hkv`` is at most 128.
+
+    ``max_context``: a host-side bound on the context lengths (default: what the tables can hold) from which the
+    number of parts per sequence is chosen. A row whose sequence has no token at all comes out as zeros. ``scale``
+    defaults to ``1 / sqrt(hd)``; ``out`` (contiguous, like ``q``) receives the result.
+    """
+    _require(q.dim() == 3 and key_cache.dim() == 4 and key_cache.shape == value_cache.shape and block_tables.dim() == 2,
+             "shared_prefix_attention: q is [rows, heads, hd], the caches [blocks, block, kv_heads, hd], block_tables [n, max_blocks]")
+    total, heads, head_dim = q.shape
+    num_blocks, block_size, kv_heads, _ = key_cache.shape
+    n, max_blocks = block_tables.shape
+    device = q.device
+    _require(q_len >= 1 and total == n * q_len, f"shared_prefix_attention: {total} query rows are not {q_len} for each of {n} sequences")
+    _require(key_cache.shape[3] == head_dim and kv_heads >= 1 and heads % kv_heads == 0,
+             "shared_prefix_attention: the heads of q and of the caches do not match")
+    _require(0 <= prefix_len <= max_blocks * block_size, f"shared_prefix_attention: prefix_len {prefix_len} does not fit the block tables")
+    _require(key_cache.dtype == value_cache.dtype == q.dtype and key_cache.device == value_cache.device == device,
+             "shared_prefix_attention: q and the caches must have one type and one device")
+    _int32("shared_prefix_attention", device, block_tables=block_tables, context_lens=context_lens)
+    _require(context_lens.shape == (n,), "shared_prefix_attention: context_lens has one entry per sequence")
+    if out is not None:
+        _require(out.shape == q.shape and out.dtype == q.dtype and out.device == device and out.is_contiguous() and not _overlap(out, q),
+                 "shared_prefix_attention: out must be contiguous, shaped like q and apart from it")
+    scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
+    if device.type != "cuda":
+        found = reference.shared_prefix_attention(q, key_cache, value_cache, block_tables, context_lens, prefix_len, q_len, scale)
+        return found if out is None else out.copy_(found)
+    if q.dtype != torch.bfloat16:
+        raise TypeError(f"shared_prefix_attention: CUDA tensors must be bfloat16 (got {q.dtype})")
+    _require(key_cache.is_contiguous() and value_cache.is_contiguous(), "shared_prefix_attention: the caches must be contiguous")
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return shared_prefix_attention(q, key_cache, value_cache, block_tables, context_lens, prefix_len, q_len=q_len,
+                                           scale=scale, max_context=max_context, out=out)
+    if q.stride(2) != 1 or q.stride(1) != head_dim or q.stride(0) % 8 or q.data_ptr() % 16:
+        q = q.contiguous()
+    if out is None:
+        out = torch.empty(total, heads, head_dim, dtype=torch.bfloat16, device=device)
+    if total == 0:
+        return out
+    shared = prefix_len // block_size * block_size
+    group = heads // kv_heads
+    parts = prefix_parts(total * group, kv_heads, shared) if shared else 0
+    chunk = q_len if group * q_len <= 32 else max(1, min(q_len, _PREFIX_TILE // group))
+    behind = min(max_context if max_context is not None else max_blocks * block_size, max_blocks * block_size) - shared
+    splits = paged_splits(n * kv_heads * -(-q_len // chunk), max(0, behind))
+    # fp32 parts of every (row, head): un-normalised outputs, then (reference maximum, sum) pairs
+    count = total * heads * (parts + splits)
+    workspace = torch.empty(count * (head_dim + 2), dtype=torch.float32, device=device)
+    native.call("ajb_shared_prefix_attention", q.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
+                context_lens.data_ptr(), out.data_ptr(), q.stride(0), n, num_blocks, block_size, max_blocks, heads, kv_heads,
+                head_dim, q_len, shared, scale, parts, splits, workspace.data_ptr(), workspace.data_ptr() + 4 * count * head_dim,
+                native.stream_ptr())
+    return out
+
+
+# ----------------------------------------------------------------------------- logits processing
+
+
+def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, prompt_lens: torch.Tensor | None = None,
+                   history_lens: torch.Tensor | None = None, repetition: torch.Tensor | None = None,
+                   presence: torch.Tensor | None = None, frequency: torch.Tensor | None = None,
+                   bias_ids: torch.Tensor | None = None, bias_values: torch.Tensor | None = None,
+                   token_mask: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Penalties for repeated tokens, token biases and a grammar mask on ``logits`` ``[rows, vocab]`` (bf16 or fp32);
+    returns new fp32 logits for the sampler. In this order, for token ``v`` of a row:
+
+    * ``history`` (int32 ``[rows, width]``; the first ``prompt_lens[row]`` of its ``history_lens[row]`` tokens are the
+      prompt, the rest was generated; ids outside the vocabulary are skipped): a logit of any token in it is divided
+      by ``repetition[row]`` if positive, multiplied with it otherwise; then ``frequency[row]`` times the number of
+      times ``v`` was generated is taken off, and ``presence[row]`` if it was generated at all (fp32 ``[rows]``,
+      ``None`` = no such penalty);
+    * ``bias_values[row, j]`` is added to token ``bias_ids[row, j]`` (fp32 / int32 ``[rows, biases]``, ids outside the
+      vocabulary are skipped, equal ids are added one after another);
+    * tokens whose bit is not set in ``token_mask`` (int32 ``[rows, ceil(vocab / 32)]``, bit ``v % 32`` of word
+      ``v // 32``) become ``-inf``, whatever their logit was. A row whose mask leaves nothing is ``-inf`` throughout.
+
+    ``out`` (fp32 ``[rows, vocab]``, contiguous, apart from ``logits``) receives the result.
+    """
+    _require(logits.dim() == 2, "process_logits: logits must be [rows, vocab]")
+    rows, vocab = logits.shape
+    device = logits.device
+    if logits.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"process_logits: logits must be bfloat16 or float32 (got {logits.dtype})")
+    _require(vocab >= 1, "process_logits: the vocabulary is empty")
+    width = biases = 0
+    if history is not None:
+        _require(prompt_lens is not None and history_lens is not None, "process_logits: a history comes with prompt_lens and history_lens")
+        _int32("process_logits", device, history=history, prompt_lens=prompt_lens, history_lens=history_lens)
+        _require(history.dim() == 2 and history.shape[0] == rows and prompt_lens.shape == history_lens.shape == (rows,),
+                 "process_logits: history is [rows, width], prompt_lens and history_lens [rows]")
+        width = history.shape[1]
+        for name, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
+            _require(t is None or (t.dtype == torch.float32 and t.device == device and t.shape == (rows,) and t.is_contiguous()),
+                     f"process_logits: {name} must be a contiguous float32 [rows] tensor on {device}")
+    else:
+        _require(repetition is None and presence is None and frequency is None and prompt_lens is None and history_lens is None,
+                 "process_logits: penalties need a history")
+    if bias_ids is not None or bias_values is not None:
+        _require(bias_ids is not None and bias_values is not None, "process_logits: bias_ids and bias_values come together")
+        _int32("process_logits", device, bias_ids=bias_ids)
+        _require(bias_ids.dim() == 2 and bias_ids.shape[0] == rows and bias_values.shape == bias_ids.shape
+                 and bias_values.dtype == torch.float32 and bias_values.device == device and bias_values.is_contiguous(),
+                 "process_logits: bias_ids is [rows, biases], bias_values a contiguous float32 tensor of the same shape")
+        biases = bias_ids.shape[1]
+    if token_mask is not None:
+        _int32("process_logits", device, token_mask=token_mask)
+        _require(token_mask.shape == (rows, (vocab + 31) // 32), "process_logits: token_mask must be [rows, ceil(vocab / 32)]")
+    if out is not None:
+        _require(out.shape == logits.shape and out.dtype == torch.float32 and out.device == device and out.is_contiguous()
+                 and not _overlap(out, logits), "process_logits: out must be contiguous float32 [rows, vocab] apart from the logits")
+    if device.type != "cuda":
+        found = reference.process_logits(logits, history, prompt_lens, history_lens, repetition, presence, frequency, bias_ids,
+                                         bias_values, token_mask)
+        return found if out is None else out.copy_(found)
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return process_logits(logits, history=history, prompt_lens=prompt_lens, history_lens=history_lens, repetition=repetition,
+                                  presence=presence, frequency=frequency, bias_ids=bias_ids, bias_values=bias_values,
+                                  token_mask=token_mask, out=out)
+    if logits.stride(1) != 1:
+        logits = logits.contiguous()
+    if out is None:
+        out = torch.empty(rows, vocab, dtype=torch.float32, device=device)
+    native.call("ajb_process_logits", logits.data_ptr(), 0 if logits.dtype == torch.bfloat16 else 1, logits.stride(0), out.data_ptr(),
+                rows, vocab, native.ptr(history) if width else None, width, width, native.ptr(prompt_lens), native.ptr(history_lens),
+                native.ptr(repetition), native.ptr(presence), native.ptr(frequency), native.ptr(bias_ids), native.ptr(bias_values),
+                biases, native.ptr(token_mask), (vocab + 31) // 32, native.stream_ptr())
+    return out

@@ -1,0 +1,404 @@
+"""Block tables and slot maps, shared-prefix attention and logits processing on a GPU, against plain statements in
+64 bits, at the sizes and masks where they can go wrong."""
+
+import math
+
+import pytest
+import torch
+
+from ajllm_b200.ops import native, reference, serving
+
+pytestmark = pytest.mark.gpu
+
+HALF_BF16 = 2.0 ** -8           # half a step of bf16, relative
+HALF_FP32 = 2.0 ** -24
+
+
+def _dev():
+    return torch.device("cuda", 0)
+
+
+def _i32(values, device=None):
+    return torch.tensor(values, dtype=torch.int32, device=device or _dev())
+
+
+# --------------------------------------------------------------------------------------------- batch maps
+
+
+MAPS = [
+    # block ids, counts, cached, new, total, max_blocks, block, pad
+    (dict(counts=[1], cached=[0], new=[1]), 1, 1, 16),
+    (dict(counts=[3, 1, 2], cached=[17, 0, 31], new=[31, 16, 1]), 48, 3, 16),
+    (dict(counts=[2, 0, 0, 5], cached=[0, 0, 0, 70], new=[0, 0, 0, 7]), 7, 7, 16),            # sequences without tokens
+    (dict(counts=[2, 4], cached=[30, 5], new=[9, 59]), 80, 3, 16),        # too few blocks, rows behind the last, narrow table
+    (dict(counts=[], cached=[], new=[]), 5, 4, 16),                       # no sequence at all
+    (dict(counts=[], cached=[], new=[]), 0, 1, 16),
+    (dict(counts=[3, 2], cached=[1, 4], new=[6, 1]), 7, 5, 3),            # block size that is no power of two
+    (dict(counts=[-4, 2, 3], cached=[-9, 3, 0], new=[-1, 4, 40]), 44, 9, 16),     # negative lengths count as 0
+    (dict(counts=[4, 4], cached=[0, 0], new=[40, 40]), 50, 4, 16),        # more tokens than rows
+]
+
+
+@pytest.mark.parametrize("lens,total,width,block", MAPS)
+def test_batch_maps(lens, total, width, block):
+    ids = torch.randperm(100)[:sum(max(0, c) for c in lens["counts"])].to(torch.int32)
+    args = [ids, *(torch.tensor(lens[k], dtype=torch.int32) for k in ("counts", "cached", "new"))]
+    want = serving.batch_maps(*args, total, width, block_size=block, pad_block=777)
+    got = serving.batch_maps(*(a.cuda() for a in args), total, width, block_size=block, pad_block=777)
+    for name, a, b in zip(serving.BatchMaps._fields, got, want):
+        assert a.dtype == b.dtype and torch.equal(a.cpu(), b), name
+
+
+@pytest.mark.parametrize("n,most", [(257, 40), (5000, 9), (16384, 3)])
+def test_batch_maps_of_many_sequences(n, most):
+    gen = torch.Generator().manual_seed(n)
+    cached, new = (torch.randint(0, most, (n,), generator=gen) for _ in range(2))
+    counts = (cached + new + 15) // 16 + torch.randint(0, 2, (n,), generator=gen)
+    ids = torch.randint(0, 2**31 - 1, (int(counts.sum()),), generator=gen)
+    total, width = int(new.sum()), int(counts.max()) + 1
+    got = serving.batch_maps(*(_i32(t.tolist()) for t in (ids, counts, cached, new)), total, width, pad_block=3)
+    # the same by whole-tensor operations in 64 bits
+    seq = torch.repeat_interleave(torch.arange(n), new)
+    at = cached[seq] + torch.arange(total) - (torch.cumsum(new, 0) - new)[seq]
+    first = torch.cumsum(counts, 0) - counts
+    assert torch.equal(got.positions.cpu().long(), at)
+    assert torch.equal(got.slots.cpu(), ids[first[seq] + at // 16] * 16 + at % 16)              # block ids near 2^31: slots pass 32 bits
+    column = torch.arange(width)
+    tables = torch.where(column < counts[:, None], ids[(first[:, None] + column).clamp(max=ids.numel() - 1)], 3)
+    assert torch.equal(got.tables.cpu().long(), tables)
+    assert got.q_start.tolist() == [0] + torch.cumsum(new, 0).tolist() and got.context_lens.tolist() == (cached + new).tolist()
+
+
+def test_batch_maps_survives_absurd_lengths_and_keeps_to_its_buffers():
+    big = 2**31 - 1
+    guard = 64
+    kept, views = [], []
+    for shape, dtype in (((4, 8), torch.int32), ((32,), torch.int32), ((32,), torch.int64), ((5,), torch.int32), ((4,), torch.int32)):
+        flat = torch.full((math.prod(shape) + 2 * guard,), -5, dtype=dtype, device=_dev())
+        kept.append(flat)
+        views.append(flat[guard:guard + math.prod(shape)].view(shape))
+    got = serving.batch_maps(_i32([5, 6, 7]), _i32([big, big, 2, -big]), _i32([big, 3, 0, 9]), _i32([big, 4, big, 1]), 32, 8, pad_block=1,
+                             out=tuple(views))
+    assert all(a.data_ptr() == b.data_ptr() for a, b in zip(got, views))
+    assert got.positions.tolist() == [big] * 32                  # the first sequence's tokens sit at the largest position
+    assert got.slots.tolist() == [1 * 16 + (big + j) % 16 for j in range(32)] and got.tables[0].tolist() == [5, 6, 7] + [1] * 5
+    for flat, view in zip(kept, views):
+        assert torch.all(flat[:guard] == -5) and torch.all(flat[guard + view.numel():] == -5)
+
+
+def test_batch_maps_replayed_from_a_graph():
+    ids, counts, cached, new = _i32(list(range(40))), _i32([10, 10, 10, 10]), _i32([3, 16, 31, 100]), _i32([5, 1, 2, 8])
+    out = serving.batch_maps(ids, counts, cached, new, 16, 12, pad_block=99)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        serving.batch_maps(ids, counts, cached, new, 16, 12, pad_block=99, out=out)
+    cached.copy_(_i32([0, 1, 2, 3]))
+    new.copy_(_i32([1, 1, 0, 12]))
+    graph.replay()
+    want = serving.batch_maps(ids.cpu(), counts.cpu(), cached.cpu(), new.cpu(), 16, 12, pad_block=99)
+    for a, b in zip(out, want):
+        assert torch.equal(a.cpu(), b)
+
+
+# --------------------------------------------------------------------------------------------- attention
+
+
+def _batch(heads, kv_heads, hd, q_len, prefix, suffixes, seed=0, poison=True):
+    """Queries, caches, tables and lengths of sequences with a common prefix in shuffled blocks. With ``poison`` every
+    cache slot that no sequence has written holds a NaN or an infinity."""
+    gen = torch.Generator().manual_seed(seed)
+    n, shared = len(suffixes), prefix // 16
+    context = [prefix + s for s in suffixes]
+    own = [(c + 15) // 16 - shared for c in context]
+    order = torch.randperm(shared + sum(own) + 5, generator=gen)
+    width = max(1, shared + max(own) + 1)
+    tables = torch.full((n, width), int(order[-1]), dtype=torch.int64)
+    tables[:, :shared] = order[:shared]
+    cursor = shared
+    for i, count in enumerate(own):
+        tables[i, shared:shared + count] = order[cursor:cursor + count]
+        cursor += count
+    keys, values = (torch.randn(order.numel(), 16, kv_heads, hd, generator=gen) for _ in range(2))
+    if prefix % 16:
+        at = tables[:, shared]
+        for cache in (keys, values):
+            cache[at, :prefix % 16] = cache[at[0], :prefix % 16].clone()
+    if poison:
+        used = torch.zeros(order.numel(), 16, dtype=torch.bool)
+        for i, c in enumerate(context):
+            place = torch.arange(c)
+            used[tables[i, place // 16], place % 16] = True
+        keys[~used] = math.nan
+        values[~used] = torch.tensor([math.inf, -math.inf, math.nan, 3e38])[torch.arange(int((~used).sum())) % 4][:, None, None]
+    q = 1.5 * torch.randn(n * q_len, heads, hd, generator=gen)
+    bf16 = [t.to(torch.bfloat16).cuda() for t in (q, keys, values)]
+    return (*bf16, _i32(tables.tolist()), _i32(context))
+
+
+def _oracle(q, keys, values, tables, context, q_len, scale=None):
+    """``(out, sum of p |v|)`` in 64 bits, every sequence over its own blocks in order."""
+    heads, hd = q.shape[1:]
+    kv_heads = keys.shape[2]
+    scale = scale or hd ** -0.5
+    out, size = [], []
+    for i, c in enumerate(context.tolist()):
+        place = torch.arange(c, device=q.device)
+        block = tables[i].long()[place // 16]
+        k, v = (t[block, place % 16].double().repeat_interleave(heads // kv_heads, 1) for t in (keys, values))
+        scores = torch.einsum("ihd,shd->ihs", q[i * q_len:(i + 1) * q_len].double(), k) * scale
+        last = c - q_len + torch.arange(q_len, device=q.device)
+        p = torch.softmax(scores.masked_fill(place > last[:, None, None], -math.inf), -1)
+        out.append(torch.einsum("ihs,shd->ihd", p, v))
+        size.append(torch.einsum("ihs,shd->ihd", p, v.abs()))
+    return torch.cat(out), torch.cat(size)
+
+
+def _check_attention(got, want, size):
+    # probabilities and outputs are each rounded to bf16 once (half a step of sum p |v|, half a step of the output); the
+    # rest is fp32: an exponent off by 1e-5 (128-term dot products of |s| < 100 and exp2's two steps) moves p by 1e-5
+    bound = HALF_BF16 * (size + want.abs()) + 1e-4 * size + 1e-30
+    worst = ((got.double() - want).abs() / bound).max()
+    assert torch.isfinite(got).all() and float(worst) <= 1.0, float(worst)
+    assert native.lib().ajb_check_status() == 0
+
+
+SHAPES = [
+    (8, 2, 128, 1, 512, [1, 17, 130, 500]),
+    (4, 4, 64, 1, 16, [1]),                              # one sequence, one block
+    (32, 8, 128, 1, 129, [1, 2, 64, 65, 200]),           # prefix ends one token into a block
+    (32, 8, 64, 1, 4001, [3, 400]),
+    (6, 2, 128, 1, 144, list(range(1, 51))),             # group of 3; more rows than a tile, tail tile
+    (16, 2, 64, 1, 2048, [16, 48, 64, 80]),              # suffixes of whole blocks
+    (8, 1, 128, 5, 333, [5, 6, 70]),                     # verification, 40 rows per sequence
+    (16, 4, 128, 5, 100, [5, 130]),                      # verification, 20 rows (replicated variant)
+    (128, 1, 64, 1, 260, [1, 90]),                       # as many query heads per KV head as a tile has rows
+    (48, 1, 128, 3, 64, [3, 20]),                        # 144 rows: two chunks, the second partly filled
+    (8, 2, 64, 61, 200, [61, 99]),                       # a chunk of a prompt, odd length
+    (4, 2, 128, 1, 0, [1, 33, 700]),                     # nothing shared
+    (4, 2, 128, 2, 15, [2, 33]),                         # a prefix shorter than a block
+    (1, 1, 128, 1, 1024, [1] * 130),                     # one head: rows of a tile are all different sequences
+]
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,q_len,prefix,suffixes", SHAPES)
+def test_shared_prefix_attention(heads, kv_heads, hd, q_len, prefix, suffixes):
+    q, keys, values, tables, context = _batch(heads, kv_heads, hd, q_len, prefix, suffixes)
+    got = serving.shared_prefix_attention(q, keys, values, tables, context, prefix, q_len=q_len)
+    _check_attention(got, *_oracle(q, keys, values, tables, context, q_len))
+
+
+def test_shared_prefix_attention_with_large_scores_and_a_given_scale():
+    """Scores of several hundred: the running maximum moves again and again, within the prefix and behind it."""
+    q, keys, values, tables, context = _batch(8, 2, 128, 1, 640, [40, 300, 9], seed=3)
+    ramp = torch.linspace(0.1, 3.0, keys.shape[0], device=_dev())[torch.randperm(keys.shape[0], device=_dev())]
+    keys = (keys.float() * ramp[:, None, None, None]).to(torch.bfloat16)
+    want, size = _oracle(q, keys, values, tables, context, 1, scale=1.0)
+    got = serving.shared_prefix_attention(q, keys, values, tables, context, 640, scale=1.0)
+    # products of |q k| up to 128 * 5 * 13 summed in fp32: the exponent is off by up to 128 * 2^-24 * 8e3 = 0.06
+    bound = HALF_BF16 * (size + want.abs()) + 0.065 * 2 * size
+    assert bool(((got.double() - want).abs() <= bound).all())
+    assert native.lib().ajb_check_status() == 0
+
+
+def test_shared_prefix_attention_equals_paged_attention_closely():
+    q, keys, values, tables, context = _batch(32, 8, 128, 1, 1024, [7, 260, 31], poison=False)
+    a = serving.shared_prefix_attention(q, keys, values, tables, context, 1024)
+    b = serving.paged_attention(q, keys, values, tables, None, None, [1] * 3, context.tolist())
+    want, size = _oracle(q, keys, values, tables, context, 1)
+    _check_attention(a, want, size)
+    _check_attention(b, want, size)
+
+
+def test_rows_without_a_key_are_zero():
+    q, keys, values, tables, context = _batch(4, 2, 64, 1, 0, [5, 1, 40])
+    context[1] = 0
+    got = serving.shared_prefix_attention(q, keys, values, tables, context, 0)
+    assert torch.count_nonzero(got[1]) == 0 and torch.count_nonzero(got[0]) > 0
+
+
+def test_queries_read_in_place_from_packed_rows_and_results_into_a_given_tensor():
+    q, keys, values, tables, context = _batch(8, 2, 128, 2, 200, [2, 50, 3])
+    packed = torch.full((6, 12 * 128), math.nan, dtype=torch.bfloat16, device=_dev())
+    packed[:, :1024] = q.view(6, 1024)
+    out = torch.full((8, 8, 128), 7.0, dtype=torch.bfloat16, device=_dev())
+    view, _, _ = (t for t in (packed[:, :1024].view(6, 8, 128), None, None))
+    got = serving.shared_prefix_attention(view, keys, values, tables, context, 200, q_len=2, out=out[1:7])
+    assert got.data_ptr() == out[1:].data_ptr() and torch.all(out[0] == 7) and torch.all(out[7] == 7)
+    assert torch.equal(got, serving.shared_prefix_attention(q, keys, values, tables, context, 200, q_len=2))
+    odd = torch.randn(6, 8, 130, device=_dev()).to(torch.bfloat16)[:, :, 1:129]          # rows that are not 16-byte aligned
+    assert torch.equal(serving.shared_prefix_attention(odd, keys, values, tables, context, 200, q_len=2),
+                       serving.shared_prefix_attention(odd.contiguous(), keys, values, tables, context, 200, q_len=2))
+
+
+def test_two_captured_graphs_and_eager_calls_do_not_disturb_each_other():
+    first = _batch(16, 4, 128, 1, 300, [3, 77, 12], seed=1)
+    second = _batch(8, 2, 64, 4, 500, [4, 9], seed=2)
+    side = torch.cuda.Stream()
+    graphs, outs = [], []
+    for (q, keys, values, tables, context), prefix, q_len in ((first, 300, 1), (second, 500, 4)):
+        serving.shared_prefix_attention(q, keys, values, tables, context, prefix, q_len=q_len)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(serving.shared_prefix_attention(q, keys, values, tables, context, prefix, q_len=q_len))
+        graphs.append(graph)
+    first[0].normal_()                           # replays read the inputs anew
+    first[4].sub_(_i32([1, 5, 2]))
+    for _ in range(3):
+        graphs[0].replay()
+        graphs[1].replay()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        eager = serving.shared_prefix_attention(*first, 300)
+    torch.cuda.current_stream().wait_stream(side)
+    _check_attention(outs[0], *_oracle(*first, 1))
+    _check_attention(outs[1], *_oracle(*second, 4))
+    assert torch.equal(eager, outs[0])
+
+
+def test_tables_shorter_than_the_context_bound_what_is_read():
+    """A context length beyond the block table (a caller's mistake that only the device sees) reads nothing behind it."""
+    q, keys, values, tables, context = _batch(8, 2, 128, 1, 64, [100, 30], poison=False)
+    context[0] = 10_000_000
+    got = serving.shared_prefix_attention(q, keys, values, tables, context, 64)
+    assert torch.isfinite(got).all() and native.lib().ajb_check_status() == 0
+
+
+# --------------------------------------------------------------------------------------------- logits
+
+
+def _logits_inputs(rows, vocab, dtype, width, biases, masked, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    kw = dict(history=torch.randint(-2, min(vocab + 3, 50), (rows, width), generator=gen).to(torch.int32),
+              prompt_lens=torch.randint(0, width + 1, (rows,), generator=gen).to(torch.int32),
+              history_lens=torch.randint(0, width + 1, (rows,), generator=gen).to(torch.int32),
+              repetition=0.5 + torch.rand(rows, generator=gen), presence=torch.rand(rows, generator=gen) - 0.5,
+              frequency=torch.rand(rows, generator=gen))
+    if biases:
+        kw["bias_ids"] = torch.randint(-1, min(vocab + 2, 40), (rows, biases), generator=gen).to(torch.int32)
+        kw["bias_values"] = 3 * torch.randn(rows, biases, generator=gen)
+    if masked:
+        kw["token_mask"] = torch.randint(-2**31, 2**31 - 1, (rows, (vocab + 31) // 32), generator=gen).to(torch.int32)
+    return (4 * torch.randn(rows, vocab, generator=gen)).to(dtype), kw
+
+
+def _logits_oracle(logits, kw):
+    """Token by token in 64 bits: ``(result, sum of the sizes that were added up)``."""
+    x = logits.double()
+    size = x.abs()
+    rows, vocab = x.shape
+    for r in range(rows):
+        tokens = kw["history"][r, :int(kw["history_lens"][r])].tolist() if "history" in kw else []
+        made = tokens[int(kw["prompt_lens"][r]):] if tokens else []
+        for v in {t for t in tokens if 0 <= t < vocab}:
+            f = float(kw["repetition"][r])
+            x[r, v] = x[r, v] / f if x[r, v] > 0 else x[r, v] * f
+            c = made.count(v)
+            size[r, v] = x[r, v].abs() + abs(float(kw["frequency"][r])) * c + abs(float(kw["presence"][r]))
+            x[r, v] -= float(kw["frequency"][r]) * c + (float(kw["presence"][r]) if c else 0.0)
+        for v, b in zip(kw["bias_ids"][r].tolist(), kw["bias_values"][r].tolist()) if "bias_ids" in kw else ():
+            if 0 <= v < vocab:
+                x[r, v] += b
+                size[r, v] += abs(b)
+        if "token_mask" in kw:
+            for v in range(vocab):
+                if not (int(kw["token_mask"][r, v // 32]) >> (v % 32)) & 1:
+                    x[r, v] = -math.inf
+    return x, size
+
+
+LOGITS = [
+    (1, 1, torch.float32, 3, 0, False), (2, 33, torch.bfloat16, 9, 5, True), (3, 300, torch.bfloat16, 70, 40, True),
+    (5, 8191, torch.float32, 600, 33, True), (2, 8195, torch.bfloat16, 64, 64, True), (1, 32000, torch.bfloat16, 40, 0, False),
+    (2, 1030, torch.bfloat16, 0, 3, False), (4, 64, torch.float32, 1, 1, True),
+]
+
+
+@pytest.mark.parametrize("rows,vocab,dtype,width,biases,masked", LOGITS)
+def test_process_logits(rows, vocab, dtype, width, biases, masked):
+    logits, kw = _logits_inputs(rows, vocab, dtype, width, biases, masked)
+    got = serving.process_logits(logits.cuda(), **{k: v.cuda() for k, v in kw.items()}).cpu()
+    want, size = _logits_oracle(logits, kw)
+    hidden = torch.isinf(want)
+    assert torch.equal(torch.isinf(got) & (got < 0), hidden)
+    # at most: quotient or product, frequency product, two differences, one sum per bias, each off by half a step
+    bound = (4 + biases) * HALF_FP32 * size
+    assert bool(((got.double() - want).abs()[~hidden] <= bound[~hidden]).all())
+    assert torch.equal(got, serving.process_logits(logits, **kw))              # and the same fp32 steps as on the CPU
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("offset", [0, 1, 2, 3])
+def test_process_logits_of_strided_and_misaligned_rows(dtype, offset):
+    logits, kw = _logits_inputs(7, 2051, dtype, 30, 9, True, seed=offset)
+    wide = torch.full((7, 2100 + offset), math.nan, dtype=dtype)
+    wide[:, offset:offset + 2051] = logits
+    kw = {k: v.cuda() for k, v in kw.items()}
+    got = serving.process_logits(wide.cuda()[:, offset:offset + 2051], **kw)
+    assert torch.equal(got, serving.process_logits(logits.cuda(), **kw))
+    kept = torch.full((7 * 2051 + 20,), 5.0, device=_dev())
+    again = serving.process_logits(logits.cuda(), **kw, out=kept[8:8 + 7 * 2051].view(7, 2051))
+    assert torch.equal(got, again) and torch.all(kept[:8] == 5) and torch.all(kept[8 + 7 * 2051:] == 5)
+    transposed = logits.t().contiguous().cuda().t()
+    assert torch.equal(got, serving.process_logits(transposed, **kw))
+
+
+def test_masked_places_hide_whatever_is_in_them_and_open_ones_keep_it():
+    values = torch.tensor([math.nan, math.inf, -math.inf, torch.finfo(torch.float32).min, 1.0, 0.0, -0.0, 2.0])
+    logits = values.repeat(3, 8)
+    mask = torch.tensor([[0, 0], [-1, -1], [0b11110000, 0]], dtype=torch.int32)
+    got = serving.process_logits(logits.cuda(), token_mask=mask.cuda()).cpu()
+    assert torch.all(got[0] == -math.inf)                               # nothing left
+    assert torch.equal(got[1].view(torch.int32), logits[1].view(torch.int32))
+    assert torch.all(got[2, :4] == -math.inf) and got[2, 4:8].tolist() == [1.0, 0.0, 0.0, 2.0] and torch.all(got[2, 8:] == -math.inf)
+
+
+def test_the_same_token_many_times():
+    """A history and a bias list that hold one token only: every thread of the kernel meets on it."""
+    logits = torch.ones(2, 5000, device=_dev())
+    history = torch.full((2, 4096), 4321, dtype=torch.int32, device=_dev())
+    lens = _i32([4096, 4095])
+    ids = torch.full((2, 200), 4321, dtype=torch.int32, device=_dev())
+    bias = torch.full((2, 200), 0.25, device=_dev())
+    got = serving.process_logits(logits, history=history, prompt_lens=_i32([96, 4095]), history_lens=lens,
+                                 repetition=torch.full((2,), 2.0, device=_dev()), frequency=torch.full((2,), 0.125, device=_dev()),
+                                 presence=torch.full((2,), 0.5, device=_dev()), bias_ids=ids, bias_values=bias)
+    assert got[:, 4321].tolist() == [0.5 - 500 - 0.5 + 50, 0.5 + 50]
+    got[:, 4321] = 1
+    assert torch.all(got == 1)
+
+
+def test_logits_maps_and_attention_replayed_together():
+    """One decoding step as a server runs it: maps, cache write, attention behind the prefix, logits, sampler, captured
+    once and replayed with other lengths."""
+    torch.manual_seed(0)
+    heads, kv_heads, hd, prefix, n, vocab = 8, 2, 128, 160, 3, 500
+    _, keys, values, tables, _ = _batch(heads, kv_heads, hd, 1, prefix, [40, 40, 40], seed=5, poison=False)
+    ids, counts = tables[:, :13].reshape(-1).contiguous(), _i32([13] * n)
+    cached, new = _i32([prefix + 3, prefix + 15, prefix + 38]), _i32([1] * n)
+    q, k, v = (torch.randn(n, h, hd, device=_dev()).to(torch.bfloat16) for h in (heads, kv_heads, kv_heads))
+    head = (0.05 * torch.randn(vocab, heads * hd, device=_dev())).to(torch.bfloat16)
+    history, lens = torch.randint(0, vocab, (n, 64), device=_dev(), dtype=torch.int32), _i32([10, 64, 33])
+    penalty = torch.full((n,), 1.3, device=_dev())
+    mask = torch.randint(-2**31, 2**31 - 1, (n, (vocab + 31) // 32), device=_dev()).to(torch.int32)
+    zeros, ones = torch.zeros(n, device=_dev()), torch.ones(n, device=_dev())
+    seeds = torch.arange(n, device=_dev())
+
+    def step():
+        maps = serving.batch_maps(ids, counts, cached, new, n, 13)
+        keys.view(-1, kv_heads, hd).index_copy_(0, maps.slots, k)
+        values.view(-1, kv_heads, hd).index_copy_(0, maps.slots, v)
+        attended = serving.shared_prefix_attention(q, keys, values, maps.tables, maps.context_lens, prefix)
+        raw = attended.view(n, -1) @ head.t()
+        logits = serving.process_logits(raw, history=history, prompt_lens=lens // 2, history_lens=lens, repetition=penalty, token_mask=mask)
+        return maps, attended, raw, logits, serving.sample_rows(logits, zeros, ones, seeds, seeds)
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        maps, attended, raw, logits, tokens = step()
+    cached.copy_(_i32([prefix, prefix + 31, prefix + 32]))
+    graph.replay()
+    assert maps.context_lens.tolist() == [prefix + 1, prefix + 32, prefix + 33]
+    _check_attention(attended, *_oracle(q, keys, values, maps.tables, maps.context_lens, 1))
+    want = reference.process_logits(raw.cpu(), history.cpu(), (lens // 2).cpu(), lens.cpu(), penalty.cpu(), token_mask=mask.cpu())
+    assert torch.equal(logits.cpu(), want) and tokens.tolist() == want.argmax(-1).tolist()
