@@ -8,18 +8,42 @@
 //
 // Bound by memory: 6 bytes per bf16 logit (read, write) and a bit of the mask; where a mask shuts four neighbouring
 // tokens their logits are not read. Only the few tokens of the history and of the bias list need arithmetic, so a CTA
-// first streams its piece of the row through (widen, mask), then mends those tokens one by one: it has counted the
-// history tokens of its piece in a table in shared memory, and the thread that takes a token's count out of the table
-// (an exchange with 0) is the one that writes that token. Counts are whole numbers, so the order of the additions does
-// not show. Biases follow in list order within one warp; lanes that hold the same token take turns.
+// streams its piece of the row through (widen, mask) and then mends those tokens one by one. Four more warps count the
+// history tokens of the piece in a table in shared memory while the others stream, so that neither waits for the other;
+// the thread that then takes a token's count out of the table (an atomic that leaves 0) is the one that writes that
+// token. Counts are whole numbers, so the order of the additions does not show. Biases follow in list order within one
+// warp; lanes that hold the same token take turns.
 #include "common.cuh"
 
 namespace ajb {
 namespace logits {
 
-constexpr int kThreads = 256;
+constexpr int kStreamThreads = 256;
+constexpr int kHistoryThreads = 128;             // launched in addition when there is a history
 constexpr int kUnroll = 4;
-constexpr unsigned kInPrompt = 0x80000000u;      // table entry: bit 31 = in the prompt, the rest = times generated
+constexpr int kHistoryUnroll = 4;
+constexpr unsigned kMinusInf = 0xff800000u;
+
+// Counts of the tokens of a piece. A cell has one bit for "in the prompt" and the rest for "times generated"; histories
+// of up to 32767 tokens fit 16-bit cells, two to a word of shared memory (pieces of 16384 tokens), longer ones take whole
+// words (pieces of 8192): 32 KB either way.
+template <bool kNarrow>
+struct Table {
+  static constexpr int kMaxChunk = kNarrow ? 16384 : 8192;
+  static constexpr unsigned kPrompt = kNarrow ? 0x8000u : 0x80000000u;
+  static __device__ __forceinline__ int words(int chunk) { return kNarrow ? chunk >> 1 : chunk; }
+  static __device__ __forceinline__ void add(unsigned* t, int i, bool prompt) {
+    const int shift = kNarrow ? 16 * (i & 1) : 0;
+    unsigned* word = t + (kNarrow ? i >> 1 : i);
+    if (prompt) atomicOr(word, kPrompt << shift);
+    else atomicAdd(word, 1u << shift);
+  }
+  static __device__ __forceinline__ unsigned take(unsigned* t, int i) {
+    if (!kNarrow) return atomicExch(t + i, 0u);
+    const int shift = 16 * (i & 1);
+    return (atomicAnd(t + (i >> 1), ~(0xffffu << shift)) >> shift) & 0xffffu;
+  }
+};
 
 struct Params {
   const void* in;
@@ -47,85 +71,110 @@ template <>
 __device__ __forceinline__ float load1<__nv_bfloat16>(const __nv_bfloat16* p) {
   return __uint_as_float((unsigned)__ldg(reinterpret_cast<const unsigned short*>(p)) << 16);
 }
-__device__ __forceinline__ uint4 load4(const float* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
-__device__ __forceinline__ uint4 load4(const __nv_bfloat16* p) {
-  const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-  return make_uint4(v.x << 16, v.x & 0xffff0000u, v.y << 16, v.y & 0xffff0000u);
+// four neighbouring logits, as loaded and as fp32 bits
+template <typename T>
+struct Four;
+template <>
+struct Four<float> {
+  uint4 v;
+  __device__ __forceinline__ void load(const float* p) { v = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ uint4 wide() const { return v; }
+};
+template <>
+struct Four<__nv_bfloat16> {
+  uint2 v;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = __ldg(reinterpret_cast<const uint2*>(p)); }
+  __device__ __forceinline__ uint4 wide() const { return make_uint4(v.x << 16, v.x & 0xffff0000u, v.y << 16, v.y & 0xffff0000u); }
+};
+
+__device__ __forceinline__ bool open_token(const unsigned* mask, int v) {
+  return mask == nullptr || ((__ldg(mask + (v >> 5)) >> (v & 31)) & 1u);
 }
 
-constexpr unsigned kMinusInf = 0xff800000u;
-
+// Tokens [lo, hi) of a row, widened and masked, by `threads` threads.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) process_logits_kernel(const Params p) {
+__device__ __forceinline__ void stream_piece(const T* in, float* out, const unsigned* mask, int lo, int hi, int thread, int threads) {
+  // four-token groups start where `out` is 16-byte aligned; the input rows have to agree with that to be read in groups
+  const int lead = (int)((4 - ((reinterpret_cast<uintptr_t>(out + lo) >> 2) & 3)) & 3);
+  const int first = min(hi, lo + lead);
+  const bool wide = (reinterpret_cast<uintptr_t>(in + lo + lead) & (4 * sizeof(T) - 1)) == 0;
+  auto one = [&](int v) { out[v] = open_token(mask, v) ? load1<T>(in + v) : __uint_as_float(kMinusInf); };
+  if (!wide) {
+    for (int v = lo + thread; v < hi; v += threads) one(v);
+    return;
+  }
+  for (int v = lo + thread; v < first; v += threads) one(v);
+  const int groups = (hi - first) >> 2;
+  for (int g0 = thread; g0 < groups; g0 += threads * kUnroll) {
+    unsigned open[kUnroll];
+    Four<T> x[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int g = g0 + u * threads, v = first + 4 * g;
+      open[u] = g < groups ? 15u : 0u;
+      if (mask != nullptr && g < groups) {
+        // a group lies in one word, or in two neighbours when the row does not start on a 16-byte boundary
+        const unsigned w0 = __ldg(mask + (v >> 5)), w1 = (v & 31) > 28 ? __ldg(mask + (v >> 5) + 1) : 0u;
+        open[u] = __funnelshift_r(w0, w1, v & 31) & 15u;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (open[u]) x[u].load(in + first + 4 * (g0 + u * threads));
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int g = g0 + u * threads;
+      if (g < groups) {
+        uint4 w = x[u].wide();
+        if (!(open[u] & 1u)) w.x = kMinusInf;
+        if (!(open[u] & 2u)) w.y = kMinusInf;
+        if (!(open[u] & 4u)) w.z = kMinusInf;
+        if (!(open[u] & 8u)) w.w = kMinusInf;
+        *reinterpret_cast<uint4*>(out + first + 4 * g) = w;
+      }
+    }
+  }
+  for (int v = first + 4 * groups + thread; v < hi; v += threads) one(v);
+}
+
+// visit(place, token) for the history tokens in [lo, hi); `threads` threads, several loads in flight
+template <typename Visit>
+__device__ __forceinline__ void for_history(const int* history, int len, int lo, int hi, int thread, int threads, Visit visit) {
+  for (int i0 = thread; i0 < len; i0 += threads * kHistoryUnroll) {
+    int v[kHistoryUnroll];
+#pragma unroll
+    for (int u = 0; u < kHistoryUnroll; ++u) {
+      const int i = i0 + u * threads;
+      v[u] = i < len ? __ldg(history + i) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kHistoryUnroll; ++u)
+      if (v[u] >= lo && v[u] < hi) visit(i0 + u * threads, v[u]);
+  }
+}
+
+template <typename T, bool kNarrow>
+__global__ void __launch_bounds__(kStreamThreads + kHistoryThreads) process_logits_kernel(const Params p) {
   extern __shared__ unsigned table[];
+  using Tab = Table<kNarrow>;
   const int row = (int)(blockIdx.x / (unsigned)p.chunks), part = (int)(blockIdx.x % (unsigned)p.chunks);
   const int lo = part * p.chunk, hi = min(p.vocab, lo + p.chunk);
   const T* in = reinterpret_cast<const T*>(p.in) + (size_t)row * p.in_pitch;
   float* out = p.out + (size_t)row * p.vocab;
   const unsigned* mask = p.mask != nullptr ? p.mask + (size_t)row * p.mask_pitch : nullptr;
   const int* history = p.history != nullptr ? p.history + (size_t)row * p.history_pitch : nullptr;
-  const int len = history != nullptr ? min(max(p.history_lens[row], 0), p.history_width) : 0;
+  const int thread = threadIdx.x;
+  int len = 0;
 
-  if (len > 0) {
-    for (int i = threadIdx.x; i < (p.chunk >> 2); i += kThreads) reinterpret_cast<uint4*>(table)[i] = make_uint4(0, 0, 0, 0);
-    __syncthreads();
+  if (history != nullptr) len = min(max(p.history_lens[row], 0), p.history_width);
+  if (thread < kStreamThreads) {
+    stream_piece<T>(in, out, mask, lo, hi, thread, kStreamThreads);
+  } else if (len > 0) {
+    const int t = thread - kStreamThreads;
+    for (int i = t; i < (Tab::words(p.chunk) >> 2); i += kHistoryThreads) reinterpret_cast<uint4*>(table)[i] = make_uint4(0, 0, 0, 0);
+    asm volatile("bar.sync 1, %0;" ::"n"(kHistoryThreads) : "memory");
     const int prompt = p.prompt_lens[row];
-    for (int i = threadIdx.x; i < len; i += kThreads) {
-      const int v = __ldg(history + i);
-      if (v >= lo && v < hi) {
-        if (i < prompt) atomicOr(&table[v - lo], kInPrompt);
-        else atomicAdd(&table[v - lo], 1u);
-      }
-    }
-  }
-
-  // ---- the whole piece: widen and mask
-  {
-    // four-token groups start where `out` is 16-byte aligned; the input rows have to agree with that to be read in groups
-    const int lead = (int)((4 - ((reinterpret_cast<uintptr_t>(out + lo) >> 2) & 3)) & 3);
-    const int first = min(hi, lo + lead);
-    const bool wide = (reinterpret_cast<uintptr_t>(in + lo + lead) & (4 * sizeof(T) - 1)) == 0;
-    auto one = [&](int v) {
-      const bool open = mask == nullptr || ((__ldg(mask + (v >> 5)) >> (v & 31)) & 1u);
-      out[v] = open ? load1<T>(in + v) : __uint_as_float(kMinusInf);
-    };
-    if (wide) {
-      for (int v = lo + (int)threadIdx.x; v < first; v += kThreads) one(v);
-      const int groups = (hi - first) >> 2;
-      for (int g0 = threadIdx.x; g0 < groups; g0 += kThreads * kUnroll) {
-        unsigned open[kUnroll];
-        uint4 x[kUnroll];
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-          const int g = g0 + u * kThreads, v = first + 4 * g;
-          open[u] = g < groups ? 15u : 0u;
-          if (mask != nullptr && g < groups) {
-            // a group lies in one word, or in two neighbours when the row does not start on a 16-byte boundary
-            const unsigned w0 = __ldg(mask + (v >> 5)), w1 = (v & 31) > 28 ? __ldg(mask + (v >> 5) + 1) : 0u;
-            open[u] = __funnelshift_r(w0, w1, v & 31) & 15u;
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-          x[u] = make_uint4(kMinusInf, kMinusInf, kMinusInf, kMinusInf);
-          if (open[u]) x[u] = load4(in + first + 4 * (g0 + u * kThreads));
-        }
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-          const int g = g0 + u * kThreads;
-          if (g < groups) {
-            if (!(open[u] & 1u)) x[u].x = kMinusInf;
-            if (!(open[u] & 2u)) x[u].y = kMinusInf;
-            if (!(open[u] & 4u)) x[u].z = kMinusInf;
-            if (!(open[u] & 8u)) x[u].w = kMinusInf;
-            *reinterpret_cast<uint4*>(out + first + 4 * g) = x[u];
-          }
-        }
-      }
-      for (int v = first + 4 * groups + (int)threadIdx.x; v < hi; v += kThreads) one(v);
-    } else {
-      for (int v = lo + (int)threadIdx.x; v < hi; v += kThreads) one(v);
-    }
+    for_history(history, len, lo, hi, t, kHistoryThreads, [&](int i, int v) { Tab::add(table, v - lo, i < prompt); });
   }
 
   // ---- tokens of the history
@@ -134,18 +183,15 @@ __global__ void __launch_bounds__(kThreads) process_logits_kernel(const Params p
     const float r = p.repetition != nullptr ? p.repetition[row] : 1.0f;
     const float pr = p.presence != nullptr ? p.presence[row] : 0.0f;
     const float f = p.frequency != nullptr ? p.frequency[row] : 0.0f;
-    for (int i = threadIdx.x; i < len; i += kThreads) {
-      const int v = __ldg(history + i);
-      if (v < lo || v >= hi) continue;
-      const unsigned held = atomicExch(&table[v - lo], 0u);
-      if (held == 0u || (mask != nullptr && !((__ldg(mask + (v >> 5)) >> (v & 31)) & 1u))) continue;
+    for_history(history, len, lo, hi, thread, kStreamThreads + kHistoryThreads, [&](int, int v) {
+      const unsigned held = Tab::take(table, v - lo);
+      if (held == 0u || !open_token(mask, v)) return;
       float x = load1<T>(in + v);
       x = x > 0.0f ? __fdiv_rn(x, r) : __fmul_rn(x, r);
-      const unsigned count = held & ~kInPrompt;
+      const unsigned count = held & ~Tab::kPrompt;
       x = __fsub_rn(x, __fmul_rn(f, (float)count));
-      x = __fsub_rn(x, count > 0u ? pr : 0.0f);
-      out[v] = x;
-    }
+      out[v] = __fsub_rn(x, count > 0u ? pr : 0.0f);
+    });
   }
 
   // ---- biases
@@ -157,7 +203,7 @@ __global__ void __launch_bounds__(kThreads) process_logits_kernel(const Params p
       for (int base = 0; base < p.biases; base += 32) {
         const int i = base + (int)threadIdx.x;
         const int v = i < p.biases ? __ldg(ids + i) : -1;
-        const bool mine = v >= lo && v < hi && (mask == nullptr || ((__ldg(mask + (v >> 5)) >> (v & 31)) & 1u));
+        const bool mine = v >= lo && v < hi && open_token(mask, v);
         // turn of this lane among the lanes with the same token
         const unsigned same = __match_any_sync(0xffffffffu, mine ? v : -1);
         const int turn = __popc(same & ((1u << threadIdx.x) - 1u));
@@ -201,16 +247,20 @@ extern "C" int ajb_process_logits(const void* logits, int dtype, long long in_pi
   p.mask = (const unsigned*)mask; p.mask_pitch = mask_pitch;
   // a piece of a row per CTA: large, because every piece looks at the row's whole history, but not larger than leaves
   // two CTAs for each SM
-  int chunk = 8192;
+  const bool counts = history != nullptr && history_width > 0, narrow = history_width <= 32767;
+  int chunk = narrow ? logits::Table<true>::kMaxChunk : logits::Table<false>::kMaxChunk;
   while (chunk > 1024 && (long long)rows * ((vocab + chunk - 1) / chunk) < 2ll * sm_count()) chunk >>= 1;
   p.chunk = chunk;
   p.chunks = (vocab + chunk - 1) / chunk;
   AJB_REQUIRE((long long)rows * p.chunks <= 0x7fffffffll, "process logits: %d rows of %d tokens are too many", rows, vocab);
-  const int smem = history != nullptr ? chunk * (int)sizeof(unsigned) : 0;
-  const int grid = rows * p.chunks;
+  if (!counts) p.history = nullptr;
+  const int smem = counts ? chunk * (narrow ? 2 : 4) : 0;
+  const int grid = rows * p.chunks, threads = logits::kStreamThreads + (counts ? logits::kHistoryThreads : 0);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == 0) logits::process_logits_kernel<__nv_bfloat16><<<grid, logits::kThreads, smem, s>>>(p);
-  else logits::process_logits_kernel<float><<<grid, logits::kThreads, smem, s>>>(p);
+  if (dtype == 0 && narrow) logits::process_logits_kernel<__nv_bfloat16, true><<<grid, threads, smem, s>>>(p);
+  else if (dtype == 0) logits::process_logits_kernel<__nv_bfloat16, false><<<grid, threads, smem, s>>>(p);
+  else if (narrow) logits::process_logits_kernel<float, true><<<grid, threads, smem, s>>>(p);
+  else logits::process_logits_kernel<float, false><<<grid, threads, smem, s>>>(p);
   AJB_CUDA_OK(cudaGetLastError());
   return 0;
 }

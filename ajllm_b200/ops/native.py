@@ -164,7 +164,9 @@ def sm_budget(sms: int | None):
 
 
 def stream_ptr() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """The current stream of the current device, without the stream object that ``torch.cuda.current_stream()`` builds
+    (3.2 us against 0.2 us per call; a small kernel takes less)."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def ptr(t: torch.Tensor | None) -> int | None:
@@ -180,7 +182,7 @@ launch_count = 0
 def call(name: str, *args) -> None:
     global launch_count
     launch_count += _LAUNCHES_PER_CALL.get(name, 1)
-    fn = getattr(lib(), name)
+    fn = getattr(_lib or lib(), name)
     status = fn(*args)
     if status != 0:
         message = lib().ajb_last_error()

@@ -148,15 +148,10 @@ def spec_verify(target_logits: torch.Tensor, draft_logits: torch.Tensor, draft_t
 # ----------------------------------------------------------------------------- shared by the operators below
 
 
-def _require(condition: bool, message: str) -> None:
-    if not condition:
-        raise ValueError(message)
-
-
-def _int32(op: str, device: torch.device, **tensors: torch.Tensor) -> None:
-    for name, t in tensors.items():
-        if t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
-            raise ValueError(f"{op}: {name} must be a contiguous int32 tensor on {device} (got {t.dtype} on {t.device})")
+def _dense(op: str, name: str, t: torch.Tensor, dtype: torch.dtype, device: torch.device, shape: tuple[int, ...]) -> None:
+    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{op}: {name} must be a contiguous {dtype} tensor of shape {list(shape)} on {device} "
+                         f"(got {t.dtype} {list(t.shape)} on {t.device}, strides {t.stride()})")
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -197,21 +192,24 @@ def batch_maps(block_ids: torch.Tensor, block_counts: torch.Tensor, cached_lens:
 
     ``out`` may hold the five result tensors (buffers a captured graph reads); they are overwritten and returned.
     """
-    n, device = block_counts.shape[0], block_ids.device
-    _int32("batch_maps", device, block_ids=block_ids, block_counts=block_counts, cached_lens=cached_lens, q_lens=q_lens)
-    _require(block_ids.dim() == 1 and block_counts.dim() == 1 and cached_lens.shape == block_counts.shape == q_lens.shape,
-             "batch_maps: block_ids is one flat list, block_counts / cached_lens / q_lens have one entry per sequence")
-    _require(total_tokens >= 0 and max_blocks >= 1 and block_size >= 1 and pad_block >= 0,
-             "batch_maps: total_tokens and pad_block must not be negative, max_blocks and block_size must be positive")
-    _require(n <= 16384, f"batch_maps: {n} sequences are too many (at most 16384)")
+    op, int32, device = "batch_maps", torch.int32, block_ids.device
+    if block_counts.dim() != 1 or block_ids.dim() != 1:
+        raise ValueError("batch_maps: block_ids is one flat list, block_counts has one entry per sequence")
+    n, = each = block_counts.shape
+    _dense(op, "block_ids", block_ids, int32, device, block_ids.shape)
+    _dense(op, "block_counts", block_counts, int32, device, each)
+    _dense(op, "cached_lens", cached_lens, int32, device, each)
+    _dense(op, "q_lens", q_lens, int32, device, each)
+    if not (0 <= total_tokens < 1 << 30 and max_blocks >= 1 and block_size >= 1 and pad_block >= 0 and n <= 16384):
+        raise ValueError(f"batch_maps: total_tokens {total_tokens} and pad_block {pad_block} must not be negative, max_blocks {max_blocks} "
+                         f"and block_size {block_size} must be positive, and there are at most 16384 sequences (got {n})")
     if out is not None:
         out = BatchMaps(*out)
-        _int32("batch_maps", device, tables=out.tables, positions=out.positions, q_start=out.q_start, context_lens=out.context_lens)
-        slots = out.slots
-        _require(slots.dtype == torch.int64 and slots.device == device and slots.is_contiguous() and slots.shape == (total_tokens,)
-                 and out.tables.shape == (n, max_blocks) and out.positions.shape == (total_tokens,)
-                 and out.q_start.shape == (n + 1,) and out.context_lens.shape == (n,),
-                 "batch_maps: the tensors in out do not have the shapes and types of the results")
+        _dense(op, "out.tables", out.tables, int32, device, (n, max_blocks))
+        _dense(op, "out.positions", out.positions, int32, device, (total_tokens,))
+        _dense(op, "out.slots", out.slots, torch.int64, device, (total_tokens,))
+        _dense(op, "out.q_start", out.q_start, int32, device, (n + 1,))
+        _dense(op, "out.context_lens", out.context_lens, int32, device, each)
     if device.type != "cuda":
         found = reference.batch_maps(block_ids, block_counts, cached_lens, q_lens, total_tokens, max_blocks, block_size, pad_block)
         if out is None:
@@ -267,30 +265,33 @@ def shared_prefix_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cach
     number of parts per sequence is chosen. A row whose sequence has no token at all comes out as zeros. ``scale``
     defaults to ``1 / sqrt(hd)``; ``out`` (contiguous, like ``q``) receives the result.
     """
-    _require(q.dim() == 3 and key_cache.dim() == 4 and key_cache.shape == value_cache.shape and block_tables.dim() == 2,
-             "shared_prefix_attention: q is [rows, heads, hd], the caches [blocks, block, kv_heads, hd], block_tables [n, max_blocks]")
+    op, int32, device = "shared_prefix_attention", torch.int32, q.device
+    if q.dim() != 3 or key_cache.dim() != 4 or block_tables.dim() != 2:
+        raise ValueError("shared_prefix_attention: q is [rows, heads, hd], the caches [blocks, block, kv_heads, hd], block_tables [n, max_blocks]")
     total, heads, head_dim = q.shape
-    num_blocks, block_size, kv_heads, _ = key_cache.shape
+    num_blocks, block_size, kv_heads, cache_dim = key_cache.shape
     n, max_blocks = block_tables.shape
-    device = q.device
-    _require(q_len >= 1 and total == n * q_len, f"shared_prefix_attention: {total} query rows are not {q_len} for each of {n} sequences")
-    _require(key_cache.shape[3] == head_dim and kv_heads >= 1 and heads % kv_heads == 0,
-             "shared_prefix_attention: the heads of q and of the caches do not match")
-    _require(0 <= prefix_len <= max_blocks * block_size, f"shared_prefix_attention: prefix_len {prefix_len} does not fit the block tables")
-    _require(key_cache.dtype == value_cache.dtype == q.dtype and key_cache.device == value_cache.device == device,
-             "shared_prefix_attention: q and the caches must have one type and one device")
-    _int32("shared_prefix_attention", device, block_tables=block_tables, context_lens=context_lens)
-    _require(context_lens.shape == (n,), "shared_prefix_attention: context_lens has one entry per sequence")
+    if q_len < 1 or total != n * q_len:
+        raise ValueError(f"shared_prefix_attention: {total} query rows are not {q_len} for each of {n} sequences")
+    if cache_dim != head_dim or kv_heads < 1 or heads < 1 or heads % kv_heads or num_blocks < 1 or max_blocks < 1:
+        raise ValueError(f"shared_prefix_attention: {heads} query heads of {head_dim} do not go with {kv_heads} KV heads of {cache_dim}, "
+                         "or the cache or the block tables are empty")
+    if not 0 <= prefix_len <= max_blocks * block_size:
+        raise ValueError(f"shared_prefix_attention: prefix_len {prefix_len} does not fit block tables of {max_blocks} blocks")
+    _dense(op, "key_cache", key_cache, q.dtype, device, key_cache.shape)
+    _dense(op, "value_cache", value_cache, q.dtype, device, key_cache.shape)
+    _dense(op, "block_tables", block_tables, int32, device, block_tables.shape)
+    _dense(op, "context_lens", context_lens, int32, device, (n,))
     if out is not None:
-        _require(out.shape == q.shape and out.dtype == q.dtype and out.device == device and out.is_contiguous() and not _overlap(out, q),
-                 "shared_prefix_attention: out must be contiguous, shaped like q and apart from it")
+        _dense(op, "out", out, q.dtype, device, q.shape)
+        if _overlap(out, q):
+            raise ValueError("shared_prefix_attention: out must not overlap q")
     scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
     if device.type != "cuda":
         found = reference.shared_prefix_attention(q, key_cache, value_cache, block_tables, context_lens, prefix_len, q_len, scale)
         return found if out is None else out.copy_(found)
     if q.dtype != torch.bfloat16:
         raise TypeError(f"shared_prefix_attention: CUDA tensors must be bfloat16 (got {q.dtype})")
-    _require(key_cache.is_contiguous() and value_cache.is_contiguous(), "shared_prefix_attention: the caches must be contiguous")
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
             return shared_prefix_attention(q, key_cache, value_cache, block_tables, context_lens, prefix_len, q_len=q_len,
@@ -340,38 +341,41 @@ def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
 
     ``out`` (fp32 ``[rows, vocab]``, contiguous, apart from ``logits``) receives the result.
     """
-    _require(logits.dim() == 2, "process_logits: logits must be [rows, vocab]")
+    op, int32, fp32, device, dtype = "process_logits", torch.int32, torch.float32, logits.device, logits.dtype
+    if dtype != torch.bfloat16 and dtype != fp32:
+        raise TypeError(f"process_logits: logits must be bfloat16 or float32 (got {dtype})")
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError("process_logits: logits must be [rows, vocab] with at least one token")
     rows, vocab = logits.shape
-    device = logits.device
-    if logits.dtype not in (torch.bfloat16, torch.float32):
-        raise TypeError(f"process_logits: logits must be bfloat16 or float32 (got {logits.dtype})")
-    _require(vocab >= 1, "process_logits: the vocabulary is empty")
+    each = (rows,)
     width = biases = 0
     if history is not None:
-        _require(prompt_lens is not None and history_lens is not None, "process_logits: a history comes with prompt_lens and history_lens")
-        _int32("process_logits", device, history=history, prompt_lens=prompt_lens, history_lens=history_lens)
-        _require(history.dim() == 2 and history.shape[0] == rows and prompt_lens.shape == history_lens.shape == (rows,),
-                 "process_logits: history is [rows, width], prompt_lens and history_lens [rows]")
+        if prompt_lens is None or history_lens is None or history.dim() != 2:
+            raise ValueError("process_logits: history is [rows, width] and comes with prompt_lens and history_lens")
         width = history.shape[1]
-        for name, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
-            _require(t is None or (t.dtype == torch.float32 and t.device == device and t.shape == (rows,) and t.is_contiguous()),
-                     f"process_logits: {name} must be a contiguous float32 [rows] tensor on {device}")
-    else:
-        _require(repetition is None and presence is None and frequency is None and prompt_lens is None and history_lens is None,
-                 "process_logits: penalties need a history")
+        _dense(op, "history", history, int32, device, (rows, width))
+        _dense(op, "prompt_lens", prompt_lens, int32, device, each)
+        _dense(op, "history_lens", history_lens, int32, device, each)
+        if repetition is not None:
+            _dense(op, "repetition", repetition, fp32, device, each)
+        if presence is not None:
+            _dense(op, "presence", presence, fp32, device, each)
+        if frequency is not None:
+            _dense(op, "frequency", frequency, fp32, device, each)
+    elif not (repetition is None and presence is None and frequency is None and prompt_lens is None and history_lens is None):
+        raise ValueError("process_logits: penalties need a history")
     if bias_ids is not None or bias_values is not None:
-        _require(bias_ids is not None and bias_values is not None, "process_logits: bias_ids and bias_values come together")
-        _int32("process_logits", device, bias_ids=bias_ids)
-        _require(bias_ids.dim() == 2 and bias_ids.shape[0] == rows and bias_values.shape == bias_ids.shape
-                 and bias_values.dtype == torch.float32 and bias_values.device == device and bias_values.is_contiguous(),
-                 "process_logits: bias_ids is [rows, biases], bias_values a contiguous float32 tensor of the same shape")
+        if bias_ids is None or bias_values is None or bias_ids.dim() != 2:
+            raise ValueError("process_logits: bias_ids and bias_values come together, [rows, biases] each")
         biases = bias_ids.shape[1]
+        _dense(op, "bias_ids", bias_ids, int32, device, (rows, biases))
+        _dense(op, "bias_values", bias_values, fp32, device, (rows, biases))
     if token_mask is not None:
-        _int32("process_logits", device, token_mask=token_mask)
-        _require(token_mask.shape == (rows, (vocab + 31) // 32), "process_logits: token_mask must be [rows, ceil(vocab / 32)]")
+        _dense(op, "token_mask", token_mask, int32, device, (rows, (vocab + 31) // 32))
     if out is not None:
-        _require(out.shape == logits.shape and out.dtype == torch.float32 and out.device == device and out.is_contiguous()
-                 and not _overlap(out, logits), "process_logits: out must be contiguous float32 [rows, vocab] apart from the logits")
+        _dense(op, "out", out, fp32, device, (rows, vocab))
+        if _overlap(out, logits):
+            raise ValueError("process_logits: out must not overlap the logits")
     if device.type != "cuda":
         found = reference.process_logits(logits, history, prompt_lens, history_lens, repetition, presence, frequency, bias_ids,
                                          bias_values, token_mask)
@@ -385,7 +389,7 @@ def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
         logits = logits.contiguous()
     if out is None:
         out = torch.empty(rows, vocab, dtype=torch.float32, device=device)
-    native.call("ajb_process_logits", logits.data_ptr(), 0 if logits.dtype == torch.bfloat16 else 1, logits.stride(0), out.data_ptr(),
+    native.call("ajb_process_logits", logits.data_ptr(), 1 if dtype == fp32 else 0, logits.stride(0), out.data_ptr(),
                 rows, vocab, native.ptr(history) if width else None, width, width, native.ptr(prompt_lens), native.ptr(history_lens),
                 native.ptr(repetition), native.ptr(presence), native.ptr(frequency), native.ptr(bias_ids), native.ptr(bias_values),
                 biases, native.ptr(token_mask), (vocab + 31) // 32, native.stream_ptr())

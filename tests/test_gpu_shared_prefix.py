@@ -402,3 +402,15 @@ def test_logits_maps_and_attention_replayed_together():
     _check_attention(attended, *_oracle(q, keys, values, maps.tables, maps.context_lens, 1))
     want = reference.process_logits(raw.cpu(), history.cpu(), (lens // 2).cpu(), lens.cpu(), penalty.cpu(), token_mask=mask.cpu())
     assert torch.equal(logits.cpu(), want) and tokens.tolist() == want.argmax(-1).tolist()
+
+
+def test_history_longer_than_a_16_bit_count():
+    """40000 repeats of two tokens: counts need more than 15 bits."""
+    rows, vocab, width = 2, 9000, 40000
+    history = torch.full((rows, width), 8500, dtype=torch.int32, device=_dev())
+    history[:, ::4] = 3
+    kw = dict(prompt_lens=_i32([0, 39000]), history_lens=_i32([width, width]), frequency=torch.full((rows,), 2.0 ** -10, device=_dev()))
+    got = serving.process_logits(torch.zeros(rows, vocab, device=_dev()), history=history, **kw)
+    assert got[:, 3].tolist() == [-10000 / 1024, -250 / 1024] and got[:, 8500].tolist() == [-30000 / 1024, -750 / 1024]
+    got[:, [3, 8500]] = 0
+    assert torch.count_nonzero(got) == 0
