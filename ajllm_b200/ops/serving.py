@@ -239,12 +239,20 @@ def batch_maps(block_ids: torch.Tensor, block_counts: torch.Tensor, cached_lens:
 _PREFIX_TILE = 128         # query rows and keys per step of the prefix kernel
 
 
-def prefix_parts(query_rows: int, kv_heads: int, shared: int) -> int:
-    """Parts that the shared prefix is cut into: one CTA per SM, and no part without a tile of keys."""
+def prefix_parts(query_rows: int, kv_heads: int, shared: int, suffix_tiles: int) -> int:
+    """Parts that each row's share of the prefix is cut into. A CTA of the prefix kernel keeps an SM to itself while the
+    others stream the suffixes, so the SMs are divided like the work: a step of 128 keys for up to 256 rows takes about
+    1.5 us of an SM, a 64-key tile of a suffix about 0.8 us. Up to 128 rows a CTA leaves two parts."""
     if not _SM_COUNT:
         _SM_COUNT.append(int(native.lib().ajb_sm_count()))
-    units = -(-query_rows // _PREFIX_TILE) * kv_heads
-    return max(1, min(_SM_COUNT[0] // units, -(-shared // _PREFIX_TILE), 16))
+    one_tile = query_rows <= _PREFIX_TILE
+    units = kv_heads * (1 if one_tile else -(-query_rows // (2 * _PREFIX_TILE)))
+    tiles = -(-shared // _PREFIX_TILE)
+    steps = -(-tiles // 2) if one_tile else tiles
+    prefix_work, suffix_work = 1.5 * units * steps, 0.8 * suffix_tiles
+    ctas = _SM_COUNT[0] * prefix_work / (prefix_work + suffix_work)
+    parts = max(1, min(round(ctas / units), _SM_COUNT[0] // units, steps, 16))
+    return 2 * parts if one_tile else parts
 
 
 def shared_prefix_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -304,10 +312,12 @@ def shared_prefix_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cach
         return out
     shared = prefix_len // block_size * block_size
     group = heads // kv_heads
-    parts = prefix_parts(total * group, kv_heads, shared) if shared else 0
     chunk = q_len if group * q_len <= 32 else max(1, min(q_len, _PREFIX_TILE // group))
     behind = min(max_context if max_context is not None else max_blocks * block_size, max_blocks * block_size) - shared
-    splits = paged_splits(n * kv_heads * -(-q_len // chunk), max(0, behind))
+    ctas = n * kv_heads * -(-q_len // chunk)
+    splits = paged_splits(ctas, max(0, behind))
+    # lengths are on the device: half the bound is what they are taken to be
+    parts = prefix_parts(total * group, kv_heads, shared, ctas * (behind // 128 + 1)) if shared else 0
     # fp32 parts of every (row, head): un-normalised outputs, then (reference maximum, sum) pairs
     count = total * heads * (parts + splits)
     workspace = torch.empty(count * (head_dim + 2), dtype=torch.float32, device=device)
