@@ -124,12 +124,16 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag,
                                           DeviceStatus* status, int kernel_id, int stage) {
   if (mbar_try_wait(bar, parity)) return true;
-  const unsigned long long t0 = global_timer_ns();
+  unsigned long long t0 = 0;
   uint32_t spins = 0;
   while (true) {
     if (mbar_try_wait(bar, parity)) return true;
     if (*abort_flag) return false;
-    if ((++spins & 0x3ff) == 0 && global_timer_ns() - t0 > kWaitBudgetNs) {
+    if ((++spins & 0x3ff) != 0) continue;
+    // the clock is first looked at here: reading %globaltimer takes far longer than an ordinary wait
+    const unsigned long long now = global_timer_ns();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > kWaitBudgetNs) {
       *abort_flag = 1;
       if (status != nullptr && atomicCAS(&status[kernel_id].code, 0u, (unsigned)((stage << 8) | (kernel_id + 1))) == 0u) {
         status[kernel_id].block = blockIdx.x;
@@ -178,6 +182,32 @@ __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* m
 }
 __device__ __forceinline__ void prefetch_tensor_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+
+// ---- taking over CTAs that have not started (cluster launch control): a running CTA asks for one, and if the answer in
+// shared memory (16 bytes, 16-byte aligned, completes on `bar`) says so, that CTA never starts and its index is the
+// caller's. After an answer that says no, none may be asked for again.
+__device__ __forceinline__ void launch_take_request(void* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(answer)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ bool launch_take_answer(const void* answer, int& cta /* blockIdx.x of a one-dimensional grid */) {
+  uint32_t ok;
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      ".reg .b128 h;\n"
+      "ld.shared.b128 h, [%2];\n"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n"
+      "selp.u32 %0, 1, 0, p;\n"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, _, _, _}, h;\n"
+      "}\n"
+      : "=r"(ok), "+r"(cta)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return ok != 0;
 }
 
 // ---- TMEM
@@ -396,12 +426,16 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t pa
 __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag,
                                                   DeviceStatus* status, int kernel_id, int stage) {
   if (mbar_try_wait_cluster(bar, parity)) return true;
-  const unsigned long long t0 = global_timer_ns();
+  unsigned long long t0 = 0;
   uint32_t spins = 0;
   while (true) {
     if (mbar_try_wait_cluster(bar, parity)) return true;
     if (*abort_flag) return false;
-    if ((++spins & 0x3ff) == 0 && global_timer_ns() - t0 > kWaitBudgetNs) {
+    if ((++spins & 0x3ff) != 0) continue;
+    // the clock is first looked at here: reading %globaltimer takes far longer than an ordinary wait
+    const unsigned long long now = global_timer_ns();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > kWaitBudgetNs) {
       *abort_flag = 1;
       if (status != nullptr && atomicCAS(&status[kernel_id].code, 0u, (unsigned)((stage << 8) | (kernel_id + 1))) == 0u) {
         status[kernel_id].block = blockIdx.x;

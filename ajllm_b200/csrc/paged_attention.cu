@@ -16,7 +16,7 @@
 // columns), so two CTAs share an SM and each one's chain hides behind the other's loads.
 //
 // Plain decoding has 4 to 8 real rows, all in the first quarter, and one warp would do the softmax of
-// all key columns of a tile while three idle. With at most 32 rows (REPL) the query rows are therefore staged
+// all key columns of a tile while three idle. With at most 32 rows (paged_decode_kernel) the query rows are therefore staged
 // four times, once per 32-lane quarter: the score tile then holds four identical copies, and warp q
 // works on key columns [16 q, 16 q + 16) of its own copy. The four partial row maxima (and at the end the
 // partial row sums) are exchanged through shared memory; P is assembled in rows 0..31 of the operand
@@ -54,14 +54,14 @@ constexpr int kThreads = 192;
 constexpr int kMaxRows = 64;       // group * q_len of a plain launch
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kPagedKernelId = 5;
-constexpr int kReplTileBytes = 32 * 128;   // REPL variant: the 32 meaningful rows of a probability tile (64 keys x 2 bytes per row)
+constexpr int kReplTileBytes = 32 * 128;   // paged_decode_kernel: the 32 meaningful rows of a probability tile (64 keys x 2 bytes per row)
 
 template <int HD>
 struct Cfg {
   static constexpr int kQ = QROWS * HD * 2;          // the query rows, staged once
   static constexpr int kTile = TILE * HD * 2;        // one K or V tile
   static constexpr int kP = QROWS * TILE * 2;        // probabilities of one step (A operand of P V)
-  // [parity][quarter][row] partial maxima / sums of the REPL variant live in rows 64.. of the P tile: with at most 32
+  // [parity][quarter][row] partial maxima / sums of paged_decode_kernel live in rows 64.. of the P tile: with at most 32
   // real rows those operand rows only feed accumulator rows that nobody reads
   static constexpr int kExchangeOffset = 64 * 128;
   static constexpr int kSmem = kQ + 4 * kTile /*2 x (K,V)*/ + kP + 256;
@@ -77,7 +77,8 @@ struct Params {
   const int* q_start;         // null: sequence i's rows start at i * q_total
   long long q_pitch;          // elements between the rows of two tokens in q
   int max_blocks;
-  int heads, kv_heads, q_len;
+  int heads, kv_heads, group, q_len;
+  int seqs, chunks;           // sequences; CTAs that a sequence's new tokens are cut over
   int q_total;                // new tokens per sequence; q_len of them are a CTA's, chunk after chunk
   int first_key;              // first cached token this launch looks at (a multiple of the block size)
   float scale;
@@ -88,15 +89,15 @@ struct Params {
   DeviceStatus* status;
 };
 
-// Rows [first, TILE) of a V tile become zero: they belong to no key (the unused end of the last block, or a block fetched
+// Rows [first, kRows) of a V tile become zero: they belong to no key (the unused end of the last block, or a block fetched
 // again to fill the tile), their probabilities are zero, and zero times whatever an old sequence left there (an
 // infinity, a NaN) must not reach the sums. `t` is the caller's index among the 128 threads that share the work.
-template <int HD>
+template <int HD, int kRows>
 __device__ __forceinline__ void zero_value_rows(uint8_t* tile, int first, int t) {
   constexpr int kBoxes = HD / 64;
-  for (int i = first * 8 + t; i < TILE * 8; i += 128) {
+  for (int i = first * 8 + t; i < kRows * 8; i += 128) {
 #pragma unroll
-    for (int b = 0; b < kBoxes; ++b) reinterpret_cast<uint4*>(tile + b * (TILE * 128))[i] = make_uint4(0, 0, 0, 0);
+    for (int b = 0; b < kBoxes; ++b) reinterpret_cast<uint4*>(tile + b * (kRows * 128))[i] = make_uint4(0, 0, 0, 0);
   }
 }
 
@@ -106,19 +107,16 @@ __device__ __forceinline__ void store_chunk(uint8_t* tile, int row, int ch, uint
   *reinterpret_cast<uint4*>(dst) = val;
 }
 
-template <int HD, bool REPL>
+template <int HD>
 __global__ void __launch_bounds__(kThreads, 2)
 paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                        const Params p) {
   using C = Cfg<HD>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw;
-  // Q, P, the K/V ring, barriers. P sits in front of the ring: the second probability tile of the REPL variant starts
-  // 4 KB into P and its (unused) operand rows reach into the ring, never past the end of the allocation
   uint8_t* sQ = smem;
   uint8_t* sP = sQ + C::kQ;
   uint8_t* sKV = sP + C::kP;
-  float* sExchange = reinterpret_cast<float*>(sP + C::kExchangeOffset);
   uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + 4 * C::kTile);
   if (smem_misaligned(smem, p.status, kPagedKernelId, reinterpret_cast<uint32_t*>(bars) + 60)) return;
   // K and V tiles have their own barriers: a K tile is free again after the first product of its step, long before
@@ -129,10 +127,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   uint64_t* v_empty = bars + 6;    // 2
   uint64_t* s_full = bars + 8;     // 2
   uint64_t* s_free = bars + 10;    // 2
-  uint64_t* p_ready = bars + 12;   // 2 (REPL: one per probability tile; otherwise only the first)
-  uint64_t* pv_done = bars + 14;   // 2 (likewise)
-  uint64_t* xbar = bars + 16;      // 1 (REPL: the four softmax warps exchange partial maxima / sums)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
+  uint64_t* p_ready = bars + 12;   // 1
+  uint64_t* pv_done = bars + 13;   // 1
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -163,10 +160,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       mbar_init(&v_empty[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&s_free[i], 4);
-      mbar_init(&p_ready[i], 4);
-      mbar_init(&pv_done[i], 1);
     }
-    mbar_init(xbar, 4);
+    mbar_init(p_ready, 4);
+    mbar_init(pv_done, 1);
     *abort_flag = 0;
     fence_barrier_init();
     prefetch_tensor_map(&map_k);
@@ -179,9 +175,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   // stage Q: rows beyond `rows` are zero (their scores are never used)
   if (warp >= 2) {
     const int t = threadIdx.x - 64;                 // 0..127 == tile row
-    const int qr = REPL ? (t & 31) : t;             // REPL: every quarter holds a copy of the query rows
-    const bool real = qr < rows;
-    const int h = real ? qr / q_len : 0, i = real ? qr % q_len : 0;
+    const bool real = t < rows;
+    const int h = real ? t / q_len : 0, i = real ? t % q_len : 0;
     const __nv_bfloat16* src = p.q + (size_t)(token0 + i) * p.q_pitch + (size_t)(kv_head * group + h) * HD;
 #pragma unroll
     for (int ch = 0; ch < HD / 8; ++ch) {
@@ -293,184 +288,19 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         ok = issue_s(j + 1);
         if (!ok) break;
       }
-      // REPL: probability tile j & 1 (4 KB apart), its barriers complete every other tile
-      const int pb = REPL ? (j & 1) : 0;
-      const uint32_t p_phase = REPL ? (((uint32_t)j >> 1) & 1) : ((uint32_t)j & 1);
-      if (!mbar_wait(&p_ready[pb], p_phase, abort_flag, p.status, kPagedKernelId, 5)) { ok = false; break; }
+      if (!mbar_wait(p_ready, (uint32_t)j & 1, abort_flag, p.status, kPagedKernelId, 5)) { ok = false; break; }
       if (!mbar_wait(&v_full[j & 1], ((uint32_t)j >> 1) & 1, abort_flag, p.status, kPagedKernelId, 10)) { ok = false; break; }
       tc_fence_after_sync();
       if (lane == 0) {
         const uint32_t v_mn = v_mn0 + (uint32_t)(j & 1) * kStageStep;
-        const uint32_t p_lo = p_km + (uint32_t)pb * (uint32_t)(kReplTileBytes >> 4);
-        umma_f16(tmem_base + C::kOCol, desc_at(p_lo, 0), desc_at(v_mn, 0), idesc_o, j != 0);
+        umma_f16(tmem_base + C::kOCol, desc_at(p_km, 0), desc_at(v_mn, 0), idesc_o, j != 0);
 #pragma unroll
         for (int k = 1; k < TILE / 16; ++k)
-          umma_f16_c<true>(tmem_base + C::kOCol, desc_at(p_lo, k_major_step(k, QROWS * 128)), desc_at(v_mn, mn_major_step(k)), idesc_o);
-        tc_commit(&pv_done[pb]);
+          umma_f16_c<true>(tmem_base + C::kOCol, desc_at(p_km, k_major_step(k, QROWS * 128)), desc_at(v_mn, mn_major_step(k)), idesc_o);
+        tc_commit(pv_done);
         tc_commit(&v_empty[j & 1]);
       }
       __syncwarp();
-    }
-  } else if (REPL) {
-    // ---- at most 32 query rows, copied into every quarter: warp q handles key columns [16 q, 16 q + 16)
-    const int quarter = warp & 3;
-    const bool real = lane < rows;
-    const int h = real ? lane / q_len : 0, qi = real ? lane % q_len : 0;
-    const int k_max = real ? min(ctx - q_len + qi, keys - 1) : -1;   // last visible key
-    const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
-    const float sl = p.scale * kLog2e;
-    float m_run = -INFINITY, l_run = 0.0f;              // l_run: this warp's 16 columns of every tile only
-    bool ok = true;
-    // The four warps exchange a value per row through a ring of four slots: `publish` writes this warp's value of
-    // exchange number `x` and arrives, `collect` waits (bounded) until all four have arrived for `x` and reads them.
-    // A warp collects exchange x before it publishes x + 1, so the barrier never runs two phases ahead of a waiter,
-    // and no warp can be four exchanges ahead of another (S tiles are handed back by all four warps).
-    auto publish = [&](uint32_t x, float mine) {
-      sExchange[(x & 3) * 128 + quarter * 32 + lane] = mine;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(xbar);
-    };
-    auto collect = [&](uint32_t x, float (&all)[4]) -> bool {
-      if (!mbar_wait(xbar, x & 1, abort_flag, p.status, kPagedKernelId, 9)) return false;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) all[q] = sExchange[(x & 3) * 128 + q * 32 + lane];
-      return true;
-    };
-    for (int j = 0; j < n_tiles && ok; ++j) {
-      const int s = j & 1;
-      if (!mbar_wait(&s_full[s], ((uint32_t)j >> 1) & 1, abort_flag, p.status, kPagedKernelId, 6)) { ok = false; break; }
-      tc_fence_after_sync();
-      const int k0 = (t0 + j) * TILE + quarter * 16;
-      uint32_t sv[16];
-      tmem_ld_32x16(tmem_base + lane_addr + (uint32_t)(s * TILE + quarter * 16), sv);
-      tc_wait_ld();
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s_free[s]);
-      float m_loc = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float x = __uint_as_float(sv[i]);
-        if (k0 + i > k_max) x = -INFINITY;
-        sv[i] = __float_as_uint(x);
-        m_loc = fmaxf(m_loc, x);
-      }
-      // reference maximum: the first tile waits for its own maxima; tile j > 0 takes those of tile j - 1, which were
-      // published a whole tile ago, and publishes its own for tile j + 1
-      float part[4];
-      if (j == 0) {
-        publish(0u, m_loc);
-        if (!collect(0u, part)) { ok = false; break; }
-      } else {
-        if (!collect((uint32_t)(j - 1), part)) { ok = false; break; }
-        publish((uint32_t)j, m_loc);
-      }
-      const float m_seen = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-      // lazy reference maximum (see flash_fwd.cu); every warp sees the same m_seen and decides alike
-      const bool moved = (m_seen - m_run) * sl > 8.0f;
-      const float m_new = moved ? m_seen : m_run;
-      const float m_safe = (m_new == -INFINITY) ? 0.0f : m_new;
-      const float alpha = moved ? exp2f((m_run - m_safe) * sl) : 1.0f;
-      const float neg = -m_safe * sl;
-      float l_tile = 0.0f;
-      uint32_t pk[8];
-#pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        // keys of this tile may exceed the reference of the tiles before it: the exponent is capped below overflow
-        const float p0 = exp2f(fminf(fmaf(__uint_as_float(sv[i]), sl, neg), 120.0f));
-        const float p1 = exp2f(fminf(fmaf(__uint_as_float(sv[i + 1]), sl, neg), 120.0f));
-        l_tile += p0 + p1;
-        pk[i / 2] = pack_bf16x2(p0, p1);
-      }
-      l_run = l_run * alpha + l_tile;
-      m_run = m_new;
-      // probability tile j & 1 was last read by the second product of tile j - 2
-      const int pb = j & 1;
-      if (j > 1 && !mbar_wait(&pv_done[pb], (((uint32_t)(j - 2)) >> 1) & 1, abort_flag, p.status, kPagedKernelId, 7)) { ok = false; break; }
-      // P row `lane`, key columns of this warp
-      uint8_t* tile_p = sP + pb * kReplTileBytes;
-#pragma unroll
-      for (int ch = 0; ch < 2; ++ch)
-        store_chunk(tile_p, lane, quarter * 2 + ch, make_uint4(pk[ch * 4], pk[ch * 4 + 1], pk[ch * 4 + 2], pk[ch * 4 + 3]));
-      if (ragged_tile == j) {
-        if (!mbar_wait(&v_full[s], ((uint32_t)j >> 1) & 1, abort_flag, p.status, kPagedKernelId, 11)) { ok = false; break; }
-        zero_value_rows<HD>(sKV + s * 2 * C::kTile + C::kTile, keys - (t0 + j) * TILE, quarter * 32 + lane);
-      }
-      if (j > 0 && __any_sync(0xffffffffu, moved)) {
-        // O changes scale: every product up to tile j - 1 must have landed first (all warps wait, so that none
-        // announces its part of P before the rescaled O is in place ... the first warp rescales)
-        if (!mbar_wait(&pv_done[(j - 1) & 1], (((uint32_t)(j - 1)) >> 1) & 1, abort_flag, p.status, kPagedKernelId, 7)) { ok = false; break; }
-        tc_fence_after_sync();
-        if (quarter == 0) {
-#pragma unroll 1
-          for (int c = 0; c < HD / 32; ++c) {
-            uint32_t ov[32];
-            tmem_ld_32x32(tmem_base + (uint32_t)(C::kOCol + c * 32), ov);
-            tc_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
-            tmem_st_32x32(tmem_base + (uint32_t)(C::kOCol + c * 32), ov);
-          }
-          tc_wait_st();
-        }
-      }
-      fence_proxy_async_smem();
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_ready[pb]);
-    }
-    float sums[4] = {0.f, 0.f, 0.f, 0.f};
-    if (ok && n_tiles > 0) {
-      // exchange n_tiles - 1 (the last tile's maxima) is collected first to keep the order, then the sums go round
-      float unused[4];
-      if (n_tiles > 1) ok = collect((uint32_t)(n_tiles - 1), unused);
-      if (ok) {
-        publish((uint32_t)n_tiles, l_run);
-        ok = collect((uint32_t)n_tiles, sums);
-      }
-    }
-    const size_t out_row = (size_t)(token0 + qi) * p.heads + kv_head * group + h;
-    const size_t part_row = out_row * p.part_stride + p.part_base + blockIdx.z;
-    if (p.part_stride > 0 && quarter == 0 && real && (n_tiles == 0 || !ok))
-      p.part_ml[part_row] = make_float2(0.0f, 0.0f);        // nothing to merge from this part
-    if (ok && quarter == 0 && n_tiles > 0 &&
-        mbar_wait(&pv_done[(n_tiles - 1) & 1], (((uint32_t)(n_tiles - 1)) >> 1) & 1, abort_flag, p.status, kPagedKernelId, 8)) {
-      tc_fence_after_sync();
-      const float l_all = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-      const float inv_l = l_all > 0.0f ? 1.0f / l_all : 0.0f;
-      __nv_bfloat16* dst = p.out + out_row * HD;
-      if (p.part_stride > 0) {
-        if (real) p.part_ml[part_row] = make_float2(m_run == -INFINITY ? 0.0f : m_run * sl, l_all);
-        float* part = p.part_o + part_row * HD;
-#pragma unroll 1
-        for (int c = 0; c < HD / 32; ++c) {
-          uint32_t ov[32];
-          tmem_ld_32x32(tmem_base + (uint32_t)(C::kOCol + c * 32), ov);
-          tc_wait_ld();
-          if (real) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              reinterpret_cast<uint4*>(part + c * 32)[i] = make_uint4(ov[4 * i], ov[4 * i + 1], ov[4 * i + 2], ov[4 * i + 3]);
-          }
-        }
-      } else
-#pragma unroll 1
-      for (int c = 0; c < HD / 32; ++c) {
-        uint32_t ov[32];
-        tmem_ld_32x32(tmem_base + (uint32_t)(C::kOCol + c * 32), ov);
-        tc_wait_ld();
-        if (real) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint4 q;
-            q.x = pack_bf16x2(__uint_as_float(ov[8 * i]) * inv_l, __uint_as_float(ov[8 * i + 1]) * inv_l);
-            q.y = pack_bf16x2(__uint_as_float(ov[8 * i + 2]) * inv_l, __uint_as_float(ov[8 * i + 3]) * inv_l);
-            q.z = pack_bf16x2(__uint_as_float(ov[8 * i + 4]) * inv_l, __uint_as_float(ov[8 * i + 5]) * inv_l);
-            q.w = pack_bf16x2(__uint_as_float(ov[8 * i + 6]) * inv_l, __uint_as_float(ov[8 * i + 7]) * inv_l);
-            reinterpret_cast<uint4*>(dst + c * 32)[i] = q;
-          }
-        }
-      }
     }
   } else {
     const int quarter = warp & 3;
@@ -533,7 +363,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&s_free[s]);
-      if (j > 0 && !mbar_wait(&pv_done[0], (uint32_t)(j - 1) & 1, abort_flag, p.status, kPagedKernelId, 7)) { ok = false; break; }
+      if (j > 0 && !mbar_wait(pv_done, (uint32_t)(j - 1) & 1, abort_flag, p.status, kPagedKernelId, 7)) { ok = false; break; }
       tc_fence_after_sync();
       // inactive quarters write their (zero) rows only once: they never change
       if (active || j == 0) {
@@ -542,7 +372,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       }
       if (ragged_tile == j) {
         if (!mbar_wait(&v_full[s], ((uint32_t)j >> 1) & 1, abort_flag, p.status, kPagedKernelId, 11)) { ok = false; break; }
-        zero_value_rows<HD>(sKV + s * 2 * C::kTile + C::kTile, keys - (t0 + j) * TILE, quarter * 32 + lane);
+        zero_value_rows<HD, TILE>(sKV + s * 2 * C::kTile + C::kTile, keys - (t0 + j) * TILE, quarter * 32 + lane);
       }
       if (active && j > 0 && __any_sync(0xffffffffu, moved)) {
 #pragma unroll 1
@@ -559,13 +389,13 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       fence_proxy_async_smem();
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_ready[0]);
+      if (lane == 0) mbar_arrive(p_ready);
     }
     const size_t out_row = (size_t)(token0 + qi) * p.heads + kv_head * group + h;
     const size_t part_row = out_row * p.part_stride + p.part_base + blockIdx.z;
     if (p.part_stride > 0 && real && (n_tiles == 0 || !ok))
       p.part_ml[part_row] = make_float2(0.0f, 0.0f);        // nothing to merge from this part
-    if (ok && n_tiles > 0 && mbar_wait(&pv_done[0], (uint32_t)(n_tiles - 1) & 1, abort_flag, p.status, kPagedKernelId, 8)) {
+    if (ok && n_tiles > 0 && mbar_wait(pv_done, (uint32_t)(n_tiles - 1) & 1, abort_flag, p.status, kPagedKernelId, 8)) {
       tc_fence_after_sync();
       if (active && p.part_stride > 0) {
         if (real) p.part_ml[part_row] = make_float2(m_run == -INFINITY ? 0.0f : m_run * sl, l_run);
@@ -613,6 +443,599 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   }
 }
 
+// ---------------------------------------------------------------------------------------------------------------------
+// At most 32 query rows per (sequence, KV head, part): the work of plain decoding, and of verifying a few tokens.
+//
+// Keys and head dimension fill the 128-row side of the tensor-core tile, the few query rows the narrow one:
+//   S^T [128 keys, N] = K Q^T,   O^T [hd, N] += V^T P^T    (N = 16 or 32 rows, the real ones first)
+// so a step reads every K and V byte from shared memory once and nothing else of size, each softmax thread owns one key
+// and all its query rows (4 of 16 columns used in the worst ordinary case, instead of 4 of 128 rows), and what a CTA
+// holds besides its ring of K and V tiles is a few KB. The row maxima of a tile are a warp reduction per query row and
+// one exchange between the four warps; row sums stay in registers until the end.
+//
+// A CTA does not end with its first piece of work: while it computes, it takes over a CTA of the launch that has not
+// started yet (the hardware gives out each exactly once, so sequences of any mix of lengths balance). Its producing warp
+// runs on into the next piece's keys and values as ring slots fall free, the next piece's query rows are loaded while the
+// last tile of the piece before is worked on, and barriers and tensor memory are set up once: tile, slot and exchange
+// numbers simply count over all pieces.
+// ---------------------------------------------------------------------------------------------------------------------
+constexpr int DTILE = 128;         // keys per step
+
+template <int HD, int N>
+struct DecodeCfg {
+  static constexpr int kTile = DTILE * HD * 2;                    // one K or V tile
+  static constexpr int kCtas = HD == 128 && N == 32 ? 1 : 2;      // per SM
+  static constexpr int kSlots = HD == 64 ? 5 : kCtas == 2 ? 3 : 6;
+  static constexpr int kQ = N * HD * 2;                           // query rows of a piece
+  static constexpr int kP = N * DTILE * 2;                        // probabilities of a step; two of them
+  static constexpr int kExchange = 4 * 4 * 32 * 4;                // [slot][warp][query row]
+  // 64-wide heads: the product with V^T runs 128 rows high all the same, its second half reads whatever lies behind the
+  // tile (for the last slot: 16 KB behind the ring) into accumulator rows that nobody reads
+  static constexpr int kBehind = kQ + 2 * kP + kExchange + 512;
+  static constexpr int kPad = HD == 64 && kBehind < kTile ? kTile - kBehind : 0;
+  static constexpr int kSmem = kSlots * kTile + kBehind + kPad;
+  // an SM has 228 KB, of which each CTA takes 1 KB more than it asks for
+  static_assert(kCtas * (kSmem + 1024) <= 228 * 1024, "shared memory for the CTAs of an SM");
+  static constexpr int kOCol = 2 * N;                             // S^T twice, O^T behind them
+  static constexpr int kTmemCols = N == 16 ? 64 : 128;
+};
+
+// What one CTA of a launch does, from the coordinates that the grid gives it and the lengths behind them. The producing
+// warp works it out once per piece (the divisions in it take longer than a tile's exponentials) and hands it to the
+// other warps through shared memory.
+struct Work {
+  int n_tiles;          // of 128 keys; -1: no more work
+  int t0;               // the first of them
+  int kv_head, rows;    // real query rows, packed token by token: row = new token * group + head of the group
+  int token0;           // the first new token
+  int ctx;              // keys that the last new token sees; the others see one less each
+  int keys;             // keys that there are (the block table bounds them whatever the context length says)
+  int part;
+  __device__ __forceinline__ Work() {}
+  __device__ __forceinline__ Work(const Params& p, int y, int z, int context, int first_token) {
+    int chunk = 0;
+    kv_head = y;
+    if (p.chunks > 1) { chunk = y / p.kv_heads; kv_head = y - chunk * p.kv_heads; }
+    const int q0 = chunk * p.q_len, q_len = min(p.q_len, p.q_total - q0);
+    rows = p.group * q_len;
+    token0 = first_token + q0;
+    // keys are counted from first_key
+    ctx = context - (p.q_total - q0 - q_len) - p.first_key;
+    keys = min(max(ctx, 0), p.max_blocks * BLOCK_TOKENS - p.first_key);
+    const int all_tiles = (keys + DTILE - 1) / DTILE;
+    t0 = 0;
+    n_tiles = all_tiles;
+    if (p.splits > 1) {       // this CTA's share of the sequence's tiles
+      const int per_split = (all_tiles + p.splits - 1) / p.splits;
+      t0 = min(all_tiles, z * per_split);
+      n_tiles = min(all_tiles - t0, per_split);
+    }
+    part = z;
+  }
+  // the tile that the last key does not fill, if it is this CTA's (always its last one)
+  __device__ __forceinline__ int ragged_tile() const { return (t0 + n_tiles) * DTILE > keys ? n_tiles - 1 : -1; }
+  __device__ __forceinline__ void store(int4* to) const {
+    to[0] = make_int4(n_tiles, t0, kv_head, rows);
+    to[1] = make_int4(token0, ctx, keys, part);
+  }
+  __device__ __forceinline__ void load(const int4* from) {
+    const int4 a = from[0], b = from[1];
+    n_tiles = a.x; t0 = a.y; kv_head = a.z; rows = a.w;
+    token0 = b.x; ctx = b.y; keys = b.z; part = b.w;
+  }
+};
+
+__device__ __forceinline__ float warp_max_f32(float x) {
+  float m;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(x));
+  return m;
+}
+
+template <int HD, int N>
+__global__ void __launch_bounds__(kThreads, (DecodeCfg<HD, N>::kCtas))
+paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Params p) {
+  using C = DecodeCfg<HD, N>;
+  constexpr int kSlots = C::kSlots;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* ring = smem_raw;
+  uint8_t* sQ = ring + kSlots * C::kTile;
+  uint8_t* sP = sQ + C::kQ;
+  float* sExchange = reinterpret_cast<float*>(sP + 2 * C::kP);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sP + 2 * C::kP + C::kExchange);
+  if (smem_misaligned(smem_raw, p.status, kPagedKernelId, reinterpret_cast<uint32_t*>(bars) + 120)) return;
+  uint64_t* full = bars;           // kSlots (<= 6)
+  uint64_t* empty = bars + 6;      // kSlots
+  uint64_t* s_full = bars + 12;    // 2
+  uint64_t* s_free = bars + 14;    // 2
+  uint64_t* p_ready = bars + 16;   // 2
+  uint64_t* pv_done = bars + 18;   // 2
+  uint64_t* w_full = bars + 20;    // 2: a piece of work is announced
+  uint64_t* w_empty = bars + 22;   // 2: and has been read by the five other warps
+  uint64_t* q_ready = bars + 24;   // the query rows of a piece are staged
+  uint64_t* xbar = bars + 25;      // the four softmax warps exchange maxima / sums
+  uint64_t* taken = bars + 26;     // the answer about the next piece is there
+  void* answer = bars + 28;                                     // 16 bytes
+  int4* announced = reinterpret_cast<int4*>(bars + 30);         // 2 pieces of two words each
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 38);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_free[i], 4);
+      mbar_init(&p_ready[i], 4);
+      mbar_init(&pv_done[i], 1);
+      mbar_init(&w_full[i], 1);
+      mbar_init(&w_empty[i], 5);
+    }
+    mbar_init(q_ready, 4);
+    mbar_init(xbar, 4);
+    mbar_init(taken, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    prefetch_tensor_map(&map_k);
+    prefetch_tensor_map(&map_v);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, C::kTmemCols);
+    tmem_relinquish();
+  }
+  if (warp >= 2) {
+    // query rows that no piece fills, and their probabilities, stay zero (or an earlier piece's): their columns of the
+    // accumulators are never used
+    for (int i = threadIdx.x - 64; i < (C::kQ + 2 * C::kP) / 16; i += 128) reinterpret_cast<uint4*>(sQ)[i] = make_uint4(0, 0, 0, 0);
+    fence_proxy_async_smem();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+
+  // Tiles pass through the ring in the order K0 K1 V0 K2 V1 ... K(n-1) V(n-2) V(n-1): a K tile goes out a step ahead, as
+  // its product is issued a step ahead. Number of a tile among its piece's 2 n:
+  auto k_number = [](int j) { return j == 0 ? 0 : 2 * j - 1; };
+  auto v_number = [](int j, int n) { return j < n - 1 ? 2 * j + 2 : 2 * n - 1; };
+
+  if (warp == 0) {
+    // Producer. The block ids of four tiles (32 blocks) are fetched by the 32 lanes with one coalesced load, a group
+    // ahead of their use, and handed to the issuing lane by shuffles: a dependent table lookup per block in front of
+    // its copies would cost more than the copies themselves.
+    constexpr int kBlocksPerTile = DTILE / BLOCK_TOKENS;
+    constexpr int kTilesPerGroup = 32 / kBlocksPerTile;
+    const int first_block = p.first_key / BLOCK_TOKENS, table_end = p.max_blocks - 1;
+    // The KV heads of a sequence are neighbours in the grid: their rows of a cache block are neighbours in memory, and
+    // they are read at about the same time.
+    const int columns = p.kv_heads * p.chunks;
+    int seq, y, z;
+    auto place = [&](int cta) {
+      const int rest = cta / columns;
+      y = cta - rest * columns;
+      z = 0;
+      seq = rest;
+      if (p.splits > 1) { z = rest / p.seqs; seq = rest - z * p.seqs; }
+    };
+    place(blockIdx.x);
+    int context = p.context_lens[seq], first_token = p.q_start != nullptr ? p.q_start[seq] : seq * p.q_total;
+    bool ok = true, asked = false;
+    uint32_t asked_phase = 0;
+    uint32_t base = 0;                                // tiles of all pieces before this one, K and V counted
+    auto announce = [&](uint32_t piece, const Work& what) {
+      if (lane == 0) {
+        ok = mbar_wait(&w_empty[piece & 1], ((piece >> 1) & 1) ^ 1, abort_flag, p.status, kPagedKernelId, 12);
+        if (ok) {
+          what.store(announced + 2 * (piece & 1));
+          mbar_arrive(&w_full[piece & 1]);
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+    };
+    Work w(p, y, z, context, first_token);
+    announce(0, w);
+    // ids are read up to the end of the table's row; those past the sequence's last block are not used
+    auto fetch_ids = [&](int t0, int g) {
+      return p.block_tables[(size_t)seq * p.max_blocks + min(table_end, first_block + (t0 + g * kTilesPerGroup) * kBlocksPerTile + lane)];
+    };
+    bool more = true;
+    int ids_next = 0;
+    for (uint32_t piece = 0; ok && more; ++piece) {
+      const int n_tiles = w.n_tiles;
+      const int blocks = (w.keys + BLOCK_TOKENS - 1) / BLOCK_TOKENS;
+      if (piece == 0 && n_tiles > 0) ids_next = fetch_ids(w.t0, 0);
+      // tile j of K or V as its number `number`; only the blocks that hold keys are fetched
+      auto load = [&](int j, int number, int ids, const CUtensorMap* map, int stage_id) {
+        int id[kBlocksPerTile];
+#pragma unroll
+        for (int b = 0; b < kBlocksPerTile; ++b) id[b] = __shfl_sync(0xffffffffu, ids, (j % kTilesPerGroup) * kBlocksPerTile + b);
+        if (lane == 0 && ok) {
+          const uint32_t g = base + (uint32_t)number;
+          const uint32_t s = g % kSlots;
+          ok = mbar_wait(&empty[s], ((g / kSlots) & 1) ^ 1, abort_flag, p.status, kPagedKernelId, stage_id);
+          if (ok) {
+            const int here = min(kBlocksPerTile, blocks - (w.t0 + j) * kBlocksPerTile);
+            uint8_t* tile = ring + s * C::kTile;
+            mbar_arrive_expect_tx(&full[s], (uint32_t)here * BLOCK_TOKENS * HD * 2);
+#pragma unroll
+            for (int b = 0; b < kBlocksPerTile; ++b) {
+              if (b < here) {
+#pragma unroll
+                for (int i = 0; i < HD / 64; ++i)
+                  tma_load_3d(tile + i * (DTILE * 128) + b * (BLOCK_TOKENS * 128), map, &full[s], w.kv_head * HD + 64 * i, 0, id[b]);
+              }
+            }
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+      };
+      // The next piece is asked for as the last K tile goes out: its answer takes about a microsecond, and a CTA with a
+      // long piece should not sit on another one.
+      auto ask = [&]() {
+        if (lane == 0) {
+          fence_proxy_async_smem();                   // the answer before has been read
+          mbar_arrive_expect_tx(taken, 16);
+          launch_take_request(answer, taken);
+          asked = true;
+          asked_phase = piece & 1;
+        }
+      };
+      int ids_k = ids_next, ids_prev = ids_next, k_group = -1;      // block ids of K's group of tiles and of the one before
+      for (int j = 0; j <= n_tiles && ok; ++j) {
+        if (j < n_tiles) {
+          if (j % kTilesPerGroup == 0) {
+            ids_prev = ids_k;
+            ids_k = ids_next;
+            k_group = j / kTilesPerGroup;
+            if (j + kTilesPerGroup < n_tiles) ids_next = fetch_ids(w.t0, k_group + 1);
+          }
+          load(j, k_number(j), ids_k, &map_k, 1);
+        }
+        if (j == max(0, n_tiles - 1)) ask();
+        if (j >= 1) load(j - 1, v_number(j - 1, n_tiles), (j - 1) / kTilesPerGroup == k_group ? ids_k : ids_prev, &map_v, 2);
+      }
+      base += 2u * (uint32_t)n_tiles;
+      if (!ok) break;
+      int yes = 0, cta = 0;
+      if (lane == 0) {
+        ok = mbar_wait(taken, piece & 1, abort_flag, p.status, kPagedKernelId, 13);
+        if (ok) {
+          asked = false;
+          yes = launch_take_answer(answer, cta) ? 1 : 0;
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+      more = __shfl_sync(0xffffffffu, yes, 0) != 0;
+      cta = __shfl_sync(0xffffffffu, cta, 0);
+      if (!ok) break;
+      if (more) {
+        place(cta);
+        context = p.context_lens[seq];
+        first_token = p.q_start != nullptr ? p.q_start[seq] : seq * p.q_total;
+        // a single part starts at tile 0 whatever the context is: its ids need not wait for the length
+        if (p.splits == 1) ids_next = fetch_ids(0, 0);
+        w = Work(p, y, z, context, first_token);
+        if (p.splits > 1) ids_next = fetch_ids(w.t0, 0);
+      } else {
+        w.n_tiles = -1;
+      }
+      announce(piece + 1, w);
+    }
+    // after a wait that ran out: the answer may still be on its way into this CTA's shared memory (bounded as well)
+    if (lane == 0 && asked) {
+      const unsigned long long since = global_timer_ns();
+      while (!mbar_try_wait(taken, asked_phase) && global_timer_ns() - since < kWaitBudgetNs) {}
+    }
+  } else if (warp == 1) {
+    constexpr uint32_t idesc_s = make_idesc(DTILE, N, 1, false, false);
+    constexpr uint32_t idesc_o = make_idesc(128, N, 1, true, false);
+    const uint32_t q_km = desc_lo_k_major(smem_u32(sQ)), p_km0 = desc_lo_k_major(smem_u32(sP));
+    const uint32_t k_km0 = desc_lo_k_major(smem_u32(ring));
+    const uint32_t v_mn0 = desc_lo_mn_major(smem_u32(ring), DTILE * 128);
+    constexpr uint32_t kSlotStep = C::kTile >> 4;
+    bool ok = true;
+    uint32_t base = 0, slots = 0, staged = 0;         // steps, ring tiles and pieces with keys before this piece
+    for (uint32_t piece = 0; ok; ++piece) {
+      if (!mbar_wait(&w_full[piece & 1], (piece >> 1) & 1, abort_flag, p.status, kPagedKernelId, 14)) break;
+      const int n_tiles = announced[2 * (piece & 1)].x;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&w_empty[piece & 1]);
+      if (n_tiles < 0) break;
+      if (n_tiles == 0) continue;
+      if (!mbar_wait(q_ready, staged & 1, abort_flag, p.status, kPagedKernelId, 15)) break;
+      ++staged;
+      auto issue_s = [&](int j) -> bool {
+        const uint32_t g = base + (uint32_t)j, t = slots + (uint32_t)k_number(j), slot = t % kSlots;
+        if (!mbar_wait(&full[slot], (t / kSlots) & 1, abort_flag, p.status, kPagedKernelId, 3)) return false;
+        if (!mbar_wait(&s_free[g & 1], ((g >> 1) & 1) ^ 1, abort_flag, p.status, kPagedKernelId, 4)) return false;
+        tc_fence_after_sync();
+        if (lane == 0) {
+          const uint32_t k_km = k_km0 + slot * kSlotStep;
+          const uint32_t d = tmem_base + (g & 1) * N;
+          umma_f16_c<false>(d, desc_at(k_km, 0), desc_at(q_km, 0), idesc_s);
+#pragma unroll
+          for (int k = 1; k < HD / 16; ++k)
+            umma_f16_c<true>(d, desc_at(k_km, k_major_step(k, DTILE * 128)), desc_at(q_km, k_major_step(k, N * 128)), idesc_s);
+          tc_commit(&s_full[g & 1]);
+          tc_commit(&empty[slot]);
+        }
+        __syncwarp();
+        return true;
+      };
+      ok = issue_s(0);
+      for (int j = 0; j < n_tiles && ok; ++j) {
+        if (j + 1 < n_tiles) {
+          ok = issue_s(j + 1);
+          if (!ok) break;
+        }
+        const uint32_t g = base + (uint32_t)j, t = slots + (uint32_t)v_number(j, n_tiles), slot = t % kSlots;
+        if (!mbar_wait(&p_ready[g & 1], (g >> 1) & 1, abort_flag, p.status, kPagedKernelId, 5)) { ok = false; break; }
+        if (!mbar_wait(&full[slot], (t / kSlots) & 1, abort_flag, p.status, kPagedKernelId, 10)) { ok = false; break; }
+        tc_fence_after_sync();
+        if (lane == 0) {
+          const uint32_t v_mn = v_mn0 + slot * kSlotStep, p_km = p_km0 + (g & 1) * (uint32_t)(C::kP >> 4);
+          umma_f16(tmem_base + C::kOCol, desc_at(v_mn, 0), desc_at(p_km, 0), idesc_o, j != 0);
+#pragma unroll
+          for (int k = 1; k < DTILE / 16; ++k)
+            umma_f16_c<true>(tmem_base + C::kOCol, desc_at(v_mn, mn_major_step(k)), desc_at(p_km, k_major_step(k, N * 128)), idesc_o);
+          tc_commit(&pv_done[g & 1]);
+          tc_commit(&empty[slot]);
+        }
+        __syncwarp();
+      }
+      base += (uint32_t)n_tiles;
+      slots += 2u * (uint32_t)n_tiles;
+    }
+  } else {
+    const int quarter = warp & 3;
+    const int key_lane = quarter * 32 + lane;         // this thread's key of a tile, and its row of O^T
+    const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16);
+    const float sl = p.scale * kLog2e;
+    bool ok = true;
+    // The four warps exchange one value per query row (lane r: row r) through a ring of four slots: `publish` writes
+    // this warp's value of exchange number `x` and arrives, `collect` waits (bounded) until all four have and reads them.
+    // A warp collects exchange x before it publishes x + 1, so the barrier never runs two phases ahead of a waiter.
+    auto publish = [&](uint32_t x, float mine) {
+      sExchange[(x & 3) * 128 + quarter * 32 + lane] = mine;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(xbar);
+    };
+    auto collect = [&](uint32_t x, float (&all)[4]) -> bool {
+      if (!mbar_wait(xbar, x & 1, abort_flag, p.status, kPagedKernelId, 9)) return false;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) all[q] = sExchange[(x & 3) * 128 + q * 32 + lane];
+      return true;
+    };
+    // what has been announced as piece number `piece`
+    auto read_piece = [&](uint32_t piece, Work& to) -> bool {
+      if (!mbar_wait(&w_full[piece & 1], (piece >> 1) & 1, abort_flag, p.status, kPagedKernelId, 14)) return false;
+      to.load(announced + 2 * (piece & 1));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&w_empty[piece & 1]);
+      return true;
+    };
+    // Query rows of a piece, 16 bytes at a time over the 128 threads: held in registers from the moment the piece is
+    // known, stored when the last tile of the piece before has been handed on. Which rows and pieces of them a thread
+    // moves is the same for every piece of work.
+    constexpr int kChunks = HD / 8, kHeld = N * kChunks / 128;
+    uint4 held[kHeld];
+    long long held_from[kHeld];
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) {
+      const int r = (key_lane + 128 * u) / kChunks, ch = (key_lane + 128 * u) % kChunks;
+      held_from[u] = (r / p.group) * p.q_pitch + (r % p.group) * HD + 8 * ch;
+    }
+    auto hold_queries = [&](const Work& w) {
+      const __nv_bfloat16* q = p.q + (size_t)w.token0 * p.q_pitch + (size_t)(w.kv_head * p.group) * HD;
+#pragma unroll
+      for (int u = 0; u < kHeld; ++u)
+        if ((key_lane + 128 * u) / kChunks < w.rows) held[u] = ld_nc_v4(reinterpret_cast<const uint4*>(q + held_from[u]));
+    };
+    auto stage_queries = [&](const Work& w) {         // the products of the piece before have read theirs
+#pragma unroll
+      for (int u = 0; u < kHeld; ++u) {
+        const int r = (key_lane + 128 * u) / kChunks, ch = (key_lane + 128 * u) % kChunks;
+        if (r < w.rows) *reinterpret_cast<uint4*>(sQ + (ch >> 3) * (N * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = held[u];
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_ready);
+    };
+    uint32_t base = 0, slots = 0, exchange = 0;
+    // lane r looks after query row r: new token r / group, head r % group of the KV head's group
+    const int my_token = lane / p.group, my_head = lane - my_token * p.group;
+    Work next;
+    ok = read_piece(0, next);
+    if (ok && next.n_tiles > 0) {
+      hold_queries(next);
+      stage_queries(next);
+    }
+    for (uint32_t piece = 0; ok && next.n_tiles >= 0; ++piece) {
+      const Work w = next;
+      const int n_tiles = w.n_tiles, rows = w.rows, ragged_tile = w.ragged_tile();
+      const bool real = lane < rows;
+      const int sees_least = w.ctx - (w.rows - 1) / p.group;         // keys that the first new token sees
+      const int k_max = min(sees_least + my_token, w.keys) - 1;      // last visible key of row `lane`
+      const int out_row = (w.token0 + my_token) * p.heads + w.kv_head * p.group + my_head;
+      auto look_ahead = [&]() -> bool {
+        if (!read_piece(piece + 1, next)) return false;
+        if (next.n_tiles > 0) hold_queries(next);
+        return true;
+      };
+      auto part_row = [&](int row) { return (size_t)row * p.part_stride + p.part_base + w.part; };
+      float m_run = -INFINITY;                        // of row `lane`
+      float l[N];                                     // of every row, this thread's keys only
+#pragma unroll
+      for (int r = 0; r < N; ++r) l[r] = 0.0f;
+      for (int j = 0; j < n_tiles && ok; ++j) {
+        const uint32_t g = base + (uint32_t)j;
+        const int b = g & 1;
+        const uint32_t phase = (g >> 1) & 1;
+        if (!mbar_wait(&s_full[b], phase, abort_flag, p.status, kPagedKernelId, 6)) { ok = false; break; }
+        tc_fence_after_sync();
+        uint32_t sv[N];
+        if constexpr (N == 16) tmem_ld_32x16(lane_base + (uint32_t)(b * N), sv);
+        else tmem_ld_32x32(lane_base + (uint32_t)(b * N), sv);
+        tc_wait_ld();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[b]);
+        const int key = (w.t0 + j) * DTILE + key_lane;
+        const bool masked = (w.t0 + j + 1) * DTILE > min(sees_least, w.keys);
+        float mine = -INFINITY;
+        // rows four at a time: their chains of shuffles and exponentials overlap (rows past the last one in a group of
+        // four are computed along; what comes of them is not used)
+#pragma unroll
+        for (int r = 0; r < N; r += 4) {
+          if (r < rows) {
+            if (masked) {
+#pragma unroll
+              for (int u = 0; u < 4; ++u)
+                if (key > __shfl_sync(0xffffffffu, k_max, r + u)) sv[r + u] = 0xff800000u;     // -inf
+            }
+            float m[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) m[u] = warp_max_f32(__uint_as_float(sv[r + u]));
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              if (lane == r + u) mine = m[u];
+          }
+        }
+        if (!real) mine = -INFINITY;
+        float part[4];
+        publish(exchange, mine);
+        if (!collect(exchange, part)) { ok = false; break; }
+        ++exchange;
+        const float m_tile = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+        // lazy reference maximum (see flash_fwd.cu); every warp sees the same m_tile and decides alike
+        const bool moved = (m_tile - m_run) * sl > 8.0f;
+        const float m_new = moved ? m_tile : m_run;
+        const float m_safe = (m_new == -INFINITY) ? 0.0f : m_new;
+        const float alpha = moved ? exp2f((m_run - m_safe) * sl) : 1.0f;
+        const float neg = -m_safe * sl;
+        m_run = m_new;
+        const bool any_moved = __any_sync(0xffffffffu, moved);
+        // probability tile b was last read by the second product of step g - 2
+        if (g > 1 && !mbar_wait(&pv_done[b], ((g - 2) >> 1) & 1, abort_flag, p.status, kPagedKernelId, 7)) { ok = false; break; }
+        // P^T rows are query rows, 64 keys to 128 bytes; two lanes trade so that each stores two keys of one row
+        uint8_t* tile_p = sP + b * C::kP + (quarter >> 1) * (N * 128);
+        const int pair_key = (quarter & 1) * 32 + (lane & ~1);
+#pragma unroll
+        for (int r = 0; r < N; r += 4) {
+          if (r < rows) {
+            float pr[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) pr[u] = exp2f(fmaf(__uint_as_float(sv[r + u]), sl, __shfl_sync(0xffffffffu, neg, r + u)));
+            if (any_moved) {
+#pragma unroll
+              for (int u = 0; u < 4; ++u) l[r + u] *= __shfl_sync(0xffffffffu, alpha, r + u);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) l[r + u] += pr[u];
+#pragma unroll
+            for (int u = 0; u < 4; u += 2) {
+              const float other = __shfl_xor_sync(0xffffffffu, (lane & 1) ? pr[u] : pr[u + 1], 1);
+              const int row = r + u + (lane & 1);
+              const uint32_t word = (lane & 1) ? pack_bf16x2(other, pr[u + 1]) : pack_bf16x2(pr[u], other);
+              *reinterpret_cast<uint32_t*>(tile_p + row * 128 + (((pair_key >> 3) ^ (row & 7)) << 4) + (pair_key & 7) * 2) = word;
+            }
+          }
+        }
+        if (ragged_tile == j) {
+          // Rows of the V tile that belong to no key (the unused end of the last block, blocks that were not fetched)
+          // become zero: their probabilities are zero, and zero times whatever lies there (an infinity, a NaN of an old
+          // sequence) must not reach the sums.
+          const uint32_t t = slots + (uint32_t)v_number(j, n_tiles), slot = t % kSlots;
+          if (!mbar_wait(&full[slot], (t / kSlots) & 1, abort_flag, p.status, kPagedKernelId, 11)) { ok = false; break; }
+          zero_value_rows<HD, DTILE>(ring + slot * C::kTile, w.keys - (w.t0 + j) * DTILE, key_lane);
+        }
+        if (j > 0 && any_moved) {
+          // O^T changes scale: every product up to step g - 1 must have landed first
+          if (!mbar_wait(&pv_done[b ^ 1], ((g - 1) >> 1) & 1, abort_flag, p.status, kPagedKernelId, 7)) { ok = false; break; }
+          tc_fence_after_sync();
+          uint32_t ov[N];
+          if constexpr (N == 16) tmem_ld_32x16(lane_base + C::kOCol, ov);
+          else tmem_ld_32x32(lane_base + C::kOCol, ov);
+          tc_wait_ld();
+#pragma unroll
+          for (int r = 0; r < N; ++r) ov[r] = __float_as_uint(__uint_as_float(ov[r]) * __shfl_sync(0xffffffffu, alpha, r));
+          if constexpr (N == 16) tmem_st_32x16(lane_base + C::kOCol, ov);
+          else tmem_st_32x32(lane_base + C::kOCol, ov);
+          tc_wait_st();
+        }
+        fence_proxy_async_smem();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[b]);
+      }
+      if (!ok) {
+        if (p.part_stride > 0 && quarter == 0 && real) p.part_ml[part_row(out_row)] = make_float2(0.0f, 0.0f);
+        break;
+      }
+      if (!look_ahead()) { ok = false; break; }
+      if (n_tiles == 0) {
+        if (p.part_stride > 0 && quarter == 0 && real) p.part_ml[part_row(out_row)] = make_float2(0.0f, 0.0f);     // nothing to merge from this part
+        if (next.n_tiles > 0) stage_queries(next);
+        continue;
+      }
+      float sum = 0.0f;                               // of row `lane`, this warp's keys
+#pragma unroll
+      for (int r = 0; r < N; r += 4) {
+        if (r < rows) {
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) l[r + u] += __shfl_xor_sync(0xffffffffu, l[r + u], o);
+          }
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (lane == r + u) sum = l[r + u];
+        }
+      }
+      float sums[4];
+      publish(exchange, sum);
+      if (next.n_tiles > 0) stage_queries(next);
+      if (!collect(exchange, sums)) { ok = false; break; }
+      ++exchange;
+      base += (uint32_t)n_tiles;
+      slots += 2u * (uint32_t)n_tiles;
+      const uint32_t last = base - 1;
+      if (!mbar_wait(&pv_done[last & 1], (last >> 1) & 1, abort_flag, p.status, kPagedKernelId, 8)) { ok = false; break; }
+      tc_fence_after_sync();
+      const float l_all = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+      const float inv_l = l_all > 0.0f ? 1.0f / l_all : 0.0f;
+      if (p.part_stride > 0 && quarter == 0 && real) p.part_ml[part_row(out_row)] = make_float2(m_run == -INFINITY ? 0.0f : m_run * sl, l_all);
+      if (HD == 128 || quarter < 2) {
+        uint32_t ov[N];
+        if constexpr (N == 16) tmem_ld_32x16(lane_base + C::kOCol, ov);
+        else tmem_ld_32x32(lane_base + C::kOCol, ov);
+        tc_wait_ld();
+#pragma unroll
+        for (int r = 0; r < N; ++r) {
+          if (r < rows) {
+            // 32 neighbouring elements of row r per warp
+            const int row = __shfl_sync(0xffffffffu, out_row, r);
+            const float scale = __shfl_sync(0xffffffffu, inv_l, r);
+            if (p.part_stride > 0) p.part_o[part_row(row) * HD + key_lane] = __uint_as_float(ov[r]);
+            else p.out[(size_t)row * HD + key_lane] = __float2bfloat16(__uint_as_float(ov[r]) * scale);
+          }
+        }
+      }
+      tc_fence_before_sync();
+    }
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, C::kTmemCols);
+  }
+}
+
 // out[row, head, :] = sum_z w_z O_z / sum_z w_z l_z with w_z = 2^(m_z - max m): one warp per (row, head).
 template <int HD>
 __global__ void merge_splits_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml,
@@ -649,9 +1072,35 @@ __global__ void merge_splits_kernel(const float* __restrict__ part_o, const floa
   for (int c = 0; c < kPerLane; ++c) out[out_row * HD + c * 32 + lane] = __float2bfloat16(acc[c] * inv);
 }
 
+// `kernel` on `grid`, with all the shared memory that its CTAs per SM need
+template <typename Kernel>
+static int launch_on(Kernel kernel, bool (&configured)[kMaxDevices], dim3 grid, int smem, const CUtensorMap& map_k,
+                     const CUtensorMap& map_v, const Params& p, bool beside_previous, cudaStream_t stream) {
+  // function attributes belong to a device: set once on each
+  int dev = 0;
+  AJB_CUDA_OK(cudaGetDevice(&dev));
+  if (dev >= kMaxDevices || !configured[dev]) {
+    AJB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    // two CTAs per SM need the whole shared-memory carve-out
+    AJB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+    if (dev < kMaxDevices) configured[dev] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = beside_previous ? 1 : 0;
+  AJB_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, map_k, map_v, p));
+  return 0;
+}
+
 template <int HD>
 static int launch_kernel(const Launch& a, cudaStream_t stream) {
-  using C = Cfg<HD>;
   CUtensorMap map_k, map_v;
   const uint64_t row_pitch = (uint64_t)a.kv_heads * HD * 2;
   int rc = make_tensor_map_3d(&map_k, a.k_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.num_blocks, BLOCK_TOKENS,
@@ -660,43 +1109,27 @@ static int launch_kernel(const Launch& a, cudaStream_t stream) {
   rc = make_tensor_map_3d(&map_v, a.v_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.num_blocks, BLOCK_TOKENS,
                           (uint64_t)a.kv_heads * HD, row_pitch * BLOCK_TOKENS, row_pitch, BLOCK_TOKENS, 64);
   if (rc) return rc;
-  // function attributes belong to a device: set once on each
-  static bool configured[kMaxDevices] = {};
-  int dev = 0;
-  AJB_CUDA_OK(cudaGetDevice(&dev));
-  if (dev >= kMaxDevices || !configured[dev]) {
-    AJB_CUDA_OK(cudaFuncSetAttribute(paged_attention_kernel<HD, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
-    AJB_CUDA_OK(cudaFuncSetAttribute(paged_attention_kernel<HD, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
-    // two CTAs per SM need the whole shared-memory carve-out
-    AJB_CUDA_OK(cudaFuncSetAttribute(paged_attention_kernel<HD, false>, cudaFuncAttributePreferredSharedMemoryCarveout,
-                                     cudaSharedmemCarveoutMaxShared));
-    AJB_CUDA_OK(cudaFuncSetAttribute(paged_attention_kernel<HD, true>, cudaFuncAttributePreferredSharedMemoryCarveout,
-                                     cudaSharedmemCarveoutMaxShared));
-    if (dev < kMaxDevices) configured[dev] = true;
-  }
   Params p;
   p.q = (const __nv_bfloat16*)a.q; p.out = (__nv_bfloat16*)a.out; p.block_tables = (const int*)a.block_tables;
   p.context_lens = (const int*)a.context_lens; p.q_start = (const int*)a.q_start; p.q_pitch = a.q_pitch;
-  p.max_blocks = a.max_blocks; p.heads = a.heads; p.kv_heads = a.kv_heads; p.q_len = a.q_len; p.q_total = a.q_total;
+  p.max_blocks = a.max_blocks; p.heads = a.heads; p.kv_heads = a.kv_heads; p.group = a.heads / a.kv_heads; p.q_len = a.q_len;
+  p.seqs = a.num_seqs; p.chunks = (a.q_total + a.q_len - 1) / a.q_len; p.q_total = a.q_total;
   p.first_key = a.first_key; p.scale = a.scale; p.status = device_status_buffer();
   p.splits = a.splits; p.part_stride = a.part_stride; p.part_base = a.part_base;
   p.part_o = (float*)a.part_o; p.part_ml = (float2*)a.part_ml;
-  const int chunks = (a.q_total + a.q_len - 1) / a.q_len;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.num_seqs, a.kv_heads * chunks, a.splits);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = C::kSmem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = a.beside_previous ? 1 : 0;
-  if ((a.heads / a.kv_heads) * a.q_len <= 32)
-    AJB_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_attention_kernel<HD, true>, map_k, map_v, p));
-  else
-    AJB_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_attention_kernel<HD, false>, map_k, map_v, p));
-  return 0;
+  static bool configured16[kMaxDevices] = {}, configured32[kMaxDevices] = {}, configured[kMaxDevices] = {};
+  const int rows = (a.heads / a.kv_heads) * a.q_len;
+  if (rows <= 32) {
+    const long long ctas = (long long)a.num_seqs * a.kv_heads * p.chunks * a.splits;
+    AJB_REQUIRE(ctas <= 0x7fffffffll, "paged attention: %lld CTAs are too many for one launch", ctas);
+    const dim3 grid((unsigned)ctas);
+    if (rows <= 16)
+      return launch_on(paged_decode_kernel<HD, 16>, configured16, grid, DecodeCfg<HD, 16>::kSmem, map_k, map_v, p, a.beside_previous, stream);
+    return launch_on(paged_decode_kernel<HD, 32>, configured32, grid, DecodeCfg<HD, 32>::kSmem, map_k, map_v, p, a.beside_previous, stream);
+  }
+  AJB_REQUIRE((long long)a.kv_heads * p.chunks <= 65535, "paged attention: %d new tokens per sequence are too many for one launch", a.q_total);
+  return launch_on(paged_attention_kernel<HD>, configured, dim3(a.num_seqs, a.kv_heads * p.chunks, a.splits), Cfg<HD>::kSmem, map_k, map_v, p,
+                   a.beside_previous, stream);
 }
 
 int launch(const Launch& a, int head_dim, cudaStream_t stream) {

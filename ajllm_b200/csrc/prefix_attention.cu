@@ -443,7 +443,6 @@ extern "C" int ajb_shared_prefix_attention(const void* q, const void* k_cache, c
   a.q_len = group * q_len <= 32 ? q_len : min(q_len, prefix::ROWS / group);
   a.first_key = shared; a.scale = scale; a.splits = suffix_parts; a.part_stride = prefix_parts + suffix_parts;
   a.part_base = prefix_parts; a.part_o = part_o; a.part_ml = part_ml; a.beside_previous = shared > 0;
-  AJB_REQUIRE((long long)kv_heads * ((q_len + a.q_len - 1) / a.q_len) <= 65535, "shared prefix attention: q_len %d is too long", q_len);
   int rc = 0;
   if (shared > 0)
     rc = head_dim == 128 ? prefix::launch_prefix<128>(a, shared, prefix_parts, s) : prefix::launch_prefix<64>(a, shared, prefix_parts, s);
