@@ -145,6 +145,34 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   }
 }
 
+// The same wait with its rare part (looking at the clock, giving up) out of line: kernels whose warps walk through a lot
+// of code once per piece of work lose more to instruction fetches than a call costs. Returns the time of the first look
+// at the clock, 0 once the budget is spent.
+static __device__ __noinline__ unsigned long long wait_overdue(unsigned long long since, volatile uint32_t* abort_flag,
+                                                               DeviceStatus* status, int kernel_id, int stage, uint32_t parity) {
+  const unsigned long long now = global_timer_ns();
+  if (since == 0) return now;
+  if (now - since <= kWaitBudgetNs) return since;
+  *abort_flag = 1;
+  if (status != nullptr && atomicCAS(&status[kernel_id].code, 0u, (unsigned)((stage << 8) | (kernel_id + 1))) == 0u) {
+    status[kernel_id].block = blockIdx.x;
+    status[kernel_id].detail0 = parity;
+    status[kernel_id].detail1 = threadIdx.x;
+  }
+  return 0;
+}
+__device__ __forceinline__ bool mbar_wait_compact(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag,
+                                                  DeviceStatus* status, int kernel_id, int stage) {
+  unsigned long long since = 0;
+  uint32_t spins = 0;
+#pragma unroll 1
+  while (!mbar_try_wait(bar, parity)) {
+    if (*abort_flag) return false;
+    if ((++spins & 0x3ff) == 0 && (since = wait_overdue(since, abort_flag, status, kernel_id, stage, parity)) == 0) return false;
+  }
+  return true;
+}
+
 // Swizzled operand tiles need a 1024-byte aligned base. The dynamic shared array is declared with that
 // alignment; should the runtime ever place it elsewhere, the CTA reports it and leaves before touching
 // any barrier or tensor memory. A CTA also leaves at once when an earlier CTA of the same kernel has
@@ -286,7 +314,28 @@ __device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, uint32_t (&r)[32])
       : "r"(taddr)
       : "memory");
 }
-// 32 lanes x 16 consecutive 32-bit columns.
+// 32 lanes x 4, 8 or 16 consecutive 32-bit columns.
+__device__ __forceinline__ void tmem_ld_32x4(uint32_t taddr, uint32_t (&r)[4]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld_32x8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x4(uint32_t taddr, const uint32_t (&r)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "

@@ -89,15 +89,14 @@ struct Params {
   DeviceStatus* status;
 };
 
-// Rows [first, kRows) of a V tile become zero: they belong to no key (the unused end of the last block, or a block fetched
-// again to fill the tile), their probabilities are zero, and zero times whatever an old sequence left there (an
-// infinity, a NaN) must not reach the sums. `t` is the caller's index among the 128 threads that share the work.
+// Rows [first, last) of a V tile of kRows rows become zero: they belong to no key (the unused end of the last block, or a
+// block fetched again to fill the tile), their probabilities are zero, and zero times whatever an old sequence left
+// there (an infinity, a NaN) must not reach the sums. `t` is the caller's index among the threads that share the work.
 template <int HD, int kRows>
-__device__ __forceinline__ void zero_value_rows(uint8_t* tile, int first, int t) {
-  constexpr int kBoxes = HD / 64;
-  for (int i = first * 8 + t; i < kRows * 8; i += 128) {
+__device__ __forceinline__ void zero_value_rows(uint8_t* tile, int first, int last, int t, int threads) {
+  for (int i = first * 8 + t; i < last * 8; i += threads) {
 #pragma unroll
-    for (int b = 0; b < kBoxes; ++b) reinterpret_cast<uint4*>(tile + b * (kRows * 128))[i] = make_uint4(0, 0, 0, 0);
+    for (int b = 0; b < HD / 64; ++b) reinterpret_cast<uint4*>(tile + b * (kRows * 128))[i] = make_uint4(0, 0, 0, 0);
   }
 }
 
@@ -372,7 +371,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       }
       if (ragged_tile == j) {
         if (!mbar_wait(&v_full[s], ((uint32_t)j >> 1) & 1, abort_flag, p.status, kPagedKernelId, 11)) { ok = false; break; }
-        zero_value_rows<HD, TILE>(sKV + s * 2 * C::kTile + C::kTile, keys - (t0 + j) * TILE, quarter * 32 + lane);
+        zero_value_rows<HD, TILE>(sKV + s * 2 * C::kTile + C::kTile, keys - (t0 + j) * TILE, TILE, quarter * 32 + lane, 128);
       }
       if (active && j > 0 && __any_sync(0xffffffffu, moved)) {
 #pragma unroll 1
@@ -512,8 +511,6 @@ struct Work {
     }
     part = z;
   }
-  // the tile that the last key does not fill, if it is this CTA's (always its last one)
-  __device__ __forceinline__ int ragged_tile() const { return (t0 + n_tiles) * DTILE > keys ? n_tiles - 1 : -1; }
   __device__ __forceinline__ void store(int4* to) const {
     to[0] = make_int4(n_tiles, t0, kv_head, rows);
     to[1] = make_int4(token0, ctx, keys, part);
@@ -531,9 +528,29 @@ __device__ __forceinline__ float warp_max_f32(float x) {
   return m;
 }
 
-template <int HD, int N>
-__global__ void __launch_bounds__(kThreads, (DecodeCfg<HD, N>::kCtas))
+template <int R>
+__device__ __forceinline__ void tmem_ld_rows(uint32_t taddr, uint32_t (&r)[R]) {
+  if constexpr (R == 4) tmem_ld_32x4(taddr, r);
+  else if constexpr (R == 8) tmem_ld_32x8(taddr, r);
+  else if constexpr (R == 16) tmem_ld_32x16(taddr, r);
+  else tmem_ld_32x32(taddr, r);
+}
+template <int R>
+__device__ __forceinline__ void tmem_st_rows(uint32_t taddr, const uint32_t (&r)[R]) {
+  if constexpr (R == 4) tmem_st_32x4(taddr, r);
+  else if constexpr (R == 8) tmem_st_32x8(taddr, r);
+  else if constexpr (R == 16) tmem_st_32x16(taddr, r);
+  else tmem_st_32x32(taddr, r);
+}
+
+// R: query rows that the softmax warps work on (the real ones rounded up to 4, 8, 16 or 32; what comes of the others is not
+// used). A piece of work may be a single tile, so a warp walks through most of its code once per piece: the code is kept
+// short (one place for each wait, load and product, rows as a template parameter instead of branches), as instruction
+// fetches cost short contexts more than arithmetic (256 sequences x 32..512 keys: 80 us before, 60 % of the fetches hit).
+template <int HD, int R>
+__global__ void __launch_bounds__(kThreads, (DecodeCfg<HD, (R < 16 ? 16 : R)>::kCtas))
 paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Params p) {
+  constexpr int N = R < 16 ? 16 : R;
   using C = DecodeCfg<HD, N>;
   constexpr int kSlots = C::kSlots;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -560,12 +577,17 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto wait = [&](uint64_t* bar, uint32_t parity, int stage) {
+    return mbar_wait_compact(bar, parity, abort_flag, p.status, kPagedKernelId, stage);
+  };
 
   if (threadIdx.x == 0) {
+#pragma unroll 1
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
+#pragma unroll 1
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&s_free[i], 4);
@@ -589,6 +611,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   if (warp >= 2) {
     // query rows that no piece fills, and their probabilities, stay zero (or an earlier piece's): their columns of the
     // accumulators are never used
+#pragma unroll 1
     for (int i = threadIdx.x - 64; i < (C::kQ + 2 * C::kP) / 16; i += 128) reinterpret_cast<uint4*>(sQ)[i] = make_uint4(0, 0, 0, 0);
     fence_proxy_async_smem();
   }
@@ -604,130 +627,105 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 
   if (warp == 0) {
     // Producer. The block ids of four tiles (32 blocks) are fetched by the 32 lanes with one coalesced load, a group
-    // ahead of their use, and handed to the issuing lane by shuffles: a dependent table lookup per block in front of
-    // its copies would cost more than the copies themselves.
+    // ahead of their use; for a tile, each lane then copies one box (a block's 16 tokens x 64 elements).
     constexpr int kBlocksPerTile = DTILE / BLOCK_TOKENS;
     constexpr int kTilesPerGroup = 32 / kBlocksPerTile;
+    constexpr int kBoxes = HD / 64;
     const int first_block = p.first_key / BLOCK_TOKENS, table_end = p.max_blocks - 1;
+    const int my_block = lane / kBoxes, my_box = lane % kBoxes;
     // The KV heads of a sequence are neighbours in the grid: their rows of a cache block are neighbours in memory, and
     // they are read at about the same time.
     const int columns = p.kv_heads * p.chunks;
-    int seq, y, z;
-    auto place = [&](int cta) {
-      const int rest = cta / columns;
-      y = cta - rest * columns;
-      z = 0;
-      seq = rest;
-      if (p.splits > 1) { z = rest / p.seqs; seq = rest - z * p.seqs; }
-    };
-    place(blockIdx.x);
-    int context = p.context_lens[seq], first_token = p.q_start != nullptr ? p.q_start[seq] : seq * p.q_total;
+    int cta = blockIdx.x, ids_next = 0;
     bool ok = true, asked = false;
-    uint32_t asked_phase = 0;
     uint32_t base = 0;                                // tiles of all pieces before this one, K and V counted
-    auto announce = [&](uint32_t piece, const Work& what) {
+    uint32_t piece = 0;
+#pragma unroll 1
+    for (; ok; ++piece) {
+      // ---- what the piece is
+      Work w;
+      int seq = 0;
+      if (cta >= 0) {
+        const int rest = cta / columns;
+        int z = 0;
+        seq = rest;
+        if (p.splits > 1) { z = rest / p.seqs; seq = rest - z * p.seqs; }
+        // a single part starts at tile 0 whatever the context is: its ids need not wait for the length
+        const int context = p.context_lens[seq], first_token = p.q_start != nullptr ? p.q_start[seq] : seq * p.q_total;
+        if (p.splits == 1) ids_next = p.block_tables[(size_t)seq * p.max_blocks + min(table_end, first_block + lane)];
+        w = Work(p, cta - rest * columns, z, context, first_token);
+      } else {
+        w.n_tiles = -1;
+      }
       if (lane == 0) {
-        ok = mbar_wait(&w_empty[piece & 1], ((piece >> 1) & 1) ^ 1, abort_flag, p.status, kPagedKernelId, 12);
+        ok = wait(&w_empty[piece & 1], ((piece >> 1) & 1) ^ 1, 12);
         if (ok) {
-          what.store(announced + 2 * (piece & 1));
+          w.store(announced + 2 * (piece & 1));
           mbar_arrive(&w_full[piece & 1]);
         }
       }
       ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-    };
-    Work w(p, y, z, context, first_token);
-    announce(0, w);
-    // ids are read up to the end of the table's row; those past the sequence's last block are not used
-    auto fetch_ids = [&](int t0, int g) {
-      return p.block_tables[(size_t)seq * p.max_blocks + min(table_end, first_block + (t0 + g * kTilesPerGroup) * kBlocksPerTile + lane)];
-    };
-    bool more = true;
-    int ids_next = 0;
-    for (uint32_t piece = 0; ok && more; ++piece) {
       const int n_tiles = w.n_tiles;
-      const int blocks = (w.keys + BLOCK_TOKENS - 1) / BLOCK_TOKENS;
-      if (piece == 0 && n_tiles > 0) ids_next = fetch_ids(w.t0, 0);
-      // tile j of K or V as its number `number`; only the blocks that hold keys are fetched
-      auto load = [&](int j, int number, int ids, const CUtensorMap* map, int stage_id) {
-        int id[kBlocksPerTile];
-#pragma unroll
-        for (int b = 0; b < kBlocksPerTile; ++b) id[b] = __shfl_sync(0xffffffffu, ids, (j % kTilesPerGroup) * kBlocksPerTile + b);
-        if (lane == 0 && ok) {
-          const uint32_t g = base + (uint32_t)number;
-          const uint32_t s = g % kSlots;
-          ok = mbar_wait(&empty[s], ((g / kSlots) & 1) ^ 1, abort_flag, p.status, kPagedKernelId, stage_id);
-          if (ok) {
-            const int here = min(kBlocksPerTile, blocks - (w.t0 + j) * kBlocksPerTile);
-            uint8_t* tile = ring + s * C::kTile;
-            mbar_arrive_expect_tx(&full[s], (uint32_t)here * BLOCK_TOKENS * HD * 2);
-#pragma unroll
-            for (int b = 0; b < kBlocksPerTile; ++b) {
-              if (b < here) {
-#pragma unroll
-                for (int i = 0; i < HD / 64; ++i)
-                  tma_load_3d(tile + i * (DTILE * 128) + b * (BLOCK_TOKENS * 128), map, &full[s], w.kv_head * HD + 64 * i, 0, id[b]);
-              }
-            }
-          }
-        }
-        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+      if (!ok || n_tiles < 0) break;
+      // ids are read up to the end of the table's row; those past the sequence's last block are not used
+      auto fetch_ids = [&](int j) {
+        return p.block_tables[(size_t)seq * p.max_blocks + min(table_end, first_block + (w.t0 + j) * kBlocksPerTile + lane)];
       };
-      // The next piece is asked for as the last K tile goes out: its answer takes about a microsecond, and a CTA with a
-      // long piece should not sit on another one.
-      auto ask = [&]() {
-        if (lane == 0) {
+      if (p.splits > 1 && n_tiles > 0) ids_next = fetch_ids(0);
+      const int blocks = (w.keys + BLOCK_TOKENS - 1) / BLOCK_TOKENS - w.t0 * kBlocksPerTile;
+      // ---- its tiles, and meanwhile the next piece: asked for as the last K tile goes out (the answer takes about a
+      // microsecond, and a CTA with a long piece should not sit on another one)
+      int ids_k = 0, ids_prev = 0;                    // block ids of the last K tile's group of four tiles, and of the one before
+      const int ask_at = n_tiles > 1 ? 2 * n_tiles - 3 : 0;
+#pragma unroll 1
+      for (int t = 0; t < max(1, 2 * n_tiles) && ok; ++t) {
+        if (t < 2 * n_tiles) {
+          const bool is_k = t == 0 || ((t & 1) && t < 2 * n_tiles - 1);
+          const int j = is_k ? (t + 1) >> 1 : t == 2 * n_tiles - 1 ? n_tiles - 1 : (t >> 1) - 1;
+          if (is_k && j % kTilesPerGroup == 0) {
+            ids_prev = ids_k;
+            ids_k = ids_next;
+            if (j + kTilesPerGroup < n_tiles) ids_next = fetch_ids(j + kTilesPerGroup);
+          }
+          // V of the last tile of a group goes out after K of the next group's first
+          const int ids = !is_k && j % kTilesPerGroup == kTilesPerGroup - 1 && j + 1 < n_tiles ? ids_prev : ids_k;
+          const int id = __shfl_sync(0xffffffffu, ids, (j % kTilesPerGroup) * kBlocksPerTile + my_block % kBlocksPerTile);
+          const uint32_t g = base + (uint32_t)t;
+          const uint32_t s = g % kSlots;
+          const int here = min(kBlocksPerTile, blocks - j * kBlocksPerTile);      // blocks that hold keys
+          if (lane == 0) {
+            ok = wait(&empty[s], ((g / kSlots) & 1) ^ 1, is_k ? 1 : 2);
+            if (ok) mbar_arrive_expect_tx(&full[s], (uint32_t)here * BLOCK_TOKENS * HD * 2);
+          }
+          ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+          if (ok && my_block < here)
+            tma_load_3d(ring + s * C::kTile + my_box * (DTILE * 128) + my_block * (BLOCK_TOKENS * 128), is_k ? &map_k : &map_v, &full[s],
+                        w.kv_head * HD + 64 * my_box, 0, id);
+        }
+        if (t == ask_at && lane == 0 && ok) {
           fence_proxy_async_smem();                   // the answer before has been read
           mbar_arrive_expect_tx(taken, 16);
           launch_take_request(answer, taken);
           asked = true;
-          asked_phase = piece & 1;
         }
-      };
-      int ids_k = ids_next, ids_prev = ids_next, k_group = -1;      // block ids of K's group of tiles and of the one before
-      for (int j = 0; j <= n_tiles && ok; ++j) {
-        if (j < n_tiles) {
-          if (j % kTilesPerGroup == 0) {
-            ids_prev = ids_k;
-            ids_k = ids_next;
-            k_group = j / kTilesPerGroup;
-            if (j + kTilesPerGroup < n_tiles) ids_next = fetch_ids(w.t0, k_group + 1);
-          }
-          load(j, k_number(j), ids_k, &map_k, 1);
-        }
-        if (j == max(0, n_tiles - 1)) ask();
-        if (j >= 1) load(j - 1, v_number(j - 1, n_tiles), (j - 1) / kTilesPerGroup == k_group ? ids_k : ids_prev, &map_v, 2);
       }
-      base += 2u * (uint32_t)n_tiles;
       if (!ok) break;
-      int yes = 0, cta = 0;
+      base += 2u * (uint32_t)n_tiles;
+      cta = -1;
       if (lane == 0) {
-        ok = mbar_wait(taken, piece & 1, abort_flag, p.status, kPagedKernelId, 13);
+        ok = wait(taken, piece & 1, 13);
         if (ok) {
           asked = false;
-          yes = launch_take_answer(answer, cta) ? 1 : 0;
+          if (!launch_take_answer(answer, cta)) cta = -1;
         }
       }
       ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-      more = __shfl_sync(0xffffffffu, yes, 0) != 0;
       cta = __shfl_sync(0xffffffffu, cta, 0);
-      if (!ok) break;
-      if (more) {
-        place(cta);
-        context = p.context_lens[seq];
-        first_token = p.q_start != nullptr ? p.q_start[seq] : seq * p.q_total;
-        // a single part starts at tile 0 whatever the context is: its ids need not wait for the length
-        if (p.splits == 1) ids_next = fetch_ids(0, 0);
-        w = Work(p, y, z, context, first_token);
-        if (p.splits > 1) ids_next = fetch_ids(w.t0, 0);
-      } else {
-        w.n_tiles = -1;
-      }
-      announce(piece + 1, w);
     }
     // after a wait that ran out: the answer may still be on its way into this CTA's shared memory (bounded as well)
     if (lane == 0 && asked) {
       const unsigned long long since = global_timer_ns();
-      while (!mbar_try_wait(taken, asked_phase) && global_timer_ns() - since < kWaitBudgetNs) {}
+      while (!mbar_try_wait(taken, piece & 1) && global_timer_ns() - since < kWaitBudgetNs) {}
     }
   } else if (warp == 1) {
     constexpr uint32_t idesc_s = make_idesc(DTILE, N, 1, false, false);
@@ -738,49 +736,54 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     constexpr uint32_t kSlotStep = C::kTile >> 4;
     bool ok = true;
     uint32_t base = 0, slots = 0, staged = 0;         // steps, ring tiles and pieces with keys before this piece
+#pragma unroll 1
     for (uint32_t piece = 0; ok; ++piece) {
-      if (!mbar_wait(&w_full[piece & 1], (piece >> 1) & 1, abort_flag, p.status, kPagedKernelId, 14)) break;
-      const int n_tiles = announced[2 * (piece & 1)].x;
+      if (!wait(&w_full[piece & 1], (piece >> 1) & 1, 14)) break;
+      Work w;
+      w.load(announced + 2 * (piece & 1));
+      const int n_tiles = w.n_tiles;
       __syncwarp();
       if (lane == 0) mbar_arrive(&w_empty[piece & 1]);
       if (n_tiles < 0) break;
       if (n_tiles == 0) continue;
-      if (!mbar_wait(q_ready, staged & 1, abort_flag, p.status, kPagedKernelId, 15)) break;
+      if (!wait(q_ready, staged & 1, 15)) break;
       ++staged;
-      auto issue_s = [&](int j) -> bool {
-        const uint32_t g = base + (uint32_t)j, t = slots + (uint32_t)k_number(j), slot = t % kSlots;
-        if (!mbar_wait(&full[slot], (t / kSlots) & 1, abort_flag, p.status, kPagedKernelId, 3)) return false;
-        if (!mbar_wait(&s_free[g & 1], ((g >> 1) & 1) ^ 1, abort_flag, p.status, kPagedKernelId, 4)) return false;
-        tc_fence_after_sync();
-        if (lane == 0) {
-          const uint32_t k_km = k_km0 + slot * kSlotStep;
-          const uint32_t d = tmem_base + (g & 1) * N;
-          umma_f16_c<false>(d, desc_at(k_km, 0), desc_at(q_km, 0), idesc_s);
-#pragma unroll
-          for (int k = 1; k < HD / 16; ++k)
-            umma_f16_c<true>(d, desc_at(k_km, k_major_step(k, DTILE * 128)), desc_at(q_km, k_major_step(k, N * 128)), idesc_s);
-          tc_commit(&s_full[g & 1]);
-          tc_commit(&empty[slot]);
-        }
-        __syncwarp();
-        return true;
-      };
-      ok = issue_s(0);
-      for (int j = 0; j < n_tiles && ok; ++j) {
+#pragma unroll 1
+      for (int j = -1; j < n_tiles; ++j) {
         if (j + 1 < n_tiles) {
-          ok = issue_s(j + 1);
-          if (!ok) break;
+          // S^T of step j + 1, before the second product of step j
+          const uint32_t g = base + (uint32_t)(j + 1), t = slots + (uint32_t)k_number(j + 1), slot = t % kSlots;
+          if (!wait(&full[slot], (t / kSlots) & 1, 3) || !wait(&s_free[g & 1], ((g >> 1) & 1) ^ 1, 4)) { ok = false; break; }
+          tc_fence_after_sync();
+          if (lane == 0) {
+            const uint32_t k_km = k_km0 + slot * kSlotStep, d = tmem_base + (g & 1) * N;
+            umma_f16_c<false>(d, desc_at(k_km, 0), desc_at(q_km, 0), idesc_s);
+#pragma unroll
+            for (int k = 1; k < HD / 16; ++k)
+              umma_f16_c<true>(d, desc_at(k_km, k_major_step(k, DTILE * 128)), desc_at(q_km, k_major_step(k, N * 128)), idesc_s);
+            tc_commit(&s_full[g & 1]);
+            tc_commit(&empty[slot]);
+          }
+          __syncwarp();
         }
+        if (j < 0) continue;
         const uint32_t g = base + (uint32_t)j, t = slots + (uint32_t)v_number(j, n_tiles), slot = t % kSlots;
-        if (!mbar_wait(&p_ready[g & 1], (g >> 1) & 1, abort_flag, p.status, kPagedKernelId, 5)) { ok = false; break; }
-        if (!mbar_wait(&full[slot], (t / kSlots) & 1, abort_flag, p.status, kPagedKernelId, 10)) { ok = false; break; }
+        if (!wait(&p_ready[g & 1], (g >> 1) & 1, 5) || !wait(&full[slot], (t / kSlots) & 1, 10)) { ok = false; break; }
+        // Keys of this tile, 16 to a product. The unused end of the last block becomes zero: its probabilities are zero,
+        // and zero times whatever an old sequence left there (an infinity, a NaN) must not reach the sums. Blocks past
+        // that one have not been fetched and are not multiplied.
+        const int keys = min(DTILE, w.keys - (w.t0 + j) * DTILE);
+        if (keys % BLOCK_TOKENS != 0) {
+          zero_value_rows<HD, DTILE>(ring + slot * C::kTile, keys, (keys + BLOCK_TOKENS - 1) / BLOCK_TOKENS * BLOCK_TOKENS, lane, 32);
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
         tc_fence_after_sync();
         if (lane == 0) {
           const uint32_t v_mn = v_mn0 + slot * kSlotStep, p_km = p_km0 + (g & 1) * (uint32_t)(C::kP >> 4);
-          umma_f16(tmem_base + C::kOCol, desc_at(v_mn, 0), desc_at(p_km, 0), idesc_o, j != 0);
-#pragma unroll
-          for (int k = 1; k < DTILE / 16; ++k)
-            umma_f16_c<true>(tmem_base + C::kOCol, desc_at(v_mn, mn_major_step(k)), desc_at(p_km, k_major_step(k, N * 128)), idesc_o);
+#pragma unroll 1
+          for (int k = 0; k * 16 < keys; ++k)
+            umma_f16(tmem_base + C::kOCol, desc_at(v_mn, mn_major_step(k)), desc_at(p_km, k_major_step(k, N * 128)), idesc_o, j != 0 || k != 0);
           tc_commit(&pv_done[g & 1]);
           tc_commit(&empty[slot]);
         }
@@ -795,32 +798,27 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16);
     const float sl = p.scale * kLog2e;
     bool ok = true;
-    // The four warps exchange one value per query row (lane r: row r) through a ring of four slots: `publish` writes
-    // this warp's value of exchange number `x` and arrives, `collect` waits (bounded) until all four have and reads them.
-    // A warp collects exchange x before it publishes x + 1, so the barrier never runs two phases ahead of a waiter.
-    auto publish = [&](uint32_t x, float mine) {
-      sExchange[(x & 3) * 128 + quarter * 32 + lane] = mine;
+    // The four warps exchange one value per query row (lane r: row r) through a ring of four slots: a warp writes its
+    // value of exchange number x and arrives, and waits (bounded) until all four have before it reads them. It does so
+    // before it writes x + 1, so the barrier never runs two phases ahead of a waiter.
+    uint32_t exchange = 0;
+    float* my_exchange = sExchange + quarter * 32 + lane;
+    auto publish = [&](float mine) {
+      my_exchange[(exchange & 3) * 128] = mine;
       __syncwarp();
       if (lane == 0) mbar_arrive(xbar);
     };
-    auto collect = [&](uint32_t x, float (&all)[4]) -> bool {
-      if (!mbar_wait(xbar, x & 1, abort_flag, p.status, kPagedKernelId, 9)) return false;
+    auto collect = [&](float (&all)[4]) -> bool {
+      if (!wait(xbar, exchange & 1, 9)) return false;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) all[q] = sExchange[(x & 3) * 128 + q * 32 + lane];
+      for (int q = 0; q < 4; ++q) all[q] = sExchange[(exchange & 3) * 128 + q * 32 + lane];
+      ++exchange;
       return true;
     };
-    // what has been announced as piece number `piece`
-    auto read_piece = [&](uint32_t piece, Work& to) -> bool {
-      if (!mbar_wait(&w_full[piece & 1], (piece >> 1) & 1, abort_flag, p.status, kPagedKernelId, 14)) return false;
-      to.load(announced + 2 * (piece & 1));
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&w_empty[piece & 1]);
-      return true;
-    };
-    // Query rows of a piece, 16 bytes at a time over the 128 threads: held in registers from the moment the piece is
-    // known, stored when the last tile of the piece before has been handed on. Which rows and pieces of them a thread
-    // moves is the same for every piece of work.
-    constexpr int kChunks = HD / 8, kHeld = N * kChunks / 128;
+    // Query rows of a piece, 16 bytes at a time over the 128 threads: loaded into registers as soon as the piece is known,
+    // stored when the products of the piece before have read theirs. Which of them a thread moves is the same for every
+    // piece.
+    constexpr int kChunks = HD / 8, kHeld = (R * kChunks + 127) / 128;
     uint4 held[kHeld];
     long long held_from[kHeld];
 #pragma unroll
@@ -828,87 +826,47 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       const int r = (key_lane + 128 * u) / kChunks, ch = (key_lane + 128 * u) % kChunks;
       held_from[u] = (r / p.group) * p.q_pitch + (r % p.group) * HD + 8 * ch;
     }
-    auto hold_queries = [&](const Work& w) {
-      const __nv_bfloat16* q = p.q + (size_t)w.token0 * p.q_pitch + (size_t)(w.kv_head * p.group) * HD;
-#pragma unroll
-      for (int u = 0; u < kHeld; ++u)
-        if ((key_lane + 128 * u) / kChunks < w.rows) held[u] = ld_nc_v4(reinterpret_cast<const uint4*>(q + held_from[u]));
-    };
-    auto stage_queries = [&](const Work& w) {         // the products of the piece before have read theirs
-#pragma unroll
-      for (int u = 0; u < kHeld; ++u) {
-        const int r = (key_lane + 128 * u) / kChunks, ch = (key_lane + 128 * u) % kChunks;
-        if (r < w.rows) *reinterpret_cast<uint4*>(sQ + (ch >> 3) * (N * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = held[u];
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_ready);
-    };
-    uint32_t base = 0, slots = 0, exchange = 0;
     // lane r looks after query row r: new token r / group, head r % group of the KV head's group
     const int my_token = lane / p.group, my_head = lane - my_token * p.group;
-    Work next;
-    ok = read_piece(0, next);
-    if (ok && next.n_tiles > 0) {
-      hold_queries(next);
-      stage_queries(next);
-    }
-    for (uint32_t piece = 0; ok && next.n_tiles >= 0; ++piece) {
-      const Work w = next;
-      const int n_tiles = w.n_tiles, rows = w.rows, ragged_tile = w.ragged_tile();
-      const bool real = lane < rows;
-      const int sees_least = w.ctx - (w.rows - 1) / p.group;         // keys that the first new token sees
+    uint32_t base = 0;                                // steps of all pieces before this one
+    Work w;
+    w.n_tiles = -1;                                   // nothing before the first piece
+#pragma unroll 1
+    for (uint32_t piece = 0;; ++piece) {
+      const int n_tiles = w.n_tiles, rows = w.rows;
+      const int sees_least = w.ctx - (rows - 1) / p.group;           // keys that the first new token sees
       const int k_max = min(sees_least + my_token, w.keys) - 1;      // last visible key of row `lane`
-      const int out_row = (w.token0 + my_token) * p.heads + w.kv_head * p.group + my_head;
-      auto look_ahead = [&]() -> bool {
-        if (!read_piece(piece + 1, next)) return false;
-        if (next.n_tiles > 0) hold_queries(next);
-        return true;
-      };
-      auto part_row = [&](int row) { return (size_t)row * p.part_stride + p.part_base + w.part; };
       float m_run = -INFINITY;                        // of row `lane`
-      float l[N];                                     // of every row, this thread's keys only
+      float l[R];                                     // of every row, this thread's keys only
 #pragma unroll
-      for (int r = 0; r < N; ++r) l[r] = 0.0f;
-      for (int j = 0; j < n_tiles && ok; ++j) {
+      for (int r = 0; r < R; ++r) l[r] = 0.0f;
+#pragma unroll 1
+      for (int j = 0; j < n_tiles; ++j) {
         const uint32_t g = base + (uint32_t)j;
         const int b = g & 1;
-        const uint32_t phase = (g >> 1) & 1;
-        if (!mbar_wait(&s_full[b], phase, abort_flag, p.status, kPagedKernelId, 6)) { ok = false; break; }
+        if (!wait(&s_full[b], (g >> 1) & 1, 6)) { ok = false; break; }
         tc_fence_after_sync();
-        uint32_t sv[N];
-        if constexpr (N == 16) tmem_ld_32x16(lane_base + (uint32_t)(b * N), sv);
-        else tmem_ld_32x32(lane_base + (uint32_t)(b * N), sv);
+        uint32_t sv[R];
+        tmem_ld_rows<R>(lane_base + (uint32_t)(b * N), sv);
         tc_wait_ld();
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_free[b]);
-        const int key = (w.t0 + j) * DTILE + key_lane;
-        const bool masked = (w.t0 + j + 1) * DTILE > min(sees_least, w.keys);
-        float mine = -INFINITY;
-        // rows four at a time: their chains of shuffles and exponentials overlap (rows past the last one in a group of
-        // four are computed along; what comes of them is not used)
+        if ((w.t0 + j + 1) * DTILE > min(sees_least, w.keys)) {      // some row does not see the whole tile
+          const int key = (w.t0 + j) * DTILE + key_lane;
 #pragma unroll
-        for (int r = 0; r < N; r += 4) {
-          if (r < rows) {
-            if (masked) {
-#pragma unroll
-              for (int u = 0; u < 4; ++u)
-                if (key > __shfl_sync(0xffffffffu, k_max, r + u)) sv[r + u] = 0xff800000u;     // -inf
-            }
-            float m[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) m[u] = warp_max_f32(__uint_as_float(sv[r + u]));
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-              if (lane == r + u) mine = m[u];
-          }
+          for (int r = 0; r < R; ++r)
+            if (key > __shfl_sync(0xffffffffu, k_max, r)) sv[r] = 0xff800000u;       // -inf
         }
-        if (!real) mine = -INFINITY;
+        float mine = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float m = warp_max_f32(__uint_as_float(sv[r]));
+          if (lane == r) mine = m;
+        }
+        publish(lane < rows ? mine : -INFINITY);
         float part[4];
-        publish(exchange, mine);
-        if (!collect(exchange, part)) { ok = false; break; }
-        ++exchange;
+        if (!collect(part)) { ok = false; break; }
         const float m_tile = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
         // lazy reference maximum (see flash_fwd.cu); every warp sees the same m_tile and decides alike
         const bool moved = (m_tile - m_run) * sl > 8.0f;
@@ -918,113 +876,112 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         const float neg = -m_safe * sl;
         m_run = m_new;
         const bool any_moved = __any_sync(0xffffffffu, moved);
-        // probability tile b was last read by the second product of step g - 2
-        if (g > 1 && !mbar_wait(&pv_done[b], ((g - 2) >> 1) & 1, abort_flag, p.status, kPagedKernelId, 7)) { ok = false; break; }
+        // probability tile b was last read by the second product of step g - 2, and O^T changes scale only when every
+        // product up to step g - 1 has landed
+        if (g > 1 && !wait(&pv_done[b], ((g - 2) >> 1) & 1, 7)) { ok = false; break; }
+        if (any_moved) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) l[r] *= __shfl_sync(0xffffffffu, alpha, r);
+          if (j > 0) {
+            if (!wait(&pv_done[b ^ 1], ((g - 1) >> 1) & 1, 7)) { ok = false; break; }
+            tc_fence_after_sync();
+            uint32_t ov[R];
+            tmem_ld_rows<R>(lane_base + C::kOCol, ov);
+            tc_wait_ld();
+#pragma unroll
+            for (int r = 0; r < R; ++r) ov[r] = __float_as_uint(__uint_as_float(ov[r]) * __shfl_sync(0xffffffffu, alpha, r));
+            tmem_st_rows<R>(lane_base + C::kOCol, ov);
+            tc_wait_st();
+          }
+        }
         // P^T rows are query rows, 64 keys to 128 bytes; two lanes trade so that each stores two keys of one row
         uint8_t* tile_p = sP + b * C::kP + (quarter >> 1) * (N * 128);
         const int pair_key = (quarter & 1) * 32 + (lane & ~1);
 #pragma unroll
-        for (int r = 0; r < N; r += 4) {
-          if (r < rows) {
-            float pr[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) pr[u] = exp2f(fmaf(__uint_as_float(sv[r + u]), sl, __shfl_sync(0xffffffffu, neg, r + u)));
-            if (any_moved) {
-#pragma unroll
-              for (int u = 0; u < 4; ++u) l[r + u] *= __shfl_sync(0xffffffffu, alpha, r + u);
-            }
-#pragma unroll
-            for (int u = 0; u < 4; ++u) l[r + u] += pr[u];
-#pragma unroll
-            for (int u = 0; u < 4; u += 2) {
-              const float other = __shfl_xor_sync(0xffffffffu, (lane & 1) ? pr[u] : pr[u + 1], 1);
-              const int row = r + u + (lane & 1);
-              const uint32_t word = (lane & 1) ? pack_bf16x2(other, pr[u + 1]) : pack_bf16x2(pr[u], other);
-              *reinterpret_cast<uint32_t*>(tile_p + row * 128 + (((pair_key >> 3) ^ (row & 7)) << 4) + (pair_key & 7) * 2) = word;
-            }
-          }
-        }
-        if (ragged_tile == j) {
-          // Rows of the V tile that belong to no key (the unused end of the last block, blocks that were not fetched)
-          // become zero: their probabilities are zero, and zero times whatever lies there (an infinity, a NaN of an old
-          // sequence) must not reach the sums.
-          const uint32_t t = slots + (uint32_t)v_number(j, n_tiles), slot = t % kSlots;
-          if (!mbar_wait(&full[slot], (t / kSlots) & 1, abort_flag, p.status, kPagedKernelId, 11)) { ok = false; break; }
-          zero_value_rows<HD, DTILE>(ring + slot * C::kTile, w.keys - (w.t0 + j) * DTILE, key_lane);
-        }
-        if (j > 0 && any_moved) {
-          // O^T changes scale: every product up to step g - 1 must have landed first
-          if (!mbar_wait(&pv_done[b ^ 1], ((g - 1) >> 1) & 1, abort_flag, p.status, kPagedKernelId, 7)) { ok = false; break; }
-          tc_fence_after_sync();
-          uint32_t ov[N];
-          if constexpr (N == 16) tmem_ld_32x16(lane_base + C::kOCol, ov);
-          else tmem_ld_32x32(lane_base + C::kOCol, ov);
-          tc_wait_ld();
-#pragma unroll
-          for (int r = 0; r < N; ++r) ov[r] = __float_as_uint(__uint_as_float(ov[r]) * __shfl_sync(0xffffffffu, alpha, r));
-          if constexpr (N == 16) tmem_st_32x16(lane_base + C::kOCol, ov);
-          else tmem_st_32x32(lane_base + C::kOCol, ov);
-          tc_wait_st();
+        for (int r = 0; r < R; r += 2) {
+          const float p0 = exp2f(fmaf(__uint_as_float(sv[r]), sl, __shfl_sync(0xffffffffu, neg, r)));
+          const float p1 = exp2f(fmaf(__uint_as_float(sv[r + 1]), sl, __shfl_sync(0xffffffffu, neg, r + 1)));
+          l[r] += p0;
+          l[r + 1] += p1;
+          const float other = __shfl_xor_sync(0xffffffffu, (lane & 1) ? p0 : p1, 1);
+          const int row = r + (lane & 1);
+          *reinterpret_cast<uint32_t*>(tile_p + row * 128 + (((pair_key >> 3) ^ (row & 7)) << 4) + (pair_key & 7) * 2) =
+              (lane & 1) ? pack_bf16x2(other, p1) : pack_bf16x2(p0, other);
         }
         fence_proxy_async_smem();
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_ready[b]);
       }
-      if (!ok) {
-        if (p.part_stride > 0 && quarter == 0 && real) p.part_ml[part_row(out_row)] = make_float2(0.0f, 0.0f);
-        break;
-      }
-      if (!look_ahead()) { ok = false; break; }
-      if (n_tiles == 0) {
-        if (p.part_stride > 0 && quarter == 0 && real) p.part_ml[part_row(out_row)] = make_float2(0.0f, 0.0f);     // nothing to merge from this part
-        if (next.n_tiles > 0) stage_queries(next);
-        continue;
-      }
-      float sum = 0.0f;                               // of row `lane`, this warp's keys
+      // ---- the next piece: its query rows on their way while this one's sums are joined
+      Work next;
+      ok = ok && wait(&w_full[piece & 1], (piece >> 1) & 1, 14);
+      if (ok) {
+        next.load(announced + 2 * (piece & 1));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&w_empty[piece & 1]);
+        if (next.n_tiles > 0) {
+          const __nv_bfloat16* q = p.q + (size_t)next.token0 * p.q_pitch + (size_t)(next.kv_head * p.group) * HD;
 #pragma unroll
-      for (int r = 0; r < N; r += 4) {
-        if (r < rows) {
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) {
-#pragma unroll
-            for (int u = 0; u < 4; ++u) l[r + u] += __shfl_xor_sync(0xffffffffu, l[r + u], o);
-          }
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            if (lane == r + u) sum = l[r + u];
+          for (int u = 0; u < kHeld; ++u)
+            if ((key_lane + 128 * u) / kChunks < next.rows) held[u] = ld_nc_v4(reinterpret_cast<const uint4*>(q + held_from[u]));
         }
       }
-      float sums[4];
-      publish(exchange, sum);
-      if (next.n_tiles > 0) stage_queries(next);
-      if (!collect(exchange, sums)) { ok = false; break; }
-      ++exchange;
-      base += (uint32_t)n_tiles;
-      slots += 2u * (uint32_t)n_tiles;
-      const uint32_t last = base - 1;
-      if (!mbar_wait(&pv_done[last & 1], (last >> 1) & 1, abort_flag, p.status, kPagedKernelId, 8)) { ok = false; break; }
-      tc_fence_after_sync();
-      const float l_all = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-      const float inv_l = l_all > 0.0f ? 1.0f / l_all : 0.0f;
-      if (p.part_stride > 0 && quarter == 0 && real) p.part_ml[part_row(out_row)] = make_float2(m_run == -INFINITY ? 0.0f : m_run * sl, l_all);
-      if (HD == 128 || quarter < 2) {
-        uint32_t ov[N];
-        if constexpr (N == 16) tmem_ld_32x16(lane_base + C::kOCol, ov);
-        else tmem_ld_32x32(lane_base + C::kOCol, ov);
-        tc_wait_ld();
+      const bool real = lane < rows && n_tiles >= 0;
+      const int out_row = (w.token0 + my_token) * p.heads + w.kv_head * p.group + my_head;
+      auto part_row = [&](int row) { return (size_t)row * p.part_stride + p.part_base + w.part; };
+      if (p.part_stride > 0 && quarter == 0 && real && (n_tiles == 0 || !ok)) p.part_ml[part_row(out_row)] = make_float2(0.0f, 0.0f);
+      if (!ok) break;
+      if (n_tiles > 0) {
+        float sum = 0.0f;                             // of row `lane`, this warp's keys
 #pragma unroll
-        for (int r = 0; r < N; ++r) {
-          if (r < rows) {
+        for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          if (lane == r) sum = l[r];
+        publish(sum);
+      }
+      if (next.n_tiles > 0) {
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u) {
+          const int r = (key_lane + 128 * u) / kChunks, ch = (key_lane + 128 * u) % kChunks;
+          if (r < next.rows) *reinterpret_cast<uint4*>(sQ + (ch >> 3) * (N * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = held[u];
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_ready);
+      }
+      // ---- this piece's output
+      if (n_tiles > 0) {
+        float sums[4];
+        base += (uint32_t)n_tiles;
+        if (!collect(sums) || !wait(&pv_done[(base - 1) & 1], ((base - 1) >> 1) & 1, 8)) break;
+        tc_fence_after_sync();
+        const float l_all = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+        const float inv_l = l_all > 0.0f ? 1.0f / l_all : 0.0f;
+        if (p.part_stride > 0 && quarter == 0 && real) p.part_ml[part_row(out_row)] = make_float2(m_run == -INFINITY ? 0.0f : m_run * sl, l_all);
+        if (HD == 128 || quarter < 2) {
+          uint32_t ov[R];
+          tmem_ld_rows<R>(lane_base + C::kOCol, ov);
+          tc_wait_ld();
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
             // 32 neighbouring elements of row r per warp
             const int row = __shfl_sync(0xffffffffu, out_row, r);
             const float scale = __shfl_sync(0xffffffffu, inv_l, r);
-            if (p.part_stride > 0) p.part_o[part_row(row) * HD + key_lane] = __uint_as_float(ov[r]);
-            else p.out[(size_t)row * HD + key_lane] = __float2bfloat16(__uint_as_float(ov[r]) * scale);
+            if (r < rows) {
+              if (p.part_stride > 0) p.part_o[part_row(row) * HD + key_lane] = __uint_as_float(ov[r]);
+              else p.out[(size_t)row * HD + key_lane] = __float2bfloat16(__uint_as_float(ov[r]) * scale);
+            }
           }
         }
+        tc_fence_before_sync();
       }
-      tc_fence_before_sync();
+      if (next.n_tiles < 0) break;
+      w = next;
     }
   }
 
@@ -1117,18 +1074,20 @@ static int launch_kernel(const Launch& a, cudaStream_t stream) {
   p.first_key = a.first_key; p.scale = a.scale; p.status = device_status_buffer();
   p.splits = a.splits; p.part_stride = a.part_stride; p.part_base = a.part_base;
   p.part_o = (float*)a.part_o; p.part_ml = (float2*)a.part_ml;
-  static bool configured16[kMaxDevices] = {}, configured32[kMaxDevices] = {}, configured[kMaxDevices] = {};
+  static bool configured[5][kMaxDevices] = {};
   const int rows = (a.heads / a.kv_heads) * a.q_len;
   if (rows <= 32) {
     const long long ctas = (long long)a.num_seqs * a.kv_heads * p.chunks * a.splits;
     AJB_REQUIRE(ctas <= 0x7fffffffll, "paged attention: %lld CTAs are too many for one launch", ctas);
     const dim3 grid((unsigned)ctas);
-    if (rows <= 16)
-      return launch_on(paged_decode_kernel<HD, 16>, configured16, grid, DecodeCfg<HD, 16>::kSmem, map_k, map_v, p, a.beside_previous, stream);
-    return launch_on(paged_decode_kernel<HD, 32>, configured32, grid, DecodeCfg<HD, 32>::kSmem, map_k, map_v, p, a.beside_previous, stream);
+    const int smem16 = DecodeCfg<HD, 16>::kSmem, smem32 = DecodeCfg<HD, 32>::kSmem;
+    if (rows <= 4) return launch_on(paged_decode_kernel<HD, 4>, configured[0], grid, smem16, map_k, map_v, p, a.beside_previous, stream);
+    if (rows <= 8) return launch_on(paged_decode_kernel<HD, 8>, configured[1], grid, smem16, map_k, map_v, p, a.beside_previous, stream);
+    if (rows <= 16) return launch_on(paged_decode_kernel<HD, 16>, configured[2], grid, smem16, map_k, map_v, p, a.beside_previous, stream);
+    return launch_on(paged_decode_kernel<HD, 32>, configured[3], grid, smem32, map_k, map_v, p, a.beside_previous, stream);
   }
   AJB_REQUIRE((long long)a.kv_heads * p.chunks <= 65535, "paged attention: %d new tokens per sequence are too many for one launch", a.q_total);
-  return launch_on(paged_attention_kernel<HD>, configured, dim3(a.num_seqs, a.kv_heads * p.chunks, a.splits), Cfg<HD>::kSmem, map_k, map_v, p,
+  return launch_on(paged_attention_kernel<HD>, configured[4], dim3(a.num_seqs, a.kv_heads * p.chunks, a.splits), Cfg<HD>::kSmem, map_k, map_v, p,
                    a.beside_previous, stream);
 }
 
