@@ -117,6 +117,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   uint8_t* sP = sQ + C::kQ;
   uint8_t* sKV = sP + C::kP;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + 4 * C::kTile);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (smem_misaligned(smem, p.status, kPagedKernelId, reinterpret_cast<uint32_t*>(bars) + 60)) return;
   // K and V tiles have their own barriers: a K tile is free again after the first product of its step, long before
   // the V tile of the same step, and the issuing warp must never find the next K tile missing when it gets there
@@ -440,6 +441,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     tc_fence_after_sync();
     tmem_dealloc(tmem_base, C::kTmemCols);
   }
+  // a launch that joins the parts waits for this one only: this one does not end before the launch in front of it has
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -559,6 +562,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   uint8_t* sP = sQ + C::kQ;
   float* sExchange = reinterpret_cast<float*>(sP + 2 * C::kP);
   uint64_t* bars = reinterpret_cast<uint64_t*>(sP + 2 * C::kP + C::kExchange);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (smem_misaligned(smem_raw, p.status, kPagedKernelId, reinterpret_cast<uint32_t*>(bars) + 120)) return;
   uint64_t* full = bars;           // kSlots (<= 6)
   uint64_t* empty = bars + 6;      // kSlots
@@ -991,42 +995,80 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     tc_fence_after_sync();
     tmem_dealloc(tmem_base, C::kTmemCols);
   }
+  // a launch that joins the parts waits for this one only: this one does not end before the launch in front of it has
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-// out[row, head, :] = sum_z w_z O_z / sum_z w_z l_z with w_z = 2^(m_z - max m): one warp per (row, head).
+// out[row, head, :] = sum_z w_z O_z / sum_z w_z l_z with w_z = 2^(m_z - max m): one warp per (row, head), HD / 32
+// neighbouring elements per lane. The parts are read at once, before their weights are known: what bounds the kernel is
+// the latency of two dependent reads, not the bytes. It is launched while the launch in front of it still runs and waits
+// for it (and so for everything that one has waited for) on the device.
 template <int HD>
-__global__ void merge_splits_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml,
-                                    __nv_bfloat16* __restrict__ out, const int* __restrict__ q_start, int q_len, int heads,
-                                    int splits, long long pairs /* sequences * q_len * heads */) {
+__global__ void __launch_bounds__(128) merge_splits_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml,
+                                                           __nv_bfloat16* __restrict__ out, const int* __restrict__ q_start, int q_len,
+                                                           int heads, int splits, long long pairs /* sequences * q_len * heads */) {
   const int lane = threadIdx.x & 31;
   const long long w = (blockIdx.x * (long long)blockDim.x + threadIdx.x) >> 5;
   if (w >= pairs) return;
-  const long long local_row = w / heads;
-  const int head = (int)(w - local_row * heads);
-  const int seq = (int)(local_row / q_len), i = (int)(local_row - (long long)seq * q_len);
-  const size_t out_row = (q_start != nullptr ? (size_t)(q_start[seq] + i) : (size_t)local_row) * heads + head;
-  float m_max = -INFINITY;
-  for (int z = 0; z < splits; ++z) {
-    const float2 ml = part_ml[out_row * splits + z];
-    if (ml.y > 0.0f) m_max = fmaxf(m_max, ml.x);
+  size_t out_row = (size_t)w;
+  if (q_start != nullptr) {
+    const long long local_row = w / heads;
+    const int seq = (int)(local_row / q_len);
+    out_row = (size_t)(q_start[seq] + (int)(local_row - (long long)seq * q_len)) * heads + (size_t)(w - local_row * heads);
   }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   constexpr int kPerLane = HD / 32;
+  constexpr int kBatch = 4;
   float acc[kPerLane];
 #pragma unroll
   for (int c = 0; c < kPerLane; ++c) acc[c] = 0.0f;
-  float l_all = 0.0f;
-  for (int z = 0; z < splits; ++z) {
-    const float2 ml = part_ml[out_row * splits + z];
-    if (!(ml.y > 0.0f)) continue;
-    const float weight = exp2f(ml.x - m_max);
-    l_all += weight * ml.y;
-    const float* src = part_o + (out_row * splits + z) * HD;
+  const float* src = part_o + out_row * splits * HD + lane * kPerLane;
+  // lane z: part z (and z + 32: at most 64 parts)
+  const float2* ml = part_ml + out_row * splits;
+  const float2 none = make_float2(0.0f, 0.0f);
+  const float2 a = lane < splits ? __ldcg(ml + lane) : none, b = lane + 32 < splits ? __ldcg(ml + lane + 32) : none;
+  float weight_a = 0.0f, weight_b = 0.0f;
+  bool weighed = false;
+#pragma unroll 1
+  for (int z0 = 0; z0 < splits; z0 += kBatch) {
+    float v[kBatch][kPerLane];
 #pragma unroll
-    for (int c = 0; c < kPerLane; ++c) acc[c] += weight * src[c * 32 + lane];
+    for (int u = 0; u < kBatch; ++u) {
+      if (z0 + u < splits) {
+        if constexpr (kPerLane == 4) *reinterpret_cast<float4*>(v[u]) = __ldcg(reinterpret_cast<const float4*>(src + (size_t)(z0 + u) * HD));
+        else *reinterpret_cast<float2*>(v[u]) = __ldcg(reinterpret_cast<const float2*>(src + (size_t)(z0 + u) * HD));
+      }
+    }
+    if (!weighed) {
+      float m = fmaxf(a.y > 0.0f ? a.x : -INFINITY, b.y > 0.0f ? b.x : -INFINITY);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      weight_a = a.y > 0.0f ? exp2f(a.x - m) : 0.0f;
+      weight_b = b.y > 0.0f ? exp2f(b.x - m) : 0.0f;
+      float l = weight_a * a.y + weight_b * b.y;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      weight_a *= inv;
+      weight_b *= inv;
+      weighed = true;
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      if (z0 + u < splits) {
+        const float weight = __shfl_sync(0xffffffffu, z0 + u < 32 ? weight_a : weight_b, (z0 + u) & 31);
+        // a part that saw no key has a sum of 0 and leaves its row unwritten
+        if (weight != 0.0f) {
+#pragma unroll
+          for (int c = 0; c < kPerLane; ++c) acc[c] += weight * v[u][c];
+        }
+      }
+    }
   }
-  const float inv = l_all > 0.0f ? 1.0f / l_all : 0.0f;
-#pragma unroll
-  for (int c = 0; c < kPerLane; ++c) out[out_row * HD + c * 32 + lane] = __float2bfloat16(acc[c] * inv);
+  if constexpr (kPerLane == 4)
+    *reinterpret_cast<uint2*>(out + out_row * HD + lane * 4) = make_uint2(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]));
+  else
+    *reinterpret_cast<uint32_t*>(out + out_row * HD + lane * 2) = pack_bf16x2(acc[0], acc[1]);
 }
 
 // `kernel` on `grid`, with all the shared memory that its CTAs per SM need
@@ -1101,12 +1143,17 @@ int launch(const Launch& a, int head_dim, cudaStream_t stream) {
 template <int HD>
 static int launch_merge(const Launch& a, cudaStream_t stream) {
   const long long pairs = (long long)a.num_seqs * a.q_total * a.heads;
-  const int threads = 128;
-  const long long blocks = (pairs * 32 + threads - 1) / threads;
-  merge_splits_kernel<HD><<<(unsigned)blocks, threads, 0, stream>>>((const float*)a.part_o, (const float2*)a.part_ml,
-                                                                    (__nv_bfloat16*)a.out, (const int*)a.q_start, a.q_total,
-                                                                    a.heads, a.part_stride, pairs);
-  AJB_CUDA_OK(cudaGetLastError());
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(128);
+  cfg.gridDim = dim3((unsigned)((pairs * 32 + 127) / 128));
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  AJB_CUDA_OK(cudaLaunchKernelEx(&cfg, merge_splits_kernel<HD>, (const float*)a.part_o, (const float2*)a.part_ml, (__nv_bfloat16*)a.out,
+                                 (const int*)a.q_start, a.q_total, a.heads, a.part_stride, pairs));
   return 0;
 }
 

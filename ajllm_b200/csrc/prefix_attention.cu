@@ -161,7 +161,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
       for (int b = 0; b < kBlocksPerTile; ++b) id[b] = __shfl_sync(0xffffffffu, ids, (t % kTilesPerGroup) * kBlocksPerTile + b);
       if (lane == 0 && ok) {
         const int s = t % kStages;
-        ok = mbar_wait(&empty[s], ((uint32_t)(t / kStages) & 1) ^ 1, abort_flag, p.status, kPrefixKernelId, stage_id);
+        ok = mbar_wait_compact(&empty[s], ((uint32_t)(t / kStages) & 1) ^ 1, abort_flag, p.status, kPrefixKernelId, stage_id);
         if (ok) {
           mbar_arrive_expect_tx(&full[s], C::kTile);
 #pragma unroll
@@ -197,7 +197,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
     auto issue_s = [&](int s, int i) -> bool {
       const int t = paired ? i : 2 * i + s, slot = t % kStages;
       // S overwrites P(i - 1): the product that reads it was issued before, and the tensor pipe runs in issue order
-      if (!mbar_wait(&k_full[slot], (uint32_t)(t / kStages) & 1, abort_flag, p.status, kPrefixKernelId, 3)) return false;
+      if (!mbar_wait_compact(&k_full[slot], (uint32_t)(t / kStages) & 1, abort_flag, p.status, kPrefixKernelId, 3)) return false;
       tc_fence_after_sync();
       if (lane == 0) {
         const uint32_t k_km = k_km0 + (uint32_t)slot * kStep, q_km = q_km0 + (paired ? (uint32_t)s * kStep : 0u);
@@ -220,8 +220,8 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
       for (int s = 0; s < 2; ++s) {
         if (i >= steps[s] || !ok) continue;
         const int t = paired ? i : 2 * i + s, slot = t % kStages;
-        if (!mbar_wait(&p_ready[s], (uint32_t)i & 1, abort_flag, p.status, kPrefixKernelId, 4)) { ok = false; break; }
-        if (!mbar_wait(&v_full[slot], (uint32_t)(t / kStages) & 1, abort_flag, p.status, kPrefixKernelId, 5)) { ok = false; break; }
+        if (!mbar_wait_compact(&p_ready[s], (uint32_t)i & 1, abort_flag, p.status, kPrefixKernelId, 4)) { ok = false; break; }
+        if (!mbar_wait_compact(&v_full[slot], (uint32_t)(t / kStages) & 1, abort_flag, p.status, kPrefixKernelId, 5)) { ok = false; break; }
         tc_fence_after_sync();
         if (lane == 0) {
           const uint32_t v_mn = v_mn0 + (uint32_t)slot * kStep;
@@ -249,14 +249,14 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
     float m_run = -INFINITY, l_run = 0.0f;
     bool ok = true;
     for (int j = 0; j < n; ++j) {
-      if (!mbar_wait(&s_full[stream], (uint32_t)j & 1, abort_flag, p.status, kPrefixKernelId, 6)) { ok = false; break; }
+      if (!mbar_wait_compact(&s_full[stream], (uint32_t)j & 1, abort_flag, p.status, kPrefixKernelId, 6)) { ok = false; break; }
       const int t = paired ? j : 2 * j + stream;
       const int left = p.keys - (t0 + t) * TILE;        // keys of this tile; the last tile may have fewer than 128
       if (left < TILE) {
         // the blocks that fill the tile up are copies of the last one: their probabilities are zero, and zero times an
         // infinity must not reach the sums (paired streams both write the same zeros)
         const int slot = t % kStages;
-        if (!mbar_wait(&v_full[slot], (uint32_t)(t / kStages) & 1, abort_flag, p.status, kPrefixKernelId, 9)) { ok = false; break; }
+        if (!mbar_wait_compact(&v_full[slot], (uint32_t)(t / kStages) & 1, abort_flag, p.status, kPrefixKernelId, 9)) { ok = false; break; }
         for (int i = left * 8 + row; i < TILE * 8; i += 128) {
 #pragma unroll
           for (int b = 0; b < HD / 64; ++b)
@@ -306,7 +306,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
         l_run = l_run * alpha + (l2[0] + l2[1]);
         m_run = m_new;
         if (j > 0 && __any_sync(0xffffffffu, moved)) {
-          if (!mbar_wait(&pv_done[stream], (uint32_t)(j - 1) & 1, abort_flag, p.status, kPrefixKernelId, 7)) { ok = false; break; }
+          if (!mbar_wait_compact(&pv_done[stream], (uint32_t)(j - 1) & 1, abort_flag, p.status, kPrefixKernelId, 7)) { ok = false; break; }
           tc_fence_after_sync();
 #pragma unroll 1
           for (int c = 0; c < HD / 32; ++c) {
@@ -331,7 +331,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
     };
     const bool real = row < rows;
     if (real && (n == 0 || !ok)) p.part_ml[part_row(row)] = make_float2(0.0f, 0.0f);       // nothing to join from this part
-    if (ok && active && n > 0 && mbar_wait(&pv_done[stream], (uint32_t)(n - 1) & 1, abort_flag, p.status, kPrefixKernelId, 8)) {
+    if (ok && active && n > 0 && mbar_wait_compact(&pv_done[stream], (uint32_t)(n - 1) & 1, abort_flag, p.status, kPrefixKernelId, 8)) {
       tc_fence_after_sync();
       if (real) p.part_ml[part_row(row)] = make_float2(m_run * sl, l_run);
       // rows leave as 64-byte segments through a padded block of shared memory: four lanes per row, eight rows at a time
