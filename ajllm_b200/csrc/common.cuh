@@ -59,6 +59,11 @@ int make_tensor_map_3d(CUtensorMap* map, const void* base, CUtensorMapDataType d
                        uint64_t d2, uint64_t rows, uint64_t cols, uint64_t d2_pitch_bytes,
                        uint64_t row_pitch_bytes, uint32_t box_rows, uint32_t box_cols);
 
+// The cache of one layer, [num_blocks, 16, kv_heads, hd] bf16, so that one TMA copy fetches the hd columns of one KV head
+// of a block: 8-row groups of the two 64-column halves (one, for hd = 64) side by side, 1024 bytes each, 128-byte
+// swizzle. Coordinates (0, 0, kv_head * hd / 64, 0, block); 32 * hd bytes.
+int make_tensor_map_cache(CUtensorMap* map, const void* base, uint64_t num_blocks, int kv_heads, int hd);
+
 int sm_count();            // SMs a kernel launched by this host thread may fill (the thread's budget, else all)
 int sm_count_physical();   // SMs of the current device
 
@@ -206,6 +211,13 @@ __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* m
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
       ::"r"(smem_u32(smem_dst)), "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_5d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2, int c3,
+                                            int c4) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+      ::"r"(smem_u32(smem_dst)), "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
       : "memory");
 }
 __device__ __forceinline__ void prefetch_tensor_map(const CUtensorMap* map) {
@@ -412,6 +424,20 @@ __device__ __forceinline__ uint32_t desc_lo_mn_major(uint32_t tile_addr, uint32_
 __device__ __forceinline__ uint64_t desc_at(uint32_t lo, uint32_t byte_offset) {
   return (uint64_t(kDescHi) << 32) | (lo + (byte_offset >> 4));
 }
+// The same for tiles of cache blocks (make_tensor_map_cache): 8-row groups are hd * 16 bytes apart, 64-column halves 1024.
+template <int HD>
+__device__ __forceinline__ uint64_t desc_cache(uint32_t lo, uint32_t byte_offset) {
+  constexpr uint32_t hi = ((HD * 16u) >> 4) | (1u << 14) | (2u << 29);
+  return (uint64_t(hi) << 32) | (lo + (byte_offset >> 4));
+}
+// k-step `k` of such a tile: 16 columns of all rows (the K operand), or 16 rows (the V operand, MN-major)
+__host__ __device__ constexpr uint32_t cache_column_step(int k) { return uint32_t(k / 4) * 1024u + uint32_t(k % 4) * 32u; }
+template <int HD>
+__host__ __device__ constexpr uint32_t cache_row_step(int k) { return uint32_t(k) * (2u * HD * 16u); }
+// Byte offset of 16-byte chunk `ch` (of hd / 8) of row `row` in such a tile, before the swizzle
+template <int HD>
+__host__ __device__ constexpr uint32_t cache_row_offset(int row) { return uint32_t(row >> 3) * (HD * 16u) + uint32_t(row & 7) * 128u; }
+
 // Byte offset of k-step `k` (16 elements) inside a K-major tile whose 64-element boxes are `box_bytes` apart.
 __host__ __device__ constexpr uint32_t k_major_step(int k, uint32_t box_bytes) {
   return uint32_t(k / 4) * box_bytes + uint32_t(k % 4) * 32u;

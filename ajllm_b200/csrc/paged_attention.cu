@@ -89,14 +89,14 @@ struct Params {
   DeviceStatus* status;
 };
 
-// Rows [first, last) of a V tile of kRows rows become zero: they belong to no key (the unused end of the last block, or a
-// block fetched again to fill the tile), their probabilities are zero, and zero times whatever an old sequence left
-// there (an infinity, a NaN) must not reach the sums. `t` is the caller's index among the threads that share the work.
-template <int HD, int kRows>
-__device__ __forceinline__ void zero_value_rows(uint8_t* tile, int first, int last, int t, int threads) {
-  for (int i = first * 8 + t; i < last * 8; i += threads) {
+// Rows [first, TILE) of a V tile become zero: they belong to no key (the unused end of the last block, or a block fetched
+// again to fill the tile), their probabilities are zero, and zero times whatever an old sequence left there (an
+// infinity, a NaN) must not reach the sums. `t` is the caller's index among the 128 threads that share the work.
+template <int HD>
+__device__ __forceinline__ void zero_value_rows(uint8_t* tile, int first, int t) {
+  for (int i = first * 8 + t; i < TILE * 8; i += 128) {
 #pragma unroll
-    for (int b = 0; b < HD / 64; ++b) reinterpret_cast<uint4*>(tile + b * (kRows * 128))[i] = make_uint4(0, 0, 0, 0);
+    for (int b = 0; b < HD / 64; ++b) reinterpret_cast<uint4*>(tile + b * (TILE * 128))[i] = make_uint4(0, 0, 0, 0);
   }
 }
 
@@ -372,7 +372,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       }
       if (ragged_tile == j) {
         if (!mbar_wait(&v_full[s], ((uint32_t)j >> 1) & 1, abort_flag, p.status, kPagedKernelId, 11)) { ok = false; break; }
-        zero_value_rows<HD, TILE>(sKV + s * 2 * C::kTile + C::kTile, keys - (t0 + j) * TILE, TILE, quarter * 32 + lane, 128);
+        zero_value_rows<HD>(sKV + s * 2 * C::kTile + C::kTile, keys - (t0 + j) * TILE, quarter * 32 + lane);
       }
       if (active && j > 0 && __any_sync(0xffffffffu, moved)) {
 #pragma unroll 1
@@ -471,11 +471,9 @@ struct DecodeCfg {
   static constexpr int kQ = N * HD * 2;                           // query rows of a piece
   static constexpr int kP = N * DTILE * 2;                        // probabilities of a step; two of them
   static constexpr int kExchange = 4 * 4 * 32 * 4;                // [slot][warp][query row]
-  // 64-wide heads: the product with V^T runs 128 rows high all the same, its second half reads whatever lies behind the
-  // tile (for the last slot: 16 KB behind the ring) into accumulator rows that nobody reads
-  static constexpr int kBehind = kQ + 2 * kP + kExchange + 512;
-  static constexpr int kPad = HD == 64 && kBehind < kTile ? kTile - kBehind : 0;
-  static constexpr int kSmem = kSlots * kTile + kBehind + kPad;
+  // 64-wide heads: the product with V^T runs 128 rows high all the same, its second half reads the next 8-row groups (for
+  // the last one: up to 1 KB behind the ring) into accumulator rows that nobody reads
+  static constexpr int kSmem = kSlots * kTile + kQ + 2 * kP + kExchange + 512;
   // an SM has 228 KB, of which each CTA takes 1 KB more than it asks for
   static_assert(kCtas * (kSmem + 1024) <= 228 * 1024, "shared memory for the CTAs of an SM");
   static constexpr int kOCol = 2 * N;                             // S^T twice, O^T behind them
@@ -631,12 +629,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 
   if (warp == 0) {
     // Producer. The block ids of four tiles (32 blocks) are fetched by the 32 lanes with one coalesced load, a group
-    // ahead of their use; for a tile, each lane then copies one box (a block's 16 tokens x 64 elements).
+    // ahead of their use; for a tile, eight lanes then copy a block each.
     constexpr int kBlocksPerTile = DTILE / BLOCK_TOKENS;
     constexpr int kTilesPerGroup = 32 / kBlocksPerTile;
-    constexpr int kBoxes = HD / 64;
     const int first_block = p.first_key / BLOCK_TOKENS, table_end = p.max_blocks - 1;
-    const int my_block = lane / kBoxes, my_box = lane % kBoxes;
     // The KV heads of a sequence are neighbours in the grid: their rows of a cache block are neighbours in memory, and
     // they are read at about the same time.
     const int columns = p.kv_heads * p.chunks;
@@ -693,7 +689,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           }
           // V of the last tile of a group goes out after K of the next group's first
           const int ids = !is_k && j % kTilesPerGroup == kTilesPerGroup - 1 && j + 1 < n_tiles ? ids_prev : ids_k;
-          const int id = __shfl_sync(0xffffffffu, ids, (j % kTilesPerGroup) * kBlocksPerTile + my_block % kBlocksPerTile);
+          const int id = __shfl_sync(0xffffffffu, ids, (j % kTilesPerGroup) * kBlocksPerTile + lane % kBlocksPerTile);
           const uint32_t g = base + (uint32_t)t;
           const uint32_t s = g % kSlots;
           const int here = min(kBlocksPerTile, blocks - j * kBlocksPerTile);      // blocks that hold keys
@@ -702,9 +698,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             if (ok) mbar_arrive_expect_tx(&full[s], (uint32_t)here * BLOCK_TOKENS * HD * 2);
           }
           ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-          if (ok && my_block < here)
-            tma_load_3d(ring + s * C::kTile + my_box * (DTILE * 128) + my_block * (BLOCK_TOKENS * 128), is_k ? &map_k : &map_v, &full[s],
-                        w.kv_head * HD + 64 * my_box, 0, id);
+          if (ok && lane < here)
+            tma_load_5d(ring + s * C::kTile + lane * (BLOCK_TOKENS * HD * 2), is_k ? &map_k : &map_v, &full[s], 0, 0, w.kv_head * (HD / 64), 0, id);
         }
         if (t == ask_at && lane == 0 && ok) {
           fence_proxy_async_smem();                   // the answer before has been read
@@ -736,7 +731,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     constexpr uint32_t idesc_o = make_idesc(128, N, 1, true, false);
     const uint32_t q_km = desc_lo_k_major(smem_u32(sQ)), p_km0 = desc_lo_k_major(smem_u32(sP));
     const uint32_t k_km0 = desc_lo_k_major(smem_u32(ring));
-    const uint32_t v_mn0 = desc_lo_mn_major(smem_u32(ring), DTILE * 128);
+    const uint32_t v_mn0 = desc_lo_mn_major(smem_u32(ring), 1024);
     constexpr uint32_t kSlotStep = C::kTile >> 4;
     bool ok = true;
     uint32_t base = 0, slots = 0, staged = 0;         // steps, ring tiles and pieces with keys before this piece
@@ -761,10 +756,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           tc_fence_after_sync();
           if (lane == 0) {
             const uint32_t k_km = k_km0 + slot * kSlotStep, d = tmem_base + (g & 1) * N;
-            umma_f16_c<false>(d, desc_at(k_km, 0), desc_at(q_km, 0), idesc_s);
+            umma_f16_c<false>(d, desc_cache<HD>(k_km, 0), desc_at(q_km, 0), idesc_s);
 #pragma unroll
             for (int k = 1; k < HD / 16; ++k)
-              umma_f16_c<true>(d, desc_at(k_km, k_major_step(k, DTILE * 128)), desc_at(q_km, k_major_step(k, N * 128)), idesc_s);
+              umma_f16_c<true>(d, desc_cache<HD>(k_km, cache_column_step(k)), desc_at(q_km, k_major_step(k, N * 128)), idesc_s);
             tc_commit(&s_full[g & 1]);
             tc_commit(&empty[slot]);
           }
@@ -778,7 +773,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         // that one have not been fetched and are not multiplied.
         const int keys = min(DTILE, w.keys - (w.t0 + j) * DTILE);
         if (keys % BLOCK_TOKENS != 0) {
-          zero_value_rows<HD, DTILE>(ring + slot * C::kTile, keys, (keys + BLOCK_TOKENS - 1) / BLOCK_TOKENS * BLOCK_TOKENS, lane, 32);
+          uint8_t* tile = ring + slot * C::kTile;
+          const int rows = BLOCK_TOKENS - keys % BLOCK_TOKENS;
+#pragma unroll 1
+          for (int i = lane; i < rows * (HD / 8); i += 32)      // (row, 64-column half, 16 bytes of 128)
+            *reinterpret_cast<uint4*>(tile + cache_row_offset<HD>(keys + i / (HD / 8)) + (i % (HD / 8)) / 8 * 1024 + i % 8 * 16) = make_uint4(0, 0, 0, 0);
           fence_proxy_async_smem();
           __syncwarp();
         }
@@ -787,7 +786,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           const uint32_t v_mn = v_mn0 + slot * kSlotStep, p_km = p_km0 + (g & 1) * (uint32_t)(C::kP >> 4);
 #pragma unroll 1
           for (int k = 0; k * 16 < keys; ++k)
-            umma_f16(tmem_base + C::kOCol, desc_at(v_mn, mn_major_step(k)), desc_at(p_km, k_major_step(k, N * 128)), idesc_o, j != 0 || k != 0);
+            umma_f16(tmem_base + C::kOCol, desc_cache<HD>(v_mn, cache_row_step<HD>(k)), desc_at(p_km, k_major_step(k, N * 128)), idesc_o, j != 0 || k != 0);
           tc_commit(&pv_done[g & 1]);
           tc_commit(&empty[slot]);
         }
@@ -1100,14 +1099,6 @@ static int launch_on(Kernel kernel, bool (&configured)[kMaxDevices], dim3 grid, 
 
 template <int HD>
 static int launch_kernel(const Launch& a, cudaStream_t stream) {
-  CUtensorMap map_k, map_v;
-  const uint64_t row_pitch = (uint64_t)a.kv_heads * HD * 2;
-  int rc = make_tensor_map_3d(&map_k, a.k_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.num_blocks, BLOCK_TOKENS,
-                              (uint64_t)a.kv_heads * HD, row_pitch * BLOCK_TOKENS, row_pitch, BLOCK_TOKENS, 64);
-  if (rc) return rc;
-  rc = make_tensor_map_3d(&map_v, a.v_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.num_blocks, BLOCK_TOKENS,
-                          (uint64_t)a.kv_heads * HD, row_pitch * BLOCK_TOKENS, row_pitch, BLOCK_TOKENS, 64);
-  if (rc) return rc;
   Params p;
   p.q = (const __nv_bfloat16*)a.q; p.out = (__nv_bfloat16*)a.out; p.block_tables = (const int*)a.block_tables;
   p.context_lens = (const int*)a.context_lens; p.q_start = (const int*)a.q_start; p.q_pitch = a.q_pitch;
@@ -1122,6 +1113,10 @@ static int launch_kernel(const Launch& a, cudaStream_t stream) {
     const long long ctas = (long long)a.num_seqs * a.kv_heads * p.chunks * a.splits;
     AJB_REQUIRE(ctas <= 0x7fffffffll, "paged attention: %lld CTAs are too many for one launch", ctas);
     const dim3 grid((unsigned)ctas);
+    CUtensorMap map_k, map_v;
+    int rc = make_tensor_map_cache(&map_k, a.k_cache, a.num_blocks, a.kv_heads, HD);
+    if (rc == 0) rc = make_tensor_map_cache(&map_v, a.v_cache, a.num_blocks, a.kv_heads, HD);
+    if (rc) return rc;
     const int smem16 = DecodeCfg<HD, 16>::kSmem, smem32 = DecodeCfg<HD, 32>::kSmem;
     if (rows <= 4) return launch_on(paged_decode_kernel<HD, 4>, configured[0], grid, smem16, map_k, map_v, p, a.beside_previous, stream);
     if (rows <= 8) return launch_on(paged_decode_kernel<HD, 8>, configured[1], grid, smem16, map_k, map_v, p, a.beside_previous, stream);
@@ -1129,6 +1124,14 @@ static int launch_kernel(const Launch& a, cudaStream_t stream) {
     return launch_on(paged_decode_kernel<HD, 32>, configured[3], grid, smem32, map_k, map_v, p, a.beside_previous, stream);
   }
   AJB_REQUIRE((long long)a.kv_heads * p.chunks <= 65535, "paged attention: %d new tokens per sequence are too many for one launch", a.q_total);
+  CUtensorMap map_k, map_v;
+  const uint64_t row_pitch = (uint64_t)a.kv_heads * HD * 2;
+  int rc = make_tensor_map_3d(&map_k, a.k_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.num_blocks, BLOCK_TOKENS,
+                              (uint64_t)a.kv_heads * HD, row_pitch * BLOCK_TOKENS, row_pitch, BLOCK_TOKENS, 64);
+  if (rc) return rc;
+  rc = make_tensor_map_3d(&map_v, a.v_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.num_blocks, BLOCK_TOKENS,
+                          (uint64_t)a.kv_heads * HD, row_pitch * BLOCK_TOKENS, row_pitch, BLOCK_TOKENS, 64);
+  if (rc) return rc;
   return launch_on(paged_attention_kernel<HD>, configured[4], dim3(a.num_seqs, a.kv_heads * p.chunks, a.splits), Cfg<HD>::kSmem, map_k, map_v, p,
                    a.beside_previous, stream);
 }

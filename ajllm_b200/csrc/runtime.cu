@@ -144,6 +144,23 @@ int make_tensor_map_3d(CUtensorMap* map, const void* base, CUtensorMapDataType d
   return 0;
 }
 
+int make_tensor_map_cache(CUtensorMap* map, const void* base, uint64_t num_blocks, int kv_heads, int hd) {
+  EncodeTiledFn fn = encode_fn();
+  AJB_REQUIRE(fn != nullptr, "cuTensorMapEncodeTiled is not available from this driver");
+  AJB_REQUIRE((reinterpret_cast<uintptr_t>(base) & 15) == 0, "TMA base address must be 16-byte aligned");
+  const cuuint64_t row = (cuuint64_t)kv_heads * hd * 2;
+  cuuint64_t dims[5] = {64, 8, (cuuint64_t)kv_heads * hd / 64, 2, num_blocks};
+  cuuint64_t strides[4] = {row, 128, 8 * row, 16 * row};
+  cuuint32_t box[5] = {64, 8, (cuuint32_t)hd / 64, 2, 1};
+  cuuint32_t elem_strides[5] = {1, 1, 1, 1, 1};
+  CUresult res = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), dims, strides, box, elem_strides,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  AJB_REQUIRE(res == CUDA_SUCCESS, "cuTensorMapEncodeTiled(cache) failed with code %d (%llu blocks, %d KV heads of %d)", (int)res,
+              (unsigned long long)num_blocks, kv_heads, hd);
+  return 0;
+}
+
 }  // namespace ajb
 
 extern "C" const char* ajb_last_error() { return ajb::last_error(); }
