@@ -754,7 +754,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           const uint32_t g = base + (uint32_t)(j + 1), t = slots + (uint32_t)k_number(j + 1), slot = t % kSlots;
           if (!wait(&full[slot], (t / kSlots) & 1, 3) || !wait(&s_free[g & 1], ((g >> 1) & 1) ^ 1, 4)) { ok = false; break; }
           tc_fence_after_sync();
-          if (lane == 0) {
+          if (elect_one()) {
             const uint32_t k_km = k_km0 + slot * kSlotStep, d = tmem_base + (g & 1) * N;
             umma_f16_c<false>(d, desc_cache<HD>(k_km, 0), desc_at(q_km, 0), idesc_s);
 #pragma unroll
@@ -782,7 +782,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           __syncwarp();
         }
         tc_fence_after_sync();
-        if (lane == 0) {
+        if (elect_one()) {
           const uint32_t v_mn = v_mn0 + slot * kSlotStep, p_km = p_km0 + (g & 1) * (uint32_t)(C::kP >> 4);
 #pragma unroll 1
           for (int k = 0; k * 16 < keys; ++k)

@@ -26,7 +26,7 @@ namespace prefix {
 constexpr int TILE = 128;          // keys per step
 constexpr int ROWS = 128;          // query rows of a stream
 constexpr int BLOCK_TOKENS = 16;   // tokens per cache block
-constexpr int kThreads = 384;      // TMA warp, product warp, two idle, 2 x 4 softmax warps (one per tensor-memory quarter)
+constexpr int kThreads = 576;      // TMA warp, product warp, 16 softmax warps: per stream four tensor-memory quarters x two key halves
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kPrefixKernelId = 12;
 constexpr int kMaxParts = 32;      // parts of the prefix; as many again behind it
@@ -35,18 +35,21 @@ template <int HD>
 struct Cfg {
   static constexpr int kTile = TILE * HD * 2;            // Q, one K tile, one V tile: same size
   static constexpr int kStages = HD == 64 ? 5 : 2;       // K and V tiles held at a time
-  static constexpr int kStagePitch = 20;                 // floats per row of a store block: 16 columns and 16 bytes of padding
+  static constexpr int kStagePitch = 12;                 // floats per row of a store block: 8 columns and 16 bytes of padding
   static constexpr int kStoreBlock = 32 * kStagePitch * 4;
-  static constexpr int kSmem = kTile * (2 + 2 * kStages) + 8 * kStoreBlock + 512;
+  static constexpr int kExchange = 2 * 2 * 2 * ROWS * 4; // [stream][parity][key half][row]
+  static constexpr int kSmem = kTile * (2 + 2 * kStages) + 16 * kStoreBlock + kExchange + 512;
   static constexpr int kOCol = 2 * TILE;                 // S (and P) of stream s at s * 128, O behind them
   static constexpr int kTmemCols = 512;
-  // a CTA of the suffix launch on the same SM would wait for its tensor memory until this one leaves: it must not fit
-  static_assert(kSmem + 64 * HD * 2 * 4 + ROWS * HD * 2 + ROWS * 64 * 2 > 227 * 1024, "a suffix CTA would fit beside");
+  // a CTA of the suffix launch (three or five tiles of 128 keys at least) on the same SM would wait for its tensor memory
+  // until this one leaves: it must not fit
+  static_assert(kSmem <= 227 * 1024 && kSmem + 3 * kTile > 227 * 1024, "shared memory of a prefix CTA");
 };
 
 struct Params {
   const __nv_bfloat16* q;
   const int* table;             // block ids of the prefix
+  float inv_group;
   long long q_pitch;
   int rows;                     // tokens * group: query rows of one KV head
   int group, heads;
@@ -74,7 +77,8 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
   uint8_t* sK = sQ + 2 * C::kTile;
   uint8_t* sV = sK + kStages * C::kTile;
   uint8_t* sStore = sV + kStages * C::kTile;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sStore + 8 * C::kStoreBlock);
+  float* sExchange = reinterpret_cast<float*>(sStore + 16 * C::kStoreBlock);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sStore + 16 * C::kStoreBlock + C::kExchange);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (smem_misaligned(smem, p.status, kPrefixKernelId, reinterpret_cast<uint32_t*>(bars) + 120)) return;
   uint64_t* k_full = bars;               // kStages (<= 5)
@@ -84,10 +88,14 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
   uint64_t* s_full = bars + 20;          // per stream
   uint64_t* p_ready = bars + 22;
   uint64_t* pv_done = bars + 24;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 26);
+  uint64_t* pair_bar = bars + 26;        // per stream and quarter: the two warps that share 32 rows
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 34);
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto wait = [&](uint64_t* bar, uint32_t parity, int stage) {
+    return mbar_wait_compact(bar, parity, abort_flag, p.status, kPrefixKernelId, stage);
+  };
   // row tile pairs of one (KV head, share of the keys) are neighbours: they read the same tiles out of L2
   const bool paired = p.pairs > 0;
   const int pairs = paired ? p.pairs : 1;
@@ -101,20 +109,34 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
   // stream s: its rows, and how many steps it has; step i is tile i (paired) or 2 i + s
   auto row0_of = [&](int s) { return (paired ? 2 * pair + s : 0) * ROWS; };
   auto steps_of = [&](int s) { return paired ? (row0_of(s) < p.rows ? n_tiles : 0) : (n_tiles + 1 - s) / 2; };
-  const int steps[2] = {steps_of(0), steps_of(1)};
+
+  const int group4 = (warp - 2) >> 2;                    // of a softmax warp: four warps, one per tensor-memory quarter
+  const int stream = group4 >> 1, half = group4 & 1;
+  // query row r of a tile (0 .. 127) that starts at head `head0` of token `token0`
+  const int row0 = row0_of(stream & 1), rows = p.rows - row0;      // rows may pass 128: then all of this tile's are real
+  const int token0 = row0 / p.group, head0 = row0 - token0 * p.group;
+  auto row_place = [&](int r, int& token, int& head) {
+    const int t = (int)((float)(head0 + r) * p.inv_group + 0.5f * p.inv_group);       // below 256: exact
+    token = token0 + t;
+    head = head0 + r - t * p.group;
+  };
 
   if (threadIdx.x == 0) {
+#pragma unroll 1
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
       mbar_init(&v_full[i], 1);
       mbar_init(&v_empty[i], 1);
     }
+#pragma unroll 1
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[s], 1);
-      mbar_init(&p_ready[s], 4);
+      mbar_init(&p_ready[s], 8);
       mbar_init(&pv_done[s], 1);
     }
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) mbar_init(&pair_bar[i], 2);
     *abort_flag = 0;
     fence_barrier_init();
     prefetch_tensor_map(&map_k);
@@ -124,165 +146,181 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
     tmem_alloc(tmem_slot, C::kTmemCols);
     tmem_relinquish();
   }
-  const int stream = warp >> 2 == 2 ? 1 : 0;             // of a softmax warp (4..7, 8..11)
-  if (warp >= 4 && (paired || stream == 0)) {
+  if (warp >= 2 && (paired || stream == 0)) {
     // query rows: HD / 8 neighbouring threads per row; rows past the last are zero
-    constexpr int kChunks = HD / 8;
-    const int row0 = row0_of(stream), rows = p.rows - row0;
-#pragma unroll 4
-    for (int i = threadIdx.x & 127; i < ROWS * kChunks; i += 128) {
-      const int r = i / kChunks, ch = i % kChunks;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (r < rows) {
-        const int token = (row0 + r) / p.group, h = (row0 + r) % p.group;
-        v = reinterpret_cast<const uint4*>(p.q + (size_t)token * p.q_pitch + (size_t)(kv_head * p.group + h) * HD)[ch];
-      }
-      store_chunk(sQ + stream * C::kTile, r, ch, v);
+    constexpr int kChunks = HD / 8, kEach = ROWS * kChunks / 256;
+    const int t = (threadIdx.x - 64) & 255;
+    uint4 v[kEach];
+#pragma unroll
+    for (int u = 0; u < kEach; ++u) {
+      const int r = (t + 256 * u) / kChunks, ch = (t + 256 * u) % kChunks;
+      int token, h;
+      row_place(r, token, h);
+      v[u] = make_uint4(0, 0, 0, 0);
+      if (r < rows) v[u] = ld_nc_v4(reinterpret_cast<const uint4*>(p.q + (size_t)token * p.q_pitch + (size_t)(kv_head * p.group + h) * HD) + ch);
     }
+#pragma unroll
+    for (int u = 0; u < kEach; ++u) store_chunk(sQ + stream * C::kTile, (t + 256 * u) / kChunks, (t + 256 * u) % kChunks, v[u]);
     fence_proxy_async_smem();
   }
-  tc_fence_before_sync();
-  __syncthreads();
-  tc_fence_after_sync();
-  const uint32_t tmem_base = *tmem_slot;
+  if (warp != 0) {
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+  }
 
   if (warp == 0) {
-    // block ids: eight per tile, four tiles by the 32 lanes of one coalesced load, a group of tiles ahead. K tiles run
-    // one ahead of V tiles: a K slot is free again long before the V slot of the same tile.
+    // block ids: eight per tile, four tiles by the 32 lanes of one coalesced load, a group of tiles ahead; eight lanes copy
+    // a block of a tile each. K tiles run one ahead of V tiles: a K slot is free again long before the V slot of the same
+    // tile. The first tiles go out before the other warps are let go.
     constexpr int kBlocksPerTile = TILE / BLOCK_TOKENS;
     constexpr int kTilesPerGroup = 32 / kBlocksPerTile;
     const int last_block = p.keys / BLOCK_TOKENS - 1;
+    __syncwarp();
     auto fetch_ids = [&](int g) { return p.table[min(last_block, (t0 + g * kTilesPerGroup) * kBlocksPerTile + lane)]; };
-    int ids_next = n_tiles > 0 ? fetch_ids(0) : 0, ids_k = ids_next, ids_prev = ids_next, k_group = -1;
+    int ids_next = n_tiles > 0 ? fetch_ids(0) : 0, ids_k = ids_next, ids_prev = ids_next;
     bool ok = true;
-    auto load = [&](int t, int ids, uint8_t* ring, uint64_t* full, uint64_t* empty, const CUtensorMap* map, int stage_id) {
-      int id[kBlocksPerTile];
-#pragma unroll
-      for (int b = 0; b < kBlocksPerTile; ++b) id[b] = __shfl_sync(0xffffffffu, ids, (t % kTilesPerGroup) * kBlocksPerTile + b);
-      if (lane == 0 && ok) {
-        const int s = t % kStages;
-        ok = mbar_wait_compact(&empty[s], ((uint32_t)(t / kStages) & 1) ^ 1, abort_flag, p.status, kPrefixKernelId, stage_id);
-        if (ok) {
-          mbar_arrive_expect_tx(&full[s], C::kTile);
-#pragma unroll
-          for (int b = 0; b < kBlocksPerTile; ++b) {
-#pragma unroll
-            for (int i = 0; i < HD / 64; ++i)
-              tma_load_3d(ring + s * C::kTile + i * (TILE * 128) + b * (BLOCK_TOKENS * 128), map, &full[s], kv_head * HD + 64 * i, 0, id[b]);
-          }
-        }
+#pragma unroll 1
+    for (int i = 0; i < 2 * n_tiles + (n_tiles == 0); ++i) {
+      // order K0 K1 V0 K2 V1 ...
+      if (i == 3 || (i == 2 * n_tiles - 1 && i < 3) || n_tiles == 0) {
+        tc_fence_before_sync();
+        __syncthreads();
+        tc_fence_after_sync();
+        if (n_tiles == 0) break;
+      }
+      const bool is_k = i == 0 || ((i & 1) && i < 2 * n_tiles - 1);
+      const int t = is_k ? (i + 1) >> 1 : i == 2 * n_tiles - 1 ? n_tiles - 1 : (i >> 1) - 1;
+      if (is_k && t % kTilesPerGroup == 0) {
+        ids_prev = ids_k;
+        ids_k = ids_next;
+        if (t + kTilesPerGroup < n_tiles) ids_next = fetch_ids(t / kTilesPerGroup + 1);
+      }
+      // V of the last tile of a group goes out after K of the next group's first
+      const int ids = !is_k && t % kTilesPerGroup == kTilesPerGroup - 1 && t + 1 < n_tiles ? ids_prev : ids_k;
+      const int id = __shfl_sync(0xffffffffu, ids, (t % kTilesPerGroup) * kBlocksPerTile + lane % kBlocksPerTile);
+      const int slot = t % kStages;
+      uint64_t* full = (is_k ? k_full : v_full) + slot;
+      if (lane == 0) {
+        ok = wait((is_k ? k_empty : v_empty) + slot, ((uint32_t)(t / kStages) & 1) ^ 1, is_k ? 1 : 2);
+        if (ok) mbar_arrive_expect_tx(full, C::kTile);
       }
       ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-    };
-    for (int t = 0; t <= n_tiles && ok; ++t) {
-      if (t < n_tiles) {
-        if (t % kTilesPerGroup == 0) {
-          ids_prev = ids_k;
-          ids_k = ids_next;
-          k_group = t / kTilesPerGroup;
-          if (t + kTilesPerGroup < n_tiles) ids_next = fetch_ids(k_group + 1);
-        }
-        load(t, ids_k, sK, k_full, k_empty, &map_k, 1);
-      }
-      if (t >= 1) load(t - 1, (t - 1) / kTilesPerGroup == k_group ? ids_k : ids_prev, sV, v_full, v_empty, &map_v, 2);
+      if (!ok) break;
+      if (lane < kBlocksPerTile)
+        tma_load_5d((is_k ? sK : sV) + slot * C::kTile + lane * (BLOCK_TOKENS * HD * 2), is_k ? &map_k : &map_v, full, 0, 0,
+                    kv_head * (HD / 64), 0, id);
     }
   } else if (warp == 1) {
     constexpr uint32_t idesc_s = make_idesc(ROWS, TILE, 1, false, false);
     constexpr uint32_t idesc_o = make_idesc(ROWS, HD, 1, false, true);
+    const uint32_t tmem_base = *tmem_slot;
     const uint32_t q_km0 = desc_lo_k_major(smem_u32(sQ));
     const uint32_t k_km0 = desc_lo_k_major(smem_u32(sK));
-    const uint32_t v_mn0 = desc_lo_mn_major(smem_u32(sV), TILE * 128);
+    const uint32_t v_mn0 = desc_lo_mn_major(smem_u32(sV), 1024);
     constexpr uint32_t kStep = C::kTile >> 4;
-    const bool both = paired && steps[1] > 0;            // both streams use every tile; stream 1 comes second
-    auto issue_s = [&](int s, int i) -> bool {
-      const int t = paired ? i : 2 * i + s, slot = t % kStages;
-      // S overwrites P(i - 1): the product that reads it was issued before, and the tensor pipe runs in issue order
-      if (!mbar_wait_compact(&k_full[slot], (uint32_t)(t / kStages) & 1, abort_flag, p.status, kPrefixKernelId, 3)) return false;
-      tc_fence_after_sync();
-      if (lane == 0) {
-        const uint32_t k_km = k_km0 + (uint32_t)slot * kStep, q_km = q_km0 + (paired ? (uint32_t)s * kStep : 0u);
-        const uint32_t d = tmem_base + (uint32_t)(s * TILE);
-        umma_f16_c<false>(d, desc_at(q_km, 0), desc_at(k_km, 0), idesc_s);
-#pragma unroll
-        for (int k = 1; k < HD / 16; ++k)
-          umma_f16_c<true>(d, desc_at(q_km, k_major_step(k, ROWS * 128)), desc_at(k_km, k_major_step(k, TILE * 128)), idesc_s);
-        tc_commit(&s_full[s]);
-        if (!both || s == 1) tc_commit(&k_empty[slot]);
-      }
-      __syncwarp();
-      return true;
-    };
+    const int steps0 = steps_of(0), steps1 = steps_of(1);          // stream 0 never has fewer
+    const bool both = paired && steps1 > 0;              // both streams use every tile; stream 1 comes second
     bool ok = true;
-    for (int s = 0; s < 2; ++s)
-      if (steps[s] > 0 && ok) ok = issue_s(s, 0);
-    for (int i = 0; i < steps[0] && ok; ++i) {           // stream 0 never has fewer steps than stream 1
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        if (i >= steps[s] || !ok) continue;
-        const int t = paired ? i : 2 * i + s, slot = t % kStages;
-        if (!mbar_wait_compact(&p_ready[s], (uint32_t)i & 1, abort_flag, p.status, kPrefixKernelId, 4)) { ok = false; break; }
-        if (!mbar_wait_compact(&v_full[slot], (uint32_t)(t / kStages) & 1, abort_flag, p.status, kPrefixKernelId, 5)) { ok = false; break; }
+#pragma unroll 1
+    for (int x = 0; x < 2 * (steps0 + 1) && ok; ++x) {
+      // stream s: the second product of step i - 1, then the first one of step i, which overwrites the scores that P(i - 1)
+      // lay over (the tensor pipe runs in issue order)
+      const int s = x & 1, i = x >> 1, steps = s == 0 ? steps0 : steps1;
+      if (i > 0 && i <= steps) {
+        const int t = paired ? i - 1 : 2 * (i - 1) + s, slot = t % kStages;
+        if (!wait(&p_ready[s], (uint32_t)(i - 1) & 1, 4) || !wait(&v_full[slot], (uint32_t)(t / kStages) & 1, 5)) { ok = false; break; }
         tc_fence_after_sync();
-        if (lane == 0) {
+        if (elect_one()) {
           const uint32_t v_mn = v_mn0 + (uint32_t)slot * kStep;
           const uint32_t o = tmem_base + (uint32_t)(C::kOCol + s * HD), pr = tmem_base + (uint32_t)(s * TILE);
-          umma_f16_ts(o, pr, desc_at(v_mn, 0), idesc_o, i != 0);
+          umma_f16_ts(o, pr, desc_cache<HD>(v_mn, 0), idesc_o, i != 1);
 #pragma unroll
-          for (int k = 1; k < TILE / 16; ++k) umma_f16_ts_c<true>(o, pr + (uint32_t)(k * 8), desc_at(v_mn, mn_major_step(k)), idesc_o);
+          for (int k = 1; k < TILE / 16; ++k)            // keys 0..63 in columns [0, 32) of the scores, 64..127 in [64, 96)
+            umma_f16_ts_c<true>(o, pr + (uint32_t)(k < 4 ? k * 8 : 64 + (k - 4) * 8), desc_cache<HD>(v_mn, cache_row_step<HD>(k)), idesc_o);
           tc_commit(&pv_done[s]);
           if (!both || s == 1) tc_commit(&v_empty[slot]);
         }
         __syncwarp();
-        if (i + 1 < steps[s]) ok = issue_s(s, i + 1);
+      }
+      if (i < steps) {
+        const int t = paired ? i : 2 * i + s, slot = t % kStages;
+        if (!wait(&k_full[slot], (uint32_t)(t / kStages) & 1, 3)) { ok = false; break; }
+        tc_fence_after_sync();
+        if (elect_one()) {
+          const uint32_t k_km = k_km0 + (uint32_t)slot * kStep, q_km = q_km0 + (paired ? (uint32_t)s * kStep : 0u);
+          const uint32_t d = tmem_base + (uint32_t)(s * TILE);
+          umma_f16_c<false>(d, desc_at(q_km, 0), desc_cache<HD>(k_km, 0), idesc_s);
+#pragma unroll
+          for (int k = 1; k < HD / 16; ++k)
+            umma_f16_c<true>(d, desc_at(q_km, k_major_step(k, ROWS * 128)), desc_cache<HD>(k_km, cache_column_step(k)), idesc_s);
+          tc_commit(&s_full[s]);
+          if (!both || s == 1) tc_commit(&k_empty[slot]);
+        }
+        __syncwarp();
       }
     }
-  } else if (warp >= 4) {
+  } else {
+    const uint32_t tmem_base = *tmem_slot;
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
-    const int row0 = row0_of(stream), rows = p.rows - row0;      // rows may pass 128: then all of this tile's are real
-    const int n = steps[stream];
+    const int n = steps_of(stream);
     const bool active = quarter * 32 < rows;           // warp-uniform: quarters without query rows only keep the pace
     const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
-    const uint32_t s_col = tmem_base + lane_addr + (uint32_t)(stream * TILE);
-    const uint32_t o_col = tmem_base + lane_addr + (uint32_t)(C::kOCol + stream * HD);
+    const uint32_t s_col = tmem_base + lane_addr + (uint32_t)(stream * TILE + half * 64);
+    const uint32_t o_col = tmem_base + lane_addr + (uint32_t)(C::kOCol + stream * HD + half * (HD / 2));
     const float sl = p.scale * kLog2e;
-    float m_run = -INFINITY, l_run = 0.0f;
+    float m_run = -INFINITY, l_run = 0.0f;             // l_run: this warp's half of the keys only
     bool ok = true;
+    // one float per row, exchanged with the warp that holds the other half of the keys (bounded, like every wait)
+    float* slots = sExchange + stream * (4 * ROWS) + row;
+    auto exchange = [&](uint32_t phase, float mine, float& theirs) -> bool {
+      float* slot = slots + (phase & 1) * (2 * ROWS);
+      slot[half * ROWS] = mine;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&pair_bar[stream * 4 + quarter]);
+      if (!wait(&pair_bar[stream * 4 + quarter], phase & 1, 10)) return false;
+      theirs = slot[(half ^ 1) * ROWS];
+      return true;
+    };
+#pragma unroll 1
     for (int j = 0; j < n; ++j) {
-      if (!mbar_wait_compact(&s_full[stream], (uint32_t)j & 1, abort_flag, p.status, kPrefixKernelId, 6)) { ok = false; break; }
+      if (!wait(&s_full[stream], (uint32_t)j & 1, 6)) { ok = false; break; }
       const int t = paired ? j : 2 * j + stream;
       const int left = p.keys - (t0 + t) * TILE;        // keys of this tile; the last tile may have fewer than 128
       if (left < TILE) {
         // the blocks that fill the tile up are copies of the last one: their probabilities are zero, and zero times an
-        // infinity must not reach the sums (paired streams both write the same zeros)
+        // infinity must not reach the sums (all that wait for the tile write the same zeros)
         const int slot = t % kStages;
-        if (!mbar_wait_compact(&v_full[slot], (uint32_t)(t / kStages) & 1, abort_flag, p.status, kPrefixKernelId, 9)) { ok = false; break; }
-        for (int i = left * 8 + row; i < TILE * 8; i += 128) {
-#pragma unroll
-          for (int b = 0; b < HD / 64; ++b)
-            reinterpret_cast<uint4*>(sV + slot * C::kTile + b * (TILE * 128))[i] = make_uint4(0, 0, 0, 0);
-        }
+        if (!wait(&v_full[slot], (uint32_t)(t / kStages) & 1, 9)) { ok = false; break; }
+#pragma unroll 1
+        for (int i = (half * ROWS + row); i < (TILE - left) * (HD / 8); i += 256)
+          *reinterpret_cast<uint4*>(sV + slot * C::kTile + cache_row_offset<HD>(left + i / (HD / 8)) + (i % (HD / 8)) / 8 * 1024 + i % 8 * 16) =
+              make_uint4(0, 0, 0, 0);
         fence_proxy_async_smem();
       }
       if (active) {
         tc_fence_after_sync();
-        uint32_t sv[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_col + (uint32_t)(c * 32), sv[c]);
+        uint32_t sv[2][32];
+        tmem_ld_32x32(s_col, sv[0]);
+        tmem_ld_32x32(s_col + 32u, sv[1]);
         tc_wait_ld();
         if (left < TILE) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (c * 32 + i >= left) sv[c][i] = 0xff800000u;      // -inf
+              if (half * 64 + c * 32 + i >= left) sv[c][i] = 0xff800000u;      // -inf
         }
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(sv[c][i]));
-        const float m_tile = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        const float m_half = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        float m_other;
+        if (!exchange((uint32_t)j, m_half, m_other)) { ok = false; break; }
+        const float m_tile = fmaxf(m_half, m_other);
         // lazy reference maximum (see flash_fwd.cu): O is rescaled only when a row would pass 2^8
         const bool moved = (m_tile - m_run) * sl > 8.0f;
         const float m_new = moved ? m_tile : m_run;
@@ -291,7 +329,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
         const float neg = -m_safe * sl;
         float l2[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 2; ++c) {
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
@@ -306,16 +344,17 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
         l_run = l_run * alpha + (l2[0] + l2[1]);
         m_run = m_new;
         if (j > 0 && __any_sync(0xffffffffu, moved)) {
-          if (!mbar_wait_compact(&pv_done[stream], (uint32_t)(j - 1) & 1, abort_flag, p.status, kPrefixKernelId, 7)) { ok = false; break; }
+          // each half of the warps rescales half of the head's columns
+          if (!wait(&pv_done[stream], (uint32_t)(j - 1) & 1, 7)) { ok = false; break; }
           tc_fence_after_sync();
 #pragma unroll 1
           for (int c = 0; c < HD / 32; ++c) {
-            uint32_t ov[32];
-            tmem_ld_32x32(o_col + (uint32_t)(c * 32), ov);
+            uint32_t ov[16];
+            tmem_ld_32x16(o_col + (uint32_t)(c * 16), ov);
             tc_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
-            tmem_st_32x32(o_col + (uint32_t)(c * 32), ov);
+            for (int i = 0; i < 16; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
+            tmem_st_32x16(o_col + (uint32_t)(c * 16), ov);
           }
         }
         tc_wait_st();
@@ -326,36 +365,39 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
     }
     const int part = paired ? split : 2 * split + stream;
     auto part_row = [&](int r) {
-      const int token = (row0 + r) / p.group, h = (row0 + r) % p.group;
+      int token, h;
+      row_place(r, token, h);
       return ((size_t)token * p.heads + kv_head * p.group + h) * p.part_stride + part;
     };
-    const bool real = row < rows;
+    float l_other = 0.0f;
+    if (ok && active && n > 0) ok = exchange((uint32_t)n, l_run, l_other);
+    const bool real = row < rows && half == 0;
     if (real && (n == 0 || !ok)) p.part_ml[part_row(row)] = make_float2(0.0f, 0.0f);       // nothing to join from this part
-    if (ok && active && n > 0 && mbar_wait_compact(&pv_done[stream], (uint32_t)(n - 1) & 1, abort_flag, p.status, kPrefixKernelId, 8)) {
+    if (ok && active && n > 0 && wait(&pv_done[stream], (uint32_t)(n - 1) & 1, 8)) {
       tc_fence_after_sync();
-      if (real) p.part_ml[part_row(row)] = make_float2(m_run * sl, l_run);
-      // rows leave as 64-byte segments through a padded block of shared memory: four lanes per row, eight rows at a time
-      float* block = reinterpret_cast<float*>(sStore + (warp - 4) * C::kStoreBlock);
-      const int sub = lane >> 2, piece = lane & 3;
-      float* dst[4];
+      if (real) p.part_ml[part_row(row)] = make_float2(m_run * sl, l_run + l_other);
+      // rows leave as 32-byte segments through a padded block of shared memory: two lanes per row, sixteen rows at a time
+      float* block = reinterpret_cast<float*>(sStore + (warp - 2) * C::kStoreBlock);
+      const int sub = lane >> 1, piece = lane & 1;
+      float* dst[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = quarter * 32 + 8 * i + sub;
-        dst[i] = r < rows ? p.part_o + part_row(r) * HD + 4 * piece : nullptr;
+      for (int i = 0; i < 2; ++i) {
+        const int r = quarter * 32 + 16 * i + sub;
+        dst[i] = r < rows ? p.part_o + part_row(r) * HD + half * (HD / 2) + 4 * piece : nullptr;
       }
 #pragma unroll 1
       for (int c = 0; c < HD / 16; ++c) {
-        uint32_t ov[16];
-        tmem_ld_32x16(o_col + (uint32_t)(c * 16), ov);
+        uint32_t ov[8];
+        tmem_ld_32x8(o_col + (uint32_t)(c * 8), ov);
         tc_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 2; ++i)
           *reinterpret_cast<uint4*>(block + lane * C::kStagePitch + 4 * i) = make_uint4(ov[4 * i], ov[4 * i + 1], ov[4 * i + 2], ov[4 * i + 3]);
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint4 v = *reinterpret_cast<const uint4*>(block + (8 * i + sub) * C::kStagePitch + 4 * piece);
-          if (dst[i] != nullptr) *reinterpret_cast<uint4*>(dst[i] + c * 16) = v;
+        for (int i = 0; i < 2; ++i) {
+          const uint4 v = *reinterpret_cast<const uint4*>(block + (16 * i + sub) * C::kStagePitch + 4 * piece);
+          if (dst[i] != nullptr) *reinterpret_cast<uint4*>(dst[i] + c * 8) = v;
         }
         __syncwarp();
       }
@@ -366,7 +408,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
   __syncthreads();
   if (warp == 1) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem_base, C::kTmemCols);
+    tmem_dealloc(*tmem_slot, C::kTmemCols);
   }
 }
 
@@ -374,12 +416,8 @@ template <int HD>
 static int launch_prefix(const paged::Launch& a, int shared, int parts, cudaStream_t stream) {
   using C = Cfg<HD>;
   CUtensorMap map_k, map_v;
-  const uint64_t row_pitch = (uint64_t)a.kv_heads * HD * 2;
-  int rc = make_tensor_map_3d(&map_k, a.k_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.num_blocks, BLOCK_TOKENS,
-                              (uint64_t)a.kv_heads * HD, row_pitch * BLOCK_TOKENS, row_pitch, BLOCK_TOKENS, 64);
-  if (rc) return rc;
-  rc = make_tensor_map_3d(&map_v, a.v_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.num_blocks, BLOCK_TOKENS,
-                          (uint64_t)a.kv_heads * HD, row_pitch * BLOCK_TOKENS, row_pitch, BLOCK_TOKENS, 64);
+  int rc = make_tensor_map_cache(&map_k, a.k_cache, a.num_blocks, a.kv_heads, HD);
+  if (rc == 0) rc = make_tensor_map_cache(&map_v, a.v_cache, a.num_blocks, a.kv_heads, HD);
   if (rc) return rc;
   static bool configured[kMaxDevices] = {};
   int dev = 0;
@@ -392,7 +430,7 @@ static int launch_prefix(const paged::Launch& a, int shared, int parts, cudaStre
   }
   Params p;
   p.q = (const __nv_bfloat16*)a.q; p.table = (const int*)a.block_tables; p.q_pitch = a.q_pitch;
-  p.group = a.heads / a.kv_heads; p.heads = a.heads; p.rows = a.num_seqs * a.q_total * p.group; p.keys = shared;
+  p.group = a.heads / a.kv_heads; p.inv_group = 1.0f / (float)p.group; p.heads = a.heads; p.rows = a.num_seqs * a.q_total * p.group; p.keys = shared;
   p.pairs = p.rows <= ROWS ? 0 : (p.rows + 2 * ROWS - 1) / (2 * ROWS);
   p.kv_heads = a.kv_heads; p.scale = a.scale;
   p.splits = p.pairs == 0 ? parts / 2 : parts;
