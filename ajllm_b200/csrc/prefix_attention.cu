@@ -221,43 +221,54 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
     constexpr uint32_t kStep = C::kTile >> 4;
     const int steps0 = steps_of(0), steps1 = steps_of(1);          // stream 0 never has fewer
     const bool both = paired && steps1 > 0;              // both streams use every tile; stream 1 comes second
+    // Per round: the second product of stream 0's last step, then the first one of its next, which overwrites the scores
+    // that the probabilities lay over (the tensor pipe runs in issue order), then the same of stream 1. `at` is the ring
+    // slot (and phase) of the tile whose scores come next, `was` of the one whose probabilities do; with the keys divided
+    // over the streams each takes every other tile. What a product needs is known before its wait ends.
+    int at = 0;
+    uint32_t at_phase = 0;
+    int was[2] = {0, 0};
+    uint32_t was_phase[2] = {0, 0};
     bool ok = true;
 #pragma unroll 1
-    for (int x = 0; x < 2 * (steps0 + 1) && ok; ++x) {
-      // stream s: the second product of step i - 1, then the first one of step i, which overwrites the scores that P(i - 1)
-      // lay over (the tensor pipe runs in issue order)
-      const int s = x & 1, i = x >> 1, steps = s == 0 ? steps0 : steps1;
-      if (i > 0 && i <= steps) {
-        const int t = paired ? i - 1 : 2 * (i - 1) + s, slot = t % kStages;
-        if (!wait(&p_ready[s], (uint32_t)(i - 1) & 1, 4) || !wait(&v_full[slot], (uint32_t)(t / kStages) & 1, 5)) { ok = false; break; }
-        tc_fence_after_sync();
-        if (elect_one()) {
-          const uint32_t v_mn = v_mn0 + (uint32_t)slot * kStep;
-          const uint32_t o = tmem_base + (uint32_t)(C::kOCol + s * HD), pr = tmem_base + (uint32_t)(s * TILE);
-          umma_f16_ts(o, pr, desc_cache<HD>(v_mn, 0), idesc_o, i != 1);
+    for (int i = 0; i <= steps0 && ok; ++i) {
 #pragma unroll
-          for (int k = 1; k < TILE / 16; ++k)            // keys 0..63 in columns [0, 32) of the scores, 64..127 in [64, 96)
-            umma_f16_ts_c<true>(o, pr + (uint32_t)(k < 4 ? k * 8 : 64 + (k - 4) * 8), desc_cache<HD>(v_mn, cache_row_step<HD>(k)), idesc_o);
-          tc_commit(&pv_done[s]);
-          if (!both || s == 1) tc_commit(&v_empty[slot]);
-        }
-        __syncwarp();
-      }
-      if (i < steps) {
-        const int t = paired ? i : 2 * i + s, slot = t % kStages;
-        if (!wait(&k_full[slot], (uint32_t)(t / kStages) & 1, 3)) { ok = false; break; }
-        tc_fence_after_sync();
-        if (elect_one()) {
-          const uint32_t k_km = k_km0 + (uint32_t)slot * kStep, q_km = q_km0 + (paired ? (uint32_t)s * kStep : 0u);
-          const uint32_t d = tmem_base + (uint32_t)(s * TILE);
-          umma_f16_c<false>(d, desc_at(q_km, 0), desc_cache<HD>(k_km, 0), idesc_s);
+      for (int s = 0; s < 2; ++s) {
+        const int steps = s == 0 ? steps0 : steps1;
+        const uint32_t d = tmem_base + (uint32_t)(s * TILE), o = tmem_base + (uint32_t)(C::kOCol + s * HD);
+        const bool release = !both || s == 1;
+        const uint32_t q_km = q_km0 + (paired ? (uint32_t)s * kStep : 0u);
+        if (i < steps && !wait(&k_full[at], at_phase, 3)) { ok = false; break; }
+        if (i > 0 && i <= steps) {
+          const uint32_t v_mn = v_mn0 + (uint32_t)was[s] * kStep;
+          if (!wait(&v_full[was[s]], was_phase[s], 5) || !wait(&p_ready[s], (uint32_t)(i - 1) & 1, 4)) { ok = false; break; }
+          tc_fence_after_sync();
+          if (elect_one()) {
+            umma_f16_ts(o, d, desc_cache<HD>(v_mn, 0), idesc_o, i != 1);
 #pragma unroll
-          for (int k = 1; k < HD / 16; ++k)
-            umma_f16_c<true>(d, desc_at(q_km, k_major_step(k, ROWS * 128)), desc_cache<HD>(k_km, cache_column_step(k)), idesc_s);
-          tc_commit(&s_full[s]);
-          if (!both || s == 1) tc_commit(&k_empty[slot]);
+            for (int k = 1; k < TILE / 16; ++k)            // keys 0..63 in columns [0, 32) of the scores, 64..127 in [64, 96)
+              umma_f16_ts_c<true>(o, d + (uint32_t)(k < 4 ? k * 8 : 64 + (k - 4) * 8), desc_cache<HD>(v_mn, cache_row_step<HD>(k)), idesc_o);
+            tc_commit(&pv_done[s]);
+            if (release) tc_commit(&v_empty[was[s]]);
+          }
+          __syncwarp();
         }
-        __syncwarp();
+        if (i < steps) {
+          tc_fence_after_sync();
+          if (elect_one()) {
+            const uint32_t k_km = k_km0 + (uint32_t)at * kStep;
+            umma_f16_c<false>(d, desc_at(q_km, 0), desc_cache<HD>(k_km, 0), idesc_s);
+#pragma unroll
+            for (int k = 1; k < HD / 16; ++k)
+              umma_f16_c<true>(d, desc_at(q_km, k_major_step(k, ROWS * 128)), desc_cache<HD>(k_km, cache_column_step(k)), idesc_s);
+            tc_commit(&s_full[s]);
+            if (release) tc_commit(&k_empty[at]);
+          }
+          __syncwarp();
+          was[s] = at;
+          was_phase[s] = at_phase;
+          if (release && ++at == kStages) { at = 0; at_phase ^= 1; }
+        }
       }
     }
   } else {
