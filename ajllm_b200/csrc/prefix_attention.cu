@@ -12,7 +12,7 @@
 // warps turn one stream's scores into probabilities, the tensor pipe runs the other's products. A 128 x 128 step is two
 // products of 512 cycles and 16384 exponentials, 1024 cycles of the SM's exponential unit, so the two streams keep both
 // about equally busy. The streams are two row tiles that share every K and V tile; when all rows fit one tile they are
-// two halves of the keys instead (even and odd tiles, two parts).
+// two halves of the keys instead (even and odd tiles, two parts; one part when a CTA has a single tile).
 //
 // A prefix CTA has an SM to itself (shared memory), the suffix launch, which does not read what this one writes, starts
 // as soon as every CTA here has and takes the other SMs: the prefix is bound by arithmetic, the suffix by memory, and
@@ -29,7 +29,6 @@ constexpr int BLOCK_TOKENS = 16;   // tokens per cache block
 constexpr int kThreads = 576;      // TMA warp, product warp, 16 softmax warps: per stream four tensor-memory quarters x two key halves
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kPrefixKernelId = 12;
-constexpr int kMaxParts = 32;      // parts of the prefix; as many again behind it
 
 template <int HD>
 struct Cfg {
@@ -374,7 +373,9 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_ready[stream]);
     }
-    const int part = paired ? split : 2 * split + stream;
+    // with one tile per CTA the second stream has nothing to do, and no part
+    const bool lone = !paired && per_split == 1;
+    const int part = paired || lone ? split : 2 * split + stream;
     auto part_row = [&](int r) {
       int token, h;
       row_place(r, token, h);
@@ -382,7 +383,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
     };
     float l_other = 0.0f;
     if (ok && active && n > 0) ok = exchange((uint32_t)n, l_run, l_other);
-    const bool real = row < rows && half == 0;
+    const bool real = row < rows && half == 0 && !(lone && stream == 1);
     if (real && (n == 0 || !ok)) p.part_ml[part_row(row)] = make_float2(0.0f, 0.0f);       // nothing to join from this part
     if (ok && active && n > 0 && wait(&pv_done[stream], (uint32_t)(n - 1) & 1, 8)) {
       tc_fence_after_sync();
@@ -424,7 +425,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
 }
 
 template <int HD>
-static int launch_prefix(const paged::Launch& a, int shared, int parts, cudaStream_t stream) {
+static int launch_prefix(const paged::Launch& a, int shared, int splits, cudaStream_t stream) {
   using C = Cfg<HD>;
   CUtensorMap map_k, map_v;
   int rc = make_tensor_map_cache(&map_k, a.k_cache, a.num_blocks, a.kv_heads, HD);
@@ -444,7 +445,7 @@ static int launch_prefix(const paged::Launch& a, int shared, int parts, cudaStre
   p.group = a.heads / a.kv_heads; p.inv_group = 1.0f / (float)p.group; p.heads = a.heads; p.rows = a.num_seqs * a.q_total * p.group; p.keys = shared;
   p.pairs = p.rows <= ROWS ? 0 : (p.rows + 2 * ROWS - 1) / (2 * ROWS);
   p.kv_heads = a.kv_heads; p.scale = a.scale;
-  p.splits = p.pairs == 0 ? parts / 2 : parts;
+  p.splits = splits;
   p.part_stride = a.part_stride; p.part_o = (float*)a.part_o; p.part_ml = (float2*)a.part_ml;
   p.status = device_status_buffer();
   const long long grid = (long long)(p.pairs == 0 ? 1 : p.pairs) * p.kv_heads * p.splits;
@@ -459,13 +460,15 @@ static int launch_prefix(const paged::Launch& a, int shared, int parts, cudaStre
 
 // q [num_seqs * q_len, heads, head_dim] bf16 with q_pitch elements between tokens, out the same, contiguous; the first
 // `shared` tokens (a multiple of 16; 0: plain paged attention) of every sequence are the ones that the first row of
-// block_tables names.
-// part_o holds num_seqs * q_len * heads * (prefix_parts + suffix_parts) * head_dim floats, part_ml two per part.
+// block_tables names. The prefix is divided over prefix_splits CTAs per (256 query rows, KV head); parts = what they and
+// the suffix launch leave per row: suffix_splits, and prefix_splits more, or twice as many when all query rows of a KV head
+// fit 128 and a CTA has more than one tile of 128 keys. part_o holds num_seqs * q_len * heads * parts * head_dim floats,
+// part_ml two per part.
 extern "C" int ajb_shared_prefix_attention(const void* q, const void* k_cache, const void* v_cache, const void* block_tables,
                                            const void* context_lens, void* out, long long q_pitch, int num_seqs,
                                            int num_blocks, int block_size, int max_blocks, int heads, int kv_heads,
-                                           int head_dim, int q_len, int shared, float scale, int prefix_parts,
-                                           int suffix_parts, void* part_o, void* part_ml, void* stream) {
+                                           int head_dim, int q_len, int shared, float scale, int prefix_splits,
+                                           int suffix_splits, int parts, void* part_o, void* part_ml, void* stream) {
   using namespace ajb;
   AJB_REQUIRE(block_size == prefix::BLOCK_TOKENS, "shared prefix attention: cache block size must be %d", prefix::BLOCK_TOKENS);
   AJB_REQUIRE(head_dim == 64 || head_dim == 128, "shared prefix attention: head_dim %d is not supported (64 and 128 are)", head_dim);
@@ -473,28 +476,30 @@ extern "C" int ajb_shared_prefix_attention(const void* q, const void* k_cache, c
               "shared prefix attention: %d query heads cannot share %d KV heads", heads, kv_heads);
   AJB_REQUIRE(shared >= 0 && shared % prefix::BLOCK_TOKENS == 0 && shared / prefix::BLOCK_TOKENS <= max_blocks,
               "shared prefix attention: %d shared tokens are not whole blocks of the table", shared);
-  const bool one_tile = (long long)num_seqs * q_len * (heads / kv_heads) <= prefix::ROWS;
-  AJB_REQUIRE(!one_tile || prefix_parts % 2 == 0, "shared prefix attention: up to %d query rows per KV head leave their parts in pairs",
-              prefix::ROWS);
-  AJB_REQUIRE((prefix_parts > 0) == (shared > 0) && prefix_parts >= 0 && prefix_parts <= prefix::kMaxParts && suffix_parts >= 1 && suffix_parts <= prefix::kMaxParts &&
-                  part_o != nullptr && part_ml != nullptr,
-              "shared prefix attention: parts must be in [1, %d] (none of a prefix of length 0) and come with a workspace", prefix::kMaxParts);
-  AJB_REQUIRE(q_pitch % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0, "shared prefix attention: query rows must be 16-byte aligned");
   AJB_REQUIRE((long long)num_seqs * q_len * (heads / kv_heads) <= (1ll << 30), "shared prefix attention: too many query rows");
+  const int group = heads / kv_heads, tiles = (shared + prefix::TILE - 1) / prefix::TILE;
+  const bool one_tile = num_seqs * q_len * group <= prefix::ROWS;
+  AJB_REQUIRE((prefix_splits > 0) == (shared > 0) && prefix_splits >= 0 && prefix_splits <= (tiles > 0 ? tiles : 0) &&
+                  suffix_splits >= 1 && part_o != nullptr && part_ml != nullptr,
+              "shared prefix attention: %d and %d divisions of %d shared tokens and of the rest do not fit, or there is no workspace",
+              prefix_splits, suffix_splits, shared);
+  const int prefix_parts = one_tile && prefix_splits < tiles ? 2 * prefix_splits : prefix_splits;
+  AJB_REQUIRE(parts == prefix_parts + suffix_splits && parts <= 64, "shared prefix attention: %d parts per row, not %d", parts,
+              prefix_parts + suffix_splits);
+  AJB_REQUIRE(q_pitch % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0, "shared prefix attention: query rows must be 16-byte aligned");
   if (num_seqs <= 0) return 0;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const int group = heads / kv_heads;
   paged::Launch a;
   a.q = q; a.k_cache = k_cache; a.v_cache = v_cache; a.block_tables = block_tables; a.context_lens = context_lens;
   a.q_start = nullptr; a.out = out; a.q_pitch = q_pitch; a.num_seqs = num_seqs; a.num_blocks = num_blocks;
   a.max_blocks = max_blocks; a.heads = heads; a.kv_heads = kv_heads; a.q_total = q_len;
-  // up to 32 rows the paged kernel works with four replicas of them (cheaper per step); otherwise 128 rows at a time
+  // up to 32 rows run on the paged kernel that puts the keys on the tensor-core rows; otherwise 128 query rows at a time
   a.q_len = group * q_len <= 32 ? q_len : min(q_len, prefix::ROWS / group);
-  a.first_key = shared; a.scale = scale; a.splits = suffix_parts; a.part_stride = prefix_parts + suffix_parts;
+  a.first_key = shared; a.scale = scale; a.splits = suffix_splits; a.part_stride = parts;
   a.part_base = prefix_parts; a.part_o = part_o; a.part_ml = part_ml; a.beside_previous = shared > 0;
   int rc = 0;
   if (shared > 0)
-    rc = head_dim == 128 ? prefix::launch_prefix<128>(a, shared, prefix_parts, s) : prefix::launch_prefix<64>(a, shared, prefix_parts, s);
+    rc = head_dim == 128 ? prefix::launch_prefix<128>(a, shared, prefix_splits, s) : prefix::launch_prefix<64>(a, shared, prefix_splits, s);
   if (rc == 0) rc = paged::launch(a, head_dim, s);
   if (rc == 0) rc = paged::merge_parts(a, head_dim, s);
   return rc;

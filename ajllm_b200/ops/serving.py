@@ -6,6 +6,7 @@ statements of :mod:`ajllm_b200.ops.reference`)."""
 
 from __future__ import annotations
 
+import functools
 import math
 from typing import NamedTuple
 
@@ -84,6 +85,8 @@ def paged_splits(ctas: int, max_context: int) -> int:
     """Parts per sequence for the paged-attention kernel given the (sequence, KV head) pairs of a launch."""
     if not _SM_COUNT:
         _SM_COUNT.append(int(native.lib().ajb_sm_count()))
+    if 5 * ctas >= 4 * _SM_COUNT[0]:       # one each for nearly all SMs: 128 pairs x 4096 keys take 48.5 us whole, 50.5 us in two parts
+        return 1
     want = (2 * _SM_COUNT[0]) // max(1, ctas)
     tiles = max(1, (max_context + 63) // 64)
     # a part should keep enough 64-key steps to amortise its start and the merge kernel: 16 steps when the launch
@@ -239,20 +242,37 @@ def batch_maps(block_ids: torch.Tensor, block_counts: torch.Tensor, cached_lens:
 _PREFIX_TILE = 128         # query rows and keys per step of the prefix kernel
 
 
-def prefix_parts(query_rows: int, kv_heads: int, shared: int, suffix_tiles: int) -> int:
-    """Parts that each row's share of the prefix is cut into. A CTA of the prefix kernel keeps an SM to itself while the
-    others stream the suffixes, so the SMs are divided like the work: a step of 128 keys for up to 256 rows takes about
-    1.5 us of an SM, a 64-key tile of a suffix about 0.8 us. Up to 128 rows a CTA leaves two parts."""
+@functools.lru_cache(maxsize=4096)
+def prefix_plan(rows: int, kv_heads: int, head_dim: int, shared: int, pieces: int, behind: int) -> tuple[int, int]:
+    """``(CTAs that share the prefix per 256 query rows and KV head, parts they leave per row)``.
+
+    A CTA of the prefix kernel keeps an SM to itself while the others stream the ``pieces`` (sequence, KV head) suffixes
+    of up to ``behind`` tokens, so the SMs are divided like the work. Measured beside a running suffix launch: a prefix CTA
+    takes about 14 us and 2 us more per step (128 keys for up to 256 rows; two tiles make a step when 128 rows are all there
+    are), a piece occupies half an SM for 1.3 us and 2.7 us (64-wide heads: 1.3 us) per 128 keys, of which half the bound is
+    taken; a part costs its fp32 rows, written and read once at 4 TB/s. More prefix CTAs than 7 in 10 SMs left the suffix
+    waiting (33 x 5 rows behind 4001 tokens: 28 us with 96 CTAs, 42 us with 144).
+    """
+    if not shared:
+        return 0, 0
     if not _SM_COUNT:
         _SM_COUNT.append(int(native.lib().ajb_sm_count()))
-    one_tile = query_rows <= _PREFIX_TILE
-    units = kv_heads * (1 if one_tile else -(-query_rows // (2 * _PREFIX_TILE)))
+    sms = _SM_COUNT[0]
     tiles = -(-shared // _PREFIX_TILE)
-    steps = -(-tiles // 2) if one_tile else tiles
-    prefix_work, suffix_work = 1.5 * units * steps, 0.8 * suffix_tiles
-    ctas = _SM_COUNT[0] * prefix_work / (prefix_work + suffix_work)
-    parts = max(1, min(round(ctas / units), _SM_COUNT[0] // units, steps, 16))
-    return 2 * parts if one_tile else parts
+    one_tile = rows <= _PREFIX_TILE
+    units = kv_heads * (1 if one_tile else -(-rows // (2 * _PREFIX_TILE)))
+    suffix = pieces * (0.65 + (1.35 if head_dim == 128 else 0.65) * (behind / 256 + 0.5))
+    best = (math.inf, 1, 1)
+    for splits in range(1, min(tiles, 32) + 1):
+        if splits > 1 and 10 * units * splits > 7 * sms:
+            break
+        each = -(-tiles // splits)
+        parts = 2 * splits if one_tile and splits < tiles else splits
+        last = 14.0 + (1.0 if one_tile else 2.0) * each
+        time = max(last, (units * splits * last + suffix) / sms) + parts * rows * kv_heads * head_dim * 8 / 4e6
+        if time < best[0]:
+            best = (time, splits, parts)
+    return best[1], best[2]
 
 
 def shared_prefix_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -313,18 +333,19 @@ def shared_prefix_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cach
     shared = prefix_len // block_size * block_size
     group = heads // kv_heads
     chunk = q_len if group * q_len <= 32 else max(1, min(q_len, _PREFIX_TILE // group))
-    behind = min(max_context if max_context is not None else max_blocks * block_size, max_blocks * block_size) - shared
-    ctas = n * kv_heads * -(-q_len // chunk)
-    splits = paged_splits(ctas, max(0, behind))
-    # lengths are on the device: half the bound is what they are taken to be
-    parts = prefix_parts(total * group, kv_heads, shared, ctas * (behind // 128 + 1)) if shared else 0
+    room = max_blocks * block_size
+    behind = max(0, (room if max_context is None else min(max_context, room)) - shared)
+    pieces = n * kv_heads * -(-q_len // chunk)
+    splits = paged_splits(pieces, behind)
+    prefix_splits, prefix_parts = prefix_plan(total * group, kv_heads, head_dim, shared, pieces, behind)
     # fp32 parts of every (row, head): un-normalised outputs, then (reference maximum, sum) pairs
-    count = total * heads * (parts + splits)
+    parts = prefix_parts + splits
+    count = total * heads * parts
     workspace = torch.empty(count * (head_dim + 2), dtype=torch.float32, device=device)
     native.call("ajb_shared_prefix_attention", q.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
                 context_lens.data_ptr(), out.data_ptr(), q.stride(0), n, num_blocks, block_size, max_blocks, heads, kv_heads,
-                head_dim, q_len, shared, scale, parts, splits, workspace.data_ptr(), workspace.data_ptr() + 4 * count * head_dim,
-                native.stream_ptr())
+                head_dim, q_len, shared, scale, prefix_splits, splits, parts, workspace.data_ptr(),
+                workspace.data_ptr() + 4 * count * head_dim, native.stream_ptr())
     return out
 
 
