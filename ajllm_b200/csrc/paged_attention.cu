@@ -83,6 +83,7 @@ struct Params {
   int first_key;              // first cached token this launch looks at (a multiple of the block size)
   float scale;
   int splits;                 // CTAs per (sequence, KV head, chunk)
+  int prefix_splits;          // CTAs per KV head for the keys in front of first_key (0: not covered), ahead of the others
   int part_stride, part_base; // parts per row in the workspace and the first one of this launch; part_stride 0: no parts
   float* part_o;              // [tokens, Hq, part_stride, hd] fp32, un-normalised
   float2* part_ml;            // [tokens, Hq, part_stride] (reference maximum in log2 units, row sum); sum 0 = no keys seen
@@ -490,7 +491,7 @@ struct Work {
   int token0;           // the first new token
   int ctx;              // keys that the last new token sees; the others see one less each
   int keys;             // keys that there are (the block table bounds them whatever the context length says)
-  int part;
+  int part;             // its place among the parts of a row
   __device__ __forceinline__ Work() {}
   __device__ __forceinline__ Work(const Params& p, int y, int z, int context, int first_token) {
     int chunk = 0;
@@ -510,7 +511,7 @@ struct Work {
       t0 = min(all_tiles, z * per_split);
       n_tiles = min(all_tiles - t0, per_split);
     }
-    part = z;
+    part = p.part_base + z;
   }
   __device__ __forceinline__ void store(int4* to) const {
     to[0] = make_int4(n_tiles, t0, kv_head, rows);
@@ -635,7 +636,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     const int first_block = p.first_key / BLOCK_TOKENS, table_end = p.max_blocks - 1;
     // The KV heads of a sequence are neighbours in the grid: their rows of a cache block are neighbours in memory, and
     // they are read at about the same time.
-    const int columns = p.kv_heads * p.chunks;
+    const int columns = p.kv_heads * p.chunks, prefix_ctas = p.kv_heads * p.prefix_splits;
     int cta = blockIdx.x, ids_next = 0;
     bool ok = true, asked = false;
     uint32_t base = 0;                                // tiles of all pieces before this one, K and V counted
@@ -644,8 +645,21 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     for (; ok; ++piece) {
       // ---- what the piece is
       Work w;
-      int seq = 0;
-      if (cta >= 0) {
+      int seq = 0, from_block = first_block;
+      if (cta >= 0 && cta < prefix_ctas) {
+        // keys that all sequences share, for all their query rows at once
+        from_block = 0;
+        const int split = cta / p.kv_heads, tiles = (p.first_key + DTILE - 1) / DTILE, each = (tiles + p.prefix_splits - 1) / p.prefix_splits;
+        w.kv_head = cta - split * p.kv_heads;
+        w.rows = p.seqs * p.q_total * p.group;
+        w.token0 = 0;
+        w.keys = p.first_key;
+        w.ctx = p.first_key + p.seqs * p.q_total - 1;
+        w.t0 = min(tiles, split * each);
+        w.n_tiles = min(tiles - w.t0, each);
+        w.part = split;
+      } else if (cta >= 0) {
+        cta -= prefix_ctas;
         const int rest = cta / columns;
         int z = 0;
         seq = rest;
@@ -654,6 +668,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         const int context = p.context_lens[seq], first_token = p.q_start != nullptr ? p.q_start[seq] : seq * p.q_total;
         if (p.splits == 1) ids_next = p.block_tables[(size_t)seq * p.max_blocks + min(table_end, first_block + lane)];
         w = Work(p, cta - rest * columns, z, context, first_token);
+        cta += prefix_ctas;
       } else {
         w.n_tiles = -1;
       }
@@ -669,9 +684,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       if (!ok || n_tiles < 0) break;
       // ids are read up to the end of the table's row; those past the sequence's last block are not used
       auto fetch_ids = [&](int j) {
-        return p.block_tables[(size_t)seq * p.max_blocks + min(table_end, first_block + (w.t0 + j) * kBlocksPerTile + lane)];
+        return p.block_tables[(size_t)seq * p.max_blocks + min(table_end, from_block + (w.t0 + j) * kBlocksPerTile + lane)];
       };
-      if (p.splits > 1 && n_tiles > 0) ids_next = fetch_ids(0);
+      if ((p.splits > 1 || cta < prefix_ctas) && n_tiles > 0) ids_next = fetch_ids(0);
       const int blocks = (w.keys + BLOCK_TOKENS - 1) / BLOCK_TOKENS - w.t0 * kBlocksPerTile;
       // ---- its tiles, and meanwhile the next piece: asked for as the last K tile goes out (the answer takes about a
       // microsecond, and a CTA with a long piece should not sit on another one)
@@ -932,7 +947,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       }
       const bool real = lane < rows && n_tiles >= 0;
       const int out_row = (w.token0 + my_token) * p.heads + w.kv_head * p.group + my_head;
-      auto part_row = [&](int row) { return (size_t)row * p.part_stride + p.part_base + w.part; };
+      auto part_row = [&](int row) { return (size_t)row * p.part_stride + w.part; };
       if (p.part_stride > 0 && quarter == 0 && real && (n_tiles == 0 || !ok)) p.part_ml[part_row(out_row)] = make_float2(0.0f, 0.0f);
       if (!ok) break;
       if (n_tiles > 0) {
@@ -1105,24 +1120,30 @@ static int launch_kernel(const Launch& a, cudaStream_t stream) {
   p.max_blocks = a.max_blocks; p.heads = a.heads; p.kv_heads = a.kv_heads; p.group = a.heads / a.kv_heads; p.q_len = a.q_len;
   p.seqs = a.num_seqs; p.chunks = (a.q_total + a.q_len - 1) / a.q_len; p.q_total = a.q_total;
   p.first_key = a.first_key; p.scale = a.scale; p.status = device_status_buffer();
-  p.splits = a.splits; p.part_stride = a.part_stride; p.part_base = a.part_base;
+  p.splits = a.splits; p.prefix_splits = a.prefix_splits; p.part_stride = a.part_stride; p.part_base = a.part_base;
   p.part_o = (float*)a.part_o; p.part_ml = (float2*)a.part_ml;
   static bool configured[5][kMaxDevices] = {};
-  const int rows = (a.heads / a.kv_heads) * a.q_len;
+  const int rows = p.group * (a.prefix_splits > 0 ? a.num_seqs * a.q_total : a.q_len);
   if (rows <= 32) {
-    const long long ctas = (long long)a.num_seqs * a.kv_heads * p.chunks * a.splits;
+    const long long ctas = (long long)a.kv_heads * a.prefix_splits + (long long)a.num_seqs * a.kv_heads * p.chunks * a.splits;
     AJB_REQUIRE(ctas <= 0x7fffffffll, "paged attention: %lld CTAs are too many for one launch", ctas);
     const dim3 grid((unsigned)ctas);
     CUtensorMap map_k, map_v;
-    int rc = make_tensor_map_cache(&map_k, a.k_cache, a.num_blocks, a.kv_heads, HD);
-    if (rc == 0) rc = make_tensor_map_cache(&map_v, a.v_cache, a.num_blocks, a.kv_heads, HD);
-    if (rc) return rc;
+    if (a.map_k != nullptr) {
+      map_k = *a.map_k;
+      map_v = *a.map_v;
+    } else {
+      int rc = make_tensor_map_cache(&map_k, a.k_cache, a.num_blocks, a.kv_heads, HD);
+      if (rc == 0) rc = make_tensor_map_cache(&map_v, a.v_cache, a.num_blocks, a.kv_heads, HD);
+      if (rc) return rc;
+    }
     const int smem16 = DecodeCfg<HD, 16>::kSmem, smem32 = DecodeCfg<HD, 32>::kSmem;
     if (rows <= 4) return launch_on(paged_decode_kernel<HD, 4>, configured[0], grid, smem16, map_k, map_v, p, a.beside_previous, stream);
     if (rows <= 8) return launch_on(paged_decode_kernel<HD, 8>, configured[1], grid, smem16, map_k, map_v, p, a.beside_previous, stream);
     if (rows <= 16) return launch_on(paged_decode_kernel<HD, 16>, configured[2], grid, smem16, map_k, map_v, p, a.beside_previous, stream);
     return launch_on(paged_decode_kernel<HD, 32>, configured[3], grid, smem32, map_k, map_v, p, a.beside_previous, stream);
   }
+  AJB_REQUIRE(a.prefix_splits == 0, "paged attention: a shared prefix for more than 32 query rows per KV head");
   AJB_REQUIRE((long long)a.kv_heads * p.chunks <= 65535, "paged attention: %d new tokens per sequence are too many for one launch", a.q_total);
   CUtensorMap map_k, map_v;
   const uint64_t row_pitch = (uint64_t)a.kv_heads * HD * 2;
@@ -1187,9 +1208,9 @@ extern "C" int ajb_paged_attention(const void* q, const void* k_cache, const voi
   a.q = q; a.k_cache = k_cache; a.v_cache = v_cache; a.block_tables = block_tables; a.context_lens = context_lens;
   a.q_start = q_start; a.out = out; a.q_pitch = (long long)heads * head_dim;
   a.num_seqs = num_seqs; a.num_blocks = num_blocks; a.max_blocks = max_blocks; a.heads = heads; a.kv_heads = kv_heads;
-  a.q_len = q_len; a.q_total = q_len; a.first_key = 0; a.scale = scale; a.splits = splits;
+  a.q_len = q_len; a.q_total = q_len; a.first_key = 0; a.scale = scale; a.splits = splits; a.prefix_splits = 0;
   a.part_stride = splits > 1 ? splits : 0; a.part_base = 0; a.part_o = part_o; a.part_ml = part_ml;
-  a.beside_previous = false;
+  a.map_k = a.map_v = nullptr; a.beside_previous = false;
   int rc = paged::launch(a, head_dim, s);
   if (rc == 0 && splits > 1) rc = paged::merge_parts(a, head_dim, s);
   return rc;

@@ -1,5 +1,6 @@
 // Internal interface of the paged-attention kernel, for operators that combine it with parts of their own.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 namespace ajb {
@@ -16,8 +17,12 @@ struct Launch {
   int first_key;                // cached tokens in front of this one are left out (a multiple of the block size)
   float scale;
   int splits;                   // parts this launch leaves per row
+  int prefix_splits;            // > 0: this launch also covers the keys in front of first_key, the same for all sequences (row 0
+                                // of the tables), divided over that many CTAs per KV head whose parts come first; at most 32
+                                // query rows per KV head in all
   int part_stride, part_base;   // parts per row in the workspace, first one of this launch; stride 0: no parts, `out` is written
   void *part_o, *part_ml;
+  const CUtensorMap *map_k, *map_v;   // of make_tensor_map_cache, when the caller has them already (else null)
   bool beside_previous;         // may start while the launch in front of it still runs (which must have said so)
 };
 

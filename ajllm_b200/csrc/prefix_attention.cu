@@ -14,6 +14,9 @@
 // about equally busy. The streams are two row tiles that share every K and V tile; when all rows fit one tile they are
 // two halves of the keys instead (even and odd tiles, two parts; one part when a CTA has a single tile).
 //
+// Up to 32 query rows per KV head (a few sequences) the prefix runs in the paged launch itself, as more pieces of its work
+// with all query rows at once: one launch less, and products that are as narrow as the rows are few.
+//
 // A prefix CTA has an SM to itself (shared memory), the suffix launch, which does not read what this one writes, starts
 // as soon as every CTA here has and takes the other SMs: the prefix is bound by arithmetic, the suffix by memory, and
 // the number of prefix CTAs divides the SMs so that both last about as long.
@@ -427,10 +430,6 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
 template <int HD>
 static int launch_prefix(const paged::Launch& a, int shared, int splits, cudaStream_t stream) {
   using C = Cfg<HD>;
-  CUtensorMap map_k, map_v;
-  int rc = make_tensor_map_cache(&map_k, a.k_cache, a.num_blocks, a.kv_heads, HD);
-  if (rc == 0) rc = make_tensor_map_cache(&map_v, a.v_cache, a.num_blocks, a.kv_heads, HD);
-  if (rc) return rc;
   static bool configured[kMaxDevices] = {};
   int dev = 0;
   AJB_CUDA_OK(cudaGetDevice(&dev));
@@ -450,7 +449,7 @@ static int launch_prefix(const paged::Launch& a, int shared, int splits, cudaStr
   p.status = device_status_buffer();
   const long long grid = (long long)(p.pairs == 0 ? 1 : p.pairs) * p.kv_heads * p.splits;
   AJB_REQUIRE(grid <= 0x7fffffffll, "shared prefix attention: too many query rows");
-  prefix_attention_kernel<HD><<<(int)grid, kThreads, C::kSmem, stream>>>(map_k, map_v, p);
+  prefix_attention_kernel<HD><<<(int)grid, kThreads, C::kSmem, stream>>>(*a.map_k, *a.map_v, p);
   AJB_CUDA_OK(cudaGetLastError());
   return 0;
 }
@@ -461,8 +460,8 @@ static int launch_prefix(const paged::Launch& a, int shared, int splits, cudaStr
 // q [num_seqs * q_len, heads, head_dim] bf16 with q_pitch elements between tokens, out the same, contiguous; the first
 // `shared` tokens (a multiple of 16; 0: plain paged attention) of every sequence are the ones that the first row of
 // block_tables names. The prefix is divided over prefix_splits CTAs per (256 query rows, KV head); parts = what they and
-// the suffix launch leave per row: suffix_splits, and prefix_splits more, or twice as many when all query rows of a KV head
-// fit 128 and a CTA has more than one tile of 128 keys. part_o holds num_seqs * q_len * heads * parts * head_dim floats,
+// the suffix launch leave per row: suffix_splits, and prefix_splits more, or twice as many when a KV head has 33 to 128 query
+// rows in all and a CTA more than one tile of 128 keys. part_o holds num_seqs * q_len * heads * parts * head_dim floats,
 // part_ml two per part.
 extern "C" int ajb_shared_prefix_attention(const void* q, const void* k_cache, const void* v_cache, const void* block_tables,
                                            const void* context_lens, void* out, long long q_pitch, int num_seqs,
@@ -478,12 +477,13 @@ extern "C" int ajb_shared_prefix_attention(const void* q, const void* k_cache, c
               "shared prefix attention: %d shared tokens are not whole blocks of the table", shared);
   AJB_REQUIRE((long long)num_seqs * q_len * (heads / kv_heads) <= (1ll << 30), "shared prefix attention: too many query rows");
   const int group = heads / kv_heads, tiles = (shared + prefix::TILE - 1) / prefix::TILE;
-  const bool one_tile = num_seqs * q_len * group <= prefix::ROWS;
+  const int rows = num_seqs * q_len * group;      // query rows per KV head
+  const bool few = rows <= 32;                    // the paged kernel takes the prefix along
   AJB_REQUIRE((prefix_splits > 0) == (shared > 0) && prefix_splits >= 0 && prefix_splits <= (tiles > 0 ? tiles : 0) &&
                   suffix_splits >= 1 && part_o != nullptr && part_ml != nullptr,
               "shared prefix attention: %d and %d divisions of %d shared tokens and of the rest do not fit, or there is no workspace",
               prefix_splits, suffix_splits, shared);
-  const int prefix_parts = one_tile && prefix_splits < tiles ? 2 * prefix_splits : prefix_splits;
+  const int prefix_parts = !few && rows <= prefix::ROWS && prefix_splits < tiles ? 2 * prefix_splits : prefix_splits;
   AJB_REQUIRE(parts == prefix_parts + suffix_splits && parts <= 64, "shared prefix attention: %d parts per row, not %d", parts,
               prefix_parts + suffix_splits);
   AJB_REQUIRE(q_pitch % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0, "shared prefix attention: query rows must be 16-byte aligned");
@@ -496,9 +496,15 @@ extern "C" int ajb_shared_prefix_attention(const void* q, const void* k_cache, c
   // up to 32 rows run on the paged kernel that puts the keys on the tensor-core rows; otherwise 128 query rows at a time
   a.q_len = group * q_len <= 32 ? q_len : min(q_len, prefix::ROWS / group);
   a.first_key = shared; a.scale = scale; a.splits = suffix_splits; a.part_stride = parts;
-  a.part_base = prefix_parts; a.part_o = part_o; a.part_ml = part_ml; a.beside_previous = shared > 0;
-  int rc = 0;
-  if (shared > 0)
+  a.part_base = prefix_parts; a.part_o = part_o; a.part_ml = part_ml; a.beside_previous = shared > 0 && !few;
+  a.prefix_splits = few ? prefix_splits : 0;
+  CUtensorMap map_k, map_v;
+  int rc = make_tensor_map_cache(&map_k, a.k_cache, a.num_blocks, a.kv_heads, head_dim);
+  if (rc == 0) rc = make_tensor_map_cache(&map_v, a.v_cache, a.num_blocks, a.kv_heads, head_dim);
+  if (rc) return rc;
+  a.map_k = &map_k;
+  a.map_v = &map_v;
+  if (shared > 0 && !few)
     rc = head_dim == 128 ? prefix::launch_prefix<128>(a, shared, prefix_splits, s) : prefix::launch_prefix<64>(a, shared, prefix_splits, s);
   if (rc == 0) rc = paged::launch(a, head_dim, s);
   if (rc == 0) rc = paged::merge_parts(a, head_dim, s);

@@ -151,6 +151,11 @@ def spec_verify(target_logits: torch.Tensor, draft_logits: torch.Tensor, draft_t
 # ----------------------------------------------------------------------------- shared by the operators below
 
 
+# A small operator takes a few microseconds on the device, so its argument checks are one expression over cheap
+# attributes; only when it fails are the arguments gone through one by one for the message.
+_I32, _I64, _F32, _BF16 = torch.int32, torch.int64, torch.float32, torch.bfloat16
+
+
 def _dense(op: str, name: str, t: torch.Tensor, dtype: torch.dtype, device: torch.device, shape: tuple[int, ...]) -> None:
     if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{op}: {name} must be a contiguous {dtype} tensor of shape {list(shape)} on {device} "
@@ -195,46 +200,51 @@ def batch_maps(block_ids: torch.Tensor, block_counts: torch.Tensor, cached_lens:
 
     ``out`` may hold the five result tensors (buffers a captured graph reads); they are overwritten and returned.
     """
-    op, int32, device = "batch_maps", torch.int32, block_ids.device
-    if block_counts.dim() != 1 or block_ids.dim() != 1:
-        raise ValueError("batch_maps: block_ids is one flat list, block_counts has one entry per sequence")
-    n, = each = block_counts.shape
-    _dense(op, "block_ids", block_ids, int32, device, block_ids.shape)
-    _dense(op, "block_counts", block_counts, int32, device, each)
-    _dense(op, "cached_lens", cached_lens, int32, device, each)
-    _dense(op, "q_lens", q_lens, int32, device, each)
+    index, each = block_ids.get_device(), block_counts.shape
+    if not (block_ids.dtype is block_counts.dtype is cached_lens.dtype is q_lens.dtype is _I32
+            and block_counts.get_device() == index == cached_lens.get_device() == q_lens.get_device()
+            and block_ids.dim() == 1 and len(each) == 1 and cached_lens.shape == each == q_lens.shape
+            and block_ids.is_contiguous() and block_counts.is_contiguous() and cached_lens.is_contiguous() and q_lens.is_contiguous()):
+        if block_counts.dim() != 1 or block_ids.dim() != 1:
+            raise ValueError("batch_maps: block_ids is one flat list, block_counts has one entry per sequence")
+        for name, t, shape in (("block_ids", block_ids, block_ids.shape), ("block_counts", block_counts, each),
+                               ("cached_lens", cached_lens, each), ("q_lens", q_lens, each)):
+            _dense("batch_maps", name, t, _I32, block_ids.device, shape)
+    n = each[0]
     if not (0 <= total_tokens < 1 << 30 and max_blocks >= 1 and block_size >= 1 and pad_block >= 0 and n <= 16384):
         raise ValueError(f"batch_maps: total_tokens {total_tokens} and pad_block {pad_block} must not be negative, max_blocks {max_blocks} "
                          f"and block_size {block_size} must be positive, and there are at most 16384 sequences (got {n})")
     if out is not None:
-        out = BatchMaps(*out)
-        _dense(op, "out.tables", out.tables, int32, device, (n, max_blocks))
-        _dense(op, "out.positions", out.positions, int32, device, (total_tokens,))
-        _dense(op, "out.slots", out.slots, torch.int64, device, (total_tokens,))
-        _dense(op, "out.q_start", out.q_start, int32, device, (n + 1,))
-        _dense(op, "out.context_lens", out.context_lens, int32, device, each)
-    if device.type != "cuda":
+        tables, positions, slots, q_start, context_lens = out
+        if not (tables.dtype is positions.dtype is q_start.dtype is context_lens.dtype is _I32 and slots.dtype is _I64
+                and tables.get_device() == index == positions.get_device() == slots.get_device() == q_start.get_device() == context_lens.get_device()
+                and tables.shape == (n, max_blocks) and positions.shape == (total_tokens,) == slots.shape and q_start.shape == (n + 1,)
+                and context_lens.shape == each and tables.is_contiguous() and positions.is_contiguous() and slots.is_contiguous()
+                and q_start.is_contiguous() and context_lens.is_contiguous()):
+            for name, t, dtype, shape in (("tables", tables, _I32, (n, max_blocks)), ("positions", positions, _I32, (total_tokens,)),
+                                          ("slots", slots, _I64, (total_tokens,)), ("q_start", q_start, _I32, (n + 1,)),
+                                          ("context_lens", context_lens, _I32, each)):
+                _dense("batch_maps", "out." + name, t, dtype, block_ids.device, shape)
+    if index < 0:
         found = reference.batch_maps(block_ids, block_counts, cached_lens, q_lens, total_tokens, max_blocks, block_size, pad_block)
         if out is None:
             return BatchMaps(*found)
         for mine, theirs in zip(out, found):
             mine.copy_(theirs)
-        return out
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
+        return BatchMaps(*out)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
             return batch_maps(block_ids, block_counts, cached_lens, q_lens, total_tokens, max_blocks, block_size=block_size,
                               pad_block=pad_block, out=out)
     if out is None:
-        out = BatchMaps(torch.empty(n, max_blocks, dtype=torch.int32, device=device),
-                        torch.empty(total_tokens, dtype=torch.int32, device=device),
-                        torch.empty(total_tokens, dtype=torch.int64, device=device),
-                        torch.empty(n + 1, dtype=torch.int32, device=device),
-                        torch.empty(n, dtype=torch.int32, device=device))
-    tables, positions, slots, q_start, context_lens = out
+        device = block_ids.device
+        tables, positions = torch.empty(n, max_blocks, dtype=_I32, device=device), torch.empty(total_tokens, dtype=_I32, device=device)
+        slots = torch.empty(total_tokens, dtype=_I64, device=device)
+        q_start, context_lens = torch.empty(n + 1, dtype=_I32, device=device), torch.empty(n, dtype=_I32, device=device)
     native.call("ajb_batch_maps", block_ids.data_ptr(), block_counts.data_ptr(), cached_lens.data_ptr(), q_lens.data_ptr(),
                 block_ids.shape[0], n, total_tokens, max_blocks, block_size, pad_block, tables.data_ptr(), positions.data_ptr(),
                 slots.data_ptr(), q_start.data_ptr(), context_lens.data_ptr(), native.stream_ptr())
-    return out
+    return BatchMaps(tables, positions, slots, q_start, context_lens)
 
 
 # ----------------------------------------------------------------------------- attention behind a shared prefix
@@ -243,36 +253,49 @@ _PREFIX_TILE = 128         # query rows and keys per step of the prefix kernel
 
 
 @functools.lru_cache(maxsize=4096)
-def prefix_plan(rows: int, kv_heads: int, head_dim: int, shared: int, pieces: int, behind: int) -> tuple[int, int]:
-    """``(CTAs that share the prefix per 256 query rows and KV head, parts they leave per row)``.
+def prefix_plan(n: int, q_len: int, group: int, kv_heads: int, head_dim: int, shared: int, behind: int) -> tuple[int, int, int]:
+    """How a call of :func:`shared_prefix_attention` is divided: ``(CTAs that share the prefix per 256 query rows and KV
+    head, CTAs that share a suffix, parts per row in all)``.
 
-    A CTA of the prefix kernel keeps an SM to itself while the others stream the ``pieces`` (sequence, KV head) suffixes
-    of up to ``behind`` tokens, so the SMs are divided like the work. Measured beside a running suffix launch: a prefix CTA
-    takes about 14 us and 2 us more per step (128 keys for up to 256 rows; two tiles make a step when 128 rows are all there
-    are), a piece occupies half an SM for 1.3 us and 2.7 us (64-wide heads: 1.3 us) per 128 keys, of which half the bound is
-    taken; a part costs its fp32 rows, written and read once at 4 TB/s. More prefix CTAs than 7 in 10 SMs left the suffix
-    waiting (33 x 5 rows behind 4001 tokens: 28 us with 96 CTAs, 42 us with 144).
+    A CTA of the prefix kernel keeps an SM to itself while the others stream the (sequence, KV head) suffixes of up to
+    ``behind`` tokens, so the SMs are divided like the work. Measured beside a running suffix launch: a prefix CTA takes
+    about 14 us and 2 us more per step (128 keys for up to 256 rows; two tiles make a step when 128 rows are all there are),
+    a suffix occupies half an SM for 1.3 us and 2.7 us (64-wide heads: 1.3 us) per 128 keys, of which half the bound is
+    taken; a part costs its fp32 rows, written and read once at 4 TB/s. With more prefix CTAs than 7 in 10 SMs the suffix
+    hardly runs before they end (33 x 5 rows behind 4001 tokens: 28 us with 96 CTAs, 37 us with 120). Up to 32 rows per KV
+    head both are pieces of one launch, two to an SM, and a piece takes about as long for its first tile as for three more.
     """
-    if not shared:
-        return 0, 0
     if not _SM_COUNT:
         _SM_COUNT.append(int(native.lib().ajb_sm_count()))
     sms = _SM_COUNT[0]
+    chunk = q_len if group * q_len <= 32 else max(1, min(q_len, _PREFIX_TILE // group))
+    pieces = n * kv_heads * -(-q_len // chunk)
+    splits = paged_splits(pieces, behind)
+    if not shared:
+        return 0, splits, splits
+    rows = n * q_len * group
     tiles = -(-shared // _PREFIX_TILE)
+    if rows <= 32:
+        ours = max(1, min(tiles, 32, (2 * sms - pieces * splits) // kv_heads))
+        each = -(-tiles // ours)
+        ours = -(-tiles // each)                # the same longest piece from as few CTAs as give it
+        return ours, splits, ours + splits
     one_tile = rows <= _PREFIX_TILE
     units = kv_heads * (1 if one_tile else -(-rows // (2 * _PREFIX_TILE)))
     suffix = pieces * (0.65 + (1.35 if head_dim == 128 else 0.65) * (behind / 256 + 0.5))
     best = (math.inf, 1, 1)
-    for splits in range(1, min(tiles, 32) + 1):
-        if splits > 1 and 10 * units * splits > 7 * sms:
+    for ours in range(1, min(tiles, 32) + 1):
+        if ours > 1 and units * ours > sms:
             break
-        each = -(-tiles // splits)
-        parts = 2 * splits if one_tile and splits < tiles else splits
+        each = -(-tiles // ours)
+        parts = 2 * ours if one_tile and ours < tiles else ours
         last = 14.0 + (1.0 if one_tile else 2.0) * each
-        time = max(last, (units * splits * last + suffix) / sms) + parts * rows * kv_heads * head_dim * 8 / 4e6
+        time = max(last, (units * ours * last + suffix) / sms) + parts * rows * kv_heads * head_dim * 8 / 4e6
+        if 10 * units * ours > 7 * sms:
+            time += 8.0 + suffix / sms
         if time < best[0]:
-            best = (time, splits, parts)
-    return best[1], best[2]
+            best = (time, ours, parts)
+    return best[1], splits, best[2] + splits
 
 
 def shared_prefix_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -293,7 +316,6 @@ def shared_prefix_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cach
     number of parts per sequence is chosen. A row whose sequence has no token at all comes out as zeros. ``scale``
     defaults to ``1 / sqrt(hd)``; ``out`` (contiguous, like ``q``) receives the result.
     """
-    op, int32, device = "shared_prefix_attention", torch.int32, q.device
     if q.dim() != 3 or key_cache.dim() != 4 or block_tables.dim() != 2:
         raise ValueError("shared_prefix_attention: q is [rows, heads, hd], the caches [blocks, block, kv_heads, hd], block_tables [n, max_blocks]")
     total, heads, head_dim = q.shape
@@ -306,46 +328,47 @@ def shared_prefix_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cach
                          "or the cache or the block tables are empty")
     if not 0 <= prefix_len <= max_blocks * block_size:
         raise ValueError(f"shared_prefix_attention: prefix_len {prefix_len} does not fit block tables of {max_blocks} blocks")
-    _dense(op, "key_cache", key_cache, q.dtype, device, key_cache.shape)
-    _dense(op, "value_cache", value_cache, q.dtype, device, key_cache.shape)
-    _dense(op, "block_tables", block_tables, int32, device, block_tables.shape)
-    _dense(op, "context_lens", context_lens, int32, device, (n,))
+    index, dtype = q.get_device(), q.dtype
+    if not (key_cache.dtype is value_cache.dtype is dtype and block_tables.dtype is context_lens.dtype is _I32
+            and value_cache.shape == key_cache.shape and context_lens.shape == (n,)
+            and key_cache.get_device() == index == value_cache.get_device() == block_tables.get_device() == context_lens.get_device()
+            and key_cache.is_contiguous() and value_cache.is_contiguous() and block_tables.is_contiguous() and context_lens.is_contiguous()):
+        for name, t, kind, shape in (("key_cache", key_cache, dtype, key_cache.shape), ("value_cache", value_cache, dtype, key_cache.shape),
+                                     ("block_tables", block_tables, _I32, block_tables.shape), ("context_lens", context_lens, _I32, (n,))):
+            _dense("shared_prefix_attention", name, t, kind, q.device, shape)
     if out is not None:
-        _dense(op, "out", out, q.dtype, device, q.shape)
+        _dense("shared_prefix_attention", "out", out, dtype, q.device, q.shape)
         if _overlap(out, q):
             raise ValueError("shared_prefix_attention: out must not overlap q")
     scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
-    if device.type != "cuda":
+    if index < 0:
         found = reference.shared_prefix_attention(q, key_cache, value_cache, block_tables, context_lens, prefix_len, q_len, scale)
         return found if out is None else out.copy_(found)
-    if q.dtype != torch.bfloat16:
-        raise TypeError(f"shared_prefix_attention: CUDA tensors must be bfloat16 (got {q.dtype})")
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
+    if dtype is not _BF16:
+        raise TypeError(f"shared_prefix_attention: CUDA tensors must be bfloat16 (got {dtype})")
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
             return shared_prefix_attention(q, key_cache, value_cache, block_tables, context_lens, prefix_len, q_len=q_len,
                                            scale=scale, max_context=max_context, out=out)
     if q.stride(2) != 1 or q.stride(1) != head_dim or q.stride(0) % 8 or q.data_ptr() % 16:
         q = q.contiguous()
     if out is None:
-        out = torch.empty(total, heads, head_dim, dtype=torch.bfloat16, device=device)
+        out = q.new_empty(q.shape)
     if total == 0:
         return out
     shared = prefix_len // block_size * block_size
     group = heads // kv_heads
-    chunk = q_len if group * q_len <= 32 else max(1, min(q_len, _PREFIX_TILE // group))
     room = max_blocks * block_size
     behind = max(0, (room if max_context is None else min(max_context, room)) - shared)
-    pieces = n * kv_heads * -(-q_len // chunk)
-    splits = paged_splits(pieces, behind)
-    prefix_splits, prefix_parts = prefix_plan(total * group, kv_heads, head_dim, shared, pieces, behind)
+    prefix_splits, splits, parts = prefix_plan(n, q_len, group, kv_heads, head_dim, shared, behind)
     # fp32 parts of every (row, head): un-normalised outputs, then (reference maximum, sum) pairs
-    parts = prefix_parts + splits
     count = total * heads * parts
-    workspace = torch.empty(count * (head_dim + 2), dtype=torch.float32, device=device)
+    workspace = torch.empty(count * (head_dim + 2), dtype=_F32, device=q.device)
+    parts_at = workspace.data_ptr()
     native.call("ajb_shared_prefix_attention", q.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
                 context_lens.data_ptr(), out.data_ptr(), q.stride(0), n, num_blocks, block_size, max_blocks, heads, kv_heads,
-                head_dim, q_len, shared, scale, prefix_splits, splits, parts, workspace.data_ptr(),
-                workspace.data_ptr() + 4 * count * head_dim, native.stream_ptr())
+                head_dim, q_len, shared, scale, prefix_splits, splits, parts, parts_at, parts_at + 4 * count * head_dim,
+                native.stream_ptr())
     return out
 
 
@@ -372,8 +395,8 @@ def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
 
     ``out`` (fp32 ``[rows, vocab]``, contiguous, apart from ``logits``) receives the result.
     """
-    op, int32, fp32, device, dtype = "process_logits", torch.int32, torch.float32, logits.device, logits.dtype
-    if dtype != torch.bfloat16 and dtype != fp32:
+    dtype, index = logits.dtype, logits.get_device()
+    if dtype is not _BF16 and dtype is not _F32:
         raise TypeError(f"process_logits: logits must be bfloat16 or float32 (got {dtype})")
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError("process_logits: logits must be [rows, vocab] with at least one token")
@@ -384,43 +407,46 @@ def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
         if prompt_lens is None or history_lens is None or history.dim() != 2:
             raise ValueError("process_logits: history is [rows, width] and comes with prompt_lens and history_lens")
         width = history.shape[1]
-        _dense(op, "history", history, int32, device, (rows, width))
-        _dense(op, "prompt_lens", prompt_lens, int32, device, each)
-        _dense(op, "history_lens", history_lens, int32, device, each)
-        if repetition is not None:
-            _dense(op, "repetition", repetition, fp32, device, each)
-        if presence is not None:
-            _dense(op, "presence", presence, fp32, device, each)
-        if frequency is not None:
-            _dense(op, "frequency", frequency, fp32, device, each)
+        if not (history.dtype is prompt_lens.dtype is history_lens.dtype is _I32 and history.shape[0] == rows
+                and prompt_lens.shape == each == history_lens.shape
+                and history.get_device() == index == prompt_lens.get_device() == history_lens.get_device()
+                and history.is_contiguous() and prompt_lens.is_contiguous() and history_lens.is_contiguous()):
+            for name, t, shape in (("history", history, (rows, width)), ("prompt_lens", prompt_lens, each), ("history_lens", history_lens, each)):
+                _dense("process_logits", name, t, _I32, logits.device, shape)
+        for name, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
+            if t is not None and not (t.dtype is _F32 and t.shape == each and t.get_device() == index and t.is_contiguous()):
+                _dense("process_logits", name, t, _F32, logits.device, each)
     elif not (repetition is None and presence is None and frequency is None and prompt_lens is None and history_lens is None):
         raise ValueError("process_logits: penalties need a history")
     if bias_ids is not None or bias_values is not None:
         if bias_ids is None or bias_values is None or bias_ids.dim() != 2:
             raise ValueError("process_logits: bias_ids and bias_values come together, [rows, biases] each")
         biases = bias_ids.shape[1]
-        _dense(op, "bias_ids", bias_ids, int32, device, (rows, biases))
-        _dense(op, "bias_values", bias_values, fp32, device, (rows, biases))
-    if token_mask is not None:
-        _dense(op, "token_mask", token_mask, int32, device, (rows, (vocab + 31) // 32))
+        if not (bias_ids.dtype is _I32 and bias_values.dtype is _F32 and bias_ids.shape == (rows, biases) == bias_values.shape
+                and bias_ids.get_device() == index == bias_values.get_device() and bias_ids.is_contiguous() and bias_values.is_contiguous()):
+            _dense("process_logits", "bias_ids", bias_ids, _I32, logits.device, (rows, biases))
+            _dense("process_logits", "bias_values", bias_values, _F32, logits.device, (rows, biases))
+    if token_mask is not None and not (token_mask.dtype is _I32 and token_mask.shape == (rows, (vocab + 31) // 32)
+                                       and token_mask.get_device() == index and token_mask.is_contiguous()):
+        _dense("process_logits", "token_mask", token_mask, _I32, logits.device, (rows, (vocab + 31) // 32))
     if out is not None:
-        _dense(op, "out", out, fp32, device, (rows, vocab))
+        _dense("process_logits", "out", out, _F32, logits.device, (rows, vocab))
         if _overlap(out, logits):
             raise ValueError("process_logits: out must not overlap the logits")
-    if device.type != "cuda":
+    if index < 0:
         found = reference.process_logits(logits, history, prompt_lens, history_lens, repetition, presence, frequency, bias_ids,
                                          bias_values, token_mask)
         return found if out is None else out.copy_(found)
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
             return process_logits(logits, history=history, prompt_lens=prompt_lens, history_lens=history_lens, repetition=repetition,
                                   presence=presence, frequency=frequency, bias_ids=bias_ids, bias_values=bias_values,
                                   token_mask=token_mask, out=out)
     if logits.stride(1) != 1:
         logits = logits.contiguous()
     if out is None:
-        out = torch.empty(rows, vocab, dtype=torch.float32, device=device)
-    native.call("ajb_process_logits", logits.data_ptr(), 1 if dtype == fp32 else 0, logits.stride(0), out.data_ptr(),
+        out = torch.empty(rows, vocab, dtype=_F32, device=logits.device)
+    native.call("ajb_process_logits", logits.data_ptr(), 1 if dtype is _F32 else 0, logits.stride(0), out.data_ptr(),
                 rows, vocab, native.ptr(history) if width else None, width, width, native.ptr(prompt_lens), native.ptr(history_lens),
                 native.ptr(repetition), native.ptr(presence), native.ptr(frequency), native.ptr(bias_ids), native.ptr(bias_values),
                 biases, native.ptr(token_mask), (vocab + 31) // 32, native.stream_ptr())
