@@ -414,3 +414,30 @@ def test_history_longer_than_a_16_bit_count():
     assert got[:, 3].tolist() == [-10000 / 1024, -250 / 1024] and got[:, 8500].tolist() == [-30000 / 1024, -750 / 1024]
     got[:, [3, 8500]] = 0
     assert torch.count_nonzero(got) == 0
+
+
+@pytest.mark.parametrize("rows,vocab,dtype,width,biases,masked,offset", [
+    (70, 128256, torch.bfloat16, 700, 40, True, 0), (300, 31999, torch.float32, 5000, 3, True, 1), (90, 100001, torch.bfloat16, 4096, 0, False, 0),
+    (530, 16384, torch.float32, 33, 70, True, 0), (66, 128256, torch.bfloat16, 0, 5, True, 3), (65, 131072, torch.bfloat16, 1, 0, False, 0)])
+def test_process_logits_of_many_rows(rows, vocab, dtype, width, biases, masked, offset):
+    """Sizes at which the rows are streamed by one launch and mended by another; histories longer than a CTA holds."""
+    gen = torch.Generator(device="cuda").manual_seed(vocab)
+    kw = dict(device="cuda", generator=gen)
+    wide = (4 * torch.randn(rows, vocab + 5, **kw)).to(dtype)
+    logits = wide[:, offset:offset + vocab]
+    args = {}
+    if width:
+        ids = (vocab ** torch.rand(rows, width, **kw) - 1).to(torch.int32)
+        ids[torch.rand(rows, width, **kw) < 0.02] = vocab + 7
+        args = dict(history=ids, prompt_lens=torch.randint(0, width + 1, (rows,), **kw).int(), history_lens=torch.randint(0, width + 1, (rows,), **kw).int(),
+                    repetition=0.7 + torch.rand(rows, **kw), presence=torch.rand(rows, **kw), frequency=torch.rand(rows, **kw))
+    if biases:
+        args.update(bias_ids=torch.randint(-3, vocab + 3, (rows, biases), **kw).int(), bias_values=torch.randn(rows, biases, **kw))
+        args["bias_ids"][:, biases // 2:] = args["bias_ids"][:, :biases - biases // 2]             # every token twice
+    if masked:
+        args["token_mask"] = torch.randint(-2**31, 2**31 - 1, (rows, (vocab + 31) // 32), **kw).int()
+    assert rows * vocab >= 1 << 23
+    got = serving.process_logits(logits, **args)
+    want = reference.process_logits(logits, **args)               # the same fp32 steps, whole rows at a time
+    assert torch.equal(got, want)
+    assert torch.equal(got, serving.process_logits(logits.contiguous(), **args))
