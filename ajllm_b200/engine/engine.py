@@ -12,7 +12,8 @@ from dataclasses import dataclass, field
 
 import torch
 
-from ajllm_b200.engine.kv_cache import PagedKVCache
+from ajllm_b200.engine.kv_cache import OutOfBlocks, PagedKVCache
+from ajllm_b200.engine.logits import LogitsProcessor, check_params
 from ajllm_b200.engine.model_runner import ModelRunner, RunItem
 from ajllm_b200.engine.scheduler import SamplingParams, ScheduledSeq, Scheduler, Sequence
 from ajllm_b200.engine.spec_decode import verify_greedy, verify_rejection
@@ -90,10 +91,55 @@ class LLMEngine:
         self._draws: dict[int, int] = {}
         self._sampling_state = None          # (key, temps, top_ps, seeds, counters) of the previous sampling call
         self._finished: list[Sequence] = []
+        self._processor = LogitsProcessor(model.vocab_size, device)
+        self._prefix_ids = 0
+
+    # ---------------------------------------------------------------- shared prefix
+    @torch.no_grad()
+    def share_prefix(self, tokens: list[int]) -> int:
+        """Computes the keys and values of a prompt's beginning once, for every request that begins with it from now on:
+        such a request starts behind it, and decoding steps whose requests all share it read it once for the whole
+        batch. Whole cache blocks are shared; returns how many tokens that is. The blocks stay taken until
+        :meth:`release_prefix`; one prefix is shared at a time."""
+        if self.draft_runner is not None:
+            raise ValueError("a prefix cannot be shared with a draft model")
+        if self.scheduler.prefix is not None:
+            raise ValueError("a prefix is shared already: release it first")
+        if any(not 0 <= int(t) < self.model.vocab_size for t in tokens):
+            raise ValueError(f"the prefix has tokens outside the vocabulary of {self.model.vocab_size}")
+        block = self.cache.block_size
+        length = min(len(tokens), self.model.context_length - 1) // block * block
+        if length == 0:
+            return 0
+        if length // block > self.cache.allocator.free_blocks:
+            raise OutOfBlocks(f"the prefix needs {length // block} blocks, {self.cache.allocator.free_blocks} free")
+        tokens = [int(t) for t in tokens[:length]]
+        self._prefix_ids += 1
+        cache_id = -self._prefix_ids          # requests count from 0
+        try:
+            for start in range(0, length, self.scheduler.max_batched_tokens):
+                self.runner.forward([RunItem(cache_id, tokens[start:start + self.scheduler.max_batched_tokens], 0)])
+        except BaseException:
+            self.cache.free(cache_id)
+            raise
+        self.scheduler.prefix = (cache_id, tokens)
+        self.runner.set_prefix((cache_id, length))
+        return length
+
+    def release_prefix(self) -> None:
+        """Ends the sharing; requests that began behind the prefix keep its blocks until they finish."""
+        if self.scheduler.prefix is not None:
+            self.cache.free(self.scheduler.prefix[0])
+            self.scheduler.prefix = None
+            self.runner.set_prefix(None)
 
     # ---------------------------------------------------------------- requests
     def add_request(self, prompt: list[int], params: SamplingParams | None = None) -> int:
         params = params or SamplingParams()
+        if params.processes_logits:
+            if self.draft_runner is not None:
+                raise ValueError("penalties, biases and token masks cannot be used with a draft model")
+            check_params(params, self.model.vocab_size)
         seq = self.scheduler.add(prompt, params, arrival=time.perf_counter())
         gen = torch.Generator(device="cpu")
         gen.manual_seed(params.seed if params.seed is not None else self.seed * 1_000_003 + seq.request_id)
@@ -171,6 +217,7 @@ class LLMEngine:
             self.draft_cache.free(seq.request_id)
         self._generators.pop(seq.request_id, None)
         self._draws.pop(seq.request_id, None)
+        self._processor.forget(seq.request_id)
         self._finished.append(seq)
 
     def _sync_preempted(self) -> None:
@@ -187,6 +234,8 @@ class LLMEngine:
         tick = time.perf_counter()
         done_before = len(self._finished)
         plan = self.scheduler.schedule(decode_tokens=self.k + 1 if self.k else 1)
+        if not plan and self.scheduler.prefix is not None and self.scheduler.has_work():
+            raise RuntimeError("KV cache is too small to make progress beside the shared prefix: release it")
         self._sync_preempted()
         self.stats.preemptions = self.scheduler.num_preemptions
         prefill = [item for item in plan if item.is_prefill]
@@ -206,12 +255,14 @@ class LLMEngine:
             items.append(RunItem(seq.request_id, new, 1 if item.samples else 0))
             owners.append(item)
         if items:
+            sampling = [item.seq for item in owners if item.samples]
+            mask, emptied = self._processor.masks(sampling)          # before anything is written: a mask may raise
             logits = self.runner.forward(items)
             if self.draft_runner is not None:
                 # keep the draft cache in step with the target for prompt tokens
                 self.draft_runner.forward([RunItem(i.seq_id, i.token_ids, 0) for i in items])
             now = time.perf_counter()
-            sampling = [item.seq for item in owners if item.samples]
+            logits = self._processor.apply(sampling, logits, mask)
             tokens = self._sample_rows(sampling, logits)
             row = 0
             for item in owners:
@@ -220,7 +271,10 @@ class LLMEngine:
                 if item.is_prefill:
                     self.stats.prompt_tokens += item.num_new_tokens
                 if item.samples:
-                    self._emit(seq, tokens[row], now)
+                    if emptied[row]:
+                        self._finish(seq, "mask", now)
+                    else:
+                        self._emit(seq, tokens[row], now)
                     row += 1
         self._check_kernels()
         self.stats.steps += 1

@@ -57,6 +57,8 @@ class BlockTable:
     blocks: list[int] = field(default_factory=list)
     length: int = 0
     shrinks: int = 0          # how often blocks were given back (a mirror of `blocks` elsewhere must then be rebuilt)
+    parent: int | None = None # the sequence this one was forked from, and how many of its first blocks are still the parent's
+    shared_blocks: int = 0
 
 
 class PagedKVCache:
@@ -81,20 +83,23 @@ class PagedKVCache:
     def can_append(self, seq_id: int, new_tokens: int) -> bool:
         return self.blocks_needed(seq_id, new_tokens) <= self.allocator.free_blocks
 
-    def append_slots(self, seq_id: int, new_tokens: int) -> list[int]:
-        """Reserve room for ``new_tokens`` more tokens and return their flat slot ids
-        (``block * block_size + offset``)."""
+    def reserve(self, seq_id: int, new_tokens: int) -> BlockTable:
+        """Count ``new_tokens`` more tokens to a sequence, with the blocks they need; returns its block table."""
         table = self.tables.setdefault(seq_id, BlockTable())
         need = self.blocks_needed(seq_id, new_tokens)
         if need > self.allocator.free_blocks:
             raise OutOfBlocks(f"sequence {seq_id} needs {need} blocks, {self.allocator.free_blocks} free")
         for _ in range(need):
             table.blocks.append(self.allocator.allocate())
-        slots = []
-        for t in range(table.length, table.length + new_tokens):
-            slots.append(table.blocks[t // self.block_size] * self.block_size + t % self.block_size)
         table.length += new_tokens
-        return slots
+        return table
+
+    def append_slots(self, seq_id: int, new_tokens: int) -> list[int]:
+        """Reserve room for ``new_tokens`` more tokens and return their flat slot ids
+        (``block * block_size + offset``)."""
+        table = self.reserve(seq_id, new_tokens)
+        return [table.blocks[t // self.block_size] * self.block_size + t % self.block_size
+                for t in range(table.length - new_tokens, table.length)]
 
     def truncate(self, seq_id: int, new_length: int) -> None:
         """Forget the tokens past ``new_length`` (speculative rollback)."""
@@ -105,6 +110,7 @@ class PagedKVCache:
         while len(table.blocks) > keep:
             self.allocator.release(table.blocks.pop())
             table.shrinks += 1
+        table.shared_blocks = min(table.shared_blocks, keep)
 
     def fork(self, parent_id: int, child_id: int) -> None:
         """``child`` shares every block of ``parent`` (copy-on-write is the caller's duty: a shared last
@@ -112,7 +118,12 @@ class PagedKVCache:
         parent = self.tables[parent_id]
         for block in parent.blocks:
             self.allocator.share(block)
-        self.tables[child_id] = BlockTable(list(parent.blocks), parent.length)
+        self.tables[child_id] = BlockTable(list(parent.blocks), parent.length, parent=parent_id, shared_blocks=len(parent.blocks))
+
+    def shares(self, seq_id: int, parent_id: int, blocks: int) -> bool:
+        """Whether the first ``blocks`` blocks of a sequence are those of ``parent_id``, which it was forked from."""
+        table = self.tables.get(seq_id)
+        return table is not None and table.parent == parent_id and table.shared_blocks >= blocks
 
     def free(self, seq_id: int) -> None:
         table = self.tables.pop(seq_id, None)

@@ -15,6 +15,9 @@ and write a scratch cache block that no sequence owns. Under tensor parallelism 
 GEMM -> all-reduce kernels: their call numbers and arrival counts live in device memory and advance with every
 execution, captured or not, so every rank replays the same graph and the kernels pair up as in eager mode
 (NCCL collectives are not captured: without the fused kernels, tensor-parallel decoding launches step by step).
+
+While a prefix is shared (``set_prefix``), steps of two or more sequences that all begin with it read its keys and
+values once for the whole batch; these steps have graphs of their own, which go when the prefix does.
 """
 
 from __future__ import annotations
@@ -108,8 +111,9 @@ class _DecodeGraph:
     for plain decoding, ``k + 1`` for the verification pass of speculative decoding."""
 
     def __init__(self, bucket: int, q_len: int, max_blocks: int, device: torch.device, scratch_block: int,
-                 block_size: int) -> None:
+                 block_size: int, shared: int = 0) -> None:
         self.bucket, self.q_len = bucket, q_len
+        self.shared = shared          # tokens at the beginning of every sequence that are read once for the batch
         rows = bucket * q_len
         self.staging = DecodeStaging(bucket, q_len, max_blocks, scratch_block, block_size, pinned=device.type == "cuda")
         self.rows = torch.zeros(3, rows, dtype=torch.long, device=device)
@@ -130,6 +134,7 @@ class _DecodeGraph:
 class ModelRunner:
     FUSED_ALL_REDUCE_MAX_ROWS = 2048     # beyond this the partial tiles (tp copies per rank) outgrow the win
     GRAPH_BUCKETS = (1, 2, 4, 8, 16, 32, 64, 128, 256)
+    MAX_SEQUENCES = 16384                # whose maps one launch builds; a larger step runs in parts
 
     def __init__(self, model, cache: PagedKVCache, quantization: str | None = None) -> None:
         self.model = model
@@ -164,7 +169,8 @@ class ModelRunner:
             self.weights.append(entry)
         # decoding graphs: dense feed-forward blocks (expert routing has data-dependent shapes); with several ranks only
         # when every row-parallel projection runs as the fused kernel (bf16 weights)
-        self._graphs: dict[tuple[int, int], _DecodeGraph] = {}
+        self._graphs: dict[tuple[int, int, int], _DecodeGraph] = {}      # (bucket, new tokens per sequence, shared tokens)
+        self._prefix: tuple[int, int] | None = None                      # cache id and length of the shared prefix
         self._scratch_block: int | None = None
         single = self.tp is None or self.tp.size == 1
         fused_everywhere = (not single and getattr(self.tp, "fused", None) is not None
@@ -173,6 +179,24 @@ class ModelRunner:
                            and (single or fused_everywhere)
                            and not any("moe" in w for w in self.weights)
                            and os.environ.get("AJB_DECODE_GRAPHS", "1") != "0")
+
+    # ------------------------------------------------------------------ shared prefix
+    def set_prefix(self, prefix: tuple[int, int] | None) -> None:
+        """``(cache id, tokens)`` of a prefix that sequences are forked from (whole blocks), or ``None`` for none."""
+        if self._prefix is not None:
+            self._graphs = {key: graph for key, graph in self._graphs.items() if key[2] == 0}
+        self._prefix = prefix
+
+    def _shared_tokens(self, items: list[RunItem]) -> int:
+        """Length of the prefix that the whole step can read at once: two or more sequences with equally many new tokens,
+        all forked from the prefix. 0: every sequence reads its own context."""
+        if self._prefix is None or len(items) < 2 or (self.device.type == "cuda" and self.dtype != torch.bfloat16):
+            return 0
+        parent, length = self._prefix
+        q_len, blocks = len(items[0].token_ids), length // self.cache.block_size
+        shared = all(len(item.token_ids) == q_len and self.cache.shares(item.seq_id, parent, blocks)
+                     and self.cache.length(item.seq_id) >= length for item in items)
+        return length if shared and q_len > 0 else 0
 
     # ------------------------------------------------------------------ graph-replayed decoding
     def _decode_static(self, g: _DecodeGraph) -> torch.Tensor:
@@ -197,8 +221,12 @@ class ModelRunner:
             qkv = self._padded_heads(qkv, attn)
             q, k, v = ops.split_packed_qkv(qkv, attn.num_heads, attn.num_kv_heads, self.kernel_head_dim)
             cache.write(index, g.slots, k, v)
-            attended = serving.paged_attention_planned(q.contiguous(), cache.keys[index], cache.values[index], plan,
-                                                       self.softmax_scale)
+            if g.shared:
+                attended = serving.shared_prefix_attention(q.contiguous(), cache.keys[index], cache.values[index], g.tables,
+                                                           g.ctx, g.shared, q_len=g.q_len, scale=self.softmax_scale)
+            else:
+                attended = serving.paged_attention_planned(q.contiguous(), cache.keys[index], cache.values[index], plan,
+                                                           self.softmax_scale)
             attended = self._row_parallel(self._true_heads(attended.reshape(n, -1), attn), w["out"])
             stream, normed = layer.norm2.add_and_norm(stream, attended)
             if "w13" in w:
@@ -223,17 +251,19 @@ class ModelRunner:
             for bucket in self.GRAPH_BUCKETS:
                 if bucket <= top:
                     self._graph_for(bucket, q_len)
+                    if self._prefix is not None and bucket > 1:
+                        self._graph_for(bucket, q_len, self._prefix[1])
         return len(self._graphs)
 
-    def _graph_for(self, bucket: int, q_len: int) -> _DecodeGraph:
-        g = self._graphs.get((bucket, q_len))
+    def _graph_for(self, bucket: int, q_len: int, shared: int = 0) -> _DecodeGraph:
+        g = self._graphs.get((bucket, q_len, shared))
         if g is not None:
             return g
         cache = self.cache
         if self._scratch_block is None:
             self._scratch_block = cache.allocator.allocate()       # padding rows read and write this block only
         max_blocks = (self.model.context_length + cache.block_size - 1) // cache.block_size
-        g = _DecodeGraph(bucket, q_len, max_blocks, self.device, self._scratch_block, cache.block_size)
+        g = _DecodeGraph(bucket, q_len, max_blocks, self.device, self._scratch_block, cache.block_size, shared)
         g.staging.fill([], cache)            # every row is a padding row: the capture reads and writes the scratch block only
         g.upload()
         # one eager run on a side stream first (lazy kernel attributes, allocator warm-up), then the capture
@@ -248,7 +278,7 @@ class ModelRunner:
         # captures, which the default (global) mode treats as a capture violation
         with torch.cuda.graph(g.graph, capture_error_mode="thread_local"):
             g.logits = self._decode_static(g)
-        self._graphs[(bucket, q_len)] = g
+        self._graphs[(bucket, q_len, shared)] = g
         return g
 
     def _forward_decode_graph(self, items: list[RunItem]) -> torch.Tensor | None:
@@ -270,7 +300,7 @@ class ModelRunner:
             if cache.length(item.seq_id) + q_len > model.context_length:
                 raise ValueError(f"sequence {item.seq_id} would exceed the context length {model.context_length}")
         bucket = next(b for b in self.GRAPH_BUCKETS if b >= n)
-        g = self._graph_for(bucket, q_len)
+        g = self._graph_for(bucket, q_len, self._shared_tokens(items))
         g.staging.fill(items, cache)
         g.upload()
         g.graph.replay()
@@ -304,6 +334,20 @@ class ModelRunner:
             return fused.gemm_all_reduce(x, weight)
         return self._reduce(_matmul(x, weight))
 
+    def _device_maps(self, seq_ids: list[int], q_lens: list[int], ctx_lens: list[int], total: int):
+        """Block tables, positions and slots of a ragged step: the sequences' block lists and lengths go to the device in
+        one copy and are expanded there."""
+        from ajllm_b200.ops import serving
+        n = len(seq_ids)
+        blocks = [self.cache.tables[s].blocks for s in seq_ids]
+        counts = [len(b) for b in blocks]
+        host = counts + [ctx - q for q, ctx in zip(q_lens, ctx_lens)] + q_lens
+        for own in blocks:
+            host += own
+        packed = torch.tensor(host, dtype=torch.int32, device=self.device)
+        return serving.batch_maps(packed[3 * n:], packed[:n], packed[n:2 * n], packed[2 * n:3 * n], total, max(counts, default=0) or 1,
+                                  block_size=self.cache.block_size)
+
     @torch.no_grad()
     def forward(self, items: list[RunItem]) -> torch.Tensor:
         """Returns logits ``[sum_i num_logits_i, vocab]`` in item order."""
@@ -312,6 +356,10 @@ class ModelRunner:
             if logits is not None:
                 return logits
         model, cache = self.model, self.cache
+        on_gpu = self.device.type == "cuda" and self.dtype == torch.bfloat16
+        if on_gpu and len(items) > self.MAX_SEQUENCES:
+            return torch.cat([self.forward(items[:self.MAX_SEQUENCES]), self.forward(items[self.MAX_SEQUENCES:])])
+        shared = self._shared_tokens(items)
         tokens, positions, slots, q_lens, ctx_lens, seq_ids, logit_rows = [], [], [], [], [], [], []
         cursor = 0
         for item in items:
@@ -319,9 +367,12 @@ class ModelRunner:
             n = len(item.token_ids)
             if start + n > model.context_length:
                 raise ValueError(f"sequence {item.seq_id} would exceed the context length {model.context_length}")
-            slots.extend(cache.append_slots(item.seq_id, n))
+            if on_gpu:
+                cache.reserve(item.seq_id, n)
+            else:
+                slots.extend(cache.append_slots(item.seq_id, n))
+                positions.extend(range(start, start + n))
             tokens.extend(item.token_ids)
-            positions.extend(range(start, start + n))
             q_lens.append(n)
             ctx_lens.append(start + n)
             seq_ids.append(item.seq_id)
@@ -329,16 +380,16 @@ class ModelRunner:
             cursor += n
         dev = self.device
         ids = torch.tensor(tokens, dtype=torch.long, device=dev)
-        pos = torch.tensor(positions, dtype=torch.long, device=dev)
-        slot_t = torch.tensor(slots, dtype=torch.long, device=dev)
-        tables = cache.block_table_tensor(seq_ids, dev)
-        ctx_t = torch.tensor(ctx_lens, dtype=torch.int32, device=dev)
-        qlen_t = torch.tensor(q_lens, dtype=torch.int32, device=dev)
-
-        on_gpu = dev.type == "cuda" and self.dtype == torch.bfloat16
+        from ajllm_b200.ops import serving
         if on_gpu:
-            from ajllm_b200.ops import serving
-            pos32 = pos.to(torch.int32)
+            tables, pos, slot_t, _, ctx_t = self._device_maps(seq_ids, q_lens, ctx_lens, len(tokens))
+        else:
+            pos = torch.tensor(positions, dtype=torch.long, device=dev)
+            slot_t = torch.tensor(slots, dtype=torch.long, device=dev)
+            tables = cache.block_table_tensor(seq_ids, dev)
+            ctx_t = torch.tensor(ctx_lens, dtype=torch.int32, device=dev)
+            qlen_t = torch.tensor(q_lens, dtype=torch.int32, device=dev)
+        if on_gpu:
             # split the batch: long prompts with nothing cached use the training flash kernel, the rest is paged
             fresh, cached_idx, cached_qlens, cached_ctx, cached_items = [], [], [], [], []
             cursor = 0
@@ -352,7 +403,7 @@ class ModelRunner:
                     cached_items.append(i)
                 cursor += n
             cached_rows = cached_tables = None
-            if cached_idx:
+            if cached_idx and not shared:
                 cached_rows = torch.tensor(cached_idx, dtype=torch.long, device=dev)
                 cached_tables = tables if len(cached_items) == len(q_lens) else \
                     tables.index_select(0, torch.tensor(cached_items, dtype=torch.long, device=dev)).contiguous()
@@ -361,7 +412,7 @@ class ModelRunner:
                 all_cached = len(cached_idx) == len(tokens)
         stream = model.token_embeddings(ids)
         if model.position_embeddings is not None:
-            stream = stream + model.position_embeddings(pos)
+            stream = stream + model.position_embeddings(pos.long())
         pending = None
         for index, (layer, w) in enumerate(zip(model.layers, self.weights)):
             attn = layer.attention
@@ -369,7 +420,7 @@ class ModelRunner:
             qkv = _matmul(normed, w["qkv"])
             if on_gpu:
                 if attn.use_rope:
-                    serving.rope_packed_(qkv, attn.rope_cos, attn.rope_sin, pos32, attn.num_heads, attn.num_kv_heads,
+                    serving.rope_packed_(qkv, attn.rope_cos, attn.rope_sin, pos, attn.num_heads, attn.num_kv_heads,
                                          attn.head_dim)
                 khd = self.kernel_head_dim
                 qkv = self._padded_heads(qkv, attn)
@@ -379,7 +430,11 @@ class ModelRunner:
                 for lo, hi in fresh:          # prompts starting from an empty cache: tiled kernel on the packed rows
                     attended[lo:hi] = serving.prompt_attention(qkv[lo:hi], attn.num_heads, attn.num_kv_heads, khd,
                                                                self.softmax_scale)
-                if cached_rows is not None:
+                if shared:          # every sequence of the step is behind the prefix
+                    attended = serving.shared_prefix_attention(q.contiguous(), cache.keys[index], cache.values[index], tables, ctx_t,
+                                                               shared, q_len=q_lens[0], scale=self.softmax_scale,
+                                                               max_context=max(ctx_lens)).reshape(ids.shape[0], -1)
+                elif cached_rows is not None:
                     if all_cached:          # pure decode / verify step: no gather, no scatter
                         attended = serving.paged_attention_planned(q.contiguous(), cache.keys[index], cache.values[index],
                                                                    paged_plan, self.softmax_scale).reshape(ids.shape[0], -1)
@@ -394,8 +449,12 @@ class ModelRunner:
                     q = reference.rope_interleaved(q, attn.rope_cos, attn.rope_sin, pos)
                     k = reference.rope_interleaved(k, attn.rope_cos, attn.rope_sin, pos)
                 cache.write(index, slot_t, k, v)
-                attended = ops.paged_attention_ragged(q, cache.keys[index], cache.values[index], tables, ctx_t, qlen_t,
-                                                      q_lens, ctx_lens)
+                if shared:
+                    attended = serving.shared_prefix_attention(q.contiguous(), cache.keys[index], cache.values[index], tables, ctx_t,
+                                                               shared, q_len=q_lens[0])
+                else:
+                    attended = ops.paged_attention_ragged(q, cache.keys[index], cache.values[index], tables, ctx_t, qlen_t,
+                                                          q_lens, ctx_lens)
             attended = self._row_parallel(attended.reshape(ids.shape[0], -1), w["out"])
             stream, normed = layer.norm2.add_and_norm(stream, attended)
             if "moe" in w:

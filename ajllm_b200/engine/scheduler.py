@@ -5,7 +5,8 @@ verify) step, then as many waiting requests as fit (``max_num_seqs`` sequences,
 ``max_batched_tokens`` new tokens, free KV blocks). Prompts longer than the remaining token budget
 are prefilled in chunks. When a running sequence cannot get a block, the most recently admitted
 running sequence is preempted: its blocks are released and it re-enters the waiting queue with its
-generated tokens appended to its prompt (recompute on resume). The reference serves one prompt at a
+generated tokens appended to its prompt (recompute on resume). A request that begins with the shared
+prefix starts from the prefix's blocks instead of an empty table. The reference serves one prompt at a
 time with no scheduler (``ajllm/workflows/lm_generate.py:56-81``).
 """
 
@@ -13,8 +14,11 @@ from __future__ import annotations
 
 import itertools
 from collections import deque
+from collections.abc import Callable
 from dataclasses import dataclass, field
 from enum import Enum
+
+import torch
 
 from ajllm_b200.engine.kv_cache import PagedKVCache
 
@@ -32,6 +36,24 @@ class SamplingParams:
     top_p: float | None = 0.95
     eos_token_id: int | None = None
     seed: int | None = None
+    # Applied to the logits before temperature and top-p, in this order. The first penalises tokens of the prompt and the
+    # output (a positive logit is divided by it, another multiplied), the next two tokens of the output (taken off once,
+    # and once per occurrence). `token_mask` is called with the output so far before every token and returns which tokens
+    # may follow (int32 words, bit v % 32 of word v // 32 for token v; None: all); when none may, the request finishes
+    # with the reason "mask".
+    repetition_penalty: float = 1.0
+    presence_penalty: float = 0.0
+    frequency_penalty: float = 0.0
+    logit_bias: dict[int, float] | None = None
+    token_mask: Callable[[list[int]], torch.Tensor | None] | None = None
+
+    @property
+    def penalises(self) -> bool:
+        return self.repetition_penalty != 1.0 or self.presence_penalty != 0.0 or self.frequency_penalty != 0.0
+
+    @property
+    def processes_logits(self) -> bool:
+        return self.penalises or bool(self.logit_bias) or self.token_mask is not None
 
 
 @dataclass(eq=False)          # sequences are compared and hashed by identity (a field-wise == would walk the prompts)
@@ -90,6 +112,7 @@ class Scheduler:
         self.running: list[Sequence] = []
         self._ids = itertools.count()
         self.num_preemptions = 0
+        self.prefix: tuple[int, list[int]] | None = None     # cache id and tokens (whole blocks) that requests may begin with
 
     def add(self, prompt: list[int], params: SamplingParams, arrival: float = 0.0) -> Sequence:
         if not prompt:
@@ -117,6 +140,13 @@ class Scheduler:
             self.waiting.appendleft(victim)
             return True
         return False
+
+    def _begins_with_prefix(self, seq: Sequence) -> bool:
+        """Whether everything the shared prefix caches is the beginning of ``seq``, with a token behind it to run."""
+        if self.prefix is None:
+            return False
+        tokens = self.prefix[1]
+        return seq.total_len > len(tokens) and seq.token_slice(0, len(tokens)) == tokens
 
     # ---------------------------------------------------------------- one step
     def schedule(self, decode_tokens: int = 1) -> list[ScheduledSeq]:
@@ -159,10 +189,15 @@ class Scheduler:
         # 2. admit waiting requests
         while self.waiting and len(self.running) < self.max_num_seqs and budget > 0:
             seq = self.waiting[0]
-            new = min(seq.remaining_prefill, budget)
+            shares = self._begins_with_prefix(seq)
+            cached = len(self.prefix[1]) if shares else 0          # whole blocks: the new tokens start a block either way
+            new = min(seq.total_len - cached, budget)
             if not fits(seq, new):
                 break
             self.waiting.popleft()
+            if shares:
+                self.cache.fork(self.prefix[0], seq.request_id)
+                seq.computed = cached
             seq.status = SeqStatus.RUNNING
             self.running.append(seq)
             budget -= new

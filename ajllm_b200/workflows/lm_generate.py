@@ -3,7 +3,9 @@
 
 All prompts and their ``samples_per_prompt`` copies are submitted to the continuous-batching engine at
 once instead of being generated one after another; ``engine:`` may set ``block_size``,
-``max_num_seqs``, ``quantization: fp8`` and ``speculative: {draft_run_directory, k}``.
+``max_num_seqs``, ``quantization: fp8``, ``speculative: {draft_run_directory, k}`` and ``share_prefix: true``
+(what all prompts begin with is computed and read once). ``repetition_penalty``, ``presence_penalty``,
+``frequency_penalty`` and ``logit_bias`` (token id: bias) act on the logits before sampling.
 
 Launched with one process per GPU (``torchrun``), the model is served tensor-parallel over all ranks:
 every rank loads its slice of the checkpoint, row-parallel projections end in the fused
@@ -34,6 +36,15 @@ def read_prompts(data: dict[str, Any], project_root: Path) -> list[str]:
         text = project_path(project_root, data["prompt_file"]).read_text(encoding="utf-8")
         return [line.strip() for line in text.splitlines() if line.strip()]
     raise ValueError("Generation config requires prompts or prompt_file")
+
+
+def common_prefix(prompts: list[list[int]]) -> list[int]:
+    """The tokens that all prompts begin with, at least one less than the shortest has."""
+    if not prompts:
+        return []
+    low, high = min(prompts), max(prompts)
+    length = next((i for i, (a, b) in enumerate(zip(low, high)) if a != b), min(len(low), len(high)))
+    return low[:min(length, min(map(len, prompts)) - 1)]
 
 
 def run(config: LoadedConfig) -> dict[str, Any]:
@@ -77,14 +88,20 @@ def run(config: LoadedConfig) -> dict[str, Any]:
                        num_speculative_tokens=k or 4, seed=seed)
     prompts = read_prompts(data, config.project_root)
     encoded = [tokenizer.encode(p) or ([eos_id] if eos_id is not None else [0]) for p in prompts]
+    adjust = {key: float(data[key]) for key in ("repetition_penalty", "presence_penalty", "frequency_penalty")
+              if data.get(key) is not None}
+    if data.get("logit_bias"):
+        adjust["logit_bias"] = {int(token): float(bias) for token, bias in data["logit_bias"].items()}
     requests, owners = [], []
     for index, ids in enumerate(encoded):
         room = max(1, min(max_new, model.context_length + 1 - len(ids)))
         for sample in range(samples):
             requests.append((ids, SamplingParams(room, temperature, top_p, eos_id,
-                                                 seed=seed * 1_000_003 + index * 1009 + sample)))
+                                                 seed=seed * 1_000_003 + index * 1009 + sample, **adjust)))
             owners.append(index)
     started = time.perf_counter()
+    if engine_cfg.get("share_prefix") and len(requests) > 1:
+        engine.share_prefix(common_prefix(encoded))
     outputs = engine.generate([r[0] for r in requests], [r[1] for r in requests])
     elapsed = time.perf_counter() - started
     results = [{"prompt": p, "completions": []} for p in prompts]
@@ -99,7 +116,7 @@ def run(config: LoadedConfig) -> dict[str, Any]:
     payload = {
         "training_run": str(training_run), "checkpoint": checkpoint,
         "parameters": {"max_new_tokens": max_new, "temperature": temperature, "top_p": top_p,
-                       "samples_per_prompt": samples, "seed": seed},
+                       "samples_per_prompt": samples, "seed": seed, **adjust},
         "throughput": {"output_tokens": engine.stats.output_tokens, "elapsed_seconds": elapsed,
                        "output_tokens_per_second": engine.stats.output_tokens / max(elapsed, 1e-9)},
         "tensor_parallel": {"size": world, "backend": tp_backend(tp)},

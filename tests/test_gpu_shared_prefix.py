@@ -441,3 +441,112 @@ def test_process_logits_of_many_rows(rows, vocab, dtype, width, biases, masked, 
     want = reference.process_logits(logits, **args)               # the same fp32 steps, whole rows at a time
     assert torch.equal(got, want)
     assert torch.equal(got, serving.process_logits(logits.contiguous(), **args))
+
+
+# ----------------------------------------------------------------------------- the serving engine
+
+ENGINE_CFG = {"name": "s", "context_length": 512, "d_model": 512, "num_layers": 2, "num_heads": 4, "num_kv_heads": 2,
+              "d_ff": 1408, "init": {"type": "normal", "std": 0.05}}
+
+
+@pytest.fixture(scope="module")
+def engine_model():
+    from ajllm_b200.models import build_model
+    torch.manual_seed(0)
+    return build_model(ENGINE_CFG, 1000).to(device=torch.device("cuda", 0), dtype=torch.bfloat16)
+
+
+def _engine_prompts():
+    gen = torch.Generator().manual_seed(3)
+    head = torch.randint(0, 1000, (150,), generator=gen).tolist()
+    return head, [head + torch.randint(0, 1000, (n,), generator=gen).tolist() for n in (5, 40, 1, 130, 17, 64, 9)]
+
+
+@pytest.mark.parametrize("graphs", ["1", "0"])
+@pytest.mark.parametrize("count", [2, 7])
+def test_runner_steps_behind_a_prefix(engine_model, monkeypatch, graphs, count):
+    """Prefill and decoding steps behind a shared prefix against the model run on each whole sequence."""
+    from ajllm_b200.engine import LLMEngine
+    from ajllm_b200.engine.model_runner import RunItem
+    monkeypatch.setenv("AJB_DECODE_GRAPHS", graphs)
+    head, prompts = _engine_prompts()
+    engine = LLMEngine(engine_model, num_blocks=256)
+    assert engine.runner.use_graphs == (graphs == "1")
+    assert engine.share_prefix(head) == 144
+    parent = engine.scheduler.prefix[0]
+    sequences = [list(p) for p in prompts[:count]]
+    for i in range(count):
+        engine.cache.fork(parent, i)
+    calls = []
+    real = serving.shared_prefix_attention
+    monkeypatch.setattr(serving, "shared_prefix_attention", lambda *a, **k: calls.append(1) or real(*a, **k))
+    logits = engine.runner.forward([RunItem(i, s[144:], 1) for i, s in enumerate(sequences)])
+    assert not calls                                        # ragged: every sequence reads its own context
+    for step in range(3):
+        for i, sequence in enumerate(sequences):
+            with torch.no_grad():
+                want = engine_model(torch.tensor([sequence], device=logits.device))[0, -1].float()
+            assert float((logits[i] - want).abs().max()) < 0.08 * float(want.abs().max())
+            sequence.append(int(want.argmax()))
+        logits = engine.runner.forward([RunItem(i, s[-1:], 1) for i, s in enumerate(sequences)])
+    assert calls
+    before = len(engine.runner._graphs)
+    engine.release_prefix()
+    assert len(engine.runner._graphs) == (before - 1 if graphs == "1" else 0)
+    logits = engine.runner.forward([RunItem(i, [1], 1) for i in range(count)])       # the blocks outlive the prefix's own hold
+    with torch.no_grad():
+        want = engine_model(torch.tensor([sequences[0] + [1]], device=logits.device))[0, -1].float()
+    assert float((logits[0] - want).abs().max()) < 0.08 * float(want.abs().max())
+    assert native.lib().ajb_check_status() == 0
+
+
+def test_engine_serves_requests_behind_a_prefix(engine_model):
+    from ajllm_b200.engine import LLMEngine, SamplingParams
+    head, prompts = _engine_prompts()
+    params = SamplingParams(12, 0.0, None)
+    plain = LLMEngine(engine_model, num_blocks=256, max_num_seqs=4).generate(prompts, params)
+    engine = LLMEngine(engine_model, num_blocks=256, max_num_seqs=4)
+    engine.share_prefix(head)
+    graphs = engine.warm_up()
+    outs = engine.generate(prompts, params)
+    assert len(engine.runner._graphs) == graphs == 5           # 1, 2, 4 sequences, and 2 and 4 behind the prefix
+    # The logits are bf16: two evaluations that sum in another order can round a logit to neighbouring values, one step of
+    # 2^-8 to 2^-7 of it apart, so two logits that differ by two steps of the larger at most can change places. The first
+    # token that differs from the plain engine's has to be such a case (what follows it then differs for good).
+    for a, b in zip(plain, outs):
+        first = next((i for i, (x, y) in enumerate(zip(a.output, b.output)) if x != y), None)
+        if first is not None:
+            with torch.no_grad():
+                logits = engine_model(torch.tensor([a.prompt + a.output[:first]], device=_dev()))[0, -1].float()
+            one, other = float(logits[a.output[first]]), float(logits[b.output[first]])
+            assert abs(one - other) <= 2 * 2.0 ** -7 * max(abs(one), abs(other))
+    assert engine.cache.allocator.free_blocks == 256 - 9 - 1
+    assert native.lib().ajb_check_status() == 0
+
+
+def test_engine_processes_logits(engine_model):
+    """Penalties, biases and masks of a changing batch: every greedy token is the best of the formula on the model's logits."""
+    from ajllm_b200.engine import LLMEngine, SamplingParams
+    head, prompts = _engine_prompts()
+    words = torch.zeros(32, dtype=torch.int32)
+    words[5] = 0b1111
+    params = [SamplingParams(9, 0.0, None, repetition_penalty=1.3), SamplingParams(5, 0.0, None, frequency_penalty=2.0, presence_penalty=0.5),
+              SamplingParams(9, 0.0, None, token_mask=lambda output: words if len(output) < 4 else torch.zeros_like(words)),
+              SamplingParams(7, 0.0, None, logit_bias={3: 100.0}, frequency_penalty=30.0), SamplingParams(9, 0.0, None), None, None]
+    engine = LLMEngine(engine_model, num_blocks=256, max_num_seqs=3)
+    engine.share_prefix(head)
+    outs = engine.generate(prompts[:5], params[:5])
+    assert [len(o.output) for o in outs] == [9, 5, 4, 7, 9] and outs[2].finish_reason == "mask"
+    assert all(160 <= token < 164 for token in outs[2].output)
+    assert outs[3].output[:3] == [3, 3, 3] and outs[3].output != [3] * 7
+    for prompt, p, out in zip(prompts[:2], params[:2], outs[:2]):
+        tokens = list(prompt)
+        for token in out.output:
+            with torch.no_grad():
+                x = engine_model(torch.tensor([tokens], device=torch.device("cuda", 0)))[0, -1:].float().cpu()
+            one = lambda v: torch.tensor([v])
+            want = reference.process_logits(x, torch.tensor([tokens]).int(), one(len(prompt)).int(), one(len(tokens)).int(), one(p.repetition_penalty),
+                                            one(p.presence_penalty), one(p.frequency_penalty))[0]
+            assert float(want[token]) > float(want.max()) - 0.08 * float(x.abs().max())      # as far as the forwards may differ
+            tokens.append(token)
+    assert native.lib().ajb_check_status() == 0
