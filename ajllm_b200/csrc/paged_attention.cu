@@ -83,7 +83,9 @@ struct Params {
   int first_key;              // first cached token this launch looks at (a multiple of the block size)
   float scale;
   int splits;                 // CTAs per (sequence, KV head, chunk)
-  int prefix_splits;          // CTAs per KV head for the keys in front of first_key (0: not covered), ahead of the others
+  int prefix_splits;          // divisions of the keys in front of first_key (0: not covered); their CTAs are ahead of the others
+  int prefix_tokens;          // query tokens that one of these CTAs takes
+  int prefix_pieces;          // and how many of them a KV head's query tokens are
   int part_stride, part_base; // parts per row in the workspace and the first one of this launch; part_stride 0: no parts
   float* part_o;              // [tokens, Hq, part_stride, hd] fp32, un-normalised
   float2* part_ml;            // [tokens, Hq, part_stride] (reference maximum in log2 units, row sum); sum 0 = no keys seen
@@ -636,7 +638,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     const int first_block = p.first_key / BLOCK_TOKENS, table_end = p.max_blocks - 1;
     // The KV heads of a sequence are neighbours in the grid: their rows of a cache block are neighbours in memory, and
     // they are read at about the same time.
-    const int columns = p.kv_heads * p.chunks, prefix_ctas = p.kv_heads * p.prefix_splits;
+    const int columns = p.kv_heads * p.chunks, prefix_ctas = p.kv_heads * p.prefix_pieces * p.prefix_splits;
     int cta = blockIdx.x, ids_next = 0;
     bool ok = true, asked = false;
     uint32_t base = 0;                                // tiles of all pieces before this one, K and V counted
@@ -647,14 +649,16 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       Work w;
       int seq = 0, from_block = first_block;
       if (cta >= 0 && cta < prefix_ctas) {
-        // keys that all sequences share, for all their query rows at once
+        // keys that all sequences share, for as many of their query rows as the launch's CTAs hold
         from_block = 0;
-        const int split = cta / p.kv_heads, tiles = (p.first_key + DTILE - 1) / DTILE, each = (tiles + p.prefix_splits - 1) / p.prefix_splits;
-        w.kv_head = cta - split * p.kv_heads;
-        w.rows = p.seqs * p.q_total * p.group;
-        w.token0 = 0;
+        const int units = p.kv_heads * p.prefix_pieces, split = cta / units, unit = cta - split * units, piece_of = unit / p.kv_heads;
+        const int tiles = (p.first_key + DTILE - 1) / DTILE, each = (tiles + p.prefix_splits - 1) / p.prefix_splits;
+        w.kv_head = unit - piece_of * p.kv_heads;
+        w.token0 = piece_of * p.prefix_tokens;
+        const int tokens = min(p.prefix_tokens, p.seqs * p.q_total - w.token0);
+        w.rows = tokens * p.group;
         w.keys = p.first_key;
-        w.ctx = p.first_key + p.seqs * p.q_total - 1;
+        w.ctx = p.first_key + tokens - 1;
         w.t0 = min(tiles, split * each);
         w.n_tiles = min(tiles - w.t0, each);
         w.part = split;
@@ -1123,9 +1127,11 @@ static int launch_kernel(const Launch& a, cudaStream_t stream) {
   p.splits = a.splits; p.prefix_splits = a.prefix_splits; p.part_stride = a.part_stride; p.part_base = a.part_base;
   p.part_o = (float*)a.part_o; p.part_ml = (float2*)a.part_ml;
   static bool configured[5][kMaxDevices] = {};
-  const int rows = p.group * (a.prefix_splits > 0 ? a.num_seqs * a.q_total : a.q_len);
+  p.prefix_tokens = a.prefix_tokens;
+  p.prefix_pieces = a.prefix_splits > 0 ? (a.num_seqs * a.q_total + a.prefix_tokens - 1) / a.prefix_tokens : 0;
+  const int rows = p.group * (a.prefix_splits > 0 ? max(a.q_len, min(a.prefix_tokens, a.num_seqs * a.q_total)) : a.q_len);
   if (rows <= 32) {
-    const long long ctas = (long long)a.kv_heads * a.prefix_splits + (long long)a.num_seqs * a.kv_heads * p.chunks * a.splits;
+    const long long ctas = (long long)a.kv_heads * p.prefix_pieces * a.prefix_splits + (long long)a.num_seqs * a.kv_heads * p.chunks * a.splits;
     AJB_REQUIRE(ctas <= 0x7fffffffll, "paged attention: %lld CTAs are too many for one launch", ctas);
     const dim3 grid((unsigned)ctas);
     CUtensorMap map_k, map_v;
@@ -1143,7 +1149,7 @@ static int launch_kernel(const Launch& a, cudaStream_t stream) {
     if (rows <= 16) return launch_on(paged_decode_kernel<HD, 16>, configured[2], grid, smem16, map_k, map_v, p, a.beside_previous, stream);
     return launch_on(paged_decode_kernel<HD, 32>, configured[3], grid, smem32, map_k, map_v, p, a.beside_previous, stream);
   }
-  AJB_REQUIRE(a.prefix_splits == 0, "paged attention: a shared prefix for more than 32 query rows per KV head");
+  AJB_REQUIRE(a.prefix_splits == 0, "paged attention: more than 32 query rows per CTA cannot take a shared prefix along");
   AJB_REQUIRE((long long)a.kv_heads * p.chunks <= 65535, "paged attention: %d new tokens per sequence are too many for one launch", a.q_total);
   CUtensorMap map_k, map_v;
   const uint64_t row_pitch = (uint64_t)a.kv_heads * HD * 2;
@@ -1208,7 +1214,7 @@ extern "C" int ajb_paged_attention(const void* q, const void* k_cache, const voi
   a.q = q; a.k_cache = k_cache; a.v_cache = v_cache; a.block_tables = block_tables; a.context_lens = context_lens;
   a.q_start = q_start; a.out = out; a.q_pitch = (long long)heads * head_dim;
   a.num_seqs = num_seqs; a.num_blocks = num_blocks; a.max_blocks = max_blocks; a.heads = heads; a.kv_heads = kv_heads;
-  a.q_len = q_len; a.q_total = q_len; a.first_key = 0; a.scale = scale; a.splits = splits; a.prefix_splits = 0;
+  a.q_len = q_len; a.q_total = q_len; a.first_key = 0; a.scale = scale; a.splits = splits; a.prefix_splits = a.prefix_tokens = 0;
   a.part_stride = splits > 1 ? splits : 0; a.part_base = 0; a.part_o = part_o; a.part_ml = part_ml;
   a.map_k = a.map_v = nullptr; a.beside_previous = false;
   int rc = paged::launch(a, head_dim, s);

@@ -18,8 +18,8 @@ struct Launch {
   float scale;
   int splits;                   // parts this launch leaves per row
   int prefix_splits;            // > 0: this launch also covers the keys in front of first_key, the same for all sequences (row 0
-                                // of the tables), divided over that many CTAs per KV head whose parts come first; at most 32
-                                // query rows per KV head in all
+                                // of the tables), divided in that many parts per row, which come first; at most 32 query
+  int prefix_tokens;            // rows per CTA: so many tokens of the batch for these keys, q_len tokens of a sequence for its own
   int part_stride, part_base;   // parts per row in the workspace, first one of this launch; stride 0: no parts, `out` is written
   void *part_o, *part_ml;
   const CUtensorMap *map_k, *map_v;   // of make_tensor_map_cache, when the caller has them already (else null)

@@ -459,15 +459,16 @@ static int launch_prefix(const paged::Launch& a, int shared, int splits, cudaStr
 
 // q [num_seqs * q_len, heads, head_dim] bf16 with q_pitch elements between tokens, out the same, contiguous; the first
 // `shared` tokens (a multiple of 16; 0: plain paged attention) of every sequence are the ones that the first row of
-// block_tables names. The prefix is divided over prefix_splits CTAs per (256 query rows, KV head); parts = what they and
-// the suffix launch leave per row: suffix_splits, and prefix_splits more, or twice as many when a KV head has 33 to 128 query
-// rows in all and a CTA more than one tile of 128 keys. part_o holds num_seqs * q_len * heads * parts * head_dim floats,
+// block_tables names. With prefix_tokens > 0 it is pieces of the paged launch, prefix_splits of them for each KV head and
+// prefix_tokens query tokens (32 query rows at most); otherwise the prefix kernel divides it over prefix_splits CTAs per
+// (256 query rows, KV head). parts = what is left per row: suffix_splits, and prefix_splits more, or twice as many when the
+// prefix kernel has at most 128 query rows per KV head and a CTA more than one tile of 128 keys. part_o holds num_seqs * q_len * heads * parts * head_dim floats,
 // part_ml two per part.
 extern "C" int ajb_shared_prefix_attention(const void* q, const void* k_cache, const void* v_cache, const void* block_tables,
                                            const void* context_lens, void* out, long long q_pitch, int num_seqs,
                                            int num_blocks, int block_size, int max_blocks, int heads, int kv_heads,
-                                           int head_dim, int q_len, int shared, float scale, int prefix_splits,
-                                           int suffix_splits, int parts, void* part_o, void* part_ml, void* stream) {
+                                           int head_dim, int q_len, int shared, float scale, int prefix_tokens,
+                                           int prefix_splits, int suffix_splits, int parts, void* part_o, void* part_ml, void* stream) {
   using namespace ajb;
   AJB_REQUIRE(block_size == prefix::BLOCK_TOKENS, "shared prefix attention: cache block size must be %d", prefix::BLOCK_TOKENS);
   AJB_REQUIRE(head_dim == 64 || head_dim == 128, "shared prefix attention: head_dim %d is not supported (64 and 128 are)", head_dim);
@@ -478,7 +479,9 @@ extern "C" int ajb_shared_prefix_attention(const void* q, const void* k_cache, c
   AJB_REQUIRE((long long)num_seqs * q_len * (heads / kv_heads) <= (1ll << 30), "shared prefix attention: too many query rows");
   const int group = heads / kv_heads, tiles = (shared + prefix::TILE - 1) / prefix::TILE;
   const int rows = num_seqs * q_len * group;      // query rows per KV head
-  const bool few = rows <= 32;                    // the paged kernel takes the prefix along
+  const bool few = prefix_tokens > 0;             // the paged kernel takes the prefix along
+  AJB_REQUIRE(!few || (shared > 0 && prefix_tokens * group <= 32 && q_len * group <= 32),
+              "shared prefix attention: CTAs of %d and %d tokens with %d query heads each are too large", prefix_tokens, q_len, group);
   AJB_REQUIRE((prefix_splits > 0) == (shared > 0) && prefix_splits >= 0 && prefix_splits <= (tiles > 0 ? tiles : 0) &&
                   suffix_splits >= 1 && part_o != nullptr && part_ml != nullptr,
               "shared prefix attention: %d and %d divisions of %d shared tokens and of the rest do not fit, or there is no workspace",
@@ -498,6 +501,7 @@ extern "C" int ajb_shared_prefix_attention(const void* q, const void* k_cache, c
   a.first_key = shared; a.scale = scale; a.splits = suffix_splits; a.part_stride = parts;
   a.part_base = prefix_parts; a.part_o = part_o; a.part_ml = part_ml; a.beside_previous = shared > 0 && !few;
   a.prefix_splits = few ? prefix_splits : 0;
+  a.prefix_tokens = prefix_tokens;
   CUtensorMap map_k, map_v;
   int rc = make_tensor_map_cache(&map_k, a.k_cache, a.num_blocks, a.kv_heads, head_dim);
   if (rc == 0) rc = make_tensor_map_cache(&map_v, a.v_cache, a.num_blocks, a.kv_heads, head_dim);

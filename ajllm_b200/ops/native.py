@@ -71,7 +71,7 @@ _SIGNATURES: dict[str, list] = {
     "ajb_sample_rows": [c_void, c_long, c_int, c_int, c_void, c_void, c_void, c_void, c_void, c_int, c_void, c_void],
     "ajb_spec_verify": [c_void, c_void, c_void, c_int, c_int, c_int, c_void, c_void, c_void, c_void, c_void],
     "ajb_paged_attention": [c_void] * 7 + [c_int] * 8 + [c_float, c_int, c_void, c_void, c_void],
-    "ajb_shared_prefix_attention": [c_void] * 6 + [c_long] + [c_int] * 9 + [c_float, c_int, c_int, c_int, c_void, c_void, c_void],
+    "ajb_shared_prefix_attention": [c_void] * 6 + [c_long] + [c_int] * 9 + [c_float, c_int, c_int, c_int, c_int, c_void, c_void, c_void],
     "ajb_batch_maps": [c_void] * 4 + [c_int] * 6 + [c_void] * 6,
     "ajb_process_logits": [c_void, c_int, c_long, c_void, c_int, c_int, c_void, c_long, c_int] + [c_void] * 7 + [c_int, c_void, c_long, c_void],
     "ajb_flash_bwd": [c_void, c_void, c_void, c_void, c_void, c_void, c_void, c_int, c_int, c_int, c_int, c_int,

@@ -250,52 +250,94 @@ def batch_maps(block_ids: torch.Tensor, block_counts: torch.Tensor, cached_lens:
 # ----------------------------------------------------------------------------- attention behind a shared prefix
 
 _PREFIX_TILE = 128         # query rows and keys per step of the prefix kernel
+_EXPECTED_SUFFIX = 256     # tokens behind the prefix when the caller gives no bound: block tables are often much wider than contexts
 
 
 @functools.lru_cache(maxsize=4096)
-def prefix_plan(n: int, q_len: int, group: int, kv_heads: int, head_dim: int, shared: int, behind: int) -> tuple[int, int, int]:
-    """How a call of :func:`shared_prefix_attention` is divided: ``(CTAs that share the prefix per 256 query rows and KV
-    head, CTAs that share a suffix, parts per row in all)``.
-
-    A CTA of the prefix kernel keeps an SM to itself while the others stream the (sequence, KV head) suffixes of up to
-    ``behind`` tokens, so the SMs are divided like the work. Measured beside a running suffix launch: a prefix CTA takes
-    about 14 us and 2 us more per step (128 keys for up to 256 rows; two tiles make a step when 128 rows are all there are),
-    a suffix occupies half an SM for 1.3 us and 2.7 us (64-wide heads: 1.3 us) per 128 keys, of which half the bound is
-    taken; a part costs its fp32 rows, written and read once at 4 TB/s. With more prefix CTAs than 7 in 10 SMs the suffix
-    hardly runs before they end (33 x 5 rows behind 4001 tokens: 28 us with 96 CTAs, 37 us with 120). Up to 32 rows per KV
-    head both are pieces of one launch, two to an SM, and a piece takes about as long for its first tile as for three more.
-    """
+def prefix_plan(n: int, q_len: int, group: int, kv_heads: int, head_dim: int, shared: int, behind: int,
+                expected: int) -> tuple[int, int, int, int]:
+    """How a call of :func:`shared_prefix_attention` is divided: ``(query tokens per piece of the prefix in the paged launch,
+    or 0 for the prefix kernel; divisions of the prefix; divisions of a suffix; parts per row in all)``. Suffixes have at most
+    ``behind`` tokens and about ``expected`` at the most. Whichever of the two forms is estimated to end first is taken (in
+    us, from measurements of 16 to 1024 query rows per KV head, prefixes of 512 to 7680 and suffixes of 32 to 1024 tokens)."""
     if not _SM_COUNT:
         _SM_COUNT.append(int(native.lib().ajb_sm_count()))
     sms = _SM_COUNT[0]
     chunk = q_len if group * q_len <= 32 else max(1, min(q_len, _PREFIX_TILE // group))
     pieces = n * kv_heads * -(-q_len // chunk)
-    splits = paged_splits(pieces, behind)
+    # where the suffixes are not known to be long, they are divided as if alone, which costs little if they are short
+    bound_splits = paged_splits(pieces, behind)
     if not shared:
-        return 0, splits, splits
+        return 0, 0, bound_splits, bound_splits
+    tiles, suffix_tiles = -(-shared // _PREFIX_TILE), -(-expected // _PREFIX_TILE)
+    divisions = {min(8, bound_splits)} if expected < behind else range(1, min(16, max(1, suffix_tiles)) + 1)
     rows = n * q_len * group
-    tiles = -(-shared // _PREFIX_TILE)
-    if rows <= 32:
-        ours = max(1, min(tiles, 32, (2 * sms - pieces * splits) // kv_heads))
-        each = -(-tiles // ours)
-        ours = -(-tiles // each)                # the same longest piece from as few CTAs as give it
-        return ours, splits, ours + splits
+    least = 3.0 + (n * expected + shared) * kv_heads * head_dim * 4 / 6.5e6       # reading the caches once
+    best = _kernel_plan(rows, pieces, kv_heads, head_dim, tiles, suffix_tiles, expected, divisions, least, sms)
+    if group * q_len <= 32:
+        best = min(best, _pieces_plan(n, q_len, group, kv_heads, head_dim, tiles, suffix_tiles, divisions, least, sms))
+    return best[1]
+
+
+def _pieces_plan(n, q_len, group, kv_heads, head_dim, tiles, suffix_tiles, divisions, least, sms):
+    """The prefix in pieces of the paged launch, for 16 query rows each (32 where a sequence has more than 16): a second read
+    of the prefix from L2 costs less than pieces of 32 rows, of which an SM holds one instead of two (8 sequences of 4 rows,
+    512 + 32 tokens: 9.0 us against 10.7). A piece takes 3 us and 1.1 us per 128 keys (32 rows: 1.5 us)."""
+    height = 16 if group * q_len <= 16 else 32
+    tokens = height // group
+    slots = sms * (2 if height == 16 or head_dim == 64 else 1)
+    step = 1.1 if height == 16 else 1.5
+    units = kv_heads * -(-n * q_len // tokens)
+    per_part = 0.1 + 0.0005 * n * q_len * group * kv_heads
+    best = (math.inf, (0, 0, 0, 0))
+    for splits in divisions:
+        back, back_time = n * kv_heads * max(1, min(splits, suffix_tiles)), 3.0 + step * -(-suffix_tiles // splits)
+        for ours in sorted({-(-tiles // length) for length in range(1, tiles + 1)}):
+            if ours > 32:
+                break
+            front_time = 3.0 + step * -(-tiles // ours)
+            # the prefix's pieces start first; the suffixes fill the slots beside them, then those behind them
+            rounds, front = divmod(units * ours - 1, slots)
+            front += 1
+            k = -(-back // slots)
+            while (slots - front) * k + front * max(0, int((k * back_time - front_time) / back_time)) < back:
+                k += 1
+            time = max(rounds * front_time + max(front_time, k * back_time) + 3.0, least) + per_part * (ours + splits)
+            best = min(best, (time, (tokens, ours, splits, ours + splits)))
+    return best
+
+
+def _kernel_plan(rows, pieces, kv_heads, head_dim, tiles, suffix_tiles, expected, divisions, least, sms):
+    """The prefix kernel beside the suffixes' launch. A CTA of it keeps an SM to itself while the others stream the suffixes,
+    so the SMs are divided like the work: a prefix CTA takes about 14 us and 2 us more per step (128 keys for up to 256 rows;
+    two tiles make a step when 128 rows are all there are, and it starts 3 us sooner), a suffix occupies half an SM for 1.3 us
+    and 2.7 us (64-wide heads: 1.3 us) per 128 keys; a part costs its fp32 rows, written and read once at 4 TB/s. With more
+    prefix CTAs than 7 in 10 SMs the suffixes hardly run before they end (33 x 5 rows behind 4001 tokens: 28 us with 96 CTAs,
+    37 us with 120)."""
     one_tile = rows <= _PREFIX_TILE
     units = kv_heads * (1 if one_tile else -(-rows // (2 * _PREFIX_TILE)))
-    suffix = pieces * (0.65 + (1.35 if head_dim == 128 else 0.65) * (behind / 256 + 0.5))
-    best = (math.inf, 1, 1)
-    for ours in range(1, min(tiles, 32) + 1):
-        if ours > 1 and units * ours > sms:
-            break
-        each = -(-tiles // ours)
-        parts = 2 * ours if one_tile and ours < tiles else ours
-        last = 14.0 + (1.0 if one_tile else 2.0) * each
-        time = max(last, (units * ours * last + suffix) / sms) + parts * rows * kv_heads * head_dim * 8 / 4e6
-        if 10 * units * ours > 7 * sms:
-            time += 8.0 + suffix / sms
-        if time < best[0]:
-            best = (time, ours, parts)
-    return best[1], splits, best[2] + splits
+    step = 1.35 if head_dim == 128 else 0.65
+    suffix = pieces * (0.65 + step * (expected / 256 + 0.5))
+    per_part = rows * kv_heads * head_dim * 8 / 4e6
+    best = (math.inf, (0, 0, 0, 0))
+    for splits in divisions:
+        if splits > 1 and pieces * splits > 2 * sms:
+            continue
+        chain = 6.0 + 1.35 * -(-suffix_tiles // splits)
+        for ours in range(1, min(tiles, 32) + 1):
+            if ours > 1 and units * ours > sms:
+                break
+            parts = 2 * ours if one_tile and ours < tiles else ours
+            if parts + splits > 64:
+                continue
+            last = 11.0 + -(-tiles // ours) if one_tile else 14.0 + 2.0 * -(-tiles // ours)
+            time = max(least, last, chain, (units * ours * last + suffix) / sms) + 0.1 * last + (parts + splits) * per_part
+            if 10 * units * ours > 7 * sms:
+                time += 8.0 + suffix / sms
+            best = min(best, (time, (0, ours, splits, parts + splits)))
+    if best[1][1] == 0:          # more suffixes than the divisions allow for
+        return _kernel_plan(rows, pieces, kv_heads, head_dim, tiles, suffix_tiles, expected, {1}, least, sms)
+    return best
 
 
 def shared_prefix_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -312,8 +354,8 @@ def shared_prefix_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cach
     (``context_lens[i] - q_len >= prefix_len``): the whole prefix is visible to every row. A prefix that ends inside a
     block is shared up to that block. Heads are 64 or 128 wide, ``Hq / Hkv`` is at most 128.
 
-    ``max_context``: a host-side bound on the context lengths (default: what the tables can hold) from which the
-    number of parts per sequence is chosen. A row whose sequence has no token at all comes out as zeros. ``scale``
+    ``max_context``: a host-side bound on the context lengths from which the number of parts per sequence is chosen (without
+    one: what the tables can hold, but the work is divided for suffixes of up to 256 tokens). It bounds nothing that is read. A row whose sequence has no token at all comes out as zeros. ``scale``
     defaults to ``1 / sqrt(hd)``; ``out`` (contiguous, like ``q``) receives the result.
     """
     if q.dim() != 3 or key_cache.dim() != 4 or block_tables.dim() != 2:
@@ -360,14 +402,15 @@ def shared_prefix_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cach
     group = heads // kv_heads
     room = max_blocks * block_size
     behind = max(0, (room if max_context is None else min(max_context, room)) - shared)
-    prefix_splits, splits, parts = prefix_plan(n, q_len, group, kv_heads, head_dim, shared, behind)
+    expected = behind if max_context is not None else min(behind, _EXPECTED_SUFFIX)
+    prefix_tokens, prefix_splits, splits, parts = prefix_plan(n, q_len, group, kv_heads, head_dim, shared, behind, expected)
     # fp32 parts of every (row, head): un-normalised outputs, then (reference maximum, sum) pairs
     count = total * heads * parts
     workspace = torch.empty(count * (head_dim + 2), dtype=_F32, device=q.device)
     parts_at = workspace.data_ptr()
     native.call("ajb_shared_prefix_attention", q.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
                 context_lens.data_ptr(), out.data_ptr(), q.stride(0), n, num_blocks, block_size, max_blocks, heads, kv_heads,
-                head_dim, q_len, shared, scale, prefix_splits, splits, parts, parts_at, parts_at + 4 * count * head_dim,
+                head_dim, q_len, shared, scale, prefix_tokens, prefix_splits, splits, parts, parts_at, parts_at + 4 * count * head_dim,
                 native.stream_ptr())
     return out
 

@@ -187,6 +187,27 @@ def test_shared_prefix_attention(heads, kv_heads, hd, q_len, prefix, suffixes):
     _check_attention(got, *_oracle(q, keys, values, tables, context, q_len))
 
 
+@pytest.mark.parametrize("heads,kv_heads,hd,q_len,prefix,suffixes", [
+    (32, 2, 128, 1, 300, list(range(1, 34))),            # 16 rows per sequence, so many pieces of the prefix
+    (64, 2, 128, 1, 700, [1, 40, 7]),                    # 32 rows per sequence
+    (20, 4, 128, 1, 513, [1, 5, 200, 16, 17, 3, 8]),     # 5 heads per KV head: pieces of 15 rows, the last one of 5
+    (14, 2, 64, 2, 1000, [2, 30, 100]),                  # 14 rows per sequence: a piece of two tokens may span sequences
+    (8, 8, 128, 5, 640, [5, 129, 6, 7]),                 # one head per KV head: pieces of 16 tokens out of 20
+    (12, 4, 64, 7, 130, [7, 8, 300]),                    # 21 rows per sequence: pieces of 10 tokens out of 21
+    (8, 2, 128, 1, 4096, [3, 900] * 12),                 # few long pieces
+])
+def test_prefixes_in_pieces_of_the_paged_launch(heads, kv_heads, hd, q_len, prefix, suffixes, monkeypatch):
+    """The same through pieces of several sizes, whatever the plan would take, and through the prefix kernel."""
+    q, keys, values, tables, context = _batch(heads, kv_heads, hd, q_len, prefix, suffixes)
+    want = _oracle(q, keys, values, tables, context, q_len)
+    group, tiles, rows = heads // kv_heads, -(-(prefix // 16) // 8), len(suffixes) * q_len * heads // kv_heads
+    tokens = (16 if group * q_len <= 16 else 32) // group
+    for pieces_of, ours, splits in ((tokens, 1, 1), (tokens, tiles, 3), (1, min(tiles, 2), 2), (0, 1, 1), (0, tiles, 2)):
+        parts = splits + (2 * ours if pieces_of == 0 and rows <= 128 and ours < tiles else ours)
+        monkeypatch.setattr(serving, "prefix_plan", lambda *a: (pieces_of, ours, splits, parts))
+        _check_attention(serving.shared_prefix_attention(q, keys, values, tables, context, prefix, q_len=q_len), *want)
+
+
 def test_shared_prefix_attention_with_large_scores_and_a_given_scale():
     """Scores of several hundred: the running maximum moves again and again, within the prefix and behind it."""
     q, keys, values, tables, context = _batch(8, 2, 128, 1, 640, [40, 300, 9], seed=3)

@@ -138,6 +138,26 @@ def test_shared_prefix_attention_refuses_its_query_as_output():
         serving.shared_prefix_attention(**call, out=call["q"])
 
 
+def test_division_of_shared_prefix_attention_is_one_that_the_kernels_take(monkeypatch):
+    """Over the whole range of sizes: the limits that the entry point checks, and every key in some part."""
+    monkeypatch.setattr(serving, "_SM_COUNT", [148])
+    rng = random.Random(4)
+    for _ in range(4000):
+        n, q_len = int(2 ** rng.uniform(0, 10)), rng.choice([1, 1, 1, 2, 5, 17, 300])
+        group, kv_heads, hd = rng.choice([1, 2, 4, 6, 8, 16, 32, 71, 128]), rng.choice([1, 2, 8, 16, 32]), rng.choice([64, 128])
+        shared, behind = 16 * int(2 ** rng.uniform(-1, 11)), int(2 ** rng.uniform(-1, 15))
+        expected = rng.choice([behind, min(behind, 256)])
+        tokens, ours, splits, parts = serving.prefix_plan(n, q_len, group, kv_heads, hd, shared, behind, expected)
+        tiles, rows = -(-shared // 128), n * q_len * group
+        if not shared:
+            assert (tokens, ours) == (0, 0) and parts == splits >= 1
+            continue
+        assert 1 <= ours <= min(tiles, 32) and 1 <= splits <= 16 and parts <= 64
+        assert tokens == 0 or (tokens * group <= 32 and q_len * group <= 32)
+        twice = tokens == 0 and rows <= 128 and ours < tiles
+        assert parts == splits + (2 * ours if twice else ours)
+
+
 def _formula(x, history, prompt, total, repetition, presence, frequency, biases, allowed):
     """One row of processed logits, token by token, in 64 bits."""
     out = []
