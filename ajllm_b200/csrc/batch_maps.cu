@@ -152,10 +152,19 @@ __global__ void __launch_bounds__(kThreads) batch_maps_kernel(const Params p) {
 // ids [n_ids] block ids of all sequences, one after another; counts / cached / q_lens [seqs]; all int32 on the device.
 // tables [seqs, width], positions [total], slots [total] (int64), q_start [seqs + 1], context [seqs]; tables, positions
 // and slots 16-byte aligned.
-extern "C" int ajb_batch_maps(const void* ids, const void* counts, const void* cached, const void* q_lens, int n_ids, int seqs,
-                              int total, int width, int block_size, int pad, void* tables, void* positions, void* slots,
-                              void* q_start, void* context, void* stream) {
+struct BatchMapsArgs {          // laid out by ops/native.py
+  int size;
+  const void *ids, *counts, *cached, *q_lens;
+  int n_ids, seqs, total, width, block_size, pad;
+  void *tables, *positions, *slots, *q_start, *context, *stream;
+};
+
+extern "C" int ajb_batch_maps(const void* arguments) {
   using namespace ajb;
+  const BatchMapsArgs& args = *static_cast<const BatchMapsArgs*>(arguments);
+  AJB_REQUIRE(args.size == (int)sizeof(args), "batch maps: arguments of %d bytes, not %d", args.size, (int)sizeof(args));
+  const auto& [size, ids, counts, cached, q_lens, n_ids, seqs, total, width, block_size, pad, tables,
+               positions, slots, q_start, context, stream] = args;
   AJB_REQUIRE(seqs >= 0 && seqs <= maps::kMaxSeqs, "batch maps: %d sequences (at most %d)", seqs, maps::kMaxSeqs);
   AJB_REQUIRE(total >= 0 && total <= maps::kCap && n_ids >= 0 && n_ids <= maps::kCap && width >= 1 && block_size >= 1,
               "batch maps: %d tokens, %d block ids, %d blocks per table row, %d tokens per block are out of range", total, n_ids,

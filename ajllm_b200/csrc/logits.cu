@@ -436,12 +436,30 @@ __global__ void __launch_bounds__(kMendThreads, 6) mend_logits_kernel(const Para
 // logits [rows, vocab] (dtype 0: bf16, 1: fp32) with in_pitch elements between rows; out fp32 [rows, vocab] contiguous,
 // not overlapping the logits. Null pointers switch the parts off: history (with lens), repetition / presence /
 // frequency, bias_ids (biases = 0), mask.
-extern "C" int ajb_process_logits(const void* logits, int dtype, long long in_pitch, void* out, int rows, int vocab,
-                                  const void* history, long long history_pitch, int history_width, const void* prompt_lens,
-                                  const void* history_lens, const void* repetition, const void* presence,
-                                  const void* frequency, const void* bias_ids, const void* bias_values, int biases,
-                                  const void* mask, long long mask_pitch, void* stream) {
+struct ProcessLogitsArgs {          // laid out by ops/native.py
+  int size;
+  const void *logits;
+  int dtype;
+  long long in_pitch;
+  void *out;
+  int rows, vocab;
+  const void *history;
+  long long history_pitch;
+  int history_width;
+  const void *prompt_lens, *history_lens, *repetition, *presence, *frequency, *bias_ids, *bias_values;
+  int biases;
+  const void *mask;
+  long long mask_pitch;
+  void *stream;
+};
+
+extern "C" int ajb_process_logits(const void* arguments) {
   using namespace ajb;
+  const ProcessLogitsArgs& args = *static_cast<const ProcessLogitsArgs*>(arguments);
+  AJB_REQUIRE(args.size == (int)sizeof(args), "process logits: arguments of %d bytes, not %d", args.size, (int)sizeof(args));
+  const auto& [size, logits, dtype, in_pitch, out, rows, vocab, history, history_pitch, history_width,
+               prompt_lens, history_lens, repetition, presence, frequency, bias_ids, bias_values, biases,
+               mask, mask_pitch, stream] = args;
   AJB_REQUIRE(dtype == 0 || dtype == 1, "process logits: unknown type %d", dtype);
   AJB_REQUIRE(rows >= 0 && vocab >= 1 && vocab <= (1 << 30) && history_width >= 0 && biases >= 0, "process logits: sizes out of range");
   AJB_REQUIRE(history == nullptr || (prompt_lens != nullptr && history_lens != nullptr), "process logits: a history comes with its lengths");

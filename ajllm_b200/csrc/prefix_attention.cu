@@ -462,14 +462,26 @@ static int launch_prefix(const paged::Launch& a, int shared, int splits, cudaStr
 // block_tables names. With prefix_tokens > 0 it is pieces of the paged launch, prefix_splits of them for each KV head and
 // prefix_tokens query tokens (32 query rows at most); otherwise the prefix kernel divides it over prefix_splits CTAs per
 // (256 query rows, KV head). parts = what is left per row: suffix_splits, and prefix_splits more, or twice as many when the
-// prefix kernel has at most 128 query rows per KV head and a CTA more than one tile of 128 keys. part_o holds num_seqs * q_len * heads * parts * head_dim floats,
-// part_ml two per part.
-extern "C" int ajb_shared_prefix_attention(const void* q, const void* k_cache, const void* v_cache, const void* block_tables,
-                                           const void* context_lens, void* out, long long q_pitch, int num_seqs,
-                                           int num_blocks, int block_size, int max_blocks, int heads, int kv_heads,
-                                           int head_dim, int q_len, int shared, float scale, int prefix_tokens,
-                                           int prefix_splits, int suffix_splits, int parts, void* part_o, void* part_ml, void* stream) {
+// prefix kernel has at most 128 query rows per KV head and a CTA more than one tile of 128 keys. part_o holds
+// num_seqs * q_len * heads * parts * head_dim floats, part_ml two per part.
+struct SharedPrefixArgs {          // laid out by ops/native.py
+  int size;
+  const void *q, *k_cache, *v_cache, *block_tables, *context_lens;
+  void *out;
+  long long q_pitch;
+  int num_seqs, num_blocks, block_size, max_blocks, heads, kv_heads, head_dim, q_len, shared;
+  float scale;
+  int prefix_tokens, prefix_splits, suffix_splits, parts;
+  void *part_o, *part_ml, *stream;
+};
+
+extern "C" int ajb_shared_prefix_attention(const void* arguments) {
   using namespace ajb;
+  const SharedPrefixArgs& args = *static_cast<const SharedPrefixArgs*>(arguments);
+  AJB_REQUIRE(args.size == (int)sizeof(args), "shared prefix attention: arguments of %d bytes, not %d", args.size, (int)sizeof(args));
+  const auto& [size, q, k_cache, v_cache, block_tables, context_lens, out, q_pitch, num_seqs, num_blocks,
+               block_size, max_blocks, heads, kv_heads, head_dim, q_len, shared, scale, prefix_tokens,
+               prefix_splits, suffix_splits, parts, part_o, part_ml, stream] = args;
   AJB_REQUIRE(block_size == prefix::BLOCK_TOKENS, "shared prefix attention: cache block size must be %d", prefix::BLOCK_TOKENS);
   AJB_REQUIRE(head_dim == 64 || head_dim == 128, "shared prefix attention: head_dim %d is not supported (64 and 128 are)", head_dim);
   AJB_REQUIRE(kv_heads >= 1 && heads % kv_heads == 0 && heads / kv_heads <= prefix::ROWS && q_len >= 1,

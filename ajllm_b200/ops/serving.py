@@ -154,12 +154,17 @@ def spec_verify(target_logits: torch.Tensor, draft_logits: torch.Tensor, draft_t
 # A small operator takes a few microseconds on the device, so its argument checks are one expression over cheap
 # attributes; only when it fails are the arguments gone through one by one for the message.
 _I32, _I64, _F32, _BF16 = torch.int32, torch.int64, torch.float32, torch.bfloat16
+_CONTIGUOUS = torch.contiguous_format
 
 
 def _dense(op: str, name: str, t: torch.Tensor, dtype: torch.dtype, device: torch.device, shape: tuple[int, ...]) -> None:
     if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{op}: {name} must be a contiguous {dtype} tensor of shape {list(shape)} on {device} "
                          f"(got {t.dtype} {list(t.shape)} on {t.device}, strides {t.stride()})")
+
+
+def _ptr(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -232,7 +237,7 @@ def batch_maps(block_ids: torch.Tensor, block_counts: torch.Tensor, cached_lens:
         for mine, theirs in zip(out, found):
             mine.copy_(theirs)
         return BatchMaps(*out)
-    if index != torch.cuda.current_device():
+    if index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):
             return batch_maps(block_ids, block_counts, cached_lens, q_lens, total_tokens, max_blocks, block_size=block_size,
                               pad_block=pad_block, out=out)
@@ -241,9 +246,9 @@ def batch_maps(block_ids: torch.Tensor, block_counts: torch.Tensor, cached_lens:
         tables, positions = torch.empty(n, max_blocks, dtype=_I32, device=device), torch.empty(total_tokens, dtype=_I32, device=device)
         slots = torch.empty(total_tokens, dtype=_I64, device=device)
         q_start, context_lens = torch.empty(n + 1, dtype=_I32, device=device), torch.empty(n, dtype=_I32, device=device)
-    native.call("ajb_batch_maps", block_ids.data_ptr(), block_counts.data_ptr(), cached_lens.data_ptr(), q_lens.data_ptr(),
+    native.call_packed("ajb_batch_maps", block_ids.data_ptr(), block_counts.data_ptr(), cached_lens.data_ptr(), q_lens.data_ptr(),
                 block_ids.shape[0], n, total_tokens, max_blocks, block_size, pad_block, tables.data_ptr(), positions.data_ptr(),
-                slots.data_ptr(), q_start.data_ptr(), context_lens.data_ptr(), native.stream_ptr())
+                slots.data_ptr(), q_start.data_ptr(), context_lens.data_ptr(), native.stream_ptr(index))
     return BatchMaps(tables, positions, slots, q_start, context_lens)
 
 
@@ -388,14 +393,21 @@ def shared_prefix_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cach
         return found if out is None else out.copy_(found)
     if dtype is not _BF16:
         raise TypeError(f"shared_prefix_attention: CUDA tensors must be bfloat16 (got {dtype})")
-    if index != torch.cuda.current_device():
+    if index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):
             return shared_prefix_attention(q, key_cache, value_cache, block_tables, context_lens, prefix_len, q_len=q_len,
                                            scale=scale, max_context=max_context, out=out)
-    if q.stride(2) != 1 or q.stride(1) != head_dim or q.stride(0) % 8 or q.data_ptr() % 16:
-        q = q.contiguous()
+    q_at, pitch = q.data_ptr(), heads * head_dim
+    if not q.is_contiguous():
+        pitch = q.stride(0)
+        if q.stride(2) != 1 or q.stride(1) != head_dim or pitch % 8:
+            q, pitch = q.contiguous(), heads * head_dim
+            q_at = q.data_ptr()
+    if q_at % 16:
+        q, pitch = q.clone(memory_format=_CONTIGUOUS), heads * head_dim
+        q_at = q.data_ptr()
     if out is None:
-        out = q.new_empty(q.shape)
+        out = torch.empty_like(q, memory_format=_CONTIGUOUS)
     if total == 0:
         return out
     shared = prefix_len // block_size * block_size
@@ -408,10 +420,10 @@ def shared_prefix_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cach
     count = total * heads * parts
     workspace = torch.empty(count * (head_dim + 2), dtype=_F32, device=q.device)
     parts_at = workspace.data_ptr()
-    native.call("ajb_shared_prefix_attention", q.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
-                context_lens.data_ptr(), out.data_ptr(), q.stride(0), n, num_blocks, block_size, max_blocks, heads, kv_heads,
+    native.call_packed("ajb_shared_prefix_attention", q_at, key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
+                context_lens.data_ptr(), out.data_ptr(), pitch, n, num_blocks, block_size, max_blocks, heads, kv_heads,
                 head_dim, q_len, shared, scale, prefix_tokens, prefix_splits, splits, parts, parts_at, parts_at + 4 * count * head_dim,
-                native.stream_ptr())
+                native.stream_ptr(index))
     return out
 
 
@@ -480,7 +492,7 @@ def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
         found = reference.process_logits(logits, history, prompt_lens, history_lens, repetition, presence, frequency, bias_ids,
                                          bias_values, token_mask)
         return found if out is None else out.copy_(found)
-    if index != torch.cuda.current_device():
+    if index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):
             return process_logits(logits, history=history, prompt_lens=prompt_lens, history_lens=history_lens, repetition=repetition,
                                   presence=presence, frequency=frequency, bias_ids=bias_ids, bias_values=bias_values,
@@ -489,8 +501,8 @@ def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
         logits = logits.contiguous()
     if out is None:
         out = torch.empty(rows, vocab, dtype=_F32, device=logits.device)
-    native.call("ajb_process_logits", logits.data_ptr(), 1 if dtype is _F32 else 0, logits.stride(0), out.data_ptr(),
-                rows, vocab, native.ptr(history) if width else None, width, width, native.ptr(prompt_lens), native.ptr(history_lens),
-                native.ptr(repetition), native.ptr(presence), native.ptr(frequency), native.ptr(bias_ids), native.ptr(bias_values),
-                biases, native.ptr(token_mask), (vocab + 31) // 32, native.stream_ptr())
+    native.call_packed("ajb_process_logits", logits.data_ptr(), 1 if dtype is _F32 else 0, logits.stride(0), out.data_ptr(),
+                rows, vocab, _ptr(history) if width else 0, width, width, _ptr(prompt_lens), _ptr(history_lens),
+                _ptr(repetition), _ptr(presence), _ptr(frequency), _ptr(bias_ids), _ptr(bias_values),
+                biases, _ptr(token_mask), (vocab + 31) // 32, native.stream_ptr(index))
     return out
