@@ -222,8 +222,8 @@ __global__ void __launch_bounds__(kStreamThreads + kHistoryThreads) process_logi
       float x = load1<T>(in + v);
       x = x > 0.0f ? __fdiv_rn(x, r) : __fmul_rn(x, r);
       const unsigned count = held & ~Tab::kPrompt;
-      x = __fsub_rn(x, __fmul_rn(f, (float)count));
-      out[v] = __fsub_rn(x, count > 0u ? pr : 0.0f);
+      if (count > 0u) x = __fsub_rn(__fsub_rn(x, __fmul_rn(f, (float)count)), pr);
+      out[v] = x;
     });
   }
 
@@ -345,15 +345,17 @@ __global__ void __launch_bounds__(kMendThreads, 6) mend_logits_kernel(const Para
     auto changed = [&](float x, unsigned got) {
       x = x > 0.0f ? __fdiv_rn(x, r) : __fmul_rn(x, r);
       const unsigned count = got & ~Tab::kPrompt;
-      x = __fsub_rn(x, __fmul_rn(f, (float)count));
-      return __fsub_rn(x, count > 0u ? pr : 0.0f);
+      return count > 0u ? __fsub_rn(__fsub_rn(x, __fmul_rn(f, (float)count)), pr) : x;
     };
 #pragma unroll 1
     for (int i = thread; i < (Tab::words(cells) >> 2); i += kMendThreads) reinterpret_cast<uint4*>(table)[i] = make_uint4(0, 0, 0, 0);
     const bool held = len <= kHeld;
     if (held) {
 #pragma unroll 4
-      for (int i = thread; i < len; i += kMendThreads) tokens[i] = __ldg(history + i);
+      for (int i = thread; i < len; i += kMendThreads) {
+        const int v = __ldg(history + i);
+        tokens[i] = (unsigned)v < (unsigned)p.vocab ? v : -1;          // below -1 stand tokens whose count has been taken
+      }
     } else {
       asm volatile("griddepcontrol.wait;" ::: "memory");
     }

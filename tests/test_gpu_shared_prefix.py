@@ -571,3 +571,142 @@ def test_engine_processes_logits(engine_model):
             assert float(want[token]) > float(want.max()) - 0.08 * float(x.abs().max())      # as far as the forwards may differ
             tokens.append(token)
     assert native.lib().ajb_check_status() == 0
+
+
+# --------------------------------------------------------------------------------------------- limits and refusals
+
+
+@pytest.mark.parametrize("q_len,count", [(1, 3), (1, 70), (20, 3)])
+def test_cache_blocks_past_32_bits_and_table_entries_behind_the_context(q_len, count):
+    """The last blocks of caches of 2.3e9 elements; whatever the tables hold behind a context is not looked up."""
+    prefix, kv_heads, hd = 160, 8, 128
+    suffixes = [q_len + (7 * i) % 50 for i in range(count)]
+    q, keys, values, tables, context = _batch(16, kv_heads, hd, q_len, prefix, suffixes)
+    want = _oracle(q, keys, values, tables, context, q_len)
+    blocks = 140_000
+    far = [torch.empty(blocks, 16, kv_heads, hd, dtype=torch.bfloat16, device=_dev()) for _ in range(2)]
+    first = blocks - keys.shape[0]
+    for cache, near in zip(far, (keys, values)):
+        cache[first:] = near
+    wide = torch.full((count, tables.shape[1] + 9), 2**31 - 1, dtype=torch.int32, device=_dev())
+    wide[:, 1::2] = -7
+    for i, length in enumerate(context.tolist()):
+        wide[i, :(length + 15) // 16] = tables[i, :(length + 15) // 16] + first
+    _check_attention(serving.shared_prefix_attention(q, *far, wide, context, prefix, q_len=q_len), *want)
+
+
+def test_logits_past_32_bits():
+    rows, vocab = 16_800, 128_256                        # 2.15e9 logits
+    logits = torch.empty(rows, vocab, dtype=torch.bfloat16, device=_dev())
+    checked = [0, 1, 16_743, 16_744, rows - 1]           # 2^31 lies in row 16743
+    logits[checked] = torch.randn(len(checked), vocab, dtype=torch.bfloat16, device=_dev(), generator=torch.Generator(_dev()).manual_seed(0))
+    history = torch.randint(0, vocab, (rows, 33), dtype=torch.int32, device=_dev())
+    lens = torch.full((rows,), 33, dtype=torch.int32, device=_dev())
+    kw = dict(history=history, prompt_lens=lens // 2, history_lens=lens, presence=torch.full((rows,), 0.5, device=_dev()),
+              bias_ids=history[:, :3].contiguous(), bias_values=torch.ones(rows, 3, device=_dev()),
+              token_mask=torch.randint(-2**31, 2**31 - 1, (rows, vocab // 32), dtype=torch.int32, device=_dev()))
+    got = serving.process_logits(logits, **kw)
+    want = serving.process_logits(logits[checked], **{k: v[checked] for k, v in kw.items()})       # few rows, small offsets
+    assert torch.equal(got[checked], want)
+    plain = reference.process_logits(logits[checked].cpu(), *(None if v is None else v[checked].cpu() for v in (
+        kw["history"], kw["prompt_lens"], kw["history_lens"], None, kw["presence"], None, kw["bias_ids"], kw["bias_values"], kw["token_mask"])))
+    assert torch.equal(want.cpu(), plain)
+
+
+def test_many_rows_replayed_from_a_graph_and_calls_on_two_streams():
+    """The two-launch form captured and replayed with other inputs, and beside calls on another stream."""
+    def on_gpu(logits, kw):
+        return logits.cuda(), {name: t.cuda() for name, t in kw.items()}
+
+    logits, kw = on_gpu(*_logits_inputs(300, 32_000, torch.bfloat16, 40, 5, True))
+    other, other_kw = on_gpu(*_logits_inputs(280, 31_999, torch.float32, 77, 3, True, seed=1))
+    want_other = serving.process_logits(other, **other_kw)
+    want = serving.process_logits(logits, **kw)
+    graph, out = torch.cuda.CUDAGraph(), torch.empty_like(want)
+    with torch.cuda.graph(graph):
+        serving.process_logits(logits, **kw, out=out)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    found = []
+    for _ in range(5):
+        out.zero_()
+        graph.replay()
+        with torch.cuda.stream(side):
+            found.append(serving.process_logits(other, **other_kw))
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and all(torch.equal(f, want_other) for f in found)
+    logits.copy_(logits.flip(0))
+    kw["history"].copy_(kw["history"].flip(1))
+    graph.replay()
+    assert torch.equal(out, serving.process_logits(logits, **kw))
+
+
+def test_attention_calls_on_two_streams():
+    few = _batch(8, 2, 128, 1, 512, [1, 17, 130, 500])
+    many = _batch(32, 8, 128, 1, 2048, list(range(1, 100)))
+    calls = [(b, p, _oracle(*b, 1)) for b, p in ((few, 512), (many, 2048))]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    found = [[], []]
+    for _ in range(4):
+        for i, (batch, prefix, _) in enumerate(calls):
+            with torch.cuda.stream(streams[i]):
+                found[i].append(serving.shared_prefix_attention(*batch, prefix))
+    torch.cuda.synchronize()
+    for results, (_, _, want) in zip(found, calls):
+        for got in results:
+            _check_attention(got, *want)
+
+
+def test_results_that_cannot_be_written_are_refused():
+    q, keys, values, tables, context = _batch(8, 2, 128, 1, 64, [3, 4])
+    flat = torch.empty(q.numel() + 8, dtype=torch.bfloat16, device=_dev())
+    with pytest.raises(RuntimeError, match="aligned"):
+        serving.shared_prefix_attention(q, keys, values, tables, context, 64, out=flat[1:1 + q.numel()].view(q.shape))
+    serving.shared_prefix_attention(q, keys, values, tables, context, 64, out=flat[8:].view(q.shape))
+    for out in (q, values.flatten()[:q.numel()].view(q.shape)):
+        with pytest.raises(ValueError, match="overlap"):
+            serving.shared_prefix_attention(q, keys, values, tables, context, 64, out=out)
+    ids, counts, cached, new = _i32([3, 4]), _i32([1, 1]), _i32([2, 0]), _i32([1, 1])
+    good = serving.batch_maps(ids, counts, cached, new, 2, 2)
+    for out in (good._replace(context_lens=cached), good._replace(q_start=good.tables.flatten()[:3])):
+        with pytest.raises(RuntimeError, match="overlap"):
+            serving.batch_maps(ids, counts, cached, new, 2, 2, out=out)
+    with pytest.raises(RuntimeError, match="aligned"):
+        serving.batch_maps(ids, counts, cached, new, 2, 2, out=good._replace(positions=torch.zeros(3, dtype=torch.int32, device=_dev())[1:]))
+    logits = torch.zeros(2, 64, device=_dev())
+    mask = torch.zeros(128, device=_dev())
+    with pytest.raises(ValueError, match="overlap"):
+        serving.process_logits(logits, token_mask=mask.view(torch.int32)[:4].view(2, 2), out=mask.view(2, 64))
+    for wrong in (torch.float16, torch.float32):
+        with pytest.raises(TypeError):
+            serving.shared_prefix_attention(q.to(wrong), keys.to(wrong), values.to(wrong), tables, context, 64)
+    with pytest.raises((ValueError, TypeError)):
+        serving.shared_prefix_attention(q, keys, values, tables.cpu(), context, 64)
+    with pytest.raises(RuntimeError, match="block size"):
+        serving.shared_prefix_attention(q, keys.view(-1, 8, 2, 128), values.view(-1, 8, 2, 128), tables, context, 16)
+
+
+def test_infinite_penalties_leave_other_tokens_alone():
+    logits = torch.randn(2, 50, device=_dev())
+    kw = dict(history=_i32([[3, 4, 5], [6, 7, 8]]), prompt_lens=_i32([2, 3]), history_lens=_i32([3, 3]),
+              frequency=torch.tensor([math.inf, math.inf], device=_dev()))
+    got = serving.process_logits(logits, **kw).cpu()
+    want = reference.process_logits(logits.cpu(), *(kw[k].cpu() for k in ("history", "prompt_lens", "history_lens")), frequency=kw["frequency"].cpu())
+    assert torch.equal(got, want) and torch.isinf(got).sum() == 1 and not torch.isnan(got).any()
+
+
+@pytest.mark.parametrize("width", [9, 5000])
+@pytest.mark.parametrize("rows,vocab", [(3, 1000), (270, 32_003)])
+def test_ids_outside_the_vocabulary_are_skipped(rows, vocab, width):
+    """Whatever they are, in either form and with histories of either size."""
+    logits = torch.randn(rows, vocab, device=_dev())
+    outside = torch.tensor([-1, -2, -3, -17, -vocab, vocab, vocab + 1, 2**31 - 1, -2**31], dtype=torch.int32)
+    history = outside.repeat(rows, width // 9 + 1)[:, :width].contiguous().cuda()
+    history[:, 4] = 2
+    lens = torch.full((rows,), width, dtype=torch.int32, device=_dev())
+    got = serving.process_logits(logits, history=history, prompt_lens=lens - width, history_lens=lens, presence=torch.ones(rows, device=_dev()),
+                                 bias_ids=outside.repeat(rows, 1).cuda(), bias_values=torch.ones(rows, 9, device=_dev()))
+    want = logits.clone()
+    want[:, 2] -= 1.0
+    assert torch.equal(got, want)

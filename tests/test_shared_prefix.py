@@ -82,6 +82,14 @@ def test_batch_maps_refuses_outputs_of_another_shape():
             serving.batch_maps(*call, out=tuple(out))
 
 
+def test_batch_maps_refuses_outputs_over_its_inputs():
+    ids, counts, cached, new = _i32([0, 1]), _i32([2]), _i32([3]), _i32([1])
+    good = serving.batch_maps(ids, counts, cached, new, 1, 2)
+    for out in (good._replace(context_lens=cached), good._replace(q_start=good.tables.flatten())):
+        with pytest.raises(ValueError, match="apart"):
+            serving.batch_maps(ids, counts, cached, new, 1, 2, out=out)
+
+
 def _paged(contexts, shared, kv_heads=2, hd=8, block_size=4):
     """A cache of sequences that share their first ``shared`` tokens, its block tables, and each sequence's own keys and values."""
     gen = torch.Generator().manual_seed(len(contexts) + shared)
