@@ -171,6 +171,14 @@ extern "C" int ajb_batch_maps(const void* arguments) {
               width, block_size);
   AJB_REQUIRE(((reinterpret_cast<uintptr_t>(tables) | reinterpret_cast<uintptr_t>(positions) | reinterpret_cast<uintptr_t>(slots)) & 15) == 0,
               "batch maps: tables, positions and slots must be 16-byte aligned");
+  // every CTA reads all lengths while others write: results must lie apart from them, and from one another
+  const long long n = seqs;
+  const MemoryRange results[5] = {{tables, 4 * n * width}, {positions, 4ll * total}, {slots, 8ll * total}, {q_start, 4 * (n + 1)}, {context, 4 * n}};
+  const MemoryRange inputs[4] = {{ids, 4ll * n_ids}, {counts, 4 * n}, {cached, 4 * n}, {q_lens, 4 * n}};
+  for (int i = 0; i < 5; ++i) {
+    for (int j = 0; j < i; ++j) AJB_REQUIRE(!results[i].meets(results[j]), "batch maps: results %d and %d overlap", j, i);
+    for (int j = 0; j < 4; ++j) AJB_REQUIRE(!results[i].meets(inputs[j]), "batch maps: result %d overlaps input %d", i, j);
+  }
   maps::Params p;
   p.ids = (const int*)ids; p.counts = (const int*)counts; p.cached = (const int*)cached; p.q_lens = (const int*)q_lens;
   p.n_ids = n_ids; p.seqs = seqs; p.total = total; p.width = width; p.block_size = block_size; p.pad = pad;

@@ -37,6 +37,16 @@ const char* last_error();
     }                                       \
   } while (0)
 
+// Host side: whether two ranges of memory have a byte in common. An empty or absent range has none.
+struct MemoryRange {
+  const void* at;
+  long long bytes;
+  bool meets(const MemoryRange& other) const {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(at), b = reinterpret_cast<uintptr_t>(other.at);
+    return at != nullptr && other.at != nullptr && bytes > 0 && other.bytes > 0 && a < b + other.bytes && b < a + bytes;
+  }
+};
+
 constexpr int kMaxDevices = 16;   // devices of one process that per-device state is kept for
 
 // Device status words written by kernels whose bounded waits expired. Index = kernel id.

@@ -1,46 +1,30 @@
 // Paged-KV attention for decoding and speculative verification on sm_100a.
 //
-// One CTA serves one (sequence, KV head): the `group * q_len` query rows that share this KV head
-// (group = Hq / Hkv query heads, q_len new tokens: 1 for plain decoding, k + 1 when verifying k draft
-// tokens) form the top rows of a 128-row tcgen05 tile, so every K/V byte of the sequence is read once
-// for all of them. K/V tiles of 64 tokens are assembled from the sequence's 16-token cache blocks by
-// TMA (one box per block, addressed through the block table); S = Q K^T and O += P V run on the tensor
-// cores with accumulators in tensor memory, exactly as in the training forward kernel, but only the
-// softmax warps whose 32-row quarter holds real rows do any work. Row (head h, new token i) may see
-// keys 0 .. context_len - q_len + i.
+// A CTA's piece of work is a (sequence, KV head), or a share of its keys: the `group * q_len` query rows that share this
+// KV head (group = Hq / Hkv query heads, q_len new tokens: 1 for plain decoding, k + 1 when verifying k draft tokens) are
+// worked on together, so every K/V byte of the sequence is read once for all of them, in tiles of keys that TMA fetches
+// block by block (16 tokens, addressed through the block table). S = Q K^T and O += P V run on the tensor cores with
+// accumulators in tensor memory, the softmax between them in registers with fp32 maxima and sums. Row (head h, new token
+// i) may see keys 0 .. context_len - q_len + i.
 //
-// The kernel streams the cache once and does little arithmetic per byte, so what matters is how many bytes are in
-// flight per SM. A step (wait for the tile, one product, a softmax over it, a second product) is a dependent chain
-// of a couple of microseconds; one CTA per SM with two 128-key stages kept about one tile in flight and reached 0.4
-// of the copy bandwidth. Tiles of 64 keys halve the shared memory of a CTA (113 KB) and its tensor memory (256
-// columns), so two CTAs share an SM and each one's chain hides behind the other's loads.
+// The caches are streamed once with little arithmetic per byte, so the bytes in flight per SM and the length of a step's
+// dependent chain (wait for the tile, one product, a softmax over it, a second product) decide. There are two kernels, by
+// query rows per piece, with two CTAs per SM so that one's chain hides behind the other's loads (one for 17 to 32 rows of 128):
+//   up to 32 (paged_decode_kernel): keys on the 128-row side of the tensor-core tile, 128 of them per step;
+//   more (paged_attention_kernel): query rows on it, 64 keys per step.
+// 256 sequences of 1280 tokens, 8 KV heads of 128, 4 rows each: 195 us, 6.9 TB/s; 16 sequences of 1024: 15.5 us.
 //
-// Plain decoding has 4 to 8 real rows, all in the first quarter, and one warp would do the softmax of
-// all key columns of a tile while three idle. With at most 32 rows (paged_decode_kernel) the query rows are therefore staged
-// four times, once per 32-lane quarter: the score tile then holds four identical copies, and warp q
-// works on key columns [16 q, 16 q + 16) of its own copy. The four partial row maxima (and at the end the
-// partial row sums) are exchanged through shared memory; P is assembled in rows 0..31 of the operand
-// tile, so only the first quarter of O is meaningful and the first warp alone rescales and stores it.
+// Long contexts at small batch: with `splits` > 1 the tiles of a sequence are divided over that many pieces. Each leaves
+// its un-normalised fp32 output rows and (reference maximum, row sum) in a workspace, and a second small kernel joins them
+// with the usual log-sum-exp weights.
 //
-// In that variant the probability tile exists twice (only its first 32 rows matter, 4 KB each; the operand rows behind
-// them may hold anything, they feed accumulator rows that nobody reads), so the softmax of tile j + 1 does not wait for
-// the second product of tile j; and the partial maxima of tile j are exchanged while tile j + 1 is being computed:
-// tile j is exponentiated against the reference maximum of the tiles before it (exact for the first tile), which is
-// safe because bf16 and fp32 share the exponent range: the exponent is capped at 120, a cap that only a score jump of
-// more than 80 natural units above everything seen before could reach.
+// Layouts: q [tokens, Hq, hd] bf16 (rows of a sequence are contiguous, `q_start[seq]` is its first row); caches
+// [num_blocks, block_size = 16, Hkv, hd] bf16; block_tables [num_seqs, max_blocks] int32; out like q.
 //
-// Long contexts at small batch: with `splits` > 1 the tiles of a sequence are divided over `splits` CTAs (grid z).
-// Each writes its un-normalised fp32 output rows and (reference maximum, row sum) to a workspace, and a second small
-// kernel merges the parts with the usual log-sum-exp weights. One CTA per (sequence, KV head) walks a 4k context as
-// 32 dependent tile steps while most SMs idle; eight CTAs walk four steps each.
-//
-// Layouts: q [tokens, Hq, hd] bf16 (rows of a sequence are contiguous, `q_start[seq]` is its first
-// row); caches [num_blocks, block_size = 16, Hkv, hd] bf16; block_tables [num_seqs, max_blocks] int32;
-// out like q.
-//
-// Behind a shared prefix (csrc/prefix_attention.cu) the kernel covers the rest of every sequence: it starts at key
-// `first_key`, always leaves un-normalised parts, and sequences with more query rows than one CTA holds are cut into
-// `chunks` of q_len tokens each.
+// Behind a shared prefix (csrc/prefix_attention.cu) the kernels cover the rest of every sequence: they start at key
+// `first_key` and always leave un-normalised parts, and sequences with more query rows than one CTA holds are cut into
+// `chunks` of q_len tokens each. paged_decode_kernel may take the prefix itself along, in pieces for rows of several
+// sequences.
 #include "common.cuh"
 #include "paged_attention.h"
 
@@ -51,19 +35,15 @@ constexpr int TILE = 64;           // keys per step
 constexpr int QROWS = 128;         // rows of the query / probability operand tiles (the MMA's M)
 constexpr int BLOCK_TOKENS = 16;   // tokens per cache block
 constexpr int kThreads = 192;
-constexpr int kMaxRows = 64;       // group * q_len of a plain launch
+constexpr int kMaxRows = 64;       // group * q_len of ajb_paged_attention
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kPagedKernelId = 5;
-constexpr int kReplTileBytes = 32 * 128;   // paged_decode_kernel: the 32 meaningful rows of a probability tile (64 keys x 2 bytes per row)
 
 template <int HD>
 struct Cfg {
   static constexpr int kQ = QROWS * HD * 2;          // the query rows, staged once
   static constexpr int kTile = TILE * HD * 2;        // one K or V tile
   static constexpr int kP = QROWS * TILE * 2;        // probabilities of one step (A operand of P V)
-  // [parity][quarter][row] partial maxima / sums of paged_decode_kernel live in rows 64.. of the P tile: with at most 32
-  // real rows those operand rows only feed accumulator rows that nobody reads
-  static constexpr int kExchangeOffset = 64 * 128;
   static constexpr int kSmem = kQ + 4 * kTile /*2 x (K,V)*/ + kP + 256;
   static constexpr int kOCol = 2 * TILE;             // S0 at 0, S1 at TILE, O behind them
   static constexpr int kTmemCols = 256;              // 2 * 64 + HD <= 256: two CTAs fit the SM's 512 columns

@@ -203,7 +203,8 @@ def batch_maps(block_ids: torch.Tensor, block_counts: torch.Tensor, cached_lens:
     which must be a block that no sequence owns. Table rows keep a sequence's first ``max_blocks`` blocks and are filled
     up with ``pad_block``. At most 16384 sequences per call.
 
-    ``out`` may hold the five result tensors (buffers a captured graph reads); they are overwritten and returned.
+    ``out`` may hold the five result tensors (buffers a captured graph reads), apart from the inputs and from one another;
+    they are overwritten and returned. On a GPU the first three start on 16-byte boundaries.
     """
     index, each = block_ids.get_device(), block_counts.shape
     if not (block_ids.dtype is block_counts.dtype is cached_lens.dtype is q_lens.dtype is _I32
@@ -234,6 +235,8 @@ def batch_maps(block_ids: torch.Tensor, block_counts: torch.Tensor, cached_lens:
         found = reference.batch_maps(block_ids, block_counts, cached_lens, q_lens, total_tokens, max_blocks, block_size, pad_block)
         if out is None:
             return BatchMaps(*found)
+        if any(_overlap(a, b) for i, a in enumerate(out) for b in (*out[:i], block_ids, block_counts, cached_lens, q_lens)):
+            raise ValueError("batch_maps: out must lie apart from the inputs and from one another")
         for mine, theirs in zip(out, found):
             mine.copy_(theirs)
         return BatchMaps(*out)
@@ -360,8 +363,9 @@ def shared_prefix_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cach
     block is shared up to that block. Heads are 64 or 128 wide, ``Hq / Hkv`` is at most 128.
 
     ``max_context``: a host-side bound on the context lengths from which the number of parts per sequence is chosen (without
-    one: what the tables can hold, but the work is divided for suffixes of up to 256 tokens). It bounds nothing that is read. A row whose sequence has no token at all comes out as zeros. ``scale``
-    defaults to ``1 / sqrt(hd)``; ``out`` (contiguous, like ``q``) receives the result.
+    one: what the tables can hold, but the work is divided for suffixes of up to 256 tokens). It bounds nothing that is
+    read. A row whose sequence has no token at all comes out as zeros. ``scale`` defaults to ``1 / sqrt(hd)``; ``out``
+    (contiguous, shaped like ``q``, 16-byte aligned, apart from the inputs) receives the result.
     """
     if q.dim() != 3 or key_cache.dim() != 4 or block_tables.dim() != 2:
         raise ValueError("shared_prefix_attention: q is [rows, heads, hd], the caches [blocks, block, kv_heads, hd], block_tables [n, max_blocks]")
@@ -385,8 +389,8 @@ def shared_prefix_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cach
             _dense("shared_prefix_attention", name, t, kind, q.device, shape)
     if out is not None:
         _dense("shared_prefix_attention", "out", out, dtype, q.device, q.shape)
-        if _overlap(out, q):
-            raise ValueError("shared_prefix_attention: out must not overlap q")
+        if any(_overlap(out, t) for t in (q, key_cache, value_cache, block_tables, context_lens)):
+            raise ValueError("shared_prefix_attention: out must not overlap the inputs")
     scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
     if index < 0:
         found = reference.shared_prefix_attention(q, key_cache, value_cache, block_tables, context_lens, prefix_len, q_len, scale)
@@ -448,7 +452,7 @@ def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
     * tokens whose bit is not set in ``token_mask`` (int32 ``[rows, ceil(vocab / 32)]``, bit ``v % 32`` of word
       ``v // 32``) become ``-inf``, whatever their logit was. A row whose mask leaves nothing is ``-inf`` throughout.
 
-    ``out`` (fp32 ``[rows, vocab]``, contiguous, apart from ``logits``) receives the result.
+    ``out`` (fp32 ``[rows, vocab]``, contiguous, apart from the inputs) receives the result.
     """
     dtype, index = logits.dtype, logits.get_device()
     if dtype is not _BF16 and dtype is not _F32:
@@ -486,8 +490,9 @@ def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
         _dense("process_logits", "token_mask", token_mask, _I32, logits.device, (rows, (vocab + 31) // 32))
     if out is not None:
         _dense("process_logits", "out", out, _F32, logits.device, (rows, vocab))
-        if _overlap(out, logits):
-            raise ValueError("process_logits: out must not overlap the logits")
+        if any(t is not None and _overlap(out, t) for t in (logits, history, prompt_lens, history_lens, repetition, presence, frequency,
+                                                            bias_ids, bias_values, token_mask)):
+            raise ValueError("process_logits: out must not overlap the inputs")
     if index < 0:
         found = reference.process_logits(logits, history, prompt_lens, history_lens, repetition, presence, frequency, bias_ids,
                                          bias_values, token_mask)
