@@ -391,7 +391,10 @@ def shared_prefix_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cach
         _dense("shared_prefix_attention", "out", out, dtype, q.device, q.shape)
         if any(_overlap(out, t) for t in (q, key_cache, value_cache, block_tables, context_lens)):
             raise ValueError("shared_prefix_attention: out must not overlap the inputs")
-    scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
+    if scale is None:
+        scale = 1.0 / math.sqrt(head_dim)
+    elif not 0.0 < scale < math.inf:          # the reference maximum of a row is that of its unscaled scores
+        raise ValueError(f"shared_prefix_attention: scale must be positive (got {scale})")
     if index < 0:
         found = reference.shared_prefix_attention(q, key_cache, value_cache, block_tables, context_lens, prefix_len, q_len, scale)
         return found if out is None else out.copy_(found)

@@ -132,7 +132,8 @@ def _attention_call():
     {"prefix_len": -1}, {"prefix_len": 13}, {"context_lens": torch.zeros(2, dtype=torch.int64)}, {"context_lens": torch.zeros(3, dtype=I32)},
     {"block_tables": torch.zeros(2, 3)}, {"block_tables": torch.zeros(3, 3, dtype=I32)}, {"block_tables": torch.zeros(2, 6, dtype=I32)[:, ::2]},
     {"value_cache": torch.zeros(64, 4, 2, 4)}, {"key_cache": torch.zeros(64, 4, 2, 8).double()}, {"out": torch.zeros(2, 4, 9)},
-    {"out": torch.zeros(2, 4, 8).double()}, {"out": torch.zeros(2, 4, 16)[..., ::2]}])
+    {"out": torch.zeros(2, 4, 8).double()}, {"out": torch.zeros(2, 4, 16)[..., ::2]},
+    {"scale": 0.0}, {"scale": -0.1}, {"scale": math.nan}, {"scale": math.inf}])
 def test_shared_prefix_attention_refuses(change):
     call = _attention_call()
     serving.shared_prefix_attention(**call)
