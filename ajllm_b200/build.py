@@ -3,7 +3,8 @@
 One ``nvcc -gencode arch=compute_100a,code=sm_100a`` invocation per ``.cu`` file (in parallel), then a
 shared-library link into ``ajllm_b200/_native/libajllm_b200.so``. Objects are rebuilt only when their
 source or a header is newer. ``-Xptxas -v`` output is kept next to the objects (``*.ptxas.txt``) so
-register and shared-memory use can be read without a GPU.
+register and shared-memory use can be read without a GPU. ``csrc/fast_calls.cpp`` becomes a Python extension of its
+own (``_native/fast_calls.so``), which knows torch's tensors and calls into the library.
 """
 
 from __future__ import annotations
@@ -12,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -19,6 +21,7 @@ PACKAGE = Path(__file__).resolve().parent
 CSRC = PACKAGE / "csrc"
 OUT = PACKAGE / "_native"
 LIB = OUT / "libajllm_b200.so"
+FAST_CALLS = OUT / "fast_calls.so"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo", "--use_fast_math",
@@ -50,12 +53,26 @@ def _compile(nvcc: str, source: Path, obj: Path) -> tuple[Path, str]:
     return obj, log
 
 
+def _build_fast_calls() -> None:
+    import torch
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(find_nvcc()).resolve().parent.parent
+    done = subprocess.run(
+        ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+         "-I", sysconfig.get_paths()["include"], "-I", str(root / "include"), "-I", str(root / "include/torch/csrc/api/include"),
+         "-I", str(cuda / "include"), "-I", str(CSRC), str(CSRC / "fast_calls.cpp"), "-o", str(FAST_CALLS),
+         "-L", str(root / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"], capture_output=True, text=True)
+    if done.returncode != 0:
+        raise RuntimeError(f"g++ failed for fast_calls.cpp:\n{(done.stdout + done.stderr)[-6000:]}")
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     nvcc = find_nvcc()
     OUT.mkdir(parents=True, exist_ok=True)
     sources = sorted(CSRC.glob("*.cu"))
     headers = sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h"))
     jobs = []
+    binding = force or _needs_build(CSRC / "fast_calls.cpp", FAST_CALLS, [CSRC / "serving_args.h"])
     for source in sources:
         obj = OUT / (source.stem + ".o")
         if force or _needs_build(source, obj, headers):
@@ -66,6 +83,8 @@ def build(force: bool = False, verbose: bool = False) -> Path:
             for obj, log in pool.map(lambda job: _compile(nvcc, *job), jobs):
                 if verbose:
                     print(f"[build] {obj.name}\n{log}")
+    if binding:
+        _build_fast_calls()
     objects = [OUT / (source.stem + ".o") for source in sources]
     if jobs or not LIB.exists():
         link = [nvcc, "-shared", "-o", str(LIB), *map(str, objects), "-gencode", "arch=compute_100a,code=sm_100a",

@@ -11,6 +11,7 @@
 // reaches an index out of range: a token whose sequence has no block for it, and a row behind the last sequence, gets
 // the pad block.
 #include "common.cuh"
+#include "serving_args.h"
 
 namespace ajb {
 namespace maps {
@@ -152,13 +153,6 @@ __global__ void __launch_bounds__(kThreads) batch_maps_kernel(const Params p) {
 // ids [n_ids] block ids of all sequences, one after another; counts / cached / q_lens [seqs]; all int32 on the device.
 // tables [seqs, width], positions [total], slots [total] (int64), q_start [seqs + 1], context [seqs]; tables, positions
 // and slots 16-byte aligned.
-struct BatchMapsArgs {          // laid out by ops/native.py
-  int size;
-  const void *ids, *counts, *cached, *q_lens;
-  int n_ids, seqs, total, width, block_size, pad;
-  void *tables, *positions, *slots, *q_start, *context, *stream;
-};
-
 extern "C" int ajb_batch_maps(const void* arguments) {
   using namespace ajb;
   const BatchMapsArgs& args = *static_cast<const BatchMapsArgs*>(arguments);

@@ -19,6 +19,7 @@
 // longer looks through its row's whole history, and no streaming warp waits for one that counts (256 rows of 128256 with
 // 2560 tokens of history, biases and a mask: 56 us in one launch, 46 us in two; 36 us of that is the streaming alone).
 #include "common.cuh"
+#include "serving_args.h"
 
 namespace ajb {
 namespace logits {
@@ -438,23 +439,6 @@ __global__ void __launch_bounds__(kMendThreads, 6) mend_logits_kernel(const Para
 // logits [rows, vocab] (dtype 0: bf16, 1: fp32) with in_pitch elements between rows; out fp32 [rows, vocab] contiguous,
 // not overlapping the logits. Null pointers switch the parts off: history (with lens), repetition / presence /
 // frequency, bias_ids (biases = 0), mask.
-struct ProcessLogitsArgs {          // laid out by ops/native.py
-  int size;
-  const void *logits;
-  int dtype;
-  long long in_pitch;
-  void *out;
-  int rows, vocab;
-  const void *history;
-  long long history_pitch;
-  int history_width;
-  const void *prompt_lens, *history_lens, *repetition, *presence, *frequency, *bias_ids, *bias_values;
-  int biases;
-  const void *mask;
-  long long mask_pitch;
-  void *stream;
-};
-
 extern "C" int ajb_process_logits(const void* arguments) {
   using namespace ajb;
   const ProcessLogitsArgs& args = *static_cast<const ProcessLogitsArgs*>(arguments);

@@ -26,6 +26,7 @@
 // 13.4 us in pieces and 16.8 us with this kernel; behind 6144 + 256, 22.5 us and 20.2 us. 256 sequences behind 7680 tokens:
 // 80 us, of which the suffixes alone take 54 us.
 #include "common.cuh"
+#include "serving_args.h"
 #include "paged_attention.h"
 
 namespace ajb {
@@ -469,17 +470,6 @@ static int launch_prefix(const paged::Launch& a, int shared, int splits, cudaStr
 // (256 query rows, KV head). parts = what is left per row: suffix_splits, and prefix_splits more, or twice as many when the
 // prefix kernel has at most 128 query rows per KV head and a CTA more than one tile of 128 keys. part_o holds
 // num_seqs * q_len * heads * parts * head_dim floats, part_ml two per part.
-struct SharedPrefixArgs {          // laid out by ops/native.py
-  int size;
-  const void *q, *k_cache, *v_cache, *block_tables, *context_lens;
-  void *out;
-  long long q_pitch;
-  int num_seqs, num_blocks, block_size, max_blocks, heads, kv_heads, head_dim, q_len, shared;
-  float scale;
-  int prefix_tokens, prefix_splits, suffix_splits, parts;
-  void *part_o, *part_ml, *stream;
-};
-
 extern "C" int ajb_shared_prefix_attention(const void* arguments) {
   using namespace ajb;
   const SharedPrefixArgs& args = *static_cast<const SharedPrefixArgs*>(arguments);

@@ -10,8 +10,11 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import struct
+import warnings
 from pathlib import Path
 
 import torch
@@ -20,6 +23,7 @@ _LIB_DIR = Path(__file__).resolve().parent.parent / "_native"
 _LIB_NAME = "libajllm_b200.so"
 _lib: ctypes.CDLL | None = None
 _load_error: str | None = None
+fast = None              # the extension built from csrc/fast_calls.cpp, once the library is loaded
 
 c_void = ctypes.c_void_p
 c_int = ctypes.c_int
@@ -91,7 +95,7 @@ def library_path() -> Path:
 
 
 def _try_load() -> None:
-    global _lib, _load_error
+    global _lib, _load_error, fast
     if _lib is not None or _load_error is not None:
         return
     path = library_path()
@@ -117,6 +121,22 @@ def _try_load() -> None:
     lib.ajb_last_error.restype = ctypes.c_char_p
     lib.ajb_last_error.argtypes = []
     _lib = lib
+    fast = _load_fast_calls(lib)
+
+
+def _load_fast_calls(lib: ctypes.CDLL):
+    """The binding that checks, allocates and calls without going through ctypes. Every call works without it."""
+    path = _LIB_DIR / "fast_calls.so"
+    try:
+        loader = importlib.machinery.ExtensionFileLoader("fast_calls", str(path))
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("fast_calls", loader))
+        loader.exec_module(module)
+        module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
+                      for name in ("ajb_batch_maps", "ajb_shared_prefix_attention", "ajb_process_logits", "ajb_last_error")))
+        return module
+    except (ImportError, OSError, AttributeError) as error:
+        warnings.warn(f"{path} could not be loaded ({error}): small serving calls take longer")
+        return None
 
 
 def available() -> bool:

@@ -151,8 +151,9 @@ def spec_verify(target_logits: torch.Tensor, draft_logits: torch.Tensor, draft_t
 # ----------------------------------------------------------------------------- shared by the operators below
 
 
-# A small operator takes a few microseconds on the device, so its argument checks are one expression over cheap
-# attributes; only when it fails are the arguments gone through one by one for the message.
+# A small operator takes a few microseconds on the device. Its ordinary call on a GPU is checked, allocated and launched by
+# an extension (csrc/fast_calls.cpp), which leaves every other call to the code here. The argument checks are one expression
+# over cheap attributes; only when it fails are the arguments gone through one by one for the message.
 _I32, _I64, _F32, _BF16 = torch.int32, torch.int64, torch.float32, torch.bfloat16
 _CONTIGUOUS = torch.contiguous_format
 
@@ -206,6 +207,11 @@ def batch_maps(block_ids: torch.Tensor, block_counts: torch.Tensor, cached_lens:
     ``out`` may hold the five result tensors (buffers a captured graph reads), apart from the inputs and from one another;
     they are overwritten and returned. On a GPU the first three start on 16-byte boundaries.
     """
+    if native.fast is not None:
+        found = native.fast.batch_maps(block_ids, block_counts, cached_lens, q_lens, total_tokens, max_blocks, block_size, pad_block, out)
+        if found is not None:
+            native.launch_count += 1
+            return BatchMaps._make(out if found is True else found)
     index, each = block_ids.get_device(), block_counts.shape
     if not (block_ids.dtype is block_counts.dtype is cached_lens.dtype is q_lens.dtype is _I32
             and block_counts.get_device() == index == cached_lens.get_device() == q_lens.get_device()
@@ -367,6 +373,12 @@ def shared_prefix_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cach
     read. A row whose sequence has no token at all comes out as zeros. ``scale`` defaults to ``1 / sqrt(hd)``; ``out``
     (contiguous, shaped like ``q``, 16-byte aligned, apart from the inputs) receives the result.
     """
+    if out is None and native.fast is not None:
+        found = native.fast.shared_prefix_attention(q, key_cache, value_cache, block_tables, context_lens, prefix_len, q_len, scale,
+                                                    max_context, _EXPECTED_SUFFIX, prefix_plan)
+        if found is not None:
+            native.launch_count += 2
+            return found
     if q.dim() != 3 or key_cache.dim() != 4 or block_tables.dim() != 2:
         raise ValueError("shared_prefix_attention: q is [rows, heads, hd], the caches [blocks, block, kv_heads, hd], block_tables [n, max_blocks]")
     total, heads, head_dim = q.shape
@@ -457,6 +469,12 @@ def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
 
     ``out`` (fp32 ``[rows, vocab]``, contiguous, apart from the inputs) receives the result.
     """
+    if out is None and native.fast is not None:
+        found = native.fast.process_logits(logits, history, prompt_lens, history_lens, repetition, presence, frequency, bias_ids,
+                                           bias_values, token_mask)
+        if found is not None:
+            native.launch_count += 1
+            return found
     dtype, index = logits.dtype, logits.get_device()
     if dtype is not _BF16 and dtype is not _F32:
         raise TypeError(f"process_logits: logits must be bfloat16 or float32 (got {dtype})")

@@ -710,3 +710,63 @@ def test_ids_outside_the_vocabulary_are_skipped(rows, vocab, width):
     want = logits.clone()
     want[:, 2] -= 1.0
     assert torch.equal(got, want)
+
+
+# --------------------------------------------------------------------------------------------- the extension that makes the calls
+
+
+def _ordinary_calls():
+    maps = (_i32([3, 4, 5]), _i32([1, 2]), _i32([2, 17]), _i32([1, 9]), 12, 4)
+    attention = (*_batch(8, 2, 128, 1, 96, [3, 40]), 96)
+    logits, kw = _logits_inputs(3, 300, torch.bfloat16, 7, 4, True)
+    return [(serving.batch_maps, maps, dict(pad_block=1)), (serving.shared_prefix_attention, attention, dict(scale=0.1)),
+            (serving.shared_prefix_attention, attention, dict(max_context=200)),
+            (serving.process_logits, (logits.cuda(),), {name: t.cuda() for name, t in kw.items()})]
+
+
+def test_both_ways_to_call_give_the_same(monkeypatch):
+    """The extension, and what takes over where it does not apply: the same results, bit for bit, and launches counted alike."""
+    assert native.fast is not None
+    found = []
+    for fast in (native.fast, None):
+        monkeypatch.setattr(native, "fast", fast)
+        for fn, args, kw in _ordinary_calls():
+            before = native.launch_count
+            got = fn(*args, **kw)
+            found.append([*(got if isinstance(got, tuple) else [got]), native.launch_count - before])
+    half = len(found) // 2
+    for a, b in zip(found[:half], found[half:]):
+        assert a[-1] == b[-1] and all(torch.equal(x, y) for x, y in zip(a[:-1], b[:-1]))
+
+
+def test_ordinary_calls_go_through_the_extension(monkeypatch):
+    monkeypatch.setattr(native, "call_packed", lambda *a: pytest.fail("the call was not taken"))
+    for fn, args, kw in _ordinary_calls():
+        fn(*args, **kw)
+    out = serving.batch_maps(_i32([3]), _i32([1]), _i32([2]), _i32([1]), 1, 1)
+    assert isinstance(out, serving.BatchMaps)
+    again = serving.batch_maps(_i32([4]), _i32([1]), _i32([2]), _i32([1]), 1, 1, out=tuple(out))
+    assert isinstance(again, serving.BatchMaps) and again.tables is out.tables and out.tables.tolist() == [[4]]
+
+
+def test_calls_that_the_extension_leaves_alone():
+    logits, kw = _logits_inputs(3, 300, torch.bfloat16, 7, 4, True)
+    logits, kw = logits.cuda(), {name: t.cuda() for name, t in kw.items()}
+    want = serving.process_logits(logits, **kw)
+    assert torch.equal(serving.process_logits(torch.nn.Parameter(logits), **kw), want)                  # not a plain tensor
+    assert torch.equal(serving.process_logits(logits.t().contiguous().t(), **kw), want)                 # columns next to one another
+    q, keys, values, tables, context = _batch(8, 2, 128, 1, 96, [3, 40])
+    want = serving.shared_prefix_attention(q, keys, values, tables, context, 96)
+    wide = torch.zeros(2, 8, 160, dtype=torch.bfloat16, device=_dev())
+    wide[..., 5:133] = q
+    assert torch.equal(serving.shared_prefix_attention(wide[..., 5:133], keys, values, tables, context, 96), want)
+    assert torch.equal(serving.shared_prefix_attention(q, keys, values, tables, context, 96, scale=torch.tensor(128 ** -0.5).item()), want)
+    assert serving.shared_prefix_attention(q[:0], keys, values, tables[:0], context[:0], 96).shape == (0, 8, 128)
+    assert serving.process_logits(logits[:0]).shape == (0, 300)
+
+
+def test_a_result_that_does_not_fit_the_device_is_an_exception():
+    row = torch.zeros(1, 1 << 20, device=_dev())
+    with pytest.raises(torch.OutOfMemoryError):
+        serving.process_logits(row.expand(300_000, -1))                    # 1.2 TB of results
+    assert torch.equal(serving.process_logits(row), row)
