@@ -70,6 +70,8 @@ __device__ __forceinline__ int find(const int* sums, int n, int t) {
 }
 
 __global__ void __launch_bounds__(kThreads) batch_maps_kernel(const Params p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   extern __shared__ int sums[];
   __shared__ int warp_sums[kThreads / 32];
   int* first_block = sums;
@@ -183,8 +185,6 @@ extern "C" int ajb_batch_maps(const void* arguments) {
     AJB_CUDA_OK(cudaFuncSetAttribute(maps::batch_maps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   const long long pieces = ((long long)total + 3) / 4 + ((long long)seqs * width + 3) / 4 + 1;
   const long long blocks = (pieces + maps::kThreads - 1) / maps::kThreads;
-  maps::batch_maps_kernel<<<(int)(blocks < 4ll * sm_count() ? blocks : 4ll * sm_count()), maps::kThreads, smem,
-                            reinterpret_cast<cudaStream_t>(stream)>>>(p);
-  AJB_CUDA_OK(cudaGetLastError());
-  return 0;
+  return launch_early(maps::batch_maps_kernel, dim3((unsigned)(blocks < 4ll * sm_count() ? blocks : 4ll * sm_count())),
+                      dim3(maps::kThreads), smem, reinterpret_cast<cudaStream_t>(stream), p);
 }

@@ -190,6 +190,8 @@ __device__ __forceinline__ void add_biases(const Params& p, int row, float* out,
 template <typename T, bool kNarrow>
 __global__ void __launch_bounds__(kStreamThreads + kHistoryThreads) process_logits_kernel(const Params p) {
   extern __shared__ unsigned table[];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   using Tab = Table<kNarrow>;
   const int row = (int)(blockIdx.x / (unsigned)p.chunks), part = (int)(blockIdx.x % (unsigned)p.chunks);
   const int lo = part * p.chunk, hi = min(p.vocab, lo + p.chunk);
@@ -246,6 +248,8 @@ __global__ void __launch_bounds__(kStreamThreads, 6) stream_logits_kernel(const 
   constexpr int kWords = kStreamChunk / 32 + 1;          // one more than a piece has: groups look at the next word too
   constexpr int kEach = (kWords + kStreamThreads - 1) / kStreamThreads;
   __shared__ unsigned shared[2][kMasked ? kWords : 1];
+  // in this order: the second launch reads the inputs without waiting for anything but its start
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int thread = threadIdx.x, step = (int)gridDim.x, all = (p.vocab + 31) / 32;
   unsigned ahead[kEach];
@@ -483,8 +487,7 @@ extern "C" int ajb_process_logits(const void* arguments) {
       AJB_CUDA_OK(cudaFuncSetAttribute(stream_kernels[which], cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
       if (dev < kMaxDevices) configured[which][dev] = true;
     }
-    stream_kernels[which]<<<grid, logits::kStreamThreads, 0, s>>>(p);
-    AJB_CUDA_OK(cudaGetLastError());
+    if (const int rc = launch_early(stream_kernels[which], dim3(grid), dim3(logits::kStreamThreads), 0, s, p)) return rc;
     if (!mends) return 0;
     void (*const mend_kernels[4])(logits::Params) = {
         logits::mend_logits_kernel<__nv_bfloat16, false>, logits::mend_logits_kernel<__nv_bfloat16, true>,
@@ -499,18 +502,7 @@ extern "C" int ajb_process_logits(const void* arguments) {
       AJB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
       if (dev < kMaxDevices) done = true;
     }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(rows);
-    cfg.blockDim = dim3(logits::kMendThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    AJB_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, p));
-    return 0;
+    return launch_early(kernel, dim3(rows), dim3(logits::kMendThreads), smem, s, p);
   }
   // A piece of a row per CTA: large, because every piece looks at the row's whole history, but not larger than leaves three
   // for each SM (48 x 128256 with two: 16.6 us, with three: 13.9 us; 16 x 128256 with eight: 10.5 us, with three: 5.7 us).
@@ -520,10 +512,7 @@ extern "C" int ajb_process_logits(const void* arguments) {
   p.chunks = (vocab + chunk - 1) / chunk;
   const int smem = counts ? chunk * (narrow ? 2 : 4) : 0;
   const int grid = rows * p.chunks, threads = logits::kStreamThreads + (counts ? logits::kHistoryThreads : 0);
-  if (dtype == 0 && narrow) logits::process_logits_kernel<__nv_bfloat16, true><<<grid, threads, smem, s>>>(p);
-  else if (dtype == 0) logits::process_logits_kernel<__nv_bfloat16, false><<<grid, threads, smem, s>>>(p);
-  else if (narrow) logits::process_logits_kernel<float, true><<<grid, threads, smem, s>>>(p);
-  else logits::process_logits_kernel<float, false><<<grid, threads, smem, s>>>(p);
-  AJB_CUDA_OK(cudaGetLastError());
-  return 0;
+  auto kernel = dtype == 0 ? (narrow ? logits::process_logits_kernel<__nv_bfloat16, true> : logits::process_logits_kernel<__nv_bfloat16, false>)
+                           : (narrow ? logits::process_logits_kernel<float, true> : logits::process_logits_kernel<float, false>);
+  return launch_early(kernel, dim3(grid), dim3(threads), smem, s, p);
 }

@@ -66,6 +66,7 @@ struct Params {
   int prefix_splits;          // divisions of the keys in front of first_key (0: not covered); their CTAs are ahead of the others
   int prefix_tokens;          // query tokens that one of these CTAs takes
   int prefix_pieces;          // and how many of them a KV head's query tokens are
+  int early;                  // this launch may have started before the one in front of it ended: wait for that first
   int part_stride, part_base; // parts per row in the workspace and the first one of this launch; part_stride 0: no parts
   float* part_o;              // [tokens, Hq, part_stride, hd] fp32, un-normalised
   float2* part_ml;            // [tokens, Hq, part_stride] (reference maximum in log2 units, row sum); sum 0 = no keys seen
@@ -544,6 +545,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   float* sExchange = reinterpret_cast<float*>(sP + 2 * C::kP);
   uint64_t* bars = reinterpret_cast<uint64_t*>(sP + 2 * C::kP + C::kExchange);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (p.early) asm volatile("griddepcontrol.wait;" ::: "memory");
   if (smem_misaligned(smem_raw, p.status, kPagedKernelId, reinterpret_cast<uint32_t*>(bars) + 120)) return;
   uint64_t* full = bars;           // kSlots (<= 6)
   uint64_t* empty = bars + 6;      // kSlots
@@ -1014,6 +1016,7 @@ __global__ void __launch_bounds__(128) merge_splits_kernel(const float* __restri
     const int seq = (int)(local_row / q_len);
     out_row = (size_t)(q_start[seq] + (int)(local_row - (long long)seq * q_len)) * heads + (size_t)(w - local_row * heads);
   }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   constexpr int kPerLane = HD / 32;
   constexpr int kBatch = 4;
@@ -1104,6 +1107,7 @@ static int launch_kernel(const Launch& a, cudaStream_t stream) {
   p.max_blocks = a.max_blocks; p.heads = a.heads; p.kv_heads = a.kv_heads; p.group = a.heads / a.kv_heads; p.q_len = a.q_len;
   p.seqs = a.num_seqs; p.chunks = (a.q_total + a.q_len - 1) / a.q_len; p.q_total = a.q_total;
   p.first_key = a.first_key; p.scale = a.scale; p.status = device_status_buffer();
+  p.early = a.early;
   p.splits = a.splits; p.prefix_splits = a.prefix_splits; p.part_stride = a.part_stride; p.part_base = a.part_base;
   p.part_o = (float*)a.part_o; p.part_ml = (float2*)a.part_ml;
   static bool configured[5][kMaxDevices] = {};
@@ -1124,10 +1128,10 @@ static int launch_kernel(const Launch& a, cudaStream_t stream) {
       if (rc) return rc;
     }
     const int smem16 = DecodeCfg<HD, 16>::kSmem, smem32 = DecodeCfg<HD, 32>::kSmem;
-    if (rows <= 4) return launch_on(paged_decode_kernel<HD, 4>, configured[0], grid, smem16, map_k, map_v, p, a.beside_previous, stream);
-    if (rows <= 8) return launch_on(paged_decode_kernel<HD, 8>, configured[1], grid, smem16, map_k, map_v, p, a.beside_previous, stream);
-    if (rows <= 16) return launch_on(paged_decode_kernel<HD, 16>, configured[2], grid, smem16, map_k, map_v, p, a.beside_previous, stream);
-    return launch_on(paged_decode_kernel<HD, 32>, configured[3], grid, smem32, map_k, map_v, p, a.beside_previous, stream);
+    if (rows <= 4) return launch_on(paged_decode_kernel<HD, 4>, configured[0], grid, smem16, map_k, map_v, p, a.beside_previous || a.early, stream);
+    if (rows <= 8) return launch_on(paged_decode_kernel<HD, 8>, configured[1], grid, smem16, map_k, map_v, p, a.beside_previous || a.early, stream);
+    if (rows <= 16) return launch_on(paged_decode_kernel<HD, 16>, configured[2], grid, smem16, map_k, map_v, p, a.beside_previous || a.early, stream);
+    return launch_on(paged_decode_kernel<HD, 32>, configured[3], grid, smem32, map_k, map_v, p, a.beside_previous || a.early, stream);
   }
   AJB_REQUIRE(a.prefix_splits == 0, "paged attention: more than 32 query rows per CTA cannot take a shared prefix along");
   AJB_REQUIRE((long long)a.kv_heads * p.chunks <= 65535, "paged attention: %d new tokens per sequence are too many for one launch", a.q_total);
@@ -1153,18 +1157,8 @@ int launch(const Launch& a, int head_dim, cudaStream_t stream) {
 template <int HD>
 static int launch_merge(const Launch& a, cudaStream_t stream) {
   const long long pairs = (long long)a.num_seqs * a.q_total * a.heads;
-  cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3(128);
-  cfg.gridDim = dim3((unsigned)((pairs * 32 + 127) / 128));
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  AJB_CUDA_OK(cudaLaunchKernelEx(&cfg, merge_splits_kernel<HD>, (const float*)a.part_o, (const float2*)a.part_ml, (__nv_bfloat16*)a.out,
-                                 (const int*)a.q_start, a.q_total, a.heads, a.part_stride, pairs));
-  return 0;
+  return launch_early(merge_splits_kernel<HD>, dim3((unsigned)((pairs * 32 + 127) / 128)), dim3(128), 0, stream, (const float*)a.part_o,
+                      (const float2*)a.part_ml, (__nv_bfloat16*)a.out, (const int*)a.q_start, a.q_total, a.heads, a.part_stride, pairs);
 }
 
 int merge_parts(const Launch& a, int head_dim, cudaStream_t stream) {
@@ -1196,7 +1190,7 @@ extern "C" int ajb_paged_attention(const void* q, const void* k_cache, const voi
   a.num_seqs = num_seqs; a.num_blocks = num_blocks; a.max_blocks = max_blocks; a.heads = heads; a.kv_heads = kv_heads;
   a.q_len = q_len; a.q_total = q_len; a.first_key = 0; a.scale = scale; a.splits = splits; a.prefix_splits = a.prefix_tokens = 0;
   a.part_stride = splits > 1 ? splits : 0; a.part_base = 0; a.part_o = part_o; a.part_ml = part_ml;
-  a.map_k = a.map_v = nullptr; a.beside_previous = false;
+  a.map_k = a.map_v = nullptr; a.beside_previous = a.early = false;
   int rc = paged::launch(a, head_dim, s);
   if (rc == 0 && splits > 1) rc = paged::merge_parts(a, head_dim, s);
   return rc;

@@ -23,6 +23,7 @@ struct Launch {
   int part_stride, part_base;   // parts per row in the workspace, first one of this launch; stride 0: no parts, `out` is written
   void *part_o, *part_ml;
   const CUtensorMap *map_k, *map_v;   // of make_tensor_map_cache, when the caller has them already (else null)
+  bool early;                   // may start before the launch in front of it has ended, and waits for that (up to 32 rows per CTA)
   bool beside_previous;         // may start while the launch in front of it still runs (which must have said so)
 };
 

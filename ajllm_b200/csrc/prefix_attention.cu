@@ -510,6 +510,7 @@ extern "C" int ajb_shared_prefix_attention(const void* arguments) {
   a.part_base = prefix_parts; a.part_o = part_o; a.part_ml = part_ml; a.beside_previous = shared > 0 && !few;
   a.prefix_splits = few ? prefix_splits : 0;
   a.prefix_tokens = prefix_tokens;
+  a.early = few;
   CUtensorMap map_k, map_v;
   int rc = make_tensor_map_cache(&map_k, a.k_cache, a.num_blocks, a.kv_heads, head_dim);
   if (rc == 0) rc = make_tensor_map_cache(&map_v, a.v_cache, a.num_blocks, a.kv_heads, head_dim);
