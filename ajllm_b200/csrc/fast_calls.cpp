@@ -116,15 +116,15 @@ PyObject* fast_batch_maps(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
-// (q, key_cache, value_cache, block_tables, context_lens, prefix_len, q_len, scale or None, max_context or None, expected
-//  suffix without a bound, prefix_plan) -> the result, or None
+// (q, key_cache, value_cache, block_tables, context_lens, prefix_len, q_len, scale or None, max_context or None, prefix_plan)
+// -> the result, or None
 PyObject* fast_shared_prefix_attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
-  if (n_args != 11 || shared_prefix_entry == nullptr) Py_RETURN_NONE;
+  if (n_args != 10 || shared_prefix_entry == nullptr) Py_RETURN_NONE;
   const at::Tensor *q = tensor(a[0]), *k = tensor(a[1]), *v = tensor(a[2]), *tables = tensor(a[3]), *context = tensor(a[4]);
-  long long prefix, q_len, expected;
+  long long prefix, q_len;
   if (q == nullptr || k == nullptr || tables == nullptr || !q->is_cuda() || q->dim() != 3 || k->dim() != 4 || tables->dim() != 2 ||
-      !whole(a[5], 0, INT_MAX, prefix) || !whole(a[6], 1, INT_MAX, q_len) || !whole(a[9], 0, INT_MAX, expected))
+      !whole(a[5], 0, INT_MAX, prefix) || !whole(a[6], 1, INT_MAX, q_len))
     Py_RETURN_NONE;
   const int device = q->get_device();
   const int64_t total = q->size(0), heads = q->size(1), hd = q->size(2), blocks = k->size(0), block = k->size(1), kv_heads = k->size(2),
@@ -148,11 +148,9 @@ PyObject* fast_shared_prefix_attention(PyObject*, PyObject* const* a, Py_ssize_t
     long long bound;
     if (!whole(a[8], LLONG_MIN, LLONG_MAX, bound)) Py_RETURN_NONE;
     behind = std::max(0ll, std::min(bound, room) - shared);
-    expected = behind;
   }
-  expected = std::min(expected, behind);
-  PyObject* plan = PyObject_CallFunction(a[10], "LLLLLLLL", (long long)n, q_len, (long long)(heads / kv_heads), (long long)kv_heads,
-                                         (long long)hd, shared, behind, expected);
+  PyObject* plan = PyObject_CallFunction(a[9], "LLLLLLLL", (long long)n, q_len, (long long)(heads / kv_heads), (long long)kv_heads,
+                                         (long long)hd, shared, behind, (long long)(a[8] != Py_None));
   if (plan == nullptr) return nullptr;
   int tokens, prefix_splits, splits, parts;
   const bool understood = PyArg_ParseTuple(plan, "iiii", &tokens, &prefix_splits, &splits, &parts);

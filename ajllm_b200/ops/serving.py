@@ -264,16 +264,19 @@ def batch_maps(block_ids: torch.Tensor, block_counts: torch.Tensor, cached_lens:
 # ----------------------------------------------------------------------------- attention behind a shared prefix
 
 _PREFIX_TILE = 128         # query rows and keys per step of the prefix kernel
-_EXPECTED_SUFFIX = 256     # tokens behind the prefix when the caller gives no bound: block tables are often much wider than contexts
 
 
 @functools.lru_cache(maxsize=4096)
 def prefix_plan(n: int, q_len: int, group: int, kv_heads: int, head_dim: int, shared: int, behind: int,
-                expected: int) -> tuple[int, int, int, int]:
+                known: int) -> tuple[int, int, int, int]:
     """How a call of :func:`shared_prefix_attention` is divided: ``(query tokens per piece of the prefix in the paged launch,
     or 0 for the prefix kernel; divisions of the prefix; divisions of a suffix; parts per row in all)``. Suffixes have at most
-    ``behind`` tokens and about ``expected`` at the most. Whichever of the two forms is estimated to end first is taken (in
-    us, from measurements of 16 to 1024 query rows per KV head, prefixes of 512 to 7680 and suffixes of 32 to 1024 tokens)."""
+    ``behind`` tokens; unless that is ``known`` to be what they have, the division is the one that does best for suffixes of
+    up to that and up to half of it together, or, in tables with room for more than 1024 behind the prefix, of up to 128 and
+    up to 512 (such tables are often much wider than contexts: 64 sequences behind 2048 + 32 tokens in tables for 8192 took
+    45 us when divided for the tables, 22 us now). Whichever of the two forms is
+    estimated to end first is taken (in us, from measurements of 4 to 1024 query rows per KV head, prefixes of 512 to 7680
+    and suffixes of 32 to 1024 tokens)."""
     if not _SM_COUNT:
         _SM_COUNT.append(int(native.lib().ajb_sm_count()))
     sms = _SM_COUNT[0]
@@ -283,17 +286,20 @@ def prefix_plan(n: int, q_len: int, group: int, kv_heads: int, head_dim: int, sh
     bound_splits = paged_splits(pieces, behind)
     if not shared:
         return 0, 0, bound_splits, bound_splits
-    tiles, suffix_tiles = -(-shared // _PREFIX_TILE), -(-expected // _PREFIX_TILE)
-    divisions = {min(8, bound_splits)} if expected < behind else range(1, min(16, max(1, suffix_tiles)) + 1)
+    tiles, most = -(-shared // _PREFIX_TILE), -(-behind // _PREFIX_TILE)
+    divisions = tuple(range(1, min(16, max(1, most)) + 1)) if known or behind <= 1024 else (min(8, bound_splits),)
     rows = n * q_len * group
-    least = 3.0 + (n * expected + shared) * kv_heads * head_dim * 4 / 6.5e6       # reading the caches once
-    best = _kernel_plan(rows, pieces, kv_heads, head_dim, tiles, suffix_tiles, expected, divisions, least, sms)
-    if group * q_len <= 32:
-        best = min(best, _pieces_plan(n, q_len, group, kv_heads, head_dim, tiles, suffix_tiles, divisions, least, sms))
-    return best[1]
+    times = []
+    for expected in (behind,) if known else (behind // 2, behind) if behind <= 1024 else (128, 512):
+        least = 3.0 + (n * expected + shared) * kv_heads * head_dim * 4 / 6.5e6       # reading the caches once
+        found = _kernel_plans(rows, pieces, kv_heads, head_dim, tiles, expected, divisions, least, sms)
+        if group * q_len <= 32:
+            found.update(_pieces_plans(n, q_len, group, kv_heads, head_dim, tiles, expected, divisions, least, sms))
+        times.append((min(found.values()), found))
+    return min(times[0][1], key=lambda plan: (sum(found[plan] / best for best, found in times), plan))
 
 
-def _pieces_plan(n, q_len, group, kv_heads, head_dim, tiles, suffix_tiles, divisions, least, sms):
+def _pieces_plans(n, q_len, group, kv_heads, head_dim, tiles, expected, divisions, least, sms):
     """The prefix in pieces of the paged launch, for 16 query rows each (32 where a sequence has more than 16): a second read
     of the prefix from L2 costs less than pieces of 32 rows, of which an SM holds one instead of two (8 sequences of 4 rows,
     512 + 32 tokens: 9.0 us against 10.7). A piece takes 3 us and 1.1 us per 128 keys (32 rows: 1.5 us)."""
@@ -303,7 +309,8 @@ def _pieces_plan(n, q_len, group, kv_heads, head_dim, tiles, suffix_tiles, divis
     step = 1.1 if height == 16 else 1.5
     units = kv_heads * -(-n * q_len // tokens)
     per_part = 0.1 + 0.0005 * n * q_len * group * kv_heads
-    best = (math.inf, (0, 0, 0, 0))
+    suffix_tiles = -(-expected // _PREFIX_TILE)
+    found = {}
     for splits in divisions:
         back, back_time = n * kv_heads * max(1, min(splits, suffix_tiles)), 3.0 + step * -(-suffix_tiles // splits)
         for ours in sorted({-(-tiles // length) for length in range(1, tiles + 1)}):
@@ -317,11 +324,11 @@ def _pieces_plan(n, q_len, group, kv_heads, head_dim, tiles, suffix_tiles, divis
             while (slots - front) * k + front * max(0, int((k * back_time - front_time) / back_time)) < back:
                 k += 1
             time = max(rounds * front_time + max(front_time, k * back_time) + 3.0, least) + per_part * (ours + splits)
-            best = min(best, (time, (tokens, ours, splits, ours + splits)))
-    return best
+            found[tokens, ours, splits, ours + splits] = time
+    return found
 
 
-def _kernel_plan(rows, pieces, kv_heads, head_dim, tiles, suffix_tiles, expected, divisions, least, sms):
+def _kernel_plans(rows, pieces, kv_heads, head_dim, tiles, expected, divisions, least, sms):
     """The prefix kernel beside the suffixes' launch. A CTA of it keeps an SM to itself while the others stream the suffixes,
     so the SMs are divided like the work: a prefix CTA takes about 14 us and 2 us more per step (128 keys for up to 256 rows;
     two tiles make a step when 128 rows are all there are, and it starts 3 us sooner), a suffix occupies half an SM for 1.3 us
@@ -331,12 +338,13 @@ def _kernel_plan(rows, pieces, kv_heads, head_dim, tiles, suffix_tiles, expected
     one_tile = rows <= _PREFIX_TILE
     units = kv_heads * (1 if one_tile else -(-rows // (2 * _PREFIX_TILE)))
     step = 1.35 if head_dim == 128 else 0.65
-    suffix = pieces * (0.65 + step * (expected / 256 + 0.5))
+    suffix = pieces * (0.65 + step * (expected / 256 + 0.5))          # of `expected` at the most: half of it on average
     per_part = rows * kv_heads * head_dim * 8 / 4e6
-    best = (math.inf, (0, 0, 0, 0))
+    suffix_tiles = -(-expected // _PREFIX_TILE)
+    found = {}
     for splits in divisions:
-        if splits > 1 and pieces * splits > 2 * sms:
-            continue
+        if splits > max(1, 2 * sms // pieces) and splits > divisions[0]:
+            break
         chain = 6.0 + 1.35 * -(-suffix_tiles // splits)
         for ours in range(1, min(tiles, 32) + 1):
             if ours > 1 and units * ours > sms:
@@ -348,10 +356,8 @@ def _kernel_plan(rows, pieces, kv_heads, head_dim, tiles, suffix_tiles, expected
             time = max(least, last, chain, (units * ours * last + suffix) / sms) + 0.1 * last + (parts + splits) * per_part
             if 10 * units * ours > 7 * sms:
                 time += 8.0 + suffix / sms
-            best = min(best, (time, (0, ours, splits, parts + splits)))
-    if best[1][1] == 0:          # more suffixes than the divisions allow for
-        return _kernel_plan(rows, pieces, kv_heads, head_dim, tiles, suffix_tiles, expected, {1}, least, sms)
-    return best
+            found[0, ours, splits, parts + splits] = time
+    return found
 
 
 def shared_prefix_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -369,13 +375,13 @@ def shared_prefix_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cach
     block is shared up to that block. Heads are 64 or 128 wide, ``Hq / Hkv`` is at most 128.
 
     ``max_context``: a host-side bound on the context lengths from which the number of parts per sequence is chosen (without
-    one: what the tables can hold, but the work is divided for suffixes of up to 256 tokens). It bounds nothing that is
+    one: what the tables can hold, or 512 tokens behind the prefix if that is more than 1024). It bounds nothing that is
     read. A row whose sequence has no token at all comes out as zeros. ``scale`` defaults to ``1 / sqrt(hd)``; ``out``
     (contiguous, shaped like ``q``, 16-byte aligned, apart from the inputs) receives the result.
     """
     if out is None and native.fast is not None:
         found = native.fast.shared_prefix_attention(q, key_cache, value_cache, block_tables, context_lens, prefix_len, q_len, scale,
-                                                    max_context, _EXPECTED_SUFFIX, prefix_plan)
+                                                    max_context, prefix_plan)
         if found is not None:
             native.launch_count += 2
             return found
@@ -433,8 +439,7 @@ def shared_prefix_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cach
     group = heads // kv_heads
     room = max_blocks * block_size
     behind = max(0, (room if max_context is None else min(max_context, room)) - shared)
-    expected = behind if max_context is not None else min(behind, _EXPECTED_SUFFIX)
-    prefix_tokens, prefix_splits, splits, parts = prefix_plan(n, q_len, group, kv_heads, head_dim, shared, behind, expected)
+    prefix_tokens, prefix_splits, splits, parts = prefix_plan(n, q_len, group, kv_heads, head_dim, shared, behind, int(max_context is not None))
     # fp32 parts of every (row, head): un-normalised outputs, then (reference maximum, sum) pairs
     count = total * heads * parts
     workspace = torch.empty(count * (head_dim + 2), dtype=_F32, device=q.device)

@@ -155,8 +155,7 @@ def test_division_of_shared_prefix_attention_is_one_that_the_kernels_take(monkey
         n, q_len = int(2 ** rng.uniform(0, 10)), rng.choice([1, 1, 1, 2, 5, 17, 300])
         group, kv_heads, hd = rng.choice([1, 2, 4, 6, 8, 16, 32, 71, 128]), rng.choice([1, 2, 8, 16, 32]), rng.choice([64, 128])
         shared, behind = 16 * int(2 ** rng.uniform(-1, 11)), int(2 ** rng.uniform(-1, 15))
-        expected = rng.choice([behind, min(behind, 256)])
-        tokens, ours, splits, parts = serving.prefix_plan(n, q_len, group, kv_heads, hd, shared, behind, expected)
+        tokens, ours, splits, parts = serving.prefix_plan(n, q_len, group, kv_heads, hd, shared, behind, rng.choice([0, 1]))
         tiles, rows = -(-shared // 128), n * q_len * group
         if not shared:
             assert (tokens, ours) == (0, 0) and parts == splits >= 1
