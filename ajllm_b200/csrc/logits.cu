@@ -163,15 +163,33 @@ __device__ __forceinline__ void for_history(const int* history, int len, int lo,
   }
 }
 
+// The row's first biases, as loaded by the first warp well before they are added.
+struct FirstBiases {
+  int id[2];
+  float value[2];
+  __device__ __forceinline__ void load(const Params& p, int row) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int i = 32 * u + (int)threadIdx.x;
+      const bool there = threadIdx.x < 32 && i < p.biases;
+      id[u] = there ? __ldg(p.bias_ids + (size_t)row * p.biases + i) : -1;
+      value[u] = there ? __ldg(p.bias_values + (size_t)row * p.biases + i) : 0.0f;
+    }
+  }
+};
+
 // The row's biases of tokens in [lo, hi), by the first warp: in list order, lanes with the same token one after another.
-__device__ __forceinline__ void add_biases(const Params& p, int row, float* out, const unsigned* mask, int lo, int hi) {
+__device__ __forceinline__ void add_biases(const Params& p, const FirstBiases& ahead, int row, float* out, const unsigned* mask, int lo,
+                                           int hi) {
   if (threadIdx.x >= 32) return;
   const int* ids = p.bias_ids + (size_t)row * p.biases;
   const float* values = p.bias_values + (size_t)row * p.biases;
 #pragma unroll 1
   for (int base = 0; base < p.biases; base += 32) {
     const int i = base + (int)threadIdx.x;
-    const int v = i < p.biases ? __ldg(ids + i) : -1;
+    const bool later = base >= 64 && i < p.biases;
+    const int v = base == 0 ? ahead.id[0] : base == 32 ? ahead.id[1] : later ? __ldg(ids + i) : -1;
+    const float value = base == 0 ? ahead.value[0] : base == 32 ? ahead.value[1] : later ? __ldg(values + i) : 0.0f;
     const bool mine = v >= lo && v < hi && open_token(mask, v);
     // turn of this lane among the lanes with the same token
     const unsigned same = __match_any_sync(0xffffffffu, mine ? v : -1);
@@ -180,7 +198,7 @@ __device__ __forceinline__ void add_biases(const Params& p, int row, float* out,
     for (int k = 0; k < turns; ++k) {
       if (mine && turn == k) {
         volatile float* at = out + v;
-        *at = __fadd_rn(*at, __ldg(values + i));
+        *at = __fadd_rn(*at, value);
       }
       __syncwarp();
     }
@@ -200,9 +218,17 @@ __global__ void __launch_bounds__(kStreamThreads + kHistoryThreads) process_logi
   const unsigned* mask = p.mask != nullptr ? p.mask + (size_t)row * p.mask_pitch : nullptr;
   const int* history = p.history != nullptr ? p.history + (size_t)row * p.history_pitch : nullptr;
   const int thread = threadIdx.x;
-  int len = 0;
-
-  if (history != nullptr) len = min(max(p.history_lens[row], 0), p.history_width);
+  // what is needed behind the streaming is asked for in front of it
+  const int stored = history != nullptr ? p.history_lens[row] : 0;
+  float r = 1.0f, pr = 0.0f, f = 0.0f;
+  if (history != nullptr) {
+    if (p.repetition != nullptr) r = p.repetition[row];
+    if (p.presence != nullptr) pr = p.presence[row];
+    if (p.frequency != nullptr) f = p.frequency[row];
+  }
+  FirstBiases ahead;
+  ahead.load(p, row);
+  const int len = min(max(stored, 0), p.history_width);
   if (thread < kStreamThreads) {
     stream_piece<T>(in, out, mask, lo, hi, thread, kStreamThreads);
   } else if (len > 0) {
@@ -216,9 +242,6 @@ __global__ void __launch_bounds__(kStreamThreads + kHistoryThreads) process_logi
   // ---- tokens of the history
   if (len > 0) {
     __syncthreads();
-    const float r = p.repetition != nullptr ? p.repetition[row] : 1.0f;
-    const float pr = p.presence != nullptr ? p.presence[row] : 0.0f;
-    const float f = p.frequency != nullptr ? p.frequency[row] : 0.0f;
     for_history(history, len, lo, hi, thread, kStreamThreads + kHistoryThreads, [&](int, int v) {
       const unsigned held = Tab::take(table, v - lo);
       if (held == 0u || !open_token(mask, v)) return;
@@ -232,7 +255,7 @@ __global__ void __launch_bounds__(kStreamThreads + kHistoryThreads) process_logi
 
   if (p.biases > 0) {
     __syncthreads();
-    add_biases(p, row, out, mask, lo, hi);
+    add_biases(p, ahead, row, out, mask, lo, hi);
   }
 }
 
@@ -338,6 +361,8 @@ __global__ void __launch_bounds__(kMendThreads, 6) mend_logits_kernel(const Para
   const T* in = reinterpret_cast<const T*>(p.in) + (size_t)row * p.in_pitch;
   float* out = p.out + (size_t)row * p.vocab;
   const unsigned* mask = p.mask != nullptr ? p.mask + (size_t)row * p.mask_pitch : nullptr;
+  FirstBiases ahead;
+  ahead.load(p, row);
   if (p.history != nullptr) {
     const int cells = min(kRange, (p.vocab + 7) & ~7);
     int* tokens = reinterpret_cast<int*>(table + Tab::words(cells));
@@ -433,7 +458,7 @@ __global__ void __launch_bounds__(kMendThreads, 6) mend_logits_kernel(const Para
   }
   if (p.biases > 0) {
     __syncthreads();
-    add_biases(p, row, out, mask, 0, p.vocab);
+    add_biases(p, ahead, row, out, mask, 0, p.vocab);
   }
 }
 

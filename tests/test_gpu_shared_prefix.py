@@ -770,3 +770,102 @@ def test_a_result_that_does_not_fit_the_device_is_an_exception():
     with pytest.raises(torch.OutOfMemoryError):
         serving.process_logits(row.expand(300_000, -1))                    # 1.2 TB of results
     assert torch.equal(serving.process_logits(row), row)
+
+
+# --------------------------------------------------------------------------------------------- launches that start early
+
+
+def _slow_copies(pairs):
+    """Writes every ``src`` into its ``dst`` behind a product that takes a while, the last write directly in front of what follows."""
+    a = torch.full((4096, 4096), 1e-4, device=_dev(), dtype=torch.bfloat16)
+    for dst, src in pairs:
+        late = (a @ a).sum() * 0
+        dst.copy_(src + late.to(src.dtype))
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_inputs_written_directly_in_front_of_a_call_are_the_ones_it_reads(captured):
+    """Each operator behind a launch that writes its inputs late, and in front of one that overwrites them."""
+    logits, kw = _logits_inputs(5, 3000, torch.bfloat16, 40, 5, True)
+    many, many_kw = _logits_inputs(300, 32_000, torch.bfloat16, 40, 5, True)
+    few = _batch(8, 2, 128, 1, 512, [1, 17, 130, 500])
+    rows = _batch(32, 8, 128, 1, 2048, list(range(1, 100)))
+    maps = [_i32([3, 4, 5, 6]), _i32([1, 3]), _i32([2, 17]), _i32([1, 9])]
+
+    def move(tensors):
+        return [t.cuda() for t in tensors]
+
+    cases = []
+    for fn, given in ((lambda x, *t: serving.process_logits(x, **dict(zip(kw, t))), move([logits, *kw.values()])),
+                      (lambda x, *t: serving.process_logits(x, **dict(zip(many_kw, t))), move([many, *many_kw.values()])),
+                      (lambda *t: serving.shared_prefix_attention(*t, 512), list(few)),
+                      (lambda *t: serving.shared_prefix_attention(*t, 2048), list(rows)),
+                      (lambda *t: serving.batch_maps(*t, 12, 4, pad_block=1), maps)):
+        want = fn(*given)
+        torch.cuda.synchronize()
+        cases.append((fn, given, [t.clone() for t in given], want if isinstance(want, tuple) else (want,)))
+
+    def run():
+        found = []
+        for fn, given, kept, _ in cases:
+            _slow_copies(zip(given, kept))
+            got = fn(*given)
+            for t in given:
+                t.zero_()
+            found.append(got if isinstance(got, tuple) else (got,))
+        # and one behind another, each reading what the one in front of it has written
+        _slow_copies([(cases[0][1][0], cases[0][2][0])])
+        once = serving.process_logits(cases[0][1][0])
+        found.append((serving.process_logits(serving.process_logits(once)),))
+        return found
+
+    for _, given, _, _ in cases:
+        for t in given:
+            t.zero_()
+    if captured:
+        run()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            found = run()
+        graph.replay()
+        graph.replay()
+    else:
+        found = run()
+    torch.cuda.synchronize()
+    for got, (_, _, _, want) in zip(found, cases):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(found[-1][0], cases[0][2][0].float())
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_calls_behind_two_streams(captured):
+    """A call that follows work of its own stream and, through an event, of another one waits for both."""
+    ids, counts, cached, new = maps = [_i32([3, 4, 5, 6]), _i32([1, 3]), _i32([2, 17]), _i32([1, 9])]
+    kept = [t.clone() for t in maps]
+    want = serving.batch_maps(*maps, 12, 4, pad_block=1)
+    side = torch.cuda.Stream()
+
+    def run():
+        main = torch.cuda.current_stream()
+        for t in maps:
+            t.zero_()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            _slow_copies([(cached, kept[2]), (ids, kept[0])])
+        new.copy_(kept[3])
+        counts.copy_(kept[1])
+        main.wait_stream(side)
+        return serving.batch_maps(*maps, 12, 4, pad_block=1)
+
+    if captured:
+        run()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = run()
+        graph.replay()
+    else:
+        got = run()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
