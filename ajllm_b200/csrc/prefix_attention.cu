@@ -87,6 +87,8 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
   uint8_t* sStore = sV + kStages * C::kTile;
   float* sExchange = reinterpret_cast<float*>(sStore + 16 * C::kStoreBlock);
   uint64_t* bars = reinterpret_cast<uint64_t*>(sStore + 16 * C::kStoreBlock + C::kExchange);
+  // in this order: the suffix launch reads the inputs without waiting for anything but its start
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (smem_misaligned(smem, p.status, kPrefixKernelId, reinterpret_cast<uint32_t*>(bars) + 120)) return;
   uint64_t* k_full = bars;               // kStages (<= 5)
@@ -455,9 +457,7 @@ static int launch_prefix(const paged::Launch& a, int shared, int splits, cudaStr
   p.status = device_status_buffer();
   const long long grid = (long long)(p.pairs == 0 ? 1 : p.pairs) * p.kv_heads * p.splits;
   AJB_REQUIRE(grid <= 0x7fffffffll, "shared prefix attention: too many query rows");
-  prefix_attention_kernel<HD><<<(int)grid, kThreads, C::kSmem, stream>>>(*a.map_k, *a.map_v, p);
-  AJB_CUDA_OK(cudaGetLastError());
-  return 0;
+  return launch_early(prefix_attention_kernel<HD>, dim3((unsigned)grid), dim3(kThreads), C::kSmem, stream, *a.map_k, *a.map_v, p);
 }
 
 }  // namespace prefix
