@@ -8,15 +8,16 @@
 // key `shared` on; both leave un-normalised fp32 parts, which a small kernel joins.
 //
 // The prefix kernel takes a share of the prefix in steps of 128 keys, with two streams of 128 query rows per CTA
-// (S = Q K^T, softmax, O += P V with S, P and O in tensor memory, P written over the scores it came from): while four
+// (S = Q K^T, softmax, O += P V with S, P and O in tensor memory, P written over the scores it came from): while eight
 // warps turn one stream's scores into probabilities, the tensor pipe runs the other's products. A 128 x 128 step is two
-// products of 512 cycles and 16384 exponentials, 1024 cycles of the SM's exponential unit, so the two streams keep both
-// about equally busy. The streams are two row tiles that share every K and V tile; when all rows fit one tile they are
+// products of 512 cycles and 16384 exponentials, 1024 cycles of the SM's exponential unit, for which it takes 1600 to 1900:
+// the chain of waits (scores, maxima of the other half of the keys, probabilities, products) is what bounds it, with no
+// exponentials it is 2 % faster. The streams are two row tiles that share every K and V tile; when all rows fit one tile they are
 // two halves of the keys instead (even and odd tiles, two parts; one part when a CTA has a single tile).
 //
 // A prefix CTA has an SM to itself (shared memory), the suffix launch, which does not read what this one writes, starts
-// as soon as every CTA here has and takes the other SMs: the prefix is bound by arithmetic (a step of 256 rows x 128 keys
-// of 128 takes 1.68 us, 148 CTAs 0.95 of the 1.6 PFLOP/s that a library product reaches without the exponentials), the
+// as soon as every CTA here has and takes the other SMs: the prefix is bound by its steps (one of 256 rows x 128 keys of
+// 128 takes 1.7 us, 148 CTAs 0.95 of the 1.6 PFLOP/s that a library product reaches without the exponentials), the
 // suffix by memory, and the number of prefix CTAs divides the SMs so that both last about as long.
 //
 // This kernel starts slowly (11 to 14 us until its first parts are stored, for barriers, 512 columns of tensor memory and
