@@ -869,3 +869,16 @@ def test_calls_behind_two_streams(captured):
         got = run()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_runner_takes_a_step_of_too_many_sequences_in_parts(engine_model, monkeypatch):
+    from ajllm_b200.engine import LLMEngine
+    from ajllm_b200.engine.model_runner import ModelRunner, RunItem
+    _, prompts = _engine_prompts()
+    items = [RunItem(i, p, 1 + i % 2) for i, p in enumerate(prompts[:5])]
+    want = LLMEngine(engine_model, num_blocks=256).runner.forward(items)
+    monkeypatch.setattr(ModelRunner, "MAX_SEQUENCES", 2)
+    got = LLMEngine(engine_model, num_blocks=256).runner.forward(items)
+    assert got.shape == want.shape == (7, 1000)
+    # products of other row counts may sum in another order
+    assert float((got - want).abs().max()) < 0.08 * float(want.abs().max())

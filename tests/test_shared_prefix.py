@@ -533,3 +533,22 @@ def test_lm_generate_shares_the_prompts_beginning_and_penalises(tmp_path):
     assert [text.rstrip("A") for text in biased] == [p for p in config["prompts"] for _ in range(2)]
     assert all(text.endswith("A" * 6) for text in biased)          # 8 where the context has room for them
     assert parameters["logit_bias"] == {65: 1000.0} and parameters["frequency_penalty"] == 0.5
+
+
+def test_the_extension_leaves_cpu_tensors_alone():
+    """With the kernel library loaded, CPU calls still take the plain statements, and wrong ones their own errors."""
+    from ajllm_b200.ops import native
+    if not native.available():
+        pytest.skip("the kernel library is not built")
+    assert native.fast is not None
+    maps = (_i32([3, 4]), _i32([1, 1]), _i32([2, 0]), _i32([1, 1]))
+    assert native.fast.batch_maps(*maps, 2, 2, 16, 0, None) is None and native.fast.batch_maps() is None
+    assert serving.batch_maps(*maps, 2, 2).slots.tolist() == [3 * 16 + 2, 4 * 16]
+    assert native.fast.process_logits(*[None] * 10) is None and native.fast.process_logits(torch.zeros(1, 2), *[None] * 9) is None
+    assert serving.process_logits(torch.ones(1, 2)).tolist() == [[1.0, 1.0]]
+    call = _attention_call()
+    serving.shared_prefix_attention(**call)
+    assert native.fast.shared_prefix_attention(*call.values(), 1, None, None, serving.prefix_plan) is None
+    for wrong in (dict(prefix_len="8"), dict(q=None), dict(block_tables=3)):
+        with pytest.raises((TypeError, AttributeError, ValueError)):
+            serving.shared_prefix_attention(**{**call, **wrong})
