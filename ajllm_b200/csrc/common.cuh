@@ -181,7 +181,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
 
 // The same wait with its rare part (looking at the clock, giving up) out of line: kernels whose warps walk through a lot
 // of code once per piece of work lose more to instruction fetches than a call costs. Returns the time of the first look
-// at the clock, 0 once the budget is spent.
+// at the clock, 0 once the time is up.
 static __device__ __noinline__ unsigned long long wait_overdue(unsigned long long since, volatile uint32_t* abort_flag,
                                                                DeviceStatus* status, int kernel_id, int stage, uint32_t parity) {
   const unsigned long long now = global_timer_ns();

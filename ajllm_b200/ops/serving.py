@@ -292,7 +292,7 @@ def prefix_plan(n: int, q_len: int, group: int, kv_heads: int, head_dim: int, sh
     times = []
     for expected in (behind,) if known else (behind // 2, behind) if behind <= 1024 else (128, 512):
         least = 3.0 + (n * expected + shared) * kv_heads * head_dim * 4 / 6.5e6       # reading the caches once
-        found = _kernel_plans(rows, pieces, kv_heads, head_dim, tiles, expected, divisions, least, sms)
+        found = _kernel_plans(n, rows, pieces, kv_heads, head_dim, tiles, expected, divisions, least, sms)
         if group * q_len <= 32:
             found.update(_pieces_plans(n, q_len, group, kv_heads, head_dim, tiles, expected, divisions, least, sms))
         times.append((min(found.values()), found))
@@ -328,17 +328,17 @@ def _pieces_plans(n, q_len, group, kv_heads, head_dim, tiles, expected, division
     return found
 
 
-def _kernel_plans(rows, pieces, kv_heads, head_dim, tiles, expected, divisions, least, sms):
+def _kernel_plans(n, rows, pieces, kv_heads, head_dim, tiles, expected, divisions, least, sms):
     """The prefix kernel beside the suffixes' launch. A CTA of it keeps an SM to itself while the others stream the suffixes,
     so the SMs are divided like the work: a prefix CTA takes about 14 us and 2 us more per step (128 keys for up to 256 rows;
-    two tiles make a step when 128 rows are all there are, and it starts 3 us sooner), a suffix occupies half an SM for 1.3 us
-    and 2.7 us (64-wide heads: 1.3 us) per 128 keys; a part costs its fp32 rows, written and read once at 4 TB/s. With more
+    two tiles make a step when 128 rows are all there are, and it starts 3 us sooner), a suffix half an SM for 3.5 us and
+    1.1 us per 128 keys (sequences of more than 16 rows: 1.5 us), or longer when all of them together are bound by memory;
+    a part costs its fp32 rows, written and read once at 4 TB/s. With more
     prefix CTAs than 7 in 10 SMs the suffixes hardly run before they end (33 x 5 rows behind 4001 tokens: 28 us with 96 CTAs,
     37 us with 120)."""
     one_tile = rows <= _PREFIX_TILE
     units = kv_heads * (1 if one_tile else -(-rows // (2 * _PREFIX_TILE)))
-    step = 1.35 if head_dim == 128 else 0.65
-    suffix = pieces * (0.65 + step * (expected / 256 + 0.5))          # of `expected` at the most: half of it on average
+    step = 1.1 if rows <= 16 * n else 1.5
     per_part = rows * kv_heads * head_dim * 8 / 4e6
     suffix_tiles = -(-expected // _PREFIX_TILE)
     found = {}
@@ -346,6 +346,8 @@ def _kernel_plans(rows, pieces, kv_heads, head_dim, tiles, expected, divisions, 
         if splits > max(1, 2 * sms // pieces) and splits > divisions[0]:
             break
         chain = 6.0 + 1.35 * -(-suffix_tiles // splits)
+        many, each = pieces * splits, 3.5 + step * (expected / 256 + 0.5) / splits          # half of `expected` on average
+        alone = max(many * each / (2 * sms), least - 3.0)          # all suffixes on all SMs
         for ours in range(1, min(tiles, 32) + 1):
             if ours > 1 and units * ours > sms:
                 break
@@ -353,9 +355,10 @@ def _kernel_plans(rows, pieces, kv_heads, head_dim, tiles, expected, divisions, 
             if parts + splits > 64:
                 continue
             last = 11.0 + -(-tiles // ours) if one_tile else 14.0 + 2.0 * -(-tiles // ours)
-            time = max(least, last, chain, (units * ours * last + suffix) / sms) + 0.1 * last + (parts + splits) * per_part
+            done = min(1.0, last * 2 * max(0, sms - units * ours) / (many * each))          # of the suffixes, when the prefix ends
+            time = max(least, chain, last + (1.0 - done) * alone) + 0.1 * last + (parts + splits) * per_part
             if 10 * units * ours > 7 * sms:
-                time += 8.0 + suffix / sms
+                time += 8.0 + alone
             found[0, ours, splits, parts + splits] = time
     return found
 
