@@ -85,7 +85,6 @@ __device__ __forceinline__ int find(const int* sums, int n, int t) {
 }
 
 __global__ void __launch_bounds__(kThreads) batch_maps_kernel(const Params p) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   extern __shared__ int sums[];
   __shared__ int2 warp_sums[kThreads / 32];

@@ -37,9 +37,11 @@ const char* last_error();
     }                                       \
   } while (0)
 
-// Host side: a launch that may start before the one in front of it in its stream has ended. The kernel calls
-// griddepcontrol.wait before it reads or writes global memory, and griddepcontrol.launch_dependents where the launch behind
-// it may start likewise. Back to back this takes the 2 us between two small kernels away.
+// Host side: a launch that may be set up before the one in front of it in its stream has ended. The kernel calls
+// griddepcontrol.wait before it reads or writes global memory. Back to back this takes most of the 2 us between two small
+// kernels away; it is all that is gained: letting the next launch's CTAs in early (griddepcontrol.launch_dependents at the
+// start) takes room from this one's (maps of 64 prompts: 3.6 us without, 6.3 us with it), so only launches of one operator
+// that belong together do that.
 template <typename... Params, typename... Args>
 int launch_early(void (*kernel)(Params...), dim3 grid, dim3 block, int smem, cudaStream_t stream, const Args&... args) {
   cudaLaunchConfig_t cfg = {};

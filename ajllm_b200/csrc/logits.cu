@@ -208,7 +208,6 @@ __device__ __forceinline__ void add_biases(const Params& p, const FirstBiases& a
 template <typename T, bool kNarrow>
 __global__ void __launch_bounds__(kStreamThreads + kHistoryThreads) process_logits_kernel(const Params p) {
   extern __shared__ unsigned table[];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   using Tab = Table<kNarrow>;
   const int row = (int)(blockIdx.x / (unsigned)p.chunks), part = (int)(blockIdx.x % (unsigned)p.chunks);

@@ -1002,14 +1002,13 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 // out[row, head, :] = sum_z w_z O_z / sum_z w_z l_z with w_z = 2^(m_z - max m): one warp per (row, head), HD / 32
 // neighbouring elements per lane. The parts are read at once, before their weights are known: what bounds the kernel is
 // the latency of two dependent reads, not the bytes. It is launched while the launch in front of it still runs and waits
-// for it (and so for everything that one has waited for) on the device. Behind a prefix kernel it does not let the next
-// launch start early in turn: a prefix kernel that starts among these CTAs takes whole pairs of SMs instead of one of each,
-// and the suffixes are left with fewer of the paths to memory that pairs share (33 x 5 rows: 33 us instead of 28).
+// for it (and so for everything that one has waited for) on the device. It does not let the next launch start among its own
+// CTAs in turn: a prefix kernel then takes whole pairs of SMs instead of one of each, and the suffixes are left with fewer
+// of the paths to memory that pairs share (33 x 5 rows, back to back: 33 us instead of 28).
 template <int HD>
 __global__ void __launch_bounds__(128) merge_splits_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml,
                                                            __nv_bfloat16* __restrict__ out, const int* __restrict__ q_start, int q_len,
-                                                           int heads, int splits, long long pairs /* sequences * q_len * heads */,
-                                                           bool early) {
+                                                           int heads, int splits, long long pairs /* sequences * q_len * heads */) {
   const int lane = threadIdx.x & 31;
   const long long w = (blockIdx.x * (long long)blockDim.x + threadIdx.x) >> 5;
   if (w >= pairs) return;
@@ -1019,7 +1018,6 @@ __global__ void __launch_bounds__(128) merge_splits_kernel(const float* __restri
     const int seq = (int)(local_row / q_len);
     out_row = (size_t)(q_start[seq] + (int)(local_row - (long long)seq * q_len)) * heads + (size_t)(w - local_row * heads);
   }
-  if (early) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   constexpr int kPerLane = HD / 32;
   constexpr int kBatch = 4;
@@ -1161,7 +1159,7 @@ template <int HD>
 static int launch_merge(const Launch& a, cudaStream_t stream) {
   const long long pairs = (long long)a.num_seqs * a.q_total * a.heads;
   return launch_early(merge_splits_kernel<HD>, dim3((unsigned)((pairs * 32 + 127) / 128)), dim3(128), 0, stream, (const float*)a.part_o,
-                      (const float2*)a.part_ml, (__nv_bfloat16*)a.out, (const int*)a.q_start, a.q_total, a.heads, a.part_stride, pairs, a.early);
+                      (const float2*)a.part_ml, (__nv_bfloat16*)a.out, (const int*)a.q_start, a.q_total, a.heads, a.part_stride, pairs);
 }
 
 int merge_parts(const Launch& a, int head_dim, cudaStream_t stream) {
