@@ -197,8 +197,16 @@ extern "C" int ajb_batch_maps(const void* arguments) {
   p.tables = (int*)tables; p.positions = (int*)positions; p.slots = (long long*)slots; p.q_start = (int*)q_start;
   p.context = (int*)context;
   const int smem = 3 * (seqs + 1) * (int)sizeof(int);
-  if (smem > 48 * 1024)      // per device and cheap next to a batch of thousands of sequences: set on every such call
-    AJB_CUDA_OK(cudaFuncSetAttribute(maps::batch_maps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  // Function attributes belong to a device: raised once on each, to what the largest call takes, and never lowered, as
+  // another thread may be between this and its launch. (What a launch may use without it, 48 KB, holds the static array too.)
+  static bool configured[kMaxDevices] = {};
+  int dev = 0;
+  AJB_CUDA_OK(cudaGetDevice(&dev));
+  if (dev >= kMaxDevices || !configured[dev]) {
+    AJB_CUDA_OK(cudaFuncSetAttribute(maps::batch_maps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     3 * (maps::kMaxSeqs + 1) * (int)sizeof(int)));
+    if (dev < kMaxDevices) configured[dev] = true;
+  }
   const long long pieces = ((long long)total + 3) / 4 + ((long long)seqs * width + 3) / 4 + 1;
   const long long blocks = (pieces + maps::kThreads - 1) / maps::kThreads;
   return launch_early(maps::batch_maps_kernel, dim3((unsigned)(blocks < 4ll * sm_count() ? blocks : 4ll * sm_count())),

@@ -2,6 +2,10 @@
 64 bits, at the sizes and masks where they can go wrong."""
 
 import math
+import subprocess
+import sys
+import threading
+from pathlib import Path
 
 import pytest
 import torch
@@ -98,6 +102,44 @@ def test_batch_maps_replayed_from_a_graph():
     want = serving.batch_maps(ids.cpu(), counts.cpu(), cached.cpu(), new.cpu(), 16, 12, pad_block=99)
     for a, b in zip(out, want):
         assert torch.equal(a.cpu(), b)
+
+
+_MAPS_OF_SIZES = """
+import torch
+from ajllm_b200.ops import serving
+for n in (4089, 4090, 4095, 4096, 16384, 4095):
+    ones = torch.ones(n, dtype=torch.int32, device="cuda")
+    got = serving.batch_maps(torch.arange(n, dtype=torch.int32, device="cuda"), ones, ones - 1, ones, n, 1)
+    assert torch.equal(got.slots, 16 * torch.arange(n, device="cuda")) and int(got.q_start[n]) == n, n
+"""
+
+
+def test_batch_maps_whose_lengths_just_fill_the_ordinary_shared_memory():
+    """In a process that has made no larger call: 12 bytes per sequence and the kernel's static array pass 48 KB from 4090 on."""
+    done = subprocess.run([sys.executable, "-c", _MAPS_OF_SIZES], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_batch_maps_of_large_and_small_batches_from_two_threads():
+    failed = []
+
+    def calls(n):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                ones = torch.ones(n, dtype=torch.int32, device=_dev())
+                ids = torch.arange(n, dtype=torch.int32, device=_dev())
+                for _ in range(200):
+                    got = serving.batch_maps(ids, ones, ones - 1, ones, n, 1)
+                assert torch.equal(got.slots, 16 * ids.long())
+        except Exception as error:          # (an assertion in a thread would be lost)
+            failed.append(error)
+
+    threads = [threading.Thread(target=calls, args=(n,)) for n in (16384, 4200, 16384, 5000)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not failed
 
 
 # --------------------------------------------------------------------------------------------- attention
