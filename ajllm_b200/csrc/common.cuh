@@ -611,6 +611,54 @@ __device__ __forceinline__ uint4 ld_nc_v4(const uint4* ptr) {
   return v;
 }
 
+// Loads of what launches in front of this one write, for kernels that start before those have ended: the read-only path (.nc,
+// __ldg, const __restrict__) takes memory to be unchanged from the kernel's start on, and the compiler may then move such a
+// load in front of the wait (griddepcontrol.wait). Volatile loads stay behind it:
+__device__ __forceinline__ uint4 ld_v4(const uint4* ptr) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(ptr));
+  return v;
+}
+__device__ __forceinline__ float4 ld_l2(const float4* ptr) {          // cached in L2 only
+  float4 v;
+  asm volatile("ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(ptr));
+  return v;
+}
+__device__ __forceinline__ float2 ld_l2(const float2* ptr) {
+  float2 v;
+  asm volatile("ld.global.cg.v2.f32 {%0, %1}, [%2];\n" : "=f"(v.x), "=f"(v.y) : "l"(ptr));
+  return v;
+}
+// Others stay behind it because their address does: it has passed `behind_wait` after the wait. Among other reads and writes
+// they may move, since what they read does not change any more.
+template <typename T>
+__device__ __forceinline__ T* behind_wait(T* ptr) {
+  asm volatile("" : "+l"(ptr));
+  return ptr;
+}
+__device__ __forceinline__ unsigned ld_settled(const unsigned* ptr) {
+  unsigned v;
+  asm("ld.global.u32 %0, [%1];\n" : "=r"(v) : "l"(ptr));
+  return v;
+}
+__device__ __forceinline__ int ld_settled(const int* ptr) { return (int)ld_settled(reinterpret_cast<const unsigned*>(ptr)); }
+__device__ __forceinline__ float ld_settled(const float* ptr) { return __uint_as_float(ld_settled(reinterpret_cast<const unsigned*>(ptr))); }
+__device__ __forceinline__ unsigned short ld_settled(const unsigned short* ptr) {
+  unsigned short v;
+  asm("ld.global.u16 %0, [%1];\n" : "=h"(v) : "l"(ptr));
+  return v;
+}
+__device__ __forceinline__ uint2 ld_settled(const uint2* ptr) {
+  uint2 v;
+  asm("ld.global.v2.u32 {%0, %1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "l"(ptr));
+  return v;
+}
+__device__ __forceinline__ uint4 ld_settled(const uint4* ptr) {
+  uint4 v;
+  asm("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(ptr));
+  return v;
+}
+
 // ---- bulk copies (async proxy, no multicast)
 __device__ __forceinline__ void bulk_g2s(void* smem_dst, const void* gmem_src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(

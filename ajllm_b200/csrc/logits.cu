@@ -54,6 +54,8 @@ struct Table {
   }
 };
 
+// (Inputs are read through pointers that have passed behind_wait: the kernels start before the launch in front of them, which
+// may write those inputs, has ended.)
 struct Params {
   const void* in;
   long long in_pitch;
@@ -76,10 +78,10 @@ struct Params {
 template <typename T>
 __device__ __forceinline__ float load1(const T* p);
 template <>
-__device__ __forceinline__ float load1<float>(const float* p) { return __ldg(p); }
+__device__ __forceinline__ float load1<float>(const float* p) { return ld_settled(p); }
 template <>
 __device__ __forceinline__ float load1<__nv_bfloat16>(const __nv_bfloat16* p) {
-  return __uint_as_float((unsigned)__ldg(reinterpret_cast<const unsigned short*>(p)) << 16);
+  return __uint_as_float((unsigned)ld_settled(reinterpret_cast<const unsigned short*>(p)) << 16);
 }
 // four neighbouring logits, as loaded and as fp32 bits
 template <typename T>
@@ -87,18 +89,18 @@ struct Four;
 template <>
 struct Four<float> {
   uint4 v;
-  __device__ __forceinline__ void load(const float* p) { v = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void load(const float* p) { v = ld_settled(reinterpret_cast<const uint4*>(p)); }
   __device__ __forceinline__ uint4 wide() const { return v; }
 };
 template <>
 struct Four<__nv_bfloat16> {
   uint2 v;
-  __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = __ldg(reinterpret_cast<const uint2*>(p)); }
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = ld_settled(reinterpret_cast<const uint2*>(p)); }
   __device__ __forceinline__ uint4 wide() const { return make_uint4(v.x << 16, v.x & 0xffff0000u, v.y << 16, v.y & 0xffff0000u); }
 };
 
 __device__ __forceinline__ bool open_token(const unsigned* mask, int v) {
-  return mask == nullptr || ((__ldg(mask + (v >> 5)) >> (v & 31)) & 1u);
+  return mask == nullptr || ((ld_settled(mask + (v >> 5)) >> (v & 31)) & 1u);
 }
 
 // Tokens [lo, hi) of a row, widened and masked, by `threads` threads.
@@ -124,7 +126,7 @@ __device__ __forceinline__ void stream_piece(const T* in, float* out, const unsi
       open[u] = g < groups ? 15u : 0u;
       if (mask != nullptr && g < groups) {
         // a group lies in one word, or in two neighbours when the row does not start on a 16-byte boundary
-        const unsigned w0 = __ldg(mask + (v >> 5)), w1 = (v & 31) > 28 ? __ldg(mask + (v >> 5) + 1) : 0u;
+        const unsigned w0 = ld_settled(mask + (v >> 5)), w1 = (v & 31) > 28 ? ld_settled(mask + (v >> 5) + 1) : 0u;
         open[u] = __funnelshift_r(w0, w1, v & 31) & 15u;
       }
     }
@@ -155,7 +157,7 @@ __device__ __forceinline__ void for_history(const int* history, int len, int lo,
 #pragma unroll
     for (int u = 0; u < kHistoryUnroll; ++u) {
       const int i = i0 + u * threads;
-      v[u] = i < len ? __ldg(history + i) : -1;
+      v[u] = i < len ? ld_settled(history + i) : -1;
     }
 #pragma unroll
     for (int u = 0; u < kHistoryUnroll; ++u)
@@ -168,12 +170,14 @@ struct FirstBiases {
   int id[2];
   float value[2];
   __device__ __forceinline__ void load(const Params& p, int row) {
+    const int* ids = behind_wait(p.bias_ids);
+    const float* values = behind_wait(p.bias_values);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int i = 32 * u + (int)threadIdx.x;
       const bool there = threadIdx.x < 32 && i < p.biases;
-      id[u] = there ? __ldg(p.bias_ids + (size_t)row * p.biases + i) : -1;
-      value[u] = there ? __ldg(p.bias_values + (size_t)row * p.biases + i) : 0.0f;
+      id[u] = there ? ld_settled(ids + (size_t)row * p.biases + i) : -1;
+      value[u] = there ? ld_settled(values + (size_t)row * p.biases + i) : 0.0f;
     }
   }
 };
@@ -182,14 +186,14 @@ struct FirstBiases {
 __device__ __forceinline__ void add_biases(const Params& p, const FirstBiases& ahead, int row, float* out, const unsigned* mask, int lo,
                                            int hi) {
   if (threadIdx.x >= 32) return;
-  const int* ids = p.bias_ids + (size_t)row * p.biases;
-  const float* values = p.bias_values + (size_t)row * p.biases;
+  const int* ids = behind_wait(p.bias_ids) + (size_t)row * p.biases;
+  const float* values = behind_wait(p.bias_values) + (size_t)row * p.biases;
 #pragma unroll 1
   for (int base = 0; base < p.biases; base += 32) {
     const int i = base + (int)threadIdx.x;
     const bool later = base >= 64 && i < p.biases;
-    const int v = base == 0 ? ahead.id[0] : base == 32 ? ahead.id[1] : later ? __ldg(ids + i) : -1;
-    const float value = base == 0 ? ahead.value[0] : base == 32 ? ahead.value[1] : later ? __ldg(values + i) : 0.0f;
+    const int v = base == 0 ? ahead.id[0] : base == 32 ? ahead.id[1] : later ? ld_settled(ids + i) : -1;
+    const float value = base == 0 ? ahead.value[0] : base == 32 ? ahead.value[1] : later ? ld_settled(values + i) : 0.0f;
     const bool mine = v >= lo && v < hi && open_token(mask, v);
     // turn of this lane among the lanes with the same token
     const unsigned same = __match_any_sync(0xffffffffu, mine ? v : -1);
@@ -212,10 +216,10 @@ __global__ void __launch_bounds__(kStreamThreads + kHistoryThreads) process_logi
   using Tab = Table<kNarrow>;
   const int row = (int)(blockIdx.x / (unsigned)p.chunks), part = (int)(blockIdx.x % (unsigned)p.chunks);
   const int lo = part * p.chunk, hi = min(p.vocab, lo + p.chunk);
-  const T* in = reinterpret_cast<const T*>(p.in) + (size_t)row * p.in_pitch;
+  const T* in = behind_wait(reinterpret_cast<const T*>(p.in)) + (size_t)row * p.in_pitch;
   float* out = p.out + (size_t)row * p.vocab;
-  const unsigned* mask = p.mask != nullptr ? p.mask + (size_t)row * p.mask_pitch : nullptr;
-  const int* history = p.history != nullptr ? p.history + (size_t)row * p.history_pitch : nullptr;
+  const unsigned* mask = p.mask != nullptr ? behind_wait(p.mask) + (size_t)row * p.mask_pitch : nullptr;
+  const int* history = p.history != nullptr ? behind_wait(p.history) + (size_t)row * p.history_pitch : nullptr;
   const int thread = threadIdx.x;
   // what is needed behind the streaming is asked for in front of it
   const int stored = history != nullptr ? p.history_lens[row] : 0;
@@ -274,13 +278,15 @@ __global__ void __launch_bounds__(kStreamThreads, 6) stream_logits_kernel(const 
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int thread = threadIdx.x, step = (int)gridDim.x, all = (p.vocab + 31) / 32;
+  const T* const logits = behind_wait(reinterpret_cast<const T*>(p.in));
+  const unsigned* const mask = behind_wait(p.mask);
   unsigned ahead[kEach];
   auto load_words = [&](int piece) {
     const int row = piece / p.chunks, first = (piece - row * p.chunks) * (kStreamChunk / 32);
 #pragma unroll
     for (int u = 0; u < kEach; ++u) {
       const int i = thread + u * kStreamThreads;
-      ahead[u] = i < kWords && first + i < all ? __ldg(p.mask + (size_t)row * p.mask_pitch + first + i) : 0u;
+      ahead[u] = i < kWords && first + i < all ? ld_settled(mask + (size_t)row * p.mask_pitch + first + i) : 0u;
     }
   };
   if (kMasked && (int)blockIdx.x < p.pieces) load_words((int)blockIdx.x);
@@ -289,7 +295,7 @@ __global__ void __launch_bounds__(kStreamThreads, 6) stream_logits_kernel(const 
   for (int piece = (int)blockIdx.x; piece < p.pieces; piece += step, turn ^= 1) {
     const int row = piece / p.chunks, part = piece - row * p.chunks;
     const int lo = part * kStreamChunk, hi = min(p.vocab, lo + kStreamChunk);
-    const T* in = reinterpret_cast<const T*>(p.in) + (size_t)row * p.in_pitch;
+    const T* in = logits + (size_t)row * p.in_pitch;
     float* out = p.out + (size_t)row * p.vocab;
     const unsigned* words = shared[turn];
     if (kMasked) {
@@ -357,6 +363,7 @@ __global__ void __launch_bounds__(kMendThreads, 6) mend_logits_kernel(const Para
   using Tab = Table<kNarrow>;
   constexpr int kRange = kNarrow ? kMendRange : kMendRange / 2;
   const int row = blockIdx.x, thread = threadIdx.x;
+  // the launches that write the inputs have ended when this one starts: every CTA of the streaming launch has waited for them
   const T* in = reinterpret_cast<const T*>(p.in) + (size_t)row * p.in_pitch;
   float* out = p.out + (size_t)row * p.vocab;
   const unsigned* mask = p.mask != nullptr ? p.mask + (size_t)row * p.mask_pitch : nullptr;
@@ -382,7 +389,7 @@ __global__ void __launch_bounds__(kMendThreads, 6) mend_logits_kernel(const Para
     if (held) {
 #pragma unroll 4
       for (int i = thread; i < len; i += kMendThreads) {
-        const int v = __ldg(history + i);
+        const int v = ld_settled(history + i);
         tokens[i] = (unsigned)v < (unsigned)p.vocab ? v : -1;          // below -1 stand tokens whose count has been taken
       }
     } else {
@@ -433,7 +440,7 @@ __global__ void __launch_bounds__(kMendThreads, 6) mend_logits_kernel(const Para
           v[u] = i < len ? -2 - tokens[i] : -1;
           if (v[u] >= 0) {
             x[u] = load1<T>(in + v[u]);
-            word[u] = mask != nullptr ? __ldg(mask + (v[u] >> 5)) : 0xffffffffu;
+            word[u] = mask != nullptr ? ld_settled(mask + (v[u] >> 5)) : 0xffffffffu;
           }
         }
 #pragma unroll

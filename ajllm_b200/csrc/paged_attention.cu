@@ -928,7 +928,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           const __nv_bfloat16* q = p.q + (size_t)next.token0 * p.q_pitch + (size_t)(next.kv_head * p.group) * HD;
 #pragma unroll
           for (int u = 0; u < kHeld; ++u)
-            if ((key_lane + 128 * u) / kChunks < next.rows) held[u] = ld_nc_v4(reinterpret_cast<const uint4*>(q + held_from[u]));
+            if ((key_lane + 128 * u) / kChunks < next.rows) held[u] = ld_v4(reinterpret_cast<const uint4*>(q + held_from[u]));
         }
       }
       const bool real = lane < rows && n_tiles >= 0;
@@ -1006,8 +1006,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 // CTAs in turn: a prefix kernel then takes whole pairs of SMs instead of one of each, and the suffixes are left with fewer
 // of the paths to memory that pairs share (33 x 5 rows, back to back: 33 us instead of 28).
 template <int HD>
-__global__ void __launch_bounds__(128) merge_splits_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml,
-                                                           __nv_bfloat16* __restrict__ out, const int* __restrict__ q_start, int q_len,
+__global__ void __launch_bounds__(128) merge_splits_kernel(const float* part_o, const float2* part_ml,
+                                                           __nv_bfloat16* out, const int* q_start, int q_len,
                                                            int heads, int splits, long long pairs /* sequences * q_len * heads */) {
   const int lane = threadIdx.x & 31;
   const long long w = (blockIdx.x * (long long)blockDim.x + threadIdx.x) >> 5;
@@ -1028,7 +1028,7 @@ __global__ void __launch_bounds__(128) merge_splits_kernel(const float* __restri
   // lane z: part z (and z + 32: at most 64 parts)
   const float2* ml = part_ml + out_row * splits;
   const float2 none = make_float2(0.0f, 0.0f);
-  const float2 a = lane < splits ? __ldcg(ml + lane) : none, b = lane + 32 < splits ? __ldcg(ml + lane + 32) : none;
+  const float2 a = lane < splits ? ld_l2(ml + lane) : none, b = lane + 32 < splits ? ld_l2(ml + lane + 32) : none;
   float weight_a = 0.0f, weight_b = 0.0f;
   bool weighed = false;
 #pragma unroll 1
@@ -1037,8 +1037,8 @@ __global__ void __launch_bounds__(128) merge_splits_kernel(const float* __restri
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
       if (z0 + u < splits) {
-        if constexpr (kPerLane == 4) *reinterpret_cast<float4*>(v[u]) = __ldcg(reinterpret_cast<const float4*>(src + (size_t)(z0 + u) * HD));
-        else *reinterpret_cast<float2*>(v[u]) = __ldcg(reinterpret_cast<const float2*>(src + (size_t)(z0 + u) * HD));
+        if constexpr (kPerLane == 4) *reinterpret_cast<float4*>(v[u]) = ld_l2(reinterpret_cast<const float4*>(src + (size_t)(z0 + u) * HD));
+        else *reinterpret_cast<float2*>(v[u]) = ld_l2(reinterpret_cast<const float2*>(src + (size_t)(z0 + u) * HD));
       }
     }
     if (!weighed) {

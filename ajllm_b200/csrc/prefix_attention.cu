@@ -168,7 +168,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
       int token, h;
       row_place(r, token, h);
       v[u] = make_uint4(0, 0, 0, 0);
-      if (r < rows) v[u] = ld_nc_v4(reinterpret_cast<const uint4*>(p.q + (size_t)token * p.q_pitch + (size_t)(kv_head * p.group + h) * HD) + ch);
+      if (r < rows) v[u] = ld_v4(reinterpret_cast<const uint4*>(p.q + (size_t)token * p.q_pitch + (size_t)(kv_head * p.group + h) * HD) + ch);
     }
 #pragma unroll
     for (int u = 0; u < kEach; ++u) store_chunk(sQ + stream * C::kTile, (t + 256 * u) / kChunks, (t + 256 * u) % kChunks, v[u]);

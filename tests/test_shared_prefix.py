@@ -3,6 +3,7 @@
 
 import math
 import random
+from pathlib import Path
 
 import pytest
 import torch
@@ -552,3 +553,14 @@ def test_the_extension_leaves_cpu_tensors_alone():
     for wrong in (dict(prefix_len="8"), dict(q=None), dict(block_tables=3)):
         with pytest.raises((TypeError, AttributeError, ValueError)):
             serving.shared_prefix_attention(**{**call, **wrong})
+
+
+def test_launches_that_start_early_do_not_read_through_the_read_only_path():
+    """A kernel that runs before its inputs are written (up to its wait for them) must not promise the compiler and the caches
+    that they do not change."""
+    sources = Path(serving.__file__).resolve().parent.parent / "csrc"
+    early = [path for path in sources.glob("*.cu") if "griddepcontrol.wait" in path.read_text()]
+    assert {path.stem for path in early} >= {"batch_maps", "logits", "paged_attention", "prefix_attention"}
+    for path in early:
+        for promise in ("__ldg", "ld_nc", "__restrict__", "ld.global.nc"):
+            assert promise not in path.read_text(), (path.name, promise)
