@@ -1000,8 +1000,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 }
 
 // out[row, head, :] = sum_z w_z O_z / sum_z w_z l_z with w_z = 2^(m_z - max m): one warp per (row, head), HD / 32
-// neighbouring elements per lane. The parts are read at once, before their weights are known: what bounds the kernel is
-// the latency of two dependent reads, not the bytes. It is launched while the launch in front of it still runs and waits
+// neighbouring elements per lane. A part whose sum is 0 saw no key and has no row; any other counts, however small its weight
+// and also if its sum is NaN: what went wrong in front of the kernel must not come out as attention over the other parts. The
+// parts are read at once, before their weights are known: what bounds the kernel is the latency of two dependent reads, not
+// the bytes. It is launched while the launch in front of it still runs and waits
 // for it (and so for everything that one has waited for) on the device. It does not let the next launch start among its own
 // CTAs in turn: a prefix kernel then takes whole pairs of SMs instead of one of each, and the suffixes are left with fewer
 // of the paths to memory that pairs share (33 x 5 rows, back to back: 33 us instead of 28).
@@ -1029,6 +1031,7 @@ __global__ void __launch_bounds__(128) merge_splits_kernel(const float* part_o, 
   const float2* ml = part_ml + out_row * splits;
   const float2 none = make_float2(0.0f, 0.0f);
   const float2 a = lane < splits ? ld_l2(ml + lane) : none, b = lane + 32 < splits ? ld_l2(ml + lane + 32) : none;
+  const unsigned saw_a = __ballot_sync(0xffffffffu, a.y != 0.0f), saw_b = __ballot_sync(0xffffffffu, b.y != 0.0f);
   float weight_a = 0.0f, weight_b = 0.0f;
   bool weighed = false;
 #pragma unroll 1
@@ -1042,15 +1045,15 @@ __global__ void __launch_bounds__(128) merge_splits_kernel(const float* part_o, 
       }
     }
     if (!weighed) {
-      float m = fmaxf(a.y > 0.0f ? a.x : -INFINITY, b.y > 0.0f ? b.x : -INFINITY);
+      float m = fmaxf(a.y != 0.0f ? a.x : -INFINITY, b.y != 0.0f ? b.x : -INFINITY);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      weight_a = a.y > 0.0f ? exp2f(a.x - m) : 0.0f;
-      weight_b = b.y > 0.0f ? exp2f(b.x - m) : 0.0f;
+      weight_a = a.y != 0.0f ? exp2f(a.x - m) : 0.0f;
+      weight_b = b.y != 0.0f ? exp2f(b.x - m) : 0.0f;
       float l = weight_a * a.y + weight_b * b.y;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      const float inv = l != 0.0f ? 1.0f / l : 0.0f;
       weight_a *= inv;
       weight_b *= inv;
       weighed = true;
@@ -1059,8 +1062,7 @@ __global__ void __launch_bounds__(128) merge_splits_kernel(const float* part_o, 
     for (int u = 0; u < kBatch; ++u) {
       if (z0 + u < splits) {
         const float weight = __shfl_sync(0xffffffffu, z0 + u < 32 ? weight_a : weight_b, (z0 + u) & 31);
-        // a part that saw no key has a sum of 0 and leaves its row unwritten
-        if (weight != 0.0f) {
+        if (((z0 + u < 32 ? saw_a : saw_b) >> ((z0 + u) & 31)) & 1u) {
 #pragma unroll
           for (int c = 0; c < kPerLane; ++c) acc[c] += weight * v[u][c];
         }

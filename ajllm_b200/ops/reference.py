@@ -179,7 +179,7 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         scores = torch.einsum("ihd,shd->ihs", rows, keys) * scale
         last = (context - q_len + torch.arange(q_len, device=q.device)).clamp(min=shared - 1)
         scores = scores.masked_fill(torch.arange(length, device=q.device)[None, None, :] > last[:, None, None], float("-inf"))
-        probs = torch.nan_to_num(torch.softmax(scores, dim=-1)) if shared == 0 else torch.softmax(scores, dim=-1)
+        probs = torch.softmax(scores, dim=-1).masked_fill((last < 0)[:, None, None], 0.0)
         out[i * q_len:(i + 1) * q_len] = torch.einsum("ihs,shd->ihd", probs, values).to(q.dtype)
     return out
 

@@ -279,6 +279,65 @@ def test_rows_without_a_key_are_zero():
     assert torch.count_nonzero(got[1]) == 0 and torch.count_nonzero(got[0]) > 0
 
 
+@pytest.mark.parametrize("heads,kv_heads,hd,q_len,prefix,suffixes", [
+    (8, 2, 128, 1, 512, [1, 17, 130, 500]),              # the prefix in pieces of the paged launch
+    (32, 8, 64, 5, 2048, [5, 40] * 20),                  # the prefix kernel, two row tiles
+    (32, 8, 128, 1, 4096, [3, 900] * 12),                # the prefix kernel or long pieces, many parts
+    (48, 1, 128, 3, 64, [3, 20, 50]),                    # more than 32 rows per sequence
+    (4, 2, 64, 1, 0, [1, 33, 700]),                      # nothing shared
+])
+def test_what_is_not_a_number_is_not_lost_between_the_parts(heads, kv_heads, hd, q_len, prefix, suffixes):
+    """NaN in a query, in a visible key behind the prefix and in one of the prefix, and values whose weight is next to nothing:
+    the rows that the definition gives are NaN, and no others change. ``paged_attention``, in parts or whole, does the same."""
+    q, keys, values, tables, context = _batch(heads, kv_heads, hd, q_len, prefix, suffixes, poison=False)
+    lens = context.tolist()
+
+    def check():
+        want, size = _oracle(q, keys, values, tables, context, q_len)
+        for got in (serving.shared_prefix_attention(q, keys, values, tables, context, prefix, q_len=q_len),
+                    *([serving.paged_attention(q, keys, values, tables, None, None, [q_len] * len(lens), lens)] if heads // kv_heads * q_len <= 64 else [])):
+            assert torch.equal(got.isnan(), want.isnan())
+            real = ~want.isnan()
+            bound = HALF_BF16 * (size + want.abs()) + 1e-4 * size + 1e-30
+            assert bool(((got.double() - want).abs() <= bound)[real].all())
+        return want.isnan()
+
+    assert not check().any()
+    whole = q.clone()
+    q[0, heads - 1, 3] = math.nan
+    assert int(check().any(-1).sum()) == 1
+    q.copy_(whole)
+    last = lens[1] - q_len                              # position of the first new token of sequence 1
+    block, offset = int(tables[1, last // 16]), last % 16
+    kept = keys[block, offset, 0].clone()
+    keys[block, offset, 0] = math.nan
+    assert int(check().any(-1).sum()) == q_len * heads // kv_heads
+    keys[block, offset, 0] = kept
+    if prefix:
+        block, kept = int(tables[0, prefix // 32]), keys[int(tables[0, prefix // 32]), 7, kv_heads - 1].clone()
+        keys[block, 7, kv_heads - 1] = math.inf         # scores of both signs, or a NaN where a query's elements cancel
+        q[:, -1] = q[:, -1].abs()                       # (the last head: all positive, a score of infinity)
+        assert check()[:, -1].all()
+        keys[block, 7, kv_heads - 1] = kept
+        q.copy_(whole)
+    assert native.lib().ajb_check_status() == 0
+
+
+@pytest.mark.parametrize("q_len", [1, 20])
+def test_values_of_visible_keys_count_whatever_their_weight(q_len):
+    """A NaN value behind a prefix whose scores are 300 larger: its weight is 0 in fp32, 0 times NaN is NaN."""
+    q, keys, values, tables, context = _batch(8, 2, 128, q_len, 512, [q_len, q_len + 30], poison=False)
+    q[..., 0], keys[..., 0] = 200.0, 0.0
+    shared = tables[0, :32].long()
+    keys[shared, :, :, 0] = 20.0                        # 200 * 20 / sqrt(128) = 354 more for every key of the prefix
+    last = int(context[1]) - q_len
+    values[int(tables[1, last // 16]), last % 16, 1, 5] = math.nan
+    got = serving.shared_prefix_attention(q, keys, values, tables, context, 512, q_len=q_len)
+    want = torch.zeros_like(got, dtype=torch.bool)
+    want[q_len:, 4:, 5] = True
+    assert torch.equal(got.isnan(), want)
+
+
 def test_queries_read_in_place_from_packed_rows_and_results_into_a_given_tensor():
     q, keys, values, tables, context = _batch(8, 2, 128, 2, 200, [2, 50, 3])
     packed = torch.full((6, 12 * 128), math.nan, dtype=torch.bfloat16, device=_dev())

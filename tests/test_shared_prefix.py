@@ -122,6 +122,21 @@ def test_shared_prefix_attention_against_64_bits(contexts, shared, q_len):
             assert float((got[i * q_len + j].double() - want).abs().max()) < 50 * 2 ** -24 * float(values.abs().max())
 
 
+def test_only_rows_without_a_key_are_zero():
+    """A row that sees nothing is zeros; one whose query or visible key holds a NaN is not, with and without a prefix."""
+    for contexts, shared in (([6, 0, 9], 0), ([9, 12, 10], 8)):
+        cache, tables = _paged([max(1, c) for c in contexts], shared)
+        q = torch.randn(3, 4, 8, generator=torch.Generator().manual_seed(2))
+        q[0, 1, 0] = math.nan
+        got = serving.shared_prefix_attention(q, cache.keys[0], cache.values[0], tables, _i32(contexts), shared)
+        rows = got.isnan().all(-1)
+        assert rows[0].tolist() == [False, True, False, False] and int(got.isnan().any(-1).sum()) == 1
+        assert (torch.count_nonzero(got[1]) == 0) == (contexts[1] == 0)
+        cache.keys[0][tables[2, 0], 1, 0, 3] = math.nan                 # KV head 0: query heads 0 and 1
+        got = serving.shared_prefix_attention(q, cache.keys[0], cache.values[0], tables, _i32(contexts), shared)
+        assert got.isnan().all(-1)[2].tolist() == [True, True, False, False]
+
+
 def _attention_call():
     cache, tables = _paged([9, 12], 8)
     return dict(q=torch.zeros(2, 4, 8), key_cache=cache.keys[0], value_cache=cache.values[0], block_tables=tables,
