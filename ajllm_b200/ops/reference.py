@@ -162,7 +162,7 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     """Decode / verify attention of sequences that share their first ``prefix_len`` tokens (whole blocks of them are
     looked up in the first row of ``block_tables``). ``q`` is ``[num_seqs * q_len, Hq, hd]``; query row ``j`` of a
     sequence sees the shared blocks and its own tokens up to position ``context_len - q_len + j``; a row that sees
-    nothing comes out as zeros."""
+    nothing, or only scores of minus infinity, comes out as zeros."""
     block, kv_heads, hd = k_cache.shape[1:]
     heads = q.shape[1]
     scale = scale if scale is not None else 1.0 / math.sqrt(hd)
@@ -179,7 +179,7 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         scores = torch.einsum("ihd,shd->ihs", rows, keys) * scale
         last = (context - q_len + torch.arange(q_len, device=q.device)).clamp(min=shared - 1)
         scores = scores.masked_fill(torch.arange(length, device=q.device)[None, None, :] > last[:, None, None], float("-inf"))
-        probs = torch.softmax(scores, dim=-1).masked_fill((last < 0)[:, None, None], 0.0)
+        probs = torch.softmax(scores, dim=-1).masked_fill((scores == float("-inf")).all(-1, keepdim=True), 0.0)
         out[i * q_len:(i + 1) * q_len] = torch.einsum("ihs,shd->ihd", probs, values).to(q.dtype)
     return out
 

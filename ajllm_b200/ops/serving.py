@@ -379,7 +379,9 @@ def shared_prefix_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cach
 
     ``max_context``: a host-side bound on the context lengths from which the number of parts per sequence is chosen (without
     one: what the tables can hold, or 512 tokens behind the prefix if that is more than 1024). It bounds nothing that is
-    read. A row whose sequence has no token at all comes out as zeros. ``scale`` defaults to ``1 / sqrt(hd)``; ``out``
+    read. A row whose sequence has no token at all, or whose visible scores are all minus infinity, comes out as zeros; NaN in a
+    query or a visible key makes the row NaN, and what is not finite among the values of a sequence's tokens may reach all of its
+    rows. ``scale`` defaults to ``1 / sqrt(hd)``; ``out``
     (contiguous, shaped like ``q``, 16-byte aligned, apart from the inputs) receives the result.
     """
     if out is None and native.fast is not None:

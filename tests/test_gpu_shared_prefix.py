@@ -338,6 +338,18 @@ def test_values_of_visible_keys_count_whatever_their_weight(q_len):
     assert torch.equal(got.isnan(), want)
 
 
+@pytest.mark.parametrize("q_len,prefix,suffixes", [(1, 512, [1, 17, 130]), (20, 512, [20, 33, 150]), (1, 0, [1, 33, 700]), (1, 2048, [9] * 90)])
+def test_rows_of_scores_that_are_all_minus_infinity_are_zero(q_len, prefix, suffixes):
+    """As in the CPU form."""
+    q, keys, values, tables, context = _batch(8, 2, 128, q_len, prefix, suffixes, poison=False)
+    keys.abs_().clamp_(min=2.0 ** -10)
+    q[q_len, 2] = -math.inf
+    got = serving.shared_prefix_attention(q, keys, values, tables, context, prefix, q_len=q_len)
+    plain = serving.shared_prefix_attention(*(t.float().cpu() for t in (q, keys, values)), tables.cpu(), context.cpu(), prefix, q_len=q_len)
+    assert torch.count_nonzero(got[q_len, 2]) == 0 and torch.count_nonzero(plain[q_len, 2]) == 0
+    assert torch.isfinite(got).all() and torch.isfinite(plain).all()
+
+
 def test_queries_read_in_place_from_packed_rows_and_results_into_a_given_tensor():
     q, keys, values, tables, context = _batch(8, 2, 128, 2, 200, [2, 50, 3])
     packed = torch.full((6, 12 * 128), math.nan, dtype=torch.bfloat16, device=_dev())

@@ -137,6 +137,16 @@ def test_only_rows_without_a_key_are_zero():
         assert got.isnan().all(-1)[2].tolist() == [True, True, False, False]
 
 
+@pytest.mark.parametrize("contexts,shared", [([6, 4, 9], 0), ([9, 12, 10], 8)])
+def test_rows_of_scores_that_are_all_minus_infinity_are_zero(contexts, shared):
+    cache, tables = _paged(contexts, shared)
+    q = torch.randn(3, 4, 8, generator=torch.Generator().manual_seed(2))
+    cache.keys[0].abs_()
+    q[1, 2], q[2, 3] = -math.inf, -1e30
+    got = serving.shared_prefix_attention(q, cache.keys[0], cache.values[0], tables, _i32(contexts), shared)
+    assert torch.count_nonzero(got[1, 2]) == 0 and torch.isfinite(got).all() and torch.count_nonzero(got) == 11 * 8
+
+
 def _attention_call():
     cache, tables = _paged([9, 12], 8)
     return dict(q=torch.zeros(2, 4, 8), key_cache=cache.keys[0], value_cache=cache.values[0], block_tables=tables,
