@@ -2,7 +2,7 @@
 
 One ``nvcc -gencode arch=compute_100a,code=sm_100a`` invocation per ``.cu`` file (in parallel), then a
 shared-library link into ``ajllm_b200/_native/libajllm_b200.so``. Objects are rebuilt only when their
-source or a header is newer. ``-Xptxas -v`` output is kept next to the objects (``*.ptxas.txt``) so
+source, a header or this file is newer. ``-Xptxas -v`` output is kept next to the objects (``*.ptxas.txt``) so
 register and shared-memory use can be read without a GPU. ``csrc/fast_calls.cpp`` becomes a Python extension of its
 own (``_native/fast_calls.so``), which knows torch's tensors and calls into the library.
 """
@@ -24,9 +24,10 @@ LIB = OUT / "libajllm_b200.so"
 FAST_CALLS = OUT / "fast_calls.so"
 
 NVCC_FLAGS = [
-    "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo", "--use_fast_math",
+    "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo",
     "-Xcompiler", "-fPIC", "-Xptxas", "-v", "--expt-relaxed-constexpr",
 ]
+EXACT = {"logits"}          # compiled without fast math, which takes subnormal numbers for zero: their results are exact fp32 steps
 
 
 def find_nvcc() -> str:
@@ -44,7 +45,7 @@ def _needs_build(source: Path, obj: Path, headers: list[Path]) -> bool:
 
 
 def _compile(nvcc: str, source: Path, obj: Path) -> tuple[Path, str]:
-    cmd = [nvcc, *NVCC_FLAGS, "-I", str(CSRC), "-c", str(source), "-o", str(obj)]
+    cmd = [nvcc, *NVCC_FLAGS, *([] if source.stem in EXACT else ["--use_fast_math"]), "-I", str(CSRC), "-c", str(source), "-o", str(obj)]
     done = subprocess.run(cmd, capture_output=True, text=True)
     log = done.stdout + done.stderr
     obj.with_suffix(".ptxas.txt").write_text(log)
@@ -70,7 +71,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     nvcc = find_nvcc()
     OUT.mkdir(parents=True, exist_ok=True)
     sources = sorted(CSRC.glob("*.cu"))
-    headers = sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h"))
+    headers = sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [Path(__file__).resolve()]          # (the flags are in here)
     jobs = []
     binding = force or _needs_build(CSRC / "fast_calls.cpp", FAST_CALLS, [CSRC / "serving_args.h"])
     for source in sources:

@@ -4,7 +4,8 @@
 // For token v of a row, c(v) = how often it was generated, seen(v) = whether it is anywhere in the history (prompt and
 // generated tokens), r / p / f = the row's repetition, presence and frequency penalty:
 //   x = logit;  x = seen ? (x > 0 ? x / r : x * r) : x;  x = x - f * c - p * (c > 0);  x = x + bias;  x = masked ? -inf : x
-// Every step rounds to fp32 once and nothing is contracted, so the result equals elementary fp32 operations bit for bit.
+// Every step rounds to fp32 once and nothing is contracted (and this file is compiled without fast math, so that subnormal
+// numbers stay what they are): the result equals elementary fp32 operations bit for bit.
 //
 // Bound by memory: 6 bytes per bf16 logit (read, write) and a bit of the mask; where a mask shuts four neighbouring
 // tokens their logits are not read. Only the few tokens of the history and of the bias list need arithmetic, so the rows

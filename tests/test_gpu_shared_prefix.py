@@ -476,6 +476,27 @@ def test_process_logits_of_strided_and_misaligned_rows(dtype, offset):
     assert torch.equal(got, serving.process_logits(transposed, **kw))
 
 
+@pytest.mark.parametrize("rows", [3, 300])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_subnormal_logits_penalties_and_biases_are_not_taken_for_zero(rows, dtype):
+    """One launch and two; every kind of step with operands or results below the smallest normal number."""
+    vocab = 32_000
+    small = torch.tensor([1e-40, -1e-40, 1e-44, -1e-44, 1.3e-38, -1.3e-38, 0.0, -0.0, 1e-3, -2.0])
+    logits = small.repeat(vocab // 10).expand(rows, -1).to(dtype).contiguous()
+    history = torch.arange(200, dtype=torch.int32).repeat(rows, 1)
+    lens = torch.full((rows,), 200, dtype=torch.int32)
+    row = torch.arange(rows)
+    kw = dict(history=history, prompt_lens=lens // 2, history_lens=lens, repetition=torch.tensor([1.7, 0.6, 1e-3])[row % 3],
+              presence=torch.tensor([0.0, 3e-41, -2e-38])[row % 3], frequency=torch.tensor([1e-41, 0.0, 1.2e-38])[row % 3],
+              bias_ids=torch.arange(150, 250, dtype=torch.int32).repeat(rows, 1), bias_values=torch.tensor([5e-41, -1e-38]).repeat(50).repeat(rows, 1))
+    assert (rows * vocab >= 1 << 23) == (rows == 300)
+    got = serving.process_logits(logits.cuda(), **{name: t.cuda() for name, t in kw.items()}).cpu()
+    want = serving.process_logits(logits, **kw)
+    assert torch.equal(got.view(torch.int32), want.view(torch.int32))
+    # subnormal are 1e-40 and, in fp32, 1e-44 (bf16 ends at 9e-41), with both signs: at least 2 in 10, but for the 250 mended tokens
+    assert int(((want != 0) & (want.abs() < 2.0 ** -126)).sum()) >= rows * (vocab - 250) // 10 * 2
+
+
 def test_masked_places_hide_whatever_is_in_them_and_open_ones_keep_it():
     values = torch.tensor([math.nan, math.inf, -math.inf, torch.finfo(torch.float32).min, 1.0, 0.0, -0.0, 2.0])
     logits = values.repeat(3, 8)
