@@ -2,9 +2,11 @@
 
 One ``nvcc -gencode arch=compute_100a,code=sm_100a`` invocation per ``.cu`` file (in parallel), then a
 shared-library link into ``ajllm_b200/_native/libajllm_b200.so``. Objects are rebuilt only when their
-source, a header or this file is newer. ``-Xptxas -v`` output is kept next to the objects (``*.ptxas.txt``) so
-register and shared-memory use can be read without a GPU. ``csrc/fast_calls.cpp`` becomes a Python extension of its
-own (``_native/fast_calls.so``), which knows torch's tensors and calls into the library.
+source, a header or this file is newer, and the library is linked whenever an object is newer than it. ``-Xptxas -v``
+output is kept next to the objects (``*.ptxas.txt``) so register and shared-memory use can be read without a GPU.
+``csrc/fast_calls.cpp`` becomes a Python extension of its own, which knows torch's tensors and calls into the library. It
+reads their C++ layout, so its file is named after the Python and torch it was built for and no other is loaded; the
+framework works without it, and so a machine that cannot build it gets a warning.
 """
 
 from __future__ import annotations
@@ -14,6 +16,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -21,7 +24,6 @@ PACKAGE = Path(__file__).resolve().parent
 CSRC = PACKAGE / "csrc"
 OUT = PACKAGE / "_native"
 LIB = OUT / "libajllm_b200.so"
-FAST_CALLS = OUT / "fast_calls.so"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo",
@@ -35,6 +37,12 @@ def find_nvcc() -> str:
     if not Path(found).exists():
         raise RuntimeError("nvcc not found; the CUDA kernels cannot be built")
     return found
+
+
+def fast_calls_path() -> Path:
+    """Where the extension for this Python and this torch is."""
+    import torch
+    return OUT / f"fast_calls.{sys.implementation.cache_tag}.torch-{torch.__version__}.so"
 
 
 def _needs_build(source: Path, obj: Path, headers: list[Path]) -> bool:
@@ -54,17 +62,35 @@ def _compile(nvcc: str, source: Path, obj: Path) -> tuple[Path, str]:
     return obj, log
 
 
+def _into_place(command: list[str], target: Path) -> str | None:
+    """Runs a compiler or linker whose output goes to ``target`` only if it succeeds; otherwise returns what it printed."""
+    fresh = target.with_name(target.name + ".new")
+    try:
+        done = subprocess.run([*command, "-o", str(fresh)], capture_output=True, text=True)
+    except OSError as error:
+        return str(error)
+    if done.returncode != 0:
+        fresh.unlink(missing_ok=True)
+        return (done.stdout + done.stderr)[-6000:]
+    os.replace(fresh, target)
+    return None
+
+
 def _build_fast_calls() -> None:
     import torch
     root = Path(torch.__file__).resolve().parent
     cuda = Path(find_nvcc()).resolve().parent.parent
-    done = subprocess.run(
+    failure = _into_place(
         ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
          "-I", sysconfig.get_paths()["include"], "-I", str(root / "include"), "-I", str(root / "include/torch/csrc/api/include"),
-         "-I", str(cuda / "include"), "-I", str(CSRC), str(CSRC / "fast_calls.cpp"), "-o", str(FAST_CALLS),
-         "-L", str(root / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"], capture_output=True, text=True)
-    if done.returncode != 0:
-        raise RuntimeError(f"g++ failed for fast_calls.cpp:\n{(done.stdout + done.stderr)[-6000:]}")
+         "-I", str(cuda / "include"), "-I", str(CSRC), str(CSRC / "fast_calls.cpp"),
+         "-L", str(root / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"], fast_calls_path())
+    # one that is there was built from other sources, or for another Python or torch
+    for old in OUT.glob("fast_calls*.so"):
+        if failure is not None or old != fast_calls_path():
+            old.unlink()
+    if failure is not None:
+        warnings.warn(f"g++ failed for fast_calls.cpp (small serving calls take longer without it):\n{failure}")
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
@@ -73,7 +99,6 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     sources = sorted(CSRC.glob("*.cu"))
     headers = sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [Path(__file__).resolve()]          # (the flags are in here)
     jobs = []
-    binding = force or _needs_build(CSRC / "fast_calls.cpp", FAST_CALLS, [CSRC / "serving_args.h"])
     for source in sources:
         obj = OUT / (source.stem + ".o")
         if force or _needs_build(source, obj, headers):
@@ -84,15 +109,14 @@ def build(force: bool = False, verbose: bool = False) -> Path:
             for obj, log in pool.map(lambda job: _compile(nvcc, *job), jobs):
                 if verbose:
                     print(f"[build] {obj.name}\n{log}")
-    if binding:
-        _build_fast_calls()
     objects = [OUT / (source.stem + ".o") for source in sources]
-    if jobs or not LIB.exists():
-        link = [nvcc, "-shared", "-o", str(LIB), *map(str, objects), "-gencode", "arch=compute_100a,code=sm_100a",
+    if jobs or not LIB.exists() or LIB.stat().st_mtime < max(obj.stat().st_mtime for obj in objects):
+        link = [nvcc, "-shared", *map(str, objects), "-gencode", "arch=compute_100a,code=sm_100a",
                 "-lcudart_static", "-lpthread", "-ldl", "-lrt"]
-        done = subprocess.run(link, capture_output=True, text=True)
-        if done.returncode != 0:
-            raise RuntimeError(f"link failed:\n{done.stdout}{done.stderr}")
+        if (failure := _into_place(link, LIB)) is not None:
+            raise RuntimeError(f"link failed:\n{failure}")
+    if force or _needs_build(CSRC / "fast_calls.cpp", fast_calls_path(), [CSRC / "serving_args.h", Path(__file__).resolve()]):
+        _build_fast_calls()
     return LIB
 
 

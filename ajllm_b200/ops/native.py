@@ -19,6 +19,8 @@ from pathlib import Path
 
 import torch
 
+from ajllm_b200.build import fast_calls_path
+
 _LIB_DIR = Path(__file__).resolve().parent.parent / "_native"
 _LIB_NAME = "libajllm_b200.so"
 _lib: ctypes.CDLL | None = None
@@ -125,8 +127,9 @@ def _try_load() -> None:
 
 
 def _load_fast_calls(lib: ctypes.CDLL):
-    """The binding that checks, allocates and calls without going through ctypes. Every call works without it."""
-    path = _LIB_DIR / "fast_calls.so"
+    """The binding that checks, allocates and calls without going through ctypes, if there is one for this Python and this
+    torch. Every call works without it."""
+    path = _LIB_DIR / fast_calls_path().name
     try:
         loader = importlib.machinery.ExtensionFileLoader("fast_calls", str(path))
         module = importlib.util.module_from_spec(importlib.util.spec_from_loader("fast_calls", loader))
