@@ -140,7 +140,7 @@ PyObject* fast_shared_prefix_attention(PyObject*, PyObject* const* a, Py_ssize_t
   if (a[7] != Py_None) {
     if (!PyFloat_CheckExact(a[7])) Py_RETURN_NONE;
     scale = PyFloat_AS_DOUBLE(a[7]);
-    if (!(scale > 0.0 && std::isfinite(scale))) Py_RETURN_NONE;
+    if (!(scale >= 1e-30 && scale <= 1e3)) Py_RETURN_NONE;
   }
   const long long shared = prefix / block * block, room = max_blocks * block;
   long long behind = room - shared;

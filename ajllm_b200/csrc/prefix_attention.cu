@@ -497,6 +497,7 @@ extern "C" int ajb_shared_prefix_attention(const void* arguments) {
   const int prefix_parts = !few && rows <= prefix::ROWS && prefix_splits < tiles ? 2 * prefix_splits : prefix_splits;
   AJB_REQUIRE(parts == prefix_parts + suffix_splits && parts <= 64, "shared prefix attention: %d parts per row, not %d", parts,
               prefix_parts + suffix_splits);
+  AJB_REQUIRE(scale >= 0.99e-30f && scale <= 1000.0f, "shared prefix attention: scale %g is not between 1e-30 and 1e3", (double)scale);
   AJB_REQUIRE(q_pitch % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0, "shared prefix attention: query rows must be 16-byte aligned");
   AJB_REQUIRE((reinterpret_cast<uintptr_t>(out) & 15) == 0, "shared prefix attention: out must be 16-byte aligned");
   if (num_seqs <= 0) return 0;

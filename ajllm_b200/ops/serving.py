@@ -381,7 +381,7 @@ def shared_prefix_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cach
     one: what the tables can hold, or 512 tokens behind the prefix if that is more than 1024). It bounds nothing that is
     read. A row whose sequence has no token at all, or whose visible scores are all minus infinity, comes out as zeros; NaN in a
     query or a visible key makes the row NaN, and what is not finite among the values of a sequence's tokens may reach all of its
-    rows. ``scale`` defaults to ``1 / sqrt(hd)``; ``out``
+    rows. ``scale`` (1e-30 to 1e3) defaults to ``1 / sqrt(hd)``; ``out``
     (contiguous, shaped like ``q``, 16-byte aligned, apart from the inputs) receives the result.
     """
     if out is None and native.fast is not None:
@@ -416,8 +416,10 @@ def shared_prefix_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cach
             raise ValueError("shared_prefix_attention: out must not overlap the inputs")
     if scale is None:
         scale = 1.0 / math.sqrt(head_dim)
-    elif not 0.0 < scale < math.inf:          # the reference maximum of a row is that of its unscaled scores
-        raise ValueError(f"shared_prefix_attention: scale must be positive (got {scale})")
+    elif not 1e-30 <= scale <= 1e3:
+        # positive, as the reference maximum of a row is that of its unscaled scores, not zero in fp32, and not so large that the
+        # rounding of scale * maximum (its 2^-24th) is an exponent of its own
+        raise ValueError(f"shared_prefix_attention: scale must be positive, between 1e-30 and 1e3 (got {scale})")
     if index < 0:
         found = reference.shared_prefix_attention(q, key_cache, value_cache, block_tables, context_lens, prefix_len, q_len, scale)
         return found if out is None else out.copy_(found)

@@ -263,6 +263,24 @@ def test_shared_prefix_attention_with_large_scores_and_a_given_scale():
     assert native.lib().ajb_check_status() == 0
 
 
+def test_scales_at_the_ends_of_their_range(monkeypatch):
+    """With the smallest every visible key counts alike, with the largest only the best one does; beyond them calls are refused."""
+    for batch, prefix in ((_batch(8, 2, 128, 1, 640, [40, 300, 9]), 640), (_batch(8, 2, 64, 1, 2048, [33] * 70), 2048)):
+        q, keys, values, tables, context = batch
+        want, size = _oracle(*batch, 1, scale=1e-30)
+        _check_attention(serving.shared_prefix_attention(*batch, prefix, scale=1e-30), want, size)
+        # scores are elements of the keys, exactly: those of up to 5 make exponents of 7000, off by 7000 * 2^-24 = 4e-4, the same for
+        # every key that has the largest score (others have no weight: two bf16 numbers near 4 are 22 exponents apart)
+        q.copy_(torch.eye(8, q.shape[2], device=_dev())[None].expand_as(q))
+        want, size = _oracle(*batch, 1, scale=1e3)
+        _check_attention(serving.shared_prefix_attention(*batch, prefix, scale=1e3), want, size)
+    for fast in (native.fast, None):
+        monkeypatch.setattr(native, "fast", fast)
+        for scale in (1e-46, 1e-40, 1e39):
+            with pytest.raises(ValueError, match="between"):
+                serving.shared_prefix_attention(*batch, prefix, scale=scale)
+
+
 def test_shared_prefix_attention_equals_paged_attention_closely():
     q, keys, values, tables, context = _batch(32, 8, 128, 1, 1024, [7, 260, 31], poison=False)
     a = serving.shared_prefix_attention(q, keys, values, tables, context, 1024)

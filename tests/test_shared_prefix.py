@@ -167,6 +167,15 @@ def test_shared_prefix_attention_refuses(change):
         serving.shared_prefix_attention(**{**call, **change})
 
 
+@pytest.mark.parametrize("scale", [1e-46, 1e-40, 9e-31, 1.1e3, 1e39, 1e300])
+def test_shared_prefix_attention_refuses_a_scale_that_fp32_arithmetic_loses(scale):
+    call = _attention_call()
+    with pytest.raises(ValueError, match="between"):
+        serving.shared_prefix_attention(**call, scale=scale)
+    for kept in (1e-30, 1e3, 1):
+        assert torch.isfinite(serving.shared_prefix_attention(**call, scale=kept)).all()
+
+
 def test_shared_prefix_attention_refuses_its_query_as_output():
     call = _attention_call()
     with pytest.raises(ValueError, match="overlap"):
