@@ -147,7 +147,8 @@ PyObject* fast_shared_prefix_attention(PyObject*, PyObject* const* a, Py_ssize_t
   if (a[8] != Py_None) {
     long long bound;
     if (!whole(a[8], LLONG_MIN, LLONG_MAX, bound)) Py_RETURN_NONE;
-    behind = std::max(0ll, std::min(bound, room) - shared);
+    // in whole tiles of 128 keys, like ops/serving.py: contexts that grow by a token per step keep their plan for 128 steps
+    behind = (std::max(0ll, std::min(bound, room) - shared) + 127) / 128 * 128;
   }
   PyObject* plan = PyObject_CallFunction(a[9], "LLLLLLLL", (long long)n, q_len, (long long)(heads / kv_heads), (long long)kv_heads,
                                          (long long)hd, shared, behind, (long long)(a[8] != Py_None));

@@ -445,7 +445,9 @@ def shared_prefix_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cach
     shared = prefix_len // block_size * block_size
     group = heads // kv_heads
     room = max_blocks * block_size
-    behind = max(0, (room if max_context is None else min(max_context, room)) - shared)
+    behind = room - shared
+    if max_context is not None:          # in whole tiles: contexts that grow by a token per step keep their plan for 128 steps
+        behind = -(-max(0, min(max_context, room) - shared) // _PREFIX_TILE) * _PREFIX_TILE
     prefix_tokens, prefix_splits, splits, parts = prefix_plan(n, q_len, group, kv_heads, head_dim, shared, behind, int(max_context is not None))
     # fp32 parts of every (row, head): un-normalised outputs, then (reference maximum, sum) pairs
     count = total * heads * parts

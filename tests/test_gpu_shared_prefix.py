@@ -901,6 +901,16 @@ def test_ordinary_calls_go_through_the_extension(monkeypatch):
     assert isinstance(again, serving.BatchMaps) and again.tables is out.tables and out.tables.tolist() == [[4]]
 
 
+def test_contexts_that_grow_by_a_token_per_step_keep_their_plan(monkeypatch):
+    q, keys, values, tables, context = _batch(8, 2, 128, 1, 512, [200, 300, 600], poison=False)
+    for fast in (native.fast, None):
+        monkeypatch.setattr(native, "fast", fast)
+        serving.prefix_plan.cache_clear()
+        for most in range(700, 956):                    # 2 tiles of 128 keys
+            serving.shared_prefix_attention(q, keys, values, tables, context, 512, max_context=most)
+        assert serving.prefix_plan.cache_info().misses <= 3
+
+
 def test_calls_that_the_extension_leaves_alone():
     logits, kw = _logits_inputs(3, 300, torch.bfloat16, 7, 4, True)
     logits, kw = logits.cuda(), {name: t.cuda() for name, t in kw.items()}
