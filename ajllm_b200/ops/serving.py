@@ -66,7 +66,7 @@ def paged_attention_planned(q: torch.Tensor, key_cache: torch.Tensor, value_cach
         # two CTAs per SM (what the kernel's shared memory admits) and never more parts than the longest context has
         # 64-key tiles
         max_context = getattr(plan, "max_context", None) or tables.shape[1] * block_size
-        splits = paged_splits(count * kv_heads, max_context)
+        splits = paged_splits(count * kv_heads, max_context, heads // kv_heads * q_len, head_dim)
         part_o = part_ml = None
         if splits > 1:
             part_o = torch.empty(total, heads, splits, head_dim, dtype=torch.float32, device=q.device)
@@ -81,11 +81,15 @@ def paged_attention_planned(q: torch.Tensor, key_cache: torch.Tensor, value_cach
 _SM_COUNT: list[int] = []
 
 
-def paged_splits(ctas: int, max_context: int) -> int:
-    """Parts per sequence for the paged-attention kernel given the (sequence, KV head) pairs of a launch."""
+def paged_splits(ctas: int, max_context: int, rows: int = 1, head_dim: int = 128) -> int:
+    """Parts per sequence for the paged-attention kernels given the (sequence, KV head) pairs of a launch, the query rows of a
+    pair and the width of its heads."""
     if not _SM_COUNT:
         _SM_COUNT.append(int(native.lib().ajb_sm_count()))
-    if 5 * ctas >= 4 * _SM_COUNT[0]:       # one each for nearly all SMs: 128 pairs x 4096 keys take 48.5 us whole, 50.5 us in two parts
+    # One each for nearly all SMs. Up to 32 rows of 128-wide heads, whose CTAs fill an SM's memory path, that is best: 128 pairs
+    # x 4096 keys, 4 rows: 63.5 us whole and in two parts, 32 rows: 63.5 us whole, 67.6 us in two parts. Other CTAs want a second
+    # one beside them: 64-wide heads, 8 rows: 45.1 and 38.9 us (16384 keys: 154 and 107 us), 40 rows of 128: 82.1 and 67.6 us.
+    if 5 * ctas >= 4 * _SM_COUNT[0] and rows <= 32 and head_dim == 128:
         return 1
     want = (2 * _SM_COUNT[0]) // max(1, ctas)
     tiles = max(1, (max_context + 63) // 64)
@@ -282,10 +286,11 @@ def prefix_plan(n: int, q_len: int, group: int, kv_heads: int, head_dim: int, sh
     sms = _SM_COUNT[0]
     chunk = q_len if group * q_len <= 32 else max(1, min(q_len, _PREFIX_TILE // group))
     pieces = n * kv_heads * -(-q_len // chunk)
+    if not shared:
+        alone = paged_splits(pieces, behind, group * chunk, head_dim)
+        return 0, 0, alone, alone
     # where the suffixes are not known to be long, they are divided as if alone, which costs little if they are short
     bound_splits = paged_splits(pieces, behind)
-    if not shared:
-        return 0, 0, bound_splits, bound_splits
     tiles, most = -(-shared // _PREFIX_TILE), -(-behind // _PREFIX_TILE)
     divisions = tuple(range(1, min(16, max(1, most)) + 1)) if known or behind <= 1024 else (min(8, bound_splits),)
     rows = n * q_len * group

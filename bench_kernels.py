@@ -151,7 +151,7 @@ def run_paged(dev, small: bool) -> None:
         for label, forced in (("one CTA per (seq, kv head)", 1), ("split", None)):
             original = serving.paged_splits
             if forced is not None:
-                serving.paged_splits = lambda ctas, max_context: 1
+                serving.paged_splits = lambda *_: 1
             try:
                 t = timeit(lambda: serving.paged_attention_planned(q, cache.keys[0], cache.values[0], plan), iters=20)
                 parts = serving.paged_splits(seqs * kv_heads, ctx)

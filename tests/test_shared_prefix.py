@@ -201,6 +201,16 @@ def test_division_of_shared_prefix_attention_is_one_that_the_kernels_take(monkey
         assert parts == splits + (2 * ours if twice else ours)
 
 
+def test_parts_of_paged_attention_where_pairs_nearly_fill_the_device(monkeypatch):
+    """Long contexts are left whole only where that is the faster form: up to 32 rows of 128-wide heads."""
+    monkeypatch.setattr(serving, "_SM_COUNT", [148])
+    for pairs in (120, 128, 148):
+        assert serving.paged_splits(pairs, 4096) == serving.paged_splits(pairs, 4096, 32, 128) == 1
+        for rows, hd in ((33, 128), (64, 128), (40, 64), (8, 64)):
+            assert serving.paged_splits(pairs, 4096, rows, hd) == 2 and serving.paged_splits(pairs, 1000, rows, hd) == 1
+    assert serving.paged_splits(149, 1 << 17, 40, 64) == serving.paged_splits(149, 1 << 17) == 1
+
+
 def _formula(x, history, prompt, total, repetition, presence, frequency, biases, allowed):
     """One row of processed logits, token by token, in 64 bits."""
     out = []
