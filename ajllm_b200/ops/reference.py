@@ -187,13 +187,15 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
 def batch_maps(block_ids: torch.Tensor, block_counts: torch.Tensor, cached_lens: torch.Tensor, q_lens: torch.Tensor,
                total_tokens: int, max_blocks: int, block_size: int, pad_block: int) -> tuple[torch.Tensor, ...]:
     """Block tables ``[n, max_blocks]``, positions and cache slots ``[total_tokens]``, row offsets ``[n + 1]`` and
-    context lengths ``[n]`` of a ragged batch; what no sequence owns is filled from ``pad_block``."""
+    context lengths ``[n]`` of a ragged batch; what no sequence owns is filled from ``pad_block``. Positions and
+    context lengths stop at the largest int32."""
     n = block_counts.shape[0]
     int32 = dict(dtype=torch.int32, device=block_ids.device)
     tables = torch.full((n, max_blocks), pad_block, **int32)
     positions = torch.zeros(total_tokens, **int32)
     slots = torch.full((total_tokens,), pad_block * block_size, dtype=torch.int64, device=block_ids.device)
     starts, contexts = [0], []
+    largest = 2 ** 31 - 1
     ids = block_ids.tolist()
     first = 0
     for i, (count, cached, new) in enumerate(zip(block_counts.tolist(), cached_lens.tolist(), q_lens.tolist())):
@@ -204,11 +206,11 @@ def batch_maps(block_ids: torch.Tensor, block_counts: torch.Tensor, cached_lens:
         lo, hi = starts[-1], min(starts[-1] + new, total_tokens)
         for t in range(lo, hi):
             at = cached + t - lo
-            positions[t] = at
+            positions[t] = min(at, largest)
             block = own[at // block_size] if at // block_size < len(own) else pad_block
             slots[t] = block * block_size + at % block_size
         starts.append(hi)
-        contexts.append(cached + new)
+        contexts.append(min(cached + new, largest))
     return tables, positions, slots, torch.tensor(starts, **int32), torch.tensor(contexts, **int32)
 
 

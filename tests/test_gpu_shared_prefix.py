@@ -90,6 +90,14 @@ def test_batch_maps_survives_absurd_lengths_and_keeps_to_its_buffers():
         assert torch.all(flat[:guard] == -5) and torch.all(flat[guard + view.numel():] == -5)
 
 
+def test_batch_maps_of_lengths_past_32_bits():
+    big = 2**31 - 1
+    args = ([5, 6], [1, 1], [big - 1, big], [3, big])
+    got = serving.batch_maps(*map(_i32, args), 5, 1, pad_block=9)
+    want = serving.batch_maps(*(_i32(a, "cpu") for a in args), 5, 1, pad_block=9)
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want))
+
+
 def test_batch_maps_replayed_from_a_graph():
     ids, counts, cached, new = _i32(list(range(40))), _i32([10, 10, 10, 10]), _i32([3, 16, 31, 100]), _i32([5, 1, 2, 8])
     out = serving.batch_maps(ids, counts, cached, new, 16, 12, pad_block=99)

@@ -61,6 +61,14 @@ def test_batch_maps_without_sequences_and_with_missing_blocks():
     assert got.positions.tolist() == [15, 16] and got.slots.tolist() == [4 * 16 + 15, 9 * 16]
 
 
+def test_batch_maps_of_lengths_past_32_bits():
+    """As on a GPU: positions and context lengths stop at the largest int32, tokens without a block go to the pad block."""
+    big = 2**31 - 1
+    got = serving.batch_maps(_i32([5, 6]), _i32([1, 1]), _i32([big - 1, big]), _i32([3, big]), 5, 1, pad_block=9)
+    assert got.positions.tolist() == [big - 1] + [big] * 4 and got.context_lens.tolist() == [big, big]
+    assert got.slots.tolist() == [9 * 16 + (big - 1 + j) % 16 for j in (0, 1, 2, 1, 2)] and got.q_start.tolist() == [0, 3, 5]
+
+
 @pytest.mark.parametrize("change", [
     {"total_tokens": -1}, {"max_blocks": 0}, {"block_size": 0}, {"pad_block": -1},
     {"block_ids": torch.zeros(2, dtype=torch.int64)}, {"block_ids": torch.zeros(1, 2, dtype=I32)},
