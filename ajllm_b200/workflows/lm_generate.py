@@ -101,7 +101,8 @@ def run(config: LoadedConfig) -> dict[str, Any]:
             owners.append(index)
     started = time.perf_counter()
     if engine_cfg.get("share_prefix") and len(requests) > 1:
-        engine.share_prefix(common_prefix(encoded))
+        # (of what the scheduler leaves of prompts that are too long)
+        engine.share_prefix(common_prefix([ids[-model.context_length:] for ids in encoded]))
     outputs = engine.generate([r[0] for r in requests], [r[1] for r in requests])
     elapsed = time.perf_counter() - started
     results = [{"prompt": p, "completions": []} for p in prompts]

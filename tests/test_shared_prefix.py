@@ -588,6 +588,23 @@ def test_lm_generate_shares_the_prompts_beginning_and_penalises(tmp_path):
     assert parameters["logit_bias"] == {65: 1000.0} and parameters["frequency_penalty"] == 0.5
 
 
+def test_lm_generate_shares_the_beginning_of_what_is_left_of_prompts_that_are_too_long(tmp_path):
+    """Prompts past the context length lose their beginning: what they share behind it is shared, not what was cut off."""
+    from ajllm_b200.workflows import lm_generate, lm_train
+    from tests.helpers import loaded, make_project, prepare_artifacts, train_config
+    project = make_project(tmp_path)
+    prepare_artifacts(project)
+    run = lm_train.run(loaded(project, train_config(project, max_steps=1)))["run_directory"]
+    config = {"name": "g", "run_directory": run, "checkpoint": "final", "prompts": ["The night train ran " * 40 + end for end in ("a", "b", "c")],
+              "max_new_tokens": 3, "temperature": 0.0, "device": "cpu"}
+
+    def texts(**engine):
+        out = lm_generate.run(loaded(project, {**config, "engine": {"block_size": 1, "max_num_seqs": 1, **engine}}))
+        return [c["text"] for r in out["results"] for c in r["completions"]]
+
+    assert texts(share_prefix=True) == texts()
+
+
 def test_the_extension_leaves_cpu_tensors_alone():
     """With the kernel library loaded, CPU calls still take the plain statements, and wrong ones their own errors."""
     from ajllm_b200.ops import native
