@@ -839,7 +839,6 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     for (uint32_t piece = 0;; ++piece) {
       const int n_tiles = w.n_tiles, rows = w.rows;
       const int sees_least = w.ctx - (rows - 1) / p.group;           // keys that the first new token sees
-      const int k_max = min(sees_least + my_token, w.keys) - 1;      // last visible key of row `lane`
       float m_run = -INFINITY;                        // of row `lane`
       float l[R];                                     // of every row, this thread's keys only
 #pragma unroll
@@ -857,10 +856,12 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_free[b]);
         if ((w.t0 + j + 1) * DTILE > min(sees_least, w.keys)) {      // some row does not see the whole tile
+          // rows are packed token by token: hidden from the tokens in front of the one at this key
           const int key = (w.t0 + j) * DTILE + key_lane;
+          const int hidden = key < w.keys ? max(key - sees_least + 1, 0) * p.group : R;
 #pragma unroll
           for (int r = 0; r < R; ++r)
-            if (key > __shfl_sync(0xffffffffu, k_max, r)) sv[r] = 0xff800000u;       // -inf
+            if (r < hidden) sv[r] = 0xff800000u;       // -inf
         }
         float mine = -INFINITY;
 #pragma unroll
@@ -883,20 +884,20 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         // probability tile b was last read by the second product of step g - 2, and O^T changes scale only when every
         // product up to step g - 1 has landed
         if (g > 1 && !wait(&pv_done[b], ((g - 2) >> 1) & 1, 7)) { ok = false; break; }
-        if (any_moved) {
+        if (any_moved && j > 0) {
+          if (!wait(&pv_done[b ^ 1], ((g - 1) >> 1) & 1, 7)) { ok = false; break; }
+          tc_fence_after_sync();
+          uint32_t ov[R];
+          tmem_ld_rows<R>(lane_base + C::kOCol, ov);
+          tc_wait_ld();
 #pragma unroll
-          for (int r = 0; r < R; ++r) l[r] *= __shfl_sync(0xffffffffu, alpha, r);
-          if (j > 0) {
-            if (!wait(&pv_done[b ^ 1], ((g - 1) >> 1) & 1, 7)) { ok = false; break; }
-            tc_fence_after_sync();
-            uint32_t ov[R];
-            tmem_ld_rows<R>(lane_base + C::kOCol, ov);
-            tc_wait_ld();
-#pragma unroll
-            for (int r = 0; r < R; ++r) ov[r] = __float_as_uint(__uint_as_float(ov[r]) * __shfl_sync(0xffffffffu, alpha, r));
-            tmem_st_rows<R>(lane_base + C::kOCol, ov);
-            tc_wait_st();
+          for (int r = 0; r < R; ++r) {
+            const float shrink = __shfl_sync(0xffffffffu, alpha, r);
+            l[r] *= shrink;
+            ov[r] = __float_as_uint(__uint_as_float(ov[r]) * shrink);
           }
+          tmem_st_rows<R>(lane_base + C::kOCol, ov);
+          tc_wait_st();
         }
         // P^T rows are query rows, 64 keys to 128 bytes; two lanes trade so that each stores two keys of one row
         uint8_t* tile_p = sP + b * C::kP + (quarter >> 1) * (N * 128);
@@ -937,16 +938,20 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       if (p.part_stride > 0 && quarter == 0 && real && (n_tiles == 0 || !ok)) p.part_ml[part_row(out_row)] = make_float2(0.0f, 0.0f);
       if (!ok) break;
       if (n_tiles > 0) {
-        float sum = 0.0f;                             // of row `lane`, this warp's keys
+        // Lane r is to have the sum of row r over this warp's keys. Two lanes trade halves of their rows, then quarters, ...:
+        // R - 1 exchanges, where summing every row over all lanes takes 5 R.
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
+        for (int half = R / 2; half > 0; half >>= 1) {
+          const bool upper = (lane & half) != 0;
 #pragma unroll
-          for (int r = 0; r < R; ++r) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
+          for (int r = 0; r < half; ++r) {
+            const float theirs = upper ? l[r] : l[r + half], mine = upper ? l[r + half] : l[r];
+            l[r] = mine + __shfl_xor_sync(0xffffffffu, theirs, half);
+          }
         }
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-          if (lane == r) sum = l[r];
-        publish(sum);
+        for (int o = R; o < 32; o <<= 1) l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
+        publish(l[0]);
       }
       if (next.n_tiles > 0) {
 #pragma unroll
@@ -971,14 +976,22 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           uint32_t ov[R];
           tmem_ld_rows<R>(lane_base + C::kOCol, ov);
           tc_wait_ld();
+          // 32 neighbouring elements of row r per warp; rows and parts are counted in 32 bits (each is 256 bytes at least)
+          if (p.part_stride > 0) {
+            const int place = (int)part_row(out_row);
+            float* dst = p.part_o + key_lane;
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
-            // 32 neighbouring elements of row r per warp
-            const int row = __shfl_sync(0xffffffffu, out_row, r);
-            const float scale = __shfl_sync(0xffffffffu, inv_l, r);
-            if (r < rows) {
-              if (p.part_stride > 0) p.part_o[part_row(row) * HD + key_lane] = __uint_as_float(ov[r]);
-              else p.out[(size_t)row * HD + key_lane] = __float2bfloat16(__uint_as_float(ov[r]) * scale);
+            for (int r = 0; r < R; ++r) {
+              const int at = __shfl_sync(0xffffffffu, place, r);
+              if (r < rows) dst[(long long)at * HD] = __uint_as_float(ov[r]);
+            }
+          } else {
+            __nv_bfloat16* dst = p.out + key_lane;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+              const int at = __shfl_sync(0xffffffffu, out_row, r);
+              const float scale = __shfl_sync(0xffffffffu, inv_l, r);
+              if (r < rows) dst[(long long)at * HD] = __float2bfloat16(__uint_as_float(ov[r]) * scale);
             }
           }
         }
