@@ -7,7 +7,8 @@
 // Nothing is computed to speak of: a call lasts as long as one dependent chain (lengths -> sums -> block id -> store),
 // plus the time to write the tables when they are large. So there is one launch and no second pass over partial sums:
 // every CTA reads all lengths at once and sums them itself (a few KB out of L2, n / 256 per thread) and then takes its
-// share of the output in pieces of four elements, 16 bytes a store. 8 sequences: 3.3 us, 256: 4.3 us. Lengths are read as at least 0, and sums saturate at 2^30 - 1, so no input
+// share of the output in pieces of four elements, 16 bytes a store. 8 sequences: 3.3 us, 256: 4.1 us. Lengths are read
+// as at least 0, and sums saturate at 2^30 - 1, so no input
 // reaches an index out of range: a token whose sequence has no block for it, and a row behind the last sequence, gets
 // the pad block.
 #include "common.cuh"

@@ -4,7 +4,8 @@
 // KV head (group = Hq / Hkv query heads, q_len new tokens: 1 for plain decoding, k + 1 when verifying k draft tokens) are
 // worked on together, so every K/V byte of the sequence is read once for all of them, in tiles of keys that TMA fetches
 // block by block (16 tokens, addressed through the block table). S = Q K^T and O += P V run on the tensor cores with
-// accumulators in tensor memory, the softmax between them in registers with fp32 maxima and sums. Row (head h, new token
+// accumulators in tensor memory, the softmax between them in registers with fp32 maxima and sums; probabilities are rounded
+// to bf16 as the operand of the second product, whose other operand, the cached values, is bf16 too. Row (head h, new token
 // i) may see keys 0 .. context_len - q_len + i.
 //
 // The caches are streamed once with little arithmetic per byte, so the bytes in flight per SM and the length of a step's
@@ -12,7 +13,7 @@
 // query rows per piece, with two CTAs per SM so that one's chain hides behind the other's loads (one for 17 to 32 rows of 128):
 //   up to 32 (paged_decode_kernel): keys on the 128-row side of the tensor-core tile, 128 of them per step;
 //   more (paged_attention_kernel): query rows on it, 64 keys per step.
-// 256 sequences of 1280 tokens, 8 KV heads of 128, 4 rows each: 195 us, 6.9 TB/s; 16 sequences of 1024: 15.5 us.
+// 256 sequences of 1280 tokens, 8 KV heads of 128, 4 rows each: 191 us, 7.0 TB/s; 16 sequences of 1000: 15.7 us.
 //
 // Long contexts at small batch: with `splits` > 1 the tiles of a sequence are divided over that many pieces. Each leaves
 // its un-normalised fp32 output rows and (reference maximum, row sum) in a workspace, and a second small kernel joins them
@@ -531,7 +532,8 @@ __device__ __forceinline__ void tmem_st_rows(uint32_t taddr, const uint32_t (&r)
 // R: query rows that the softmax warps work on (the real ones rounded up to 4, 8, 16 or 32; what comes of the others is not
 // used). A piece of work may be a single tile, so a warp walks through most of its code once per piece: the code is kept
 // short (one place for each wait, load and product, rows as a template parameter instead of branches), as instruction
-// fetches cost short contexts more than arithmetic (256 sequences x 32..512 keys: 80 us before, 60 % of the fetches hit).
+// fetches cost short contexts more than arithmetic (256 sequences x 32..512 keys: 80 us before, 60 % of the fetches hit; 20
+// rows x 20 keys: 8.4 us with some 35 instructions per row, 5.9 us with some 20).
 template <int HD, int R>
 __global__ void __launch_bounds__(kThreads, (DecodeCfg<HD, (R < 16 ? 16 : R)>::kCtas))
 paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Params p) {

@@ -278,7 +278,7 @@ def prefix_plan(n: int, q_len: int, group: int, kv_heads: int, head_dim: int, sh
     ``behind`` tokens; unless that is ``known`` to be what they have, the division is the one that does best for suffixes of
     up to that and up to half of it together, or, in tables with room for more than 1024 behind the prefix, of up to 128 and
     up to 512 (such tables are often much wider than contexts: 64 sequences behind 2048 + 32 tokens in tables for 8192 took
-    45 us when divided for the tables, 22 us now). Whichever of the two forms is
+    45 us when divided for the tables, 21 us now). Whichever of the two forms is
     estimated to end first is taken (in us, from measurements of 4 to 1024 query rows per KV head, prefixes of 512 to 7680
     and suffixes of 32 to 1024 tokens)."""
     if not _SM_COUNT:
@@ -307,7 +307,7 @@ def prefix_plan(n: int, q_len: int, group: int, kv_heads: int, head_dim: int, sh
 def _pieces_plans(n, q_len, group, kv_heads, head_dim, tiles, expected, divisions, least, sms):
     """The prefix in pieces of the paged launch, for 16 query rows each (32 where a sequence has more than 16): a second read
     of the prefix from L2 costs less than pieces of 32 rows, of which an SM holds one instead of two (8 sequences of 4 rows,
-    512 + 32 tokens: 9.0 us against 10.7). A piece takes 3 us and 1.1 us per 128 keys (32 rows: 1.5 us)."""
+    512 + 32 tokens: 7.2 us against 7.8). A piece takes 3 us and 1.1 us per 128 keys (32 rows: 1.5 us)."""
     height = 16 if group * q_len <= 16 else 32
     tokens = height // group
     slots = sms * (2 if height == 16 or head_dim == 64 else 1)
