@@ -415,6 +415,22 @@ def test_two_captured_graphs_and_eager_calls_do_not_disturb_each_other():
     assert torch.equal(eager, outs[0])
 
 
+@pytest.mark.parametrize("heads,kv_heads,hd,q_len,prefix,suffixes", [
+    (32, 8, 128, 1, 1024, list(range(1, 150))),          # more pieces than run at once: which CTA takes which one varies
+    (32, 8, 64, 5, 2048, [5, 40, 300] * 30),
+    (8, 2, 64, 61, 200, [61, 99] * 8),
+])
+def test_the_same_call_repeats_itself_bit_for_bit(heads, kv_heads, hd, q_len, prefix, suffixes):
+    batch = _batch(heads, kv_heads, hd, q_len, prefix, suffixes)
+    lens = batch[4].tolist()
+    calls = [lambda: serving.shared_prefix_attention(*batch, prefix, q_len=q_len)]
+    if heads // kv_heads * q_len <= 64:
+        calls.append(lambda: serving.paged_attention(*batch[:4], None, None, [q_len] * len(lens), lens))
+    for call in calls:
+        first = call()
+        assert all(torch.equal(first, call()) for _ in range(10))
+
+
 def test_tables_shorter_than_the_context_bound_what_is_read():
     """A context length beyond the block table (a caller's mistake that only the device sees) reads nothing behind it."""
     q, keys, values, tables, context = _batch(8, 2, 128, 1, 64, [100, 30], poison=False)
